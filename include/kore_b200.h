@@ -252,6 +252,68 @@ int kb_decoder_step(kb_decoder *h, long long *tokens, int *positions, int *lens,
 /* 0 = clean; otherwise KB_ERR_TIMEOUT and the code of the bounded wait that gave up (the word is cleared) */
 int kb_decoder_status(kb_decoder *h, kb_stream stream, int *status);
 
+/* ---- serving step: norms + rotation + cache append, a KV cache held in 4 bits, attention over it, sampling ----
+ * The reference's edge runtime keeps an f32 cache, one KV head per query head and a greedy head
+ * (crates/kore-edge/src/runtime.rs:106-294); these entry points stand beside kb_rope_kv, kb_attn_decode and
+ * kb_lm_head_argmax.  Device pointers of the current device, work enqueued on `stream`.
+ *
+ * The 4-bit cache holds one row per (sequence, KV head, position).  K and V have two planes each:
+ *   codes  uint32 [n_seqs][n_kv_heads][lmax][kb_kv4_row_words(head_dim)]: dim 8w + i in bits 4i .. 4i+3 of word w, the tail
+ *          of the last word zero;
+ *   steps  uint32 [n_seqs][n_kv_heads][lmax]: two bfloat16 numbers, the step in the low half and lo in the high half.
+ * A code c stands for lo + c * step (one f32 rounding).  head_dim is a multiple of 4 up to 128, lmax a multiple of 4, the
+ * planes are 16-byte aligned.  A row is quantised from its own f32 values x:
+ *   lo = bfloat16 at or below min(x);  step = bfloat16 at or above max((max(x) - lo) / 15, 2^-100);
+ *   code = clamp(rne((x - lo) * (1 / step)), 0, 15)
+ * with every f32 operation rounded once.  A row that holds an infinity or a NaN, or whose range overflows f32, is stored
+ * with NaN for both numbers and reads back as NaN. */
+size_t kb_kv4_row_words(int head_dim);
+
+/* Per token: RMSNorm of every query and key head over its head_dim (q_gamma / k_gamma [head_dim], each nullable: no norm),
+ * half-split rotation, k and v appended to the cache, one pass over rows [q (n_heads) | k (n_kv_heads) | v (n_kv_heads)]
+ * of stride ld (0 = their width).  inv = f32(1 / sqrt(mean(x^2) + eps)) with the mean in f64, y = (x * inv) * gamma, then
+ * the rotation of kb_rope_kv; f32 operations are rounded one by one, so both forms append the same values.
+ * cos/sin tables are [max_pos][head_dim / 2]; cache_rows[t] = sequence * lmax + position.  A token whose cache row lies
+ * outside [0, n_seqs * lmax) (a negative one for padding) is not appended; one whose position lies outside [0, max_pos)
+ * is not appended either and gets NaN queries.  Two tokens of a call must not name the same cache row.
+ * kb_qknorm_rope_kv appends f32 to head-major caches [n_seqs][n_kv_heads][lmax][head_dim] (head_dim even, up to 128),
+ * kb_qknorm_rope_kv4 appends to the 4-bit planes.  n_heads a multiple of n_kv_heads. */
+int kb_qknorm_rope_kv(const float *qkv, size_t ld, const int *positions, const long long *cache_rows, const float *cos_table,
+                      const float *sin_table, size_t max_pos, const float *q_gamma, const float *k_gamma, float eps, size_t n,
+                      int n_heads, int n_kv_heads, int head_dim, size_t n_seqs, int lmax, float *q_out, float *k_cache,
+                      float *v_cache, kb_stream stream);
+int kb_qknorm_rope_kv4(const float *qkv, size_t ld, const int *positions, const long long *cache_rows, const float *cos_table,
+                       const float *sin_table, size_t max_pos, const float *q_gamma, const float *k_gamma, float eps, size_t n,
+                       int n_heads, int n_kv_heads, int head_dim, size_t n_seqs, int lmax, float *q_out, uint32_t *k_codes,
+                       uint32_t *k_steps, uint32_t *v_codes, uint32_t *v_steps, kb_stream stream);
+/* Rows read back as f32: out[i][n_kv_heads][head_dim] = the values of cache row cache_rows[i] (zeros where it lies outside
+ * the cache), for K and V in one launch; k_out or v_out may be NULL. */
+int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes, const uint32_t *v_steps,
+                const long long *cache_rows, size_t n, int n_kv_heads, int head_dim, size_t n_seqs, int lmax, float *k_out,
+                float *v_out, kb_stream stream);
+/* Attention of t query tokens per sequence over the 4-bit cache: q and out [batch][t][n_heads][head_dim], query head h
+ * reads KV head h / (n_heads / n_kv_heads).  lens[b] counts the cache positions up to and including the last query token's
+ * (clamped to 0 .. lmax): query token i sees the positions below lens[b] - (t - 1 - i).  A query that sees none gives
+ * zeros; positions it does not see have no influence, whatever they hold.  scale multiplies the scores, 0 means
+ * 1 / sqrt(head_dim).  Statistics and sums are f32.  workspace: kb_attn_kv4_workspace_bytes bytes, 16-byte aligned, no
+ * initial contents needed, not shared by calls that overlap; NULL takes it from the stream-ordered allocator. */
+int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes,
+                const uint32_t *v_steps, const int *lens, size_t batch, int t, int n_heads, int n_kv_heads, int head_dim,
+                int lmax, float scale, float *out, void *workspace, size_t workspace_bytes, kb_stream stream);
+size_t kb_attn_kv4_workspace_bytes(size_t batch, int t, int n_heads, int n_kv_heads, int head_dim, int lmax);
+/* One token per row of logits [n][vocab] (row stride ld, 0 = vocab) from one given uniform number u[i] in [0, 1) per row.
+ * Settings are device arrays of one value per row, each nullable (NULL: temperature 1, the filter off):
+ *   weights  exp((logit - max) / temperature); a temperature of 0 (or below, or NaN) takes the largest logit;
+ *   top_k    the k largest logits (<= 0: off);  min_p  weights of at least min_p times the largest (<= 0: off; above 1 is 1);
+ *   top_p    of what those two keep, the shortest run from the largest on whose weights reach top_p of the sum (>= 1: off).
+ * Runs go by logit, equal logits by index, lowest first; the largest is always kept.  The token is the first, in index
+ * order, whose running sum of kept weights exceeds u times their total.  Weights are summed as 64-bit integers of 2^-44,
+ * so the answer depends neither on the order of the sums nor on the launch.  logprobs[i] (nullable): the log of the
+ * token's share of the kept weights.  NaN logits count as -inf; a row without a larger one gives token 0 (as
+ * kb_decode_advance) and logprob NaN.  vocab up to 2^19. */
+int kb_sample(const float *logits, size_t n, size_t vocab, size_t ld, const float *temperature, const int *top_k,
+              const float *top_p, const float *min_p, const float *u, long long *tokens, float *logprobs, kb_stream stream);
+
 /* ---- forward (host pointers; what a Tensor-in/Tensor-out caller uses) ---- */
 
 /* Copies x to the device, runs kb_linear_forward, copies y back, synchronises.

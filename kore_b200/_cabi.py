@@ -54,6 +54,16 @@ SIGNATURES = {
     "kb_decoder_destroy": (None, [_vp]),
     "kb_decoder_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "kb_decoder_status": (C.c_int, [_vp, _vp, C.POINTER(C.c_int)]),
+    "kb_kv4_row_words": (_sz, [C.c_int]),
+    "kb_qknorm_rope_kv": (C.c_int, [_vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, C.c_float, _sz, C.c_int, C.c_int, C.c_int, _sz, C.c_int,
+                                    _vp, _vp, _vp, _vp]),
+    "kb_qknorm_rope_kv4": (C.c_int, [_vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, C.c_float, _sz, C.c_int, C.c_int, C.c_int, _sz, C.c_int,
+                                     _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kb_kv4_read": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _sz, C.c_int, C.c_int, _sz, C.c_int, _vp, _vp, _vp]),
+    "kb_attn_kv4": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _vp, _vp, _sz,
+                              _vp]),
+    "kb_attn_kv4_workspace_bytes": (_sz, [_sz, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "kb_sample": (C.c_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "kb_linear_forward_host": (C.c_int, [_vp, _vp, _sz, _sz, _vp]),
     "kb_linear_forward_static": (C.c_int, [_vp, _vp, _sz, _sz, _vp, _vp]),
     "kb_linear_group_create": (C.c_int, [_vp, _sz, _vp]),

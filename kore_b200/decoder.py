@@ -16,6 +16,12 @@ For one sequence a decode step is ONE launch of the library's persistent decode-
 (``kb_decoder_step``: every phase of every layer, the lm_head GEMV and the argmax inside one
 cooperative grid; it also takes two sequences, ``persistent=True``, where the graph is a few
 percent faster); larger batches run the step as a CUDA graph of the separate kernels.
+
+Beyond the reference's loop: ``kv_bits=4`` keeps the KV cache in 4 bits (``serving.KV4Cache``; decode
+attention reads the codes, prefill attention their values), ``n_kv_heads`` groups query heads over fewer KV
+heads (with the 4-bit cache), ``qk_norm`` normalises every query and key head before the rotation, and
+``set_sampling`` replaces the greedy choice by ``serving.sample``.  A step with a 4-bit cache, grouped heads
+or norms is always the graph of separate kernels.
 """
 from __future__ import annotations
 
@@ -25,7 +31,7 @@ from typing import Dict, List, Optional
 
 import numpy as np
 
-from . import _cabi, nn
+from . import _cabi, nn, serving
 
 
 @dataclass
@@ -38,10 +44,21 @@ class DecoderConfig:
     eps: float = 1e-5
     rope_base: float = 10000.0
     max_len: int = 640
+    n_kv_heads: Optional[int] = None  # None: one per query head
+    qk_norm: bool = False
+    kv_bits: int = 32  # 32: f32 cache, 4: serving.KV4Cache
 
     @property
     def head_dim(self) -> int:
         return self.d_model // self.n_heads
+
+    @property
+    def kv_heads(self) -> int:
+        return self.n_kv_heads or self.n_heads
+
+    @property
+    def kv_dim(self) -> int:
+        return self.kv_heads * self.head_dim
 
 
 def rope_tables(cfg: DecoderConfig):
@@ -64,7 +81,7 @@ def random_weights(cfg: DecoderConfig, seed: int = 4000, device: int = 0) -> Dic
     import torch
 
     d, f = cfg.d_model, cfg.d_ff
-    shapes = {"q": (d, d), "k": (d, d), "v": (d, d), "o": (d, d), "gate": (f, d), "up": (f, d), "down": (d, f)}
+    shapes = {"q": (d, d), "k": (cfg.kv_dim, d), "v": (cfg.kv_dim, d), "o": (d, d), "gate": (f, d), "up": (f, d), "down": (d, f)}
     layers = []
     for li in range(cfg.n_layers):
         entry = {}
@@ -76,6 +93,9 @@ def random_weights(cfg: DecoderConfig, seed: int = 4000, device: int = 0) -> Dic
             lay.close()
         entry["norm1"] = np.ones(d, np.float32)
         entry["norm2"] = np.ones(d, np.float32)
+        if cfg.qk_norm:
+            entry["q_norm"] = np.ones(cfg.head_dim, np.float32)
+            entry["k_norm"] = np.ones(cfg.head_dim, np.float32)
         layers.append(entry)
     g = torch.Generator().manual_seed(seed + 999)
     embed = (torch.randn((cfg.vocab, d), generator=g) * 0.02).numpy()
@@ -109,6 +129,12 @@ class BitNetDecoder:
                  persistent: Optional[bool] = None):
         import torch
 
+        if cfg.kv_bits not in (4, 32):
+            raise _cabi.KoreError(_cabi.ERR_UNSUPPORTED, f"kv_bits {cfg.kv_bits}: the cache is held in 32 or 4 bits")
+        if cfg.n_heads % cfg.kv_heads:
+            raise _cabi.KoreError(_cabi.ERR_INVALID, f"{cfg.n_heads} heads over {cfg.kv_heads} KV heads")
+        if cfg.kv_bits == 32 and cfg.kv_heads != cfg.n_heads:
+            raise _cabi.KoreError(_cabi.ERR_UNSUPPORTED, "grouped KV heads need kv_bits=4: the f32 cache has one per query head")
         self.cfg, self.batch, self.device = cfg, batch, device
         self.torch = torch
         self.lib = _cabi.lib()
@@ -121,16 +147,23 @@ class BitNetDecoder:
             mk = lambda t: nn.BitLinear.from_packed(t[0], t[1], None, t[3], t[2], device=device)
             self.layers.append({
                 "qkv": mk(qkv), "o": mk(lw["o"]), "gu": mk(gu), "down": mk(lw["down"]),
-                "norm1": torch.from_numpy(lw["norm1"]).to(self.dev), "norm2": torch.from_numpy(lw["norm2"]).to(self.dev)})
+                "norm1": torch.from_numpy(lw["norm1"]).to(self.dev), "norm2": torch.from_numpy(lw["norm2"]).to(self.dev),
+                **{g: torch.from_numpy(lw[g]).to(self.dev) if cfg.qk_norm else None for g in ("q_norm", "k_norm")}})
         self.embed = torch.from_numpy(weights["embed"]).to(self.dev)
         self.lm_head = torch.from_numpy(weights["lm_head"]).to(self.dev).contiguous()  # [vocab, d] row-major
         self.norm_f = torch.from_numpy(weights["norm_f"]).to(self.dev)
         cos, sin = rope_tables(cfg)
         self.cos, self.sin = torch.from_numpy(cos).to(self.dev), torch.from_numpy(sin).to(self.dev)
         # KV caches are head-major, [batch, heads, max_len, head_dim]: a head's keys and values are contiguous
-        kv_shape = (batch, cfg.n_heads, cfg.max_len, cfg.head_dim)
-        self.kc = [torch.zeros(kv_shape, dtype=torch.float32, device=self.dev) for _ in range(cfg.n_layers)]
-        self.vc = [torch.zeros(kv_shape, dtype=torch.float32, device=self.dev) for _ in range(cfg.n_layers)]
+        self.kv4 = None
+        self.lmax = cfg.max_len
+        if cfg.kv_bits == 4:
+            self.kv4 = [serving.KV4Cache(batch, cfg.kv_heads, cfg.max_len, cfg.head_dim, device) for _ in range(cfg.n_layers)]
+            self.lmax = self.kv4[0].max_len
+        else:
+            kv_shape = (batch, cfg.n_heads, cfg.max_len, cfg.head_dim)
+            self.kc = [torch.zeros(kv_shape, dtype=torch.float32, device=self.dev) for _ in range(cfg.n_layers)]
+            self.vc = [torch.zeros(kv_shape, dtype=torch.float32, device=self.dev) for _ in range(cfg.n_layers)]
         self.ld_d, self.ld_f = int(self.lib.kb_act_ld(d)), int(self.lib.kb_act_ld(f))
         self._bufs = {}
         self._alloc(batch)
@@ -138,20 +171,22 @@ class BitNetDecoder:
             self._alloc(max_prefill_tokens)
         self.positions = torch.zeros(batch, dtype=torch.int32, device=self.dev)
         self.lens = torch.ones(batch, dtype=torch.int32, device=self.dev)
-        self.cache_rows = (torch.arange(batch, dtype=torch.int64, device=self.dev) * cfg.max_len)
+        self.cache_rows = (torch.arange(batch, dtype=torch.int64, device=self.dev) * self.lmax)
         self.tokens = torch.zeros(batch, dtype=torch.int64, device=self.dev)
         self.logits = torch.zeros((batch, v), dtype=torch.float32, device=self.dev)
         self.att_bytes = int(self.lib.kb_attn_decode_scratch_bytes(batch, cfg.n_heads))
         self.att_scratch = torch.zeros(self.att_bytes, dtype=torch.uint8, device=self.dev)
         self.graph = None
         self.launches_per_step = 0
+        self.sampling = None  # settings of serving.sample, or None: greedy
+        self.uniform = torch.zeros(batch, dtype=torch.float32, device=self.dev)
         # persistent decode step (one launch per step) where the library supports the shape
         self.persistent = None
         self.hidden_step = torch.zeros((batch, d), dtype=torch.float32, device=self.dev)
         self.head_keys = torch.zeros(batch, dtype=torch.int64, device=self.dev)  # argmax keys of the library's head
         if persistent is None:
             persistent = batch == 1
-        if batch <= 2 and persistent:
+        if batch <= 2 and persistent and self.kv4 is None and not cfg.qk_norm:
             n = cfg.n_layers
             arr = lambda ptrs: (C.c_void_p * n)(*ptrs)
             h = C.c_void_p()
@@ -181,7 +216,7 @@ class BitNetDecoder:
         z = lambda shape, dt=torch.float32: torch.zeros(shape, dtype=dt, device=self.dev)
         ws_bytes = max(int(self.lib.kb_linear_workspace_bytes(self.layers[0]["o"].handle, n)), 256)
         self._bufs[n] = {
-            "hidden": z((n, d)), "qkv": z((n, 3 * d)), "q": z((n, d)), "attn": z((n, d)), "gu": z((n, 2 * f)),
+            "hidden": z((n, d)), "qkv": z((n, d + 2 * cfg.kv_dim)), "q": z((n, d)), "attn": z((n, d)), "gu": z((n, 2 * f)),
             "xn": z((n, d)), "xq_d": z((n, self.ld_d), torch.int8), "xq_f": z((n, self.ld_f), torch.int8),
             "sx": z(n), "sum": z(n, torch.int32), "ws": z(ws_bytes + 256, torch.uint8), "ws_bytes": ws_bytes,
             "h": z((n, f)) if n <= 2 else None, "absmax": z((2, n)) if n <= 2 else None}
@@ -206,10 +241,18 @@ class BitNetDecoder:
                                         B["xq_d"].data_ptr(), self.ld_d, B["sx"].data_ptr(), B["sum"].data_ptr(), sp))
                 ck(lib.kb_linear_forward_fused(L["qkv"].handle, None, B["xq_d"].data_ptr(), self.ld_d, B["sx"].data_ptr(),
                                                B["sum"].data_ptr(), n, None, B["qkv"].data_ptr(), 0, _cabi.PATH_AUTO, None, 0, sp))
-            ck(lib.kb_rope_kv(B["qkv"].data_ptr(), positions.data_ptr(), cache_rows.data_ptr(), self.cos.data_ptr(),
-                              self.sin.data_ptr(), n, H, hd, cfg.max_len, B["q"].data_ptr(), self.kc[li].data_ptr(),
-                              self.vc[li].data_ptr(), sp))
-            if prefill_shape is None:
+            if self.kv4 is not None or cfg.qk_norm:
+                cache = self.kv4[li] if self.kv4 is not None else (self.kc[li], self.vc[li])
+                serving.qknorm_rope_append(B["qkv"], positions, cache_rows, self.cos, self.sin, cache, H, q_gamma=L["q_norm"],
+                                           k_gamma=L["k_norm"], eps=cfg.eps, q_out=B["q"].view(n, H, hd))
+            else:
+                ck(lib.kb_rope_kv(B["qkv"].data_ptr(), positions.data_ptr(), cache_rows.data_ptr(), self.cos.data_ptr(),
+                                  self.sin.data_ptr(), n, H, hd, cfg.max_len, B["q"].data_ptr(), self.kc[li].data_ptr(),
+                                  self.vc[li].data_ptr(), sp))
+            if prefill_shape is None and self.kv4 is not None:
+                serving.attend(B["q"].view(n, H, hd), self.kv4[li], lens, out=B["attn"].view(n, H, hd))
+                launches += 2
+            elif prefill_shape is None:
                 ck(lib.kb_attn_decode(B["q"].data_ptr(), self.kc[li].data_ptr(), self.vc[li].data_ptr(), lens.data_ptr(),
                                       n, H, hd, cfg.max_len, B["attn"].data_ptr(), self.att_scratch.data_ptr(),
                                       self.att_bytes, sp))
@@ -217,9 +260,12 @@ class BitNetDecoder:
             else:
                 b, t = prefill_shape
                 qh = B["q"].view(b, t, H, hd).transpose(1, 2)
-                kh = self.kc[li][:b, :, :t]
-                vh = self.vc[li][:b, :, :t]
-                o = torch.nn.functional.scaled_dot_product_attention(qh, kh, vh, is_causal=True)
+                if self.kv4 is not None:  # the prompt attends to what the cache holds, as the decode steps will
+                    kh, vh = (x.view(b, t, cfg.kv_heads, hd).transpose(1, 2) for x in self.kv4[li].read(cache_rows))
+                else:
+                    kh = self.kc[li][:b, :, :t]
+                    vh = self.vc[li][:b, :, :t]
+                o = torch.nn.functional.scaled_dot_product_attention(qh, kh, vh, is_causal=True, enable_gqa=cfg.kv_heads != H)
                 B["attn"].view(b, t, H, hd).copy_(o.transpose(1, 2))
                 launches += 4
             ck(lib.kb_linear_forward_fused(L["o"].handle, B["attn"].data_ptr(), None, 0, None, None, n, B["hidden"].data_ptr(),
@@ -266,14 +312,14 @@ class BitNetDecoder:
         if n not in self._bufs:
             self._alloc(n)
         pos = torch.arange(t, dtype=torch.int32, device=self.dev).repeat(b)
-        rows = (torch.arange(b, dtype=torch.int64, device=self.dev)[:, None] * self.cfg.max_len
+        rows = (torch.arange(b, dtype=torch.int64, device=self.dev)[:, None] * self.lmax
                 + torch.arange(t, dtype=torch.int64, device=self.dev)[None, :]).reshape(-1)
         B = self._layers(n, prompt.reshape(-1), pos, rows, None, prefill_shape=(b, t))
         last = B["hidden"].view(b, t, -1)[:, -1].contiguous()
         logits = self._head(last)
         self.positions.fill_(t)
         self.lens.fill_(t + 1)
-        self.cache_rows.copy_(torch.arange(b, dtype=torch.int64, device=self.dev) * self.cfg.max_len + t)
+        self.cache_rows.copy_(torch.arange(b, dtype=torch.int64, device=self.dev) * self.lmax + t)
         return logits
 
     def _decode_body(self):
@@ -290,23 +336,54 @@ class BitNetDecoder:
                                               self.logits.data_ptr(), self.head_keys.data_ptr(), sp))
             _cabi.check(lib.kb_decode_advance(self.head_keys.data_ptr(), n, self.tokens.data_ptr(), self.positions.data_ptr(),
                                               self.lens.data_ptr(), self.cache_rows.data_ptr(), sp))
+            self._sample()
             return
         logits = self._head(B["hidden"])
         self.torch.argmax(logits, dim=1, out=self.tokens)
+        self._sample()
         self.positions.add_(1)
         self.lens.add_(1)
         self.cache_rows.add_(1)
 
-    def decode_step(self, use_graph: bool = True):
-        """One greedy decode step for every sequence: consumes self.tokens (the tokens chosen
-        by the previous step), leaves the next tokens in self.tokens and logits in self.logits."""
+    def set_sampling(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0):
+        """Later steps choose their tokens with ``serving.sample``.  Every setting is a number or one number per sequence; the
+        uniform numbers of the steps come from a generator of this seed.  ``temperature=None`` goes back to the greedy choice."""
         torch = self.torch
+        if (temperature is None) != (self.sampling is None):
+            self.graph = None  # captured with the other choice
+        if temperature is None:
+            self.sampling = None
+            return
+        put = lambda v, dt: torch.as_tensor(np.broadcast_to(np.asarray(v), (self.batch,)).copy(), dtype=dt).to(self.dev)
+        new = {"temperature": put(temperature, torch.float32), "top_k": put(top_k, torch.int32), "top_p": put(top_p, torch.float32),
+               "min_p": put(min_p, torch.float32)}
+        if self.sampling is None:
+            self.sampling = new
+        else:  # in place: a captured step reads these tensors
+            for name, v in new.items():
+                self.sampling[name].copy_(v)
+        self.generator = torch.Generator(device=self.dev).manual_seed(seed)
+
+    def _sample(self):
+        if self.sampling is not None:
+            serving.sample(self.logits, self.uniform, tokens=self.tokens, **self.sampling)
+
+    def _draw_uniform(self):
+        if self.sampling is not None:
+            self.torch.rand(self.batch, generator=self.generator, out=self.uniform)
+
+    def decode_step(self, use_graph: bool = True):
+        """One decode step for every sequence: consumes self.tokens (the tokens chosen by the previous step), leaves the
+        next tokens in self.tokens (the largest logits, or drawn as ``set_sampling`` says) and logits in self.logits."""
+        torch = self.torch
+        self._draw_uniform()
         if self.persistent is not None:
             sp = torch.cuda.current_stream(self.device).cuda_stream
             _cabi.check(self.lib.kb_decoder_step(self.persistent, self.tokens.data_ptr(), self.positions.data_ptr(),
                                                  self.lens.data_ptr(), self.cache_rows.data_ptr(), self.hidden_step.data_ptr(),
                                                  self.logits.data_ptr(), sp))
             self.launches_per_step = 1
+            self._sample()
             return
         if not use_graph:
             return self._decode_body()
@@ -334,10 +411,12 @@ class BitNetDecoder:
             _cabi.check(self.lib.kb_decoder_status(self.persistent, None, C.byref(st)))
 
     def generate(self, prompt, steps: int, use_graph: bool = True):
-        """Greedy generation: returns int64 [batch, steps] of new tokens."""
+        """Greedy or sampled generation: returns int64 [batch, steps] of new tokens."""
         torch = self.torch
         logits = self.prefill(prompt)
         torch.argmax(logits, dim=1, out=self.tokens)
+        self._draw_uniform()
+        self._sample()
         out = [self.tokens.clone()]
         for _ in range(steps - 1):
             self.decode_step(use_graph)
