@@ -5,6 +5,7 @@
 // stands for lo + c * step.  One pair per row keeps the unpacking out of the products: a score is
 //     step_j * sum_d(q_d c_jd) + lo_j * sum_d(q_d)      and an output      sum_j (p_j step_j) c_jd + sum_j p_j lo_j,
 // so both contractions run on bare codes and the pair touches one number per (query, position).
+#include <cuda_fp16.h>
 #include <stdlib.h>
 
 #include "common.cuh"
@@ -201,67 +202,391 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 }
 
 // ---- attention ---------------------------------------------------------------------------------
+// Bound by the bytes of the cache as long as the unpacking keeps up: at the copy bandwidth an SM receives a position (K
+// and V, 136 bytes for heads of 128) every 6 clocks, too few for a multiply-add per value on the FP32 lanes.  So both
+// products run on the matrix instruction m16n8k16 with f16 operands and f32 sums, and a 4-bit code becomes an operand by
+// masking alone: the bits 0x00f0 of a 16-bit lane ARE the f16 number code * 2^-20 (subnormal, exact, taken as such by the
+// instruction).  The factor goes into the end of the sums.  The bits 0x000f would do as well (code * 2^-24, two shifts fewer
+// per eight codes), but the instruction aligns its products by the operands' exponent fields, so leading zeros cost
+// bits of the sum: results were 1e-5 off that way.
+//   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo 2^-11
+// (22 bits of x relative to the largest of the row, for which rows are scaled by powers of two).  The terms sit in rows g
+// and g + 8 of the 16-row tile, so a warp serves 8 query rows and the second term costs nothing while the tile is not full.
+//   Lane (g, t) = (lane / 4, lane % 4).  QK^T: the contraction runs over dims in any order as long as queries and keys
+// agree, so a lane takes whole words of key row g.  The result has query row g and two positions per 8-column tile in one
+// lane, which is exactly the operand layout of the weights in the second product: no shuffle between the two.  PV: output
+// column n = g of tile j is dim 8 word(g) + j, so a lane's words of four positions give the columns of eight tiles.
+//   Positions of a 16-block are dealt so that lane t owns rows 4t .. 4t+3 (one 128-bit load of their pairs) and the four
+// rows of a load alternate in parity (64-byte rows otherwise meet in the same banks).
+//   A warp streams its own 32-position tiles through a ring of 16-byte asynchronous copies (no barrier between warps);
+// warps of a CTA deal the tiles of a chunk, chunks of a sequence go to CTAs, a second kernel joins them.
+constexpr int ATT4_WARPS = 4;
+constexpr int ATT4_STAGES = 3;
+constexpr int ATT4_TILE = 32;  // positions of a warp's tile
+constexpr int ATT4_ROWS = 8;   // query rows of a CTA
+
 struct AttnParams {
     const float *q;
     const uint32_t *k_codes, *k_steps, *v_codes, *v_steps;
     const int *lens;
-    int t, n_heads, n_kv, hd, lmax;
+    int t, n_heads, n_kv, hd, lmax, words;
+    int row_tiles, chunk, chunks;  // chunk: positions per CTA, chunks = ceil(lmax / chunk)
     float scale;
     float *out;
+    float *part;      // [rows][chunks][hd] unnormalised sums, where chunks > 1
+    float2 *part_ml;  // [rows][chunks] (largest score, sum of weights)
 };
 
-// One CTA per (sequence, query token, head); a half-warp takes one position at a time, a lane one word of its row.
-__global__ void __launch_bounds__(256) attn_kv4_kernel(AttnParams p) {
-    __shared__ float s_m[16], s_l[16], s_acc[16][KV4_MAX_HD];
-    const int lane = threadIdx.x & 31, w = lane & 15, group = threadIdx.x >> 4;
-    const long long row = blockIdx.x;
-    const int h = (int)(row % p.n_heads), i = (int)(row / p.n_heads % p.t);
-    const long long b = row / p.n_heads / p.t;
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two f32 numbers -> two f16 terms each: x = hi + lo 2^-11 to 22 bits (relative to 2^14, their upper end)
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn((x - f.x) * 2048.0f, (y - f.y) * 2048.0f);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp over the range used here (x <= 0)
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// KC = 32-bit words of a row per lane (4 lanes a row); VEC: rows of exactly 4 KC words, read as vectors
+template <int KC, bool VEC>
+__global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams p) {
+    constexpr int NBK = (KC + 1) / 2;  // blocks of 64 dims (8 words, 8 column tiles) of the output
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint4 s_q[2 * KC][32];            // query operands, in the order of the matrix instruction
+    __shared__ float s_fr[ATT4_ROWS], s_qs[ATT4_ROWS];
+    __shared__ float s_m[ATT4_WARPS][ATT4_ROWS], s_l[ATT4_WARPS][ATT4_ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int chunk_id = blockIdx.x % p.chunks, rt = blockIdx.x / p.chunks % p.row_tiles;
+    const size_t unit = blockIdx.x / p.chunks / p.row_tiles;  // sequence * n_kv + KV head
+    const int b = (int)(unit / p.n_kv), kvh = (int)(unit % p.n_kv), rep = p.n_heads / p.n_kv, W = p.words, hd = p.hd;
     release_and_wait();
-    const int words = kv4_words(p.hd), len = min(max(p.lens[b], 0), p.lmax) - (p.t - 1 - i);
-    const size_t base = ((size_t)b * p.n_kv + h / (p.n_heads / p.n_kv)) * p.lmax;
-    float q[8], qs = 0.0f, acc[8] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        q[j] = 8 * w + j < p.hd ? p.q[(size_t)row * p.hd + 8 * w + j] * p.scale : 0.0f;
-        qs += q[j];
+    const int len = min(max(p.lens[b], 0), p.lmax);
+    // rows of the tile: r = query token * rep + head of the group
+    const int r0 = rt * ATT4_ROWS, rows = min(ATT4_ROWS, p.t * rep - r0);
+    const int last = len - (p.t - 1 - (r0 + rows - 1) / rep);  // positions the tile's last row sees: no row sees more
+    const int c0 = chunk_id * p.chunk, c1 = min(last, c0 + p.chunk);
+    const bool alone = last <= p.chunk;  // one chunk holds all that these rows see
+    if (c0 >= c1 && !(chunk_id == 0)) return;
+    auto q_row = [&](int r) { return ((size_t)b * p.t + (r0 + r) / rep) * p.n_heads + kvh * rep + (r0 + r) % rep; };
+    if (last <= 0) {  // nothing is seen by any row
+        for (int i = threadIdx.x; i < rows * hd; i += ATT4_WARPS * 32) p.out[q_row(i / hd) * hd + i % hd] = 0.0f;
+        return;
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) qs += __shfl_xor_sync(0xffffffffu, qs, o);
-    for (int j0 = 0; j0 < len; j0 += 16) {
-        const int j = j0 + group;
-        const bool ok = j < len;
-        const size_t at = base + (ok ? j : j0);
-        const uint32_t kc = w < words ? p.k_codes[at * words + w] : 0u, vc = w < words ? p.v_codes[at * words + w] : 0u;
-        const uint32_t ks = p.k_steps[at], vs = p.v_steps[at];
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dot = fmaf(q[e], (float)((kc >> (4 * e)) & 15u), dot);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (!ok) continue;  // uniform over the half-warp; the shuffles above are done
-        dot = dot * kv4_step(ks) + qs * kv4_lo(ks);
-        const float m_new = fmaxf(m, dot), corr = expf(m - m_new), pj = expf(dot - m_new);
-        l = l * corr + pj;
-        const float step = pj * kv4_step(vs), lo = pj * kv4_lo(vs);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], corr, fmaf(step, (float)((vc >> (4 * e)) & 15u), lo));
-        m = m_new;
-    }
-    if (w == 0) { s_m[group] = m; s_l[group] = l; }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s_acc[group][8 * w + e] = acc[e];
-    __syncthreads();
-    if ((int)threadIdx.x < p.hd) {
-        float top = -INFINITY, cl = 0.0f, ca = 0.0f;
-        for (int g = 0; g < 16; ++g) top = fmaxf(top, s_m[g]);
-        for (int g = 0; g < 16; ++g) {
-            const float f = s_l[g] == 0.0f ? 0.0f : expf(s_m[g] - top);  // a group without positions has l = 0
-            cl += s_l[g] * f;
-            ca += s_acc[g][threadIdx.x] * f;
+
+    // the word that lane t multiplies at step c of a row
+    auto k_word = [&](int tt, int c) { return VEC ? KC * tt + c : tt + 4 * c; };
+    // ---- ring of this warp
+    const int stage_words = 2 * ATT4_TILE * W + 2 * ATT4_TILE;
+    uint32_t *ring = reinterpret_cast<uint32_t *>(smem) + warp * ATT4_STAGES * stage_words;
+    const size_t base = unit * p.lmax;
+    const uint32_t *kc = p.k_codes + base * W, *vc = p.v_codes + base * W, *ks = p.k_steps + base, *vs = p.v_steps + base;
+    const int end4 = (c1 + 3) & ~3;  // rows up to here exist (lmax is a multiple of 4)
+    auto copy16 = [&](uint32_t *dst, const uint32_t *src, bool ok) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(ok ? 16 : 0)
+                     : "memory");
+    };
+    auto issue = [&](int tile0, int stage) {  // 32 positions from tile0 on; what lies behind end4 is filled with zeros
+        if (tile0 < c1) {
+            uint32_t *s = ring + stage * stage_words;
+            const int have = min(ATT4_TILE, end4 - tile0);
+            const size_t at = (size_t)tile0 * W;
+            for (int i = lane; i < 8 * W; i += 32) {
+                const bool ok = 4 * i < have * W;
+                const size_t off = ok ? at + 4 * i : 0;
+                copy16(s + 4 * i, kc + off, ok);
+                copy16(s + ATT4_TILE * W + 4 * i, vc + off, ok);
+            }
+            if (lane < 16) {
+                const int i = lane & 7;
+                const bool ok = 4 * i < have;
+                copy16(s + 2 * ATT4_TILE * W + 4 * lane, (lane < 8 ? ks : vs) + (ok ? tile0 + 4 * i : 0), ok);
+            }
         }
-        p.out[(size_t)row * p.hd + threadIdx.x] = cl == 0.0f ? 0.0f : ca / cl;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const int first = c0 + warp * ATT4_TILE, stride = ATT4_WARPS * ATT4_TILE;
+#pragma unroll
+    for (int s = 0; s < ATT4_STAGES - 1; ++s) issue(first + s * stride, s);
+
+    // ---- queries: scaled by a power of two to [2^13, 2^14), split, laid out; a warp prepares two rows
+    for (int r = warp; r < ATT4_ROWS; r += ATT4_WARPS) {
+        const float *src = p.q + (r < rows ? q_row(r) : q_row(0)) * hd;
+        float x[4], amax = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = r < rows && lane + 32 * i < hd ? src[lane + 32 * i] : 0.0f;
+            amax = fmaxf(amax, fabsf(x[i]));
+            sum += x[i];
+        }
+        amax = warp_reduce_max(amax);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int e = amax > 0.0f && amax < INFINITY ? 13 - ilogbf(amax) : 0;
+        const float unit2 = p.scale * 1.4426950408889634f;  // scores in units of log 2
+        if (lane == 0) {
+            s_fr[r] = ldexpf(unit2, -e);
+            s_qs[r] = amax < INFINITY ? sum * unit2 : __uint_as_float(0x7fffffffu);  // a query with an infinity gives NaN
+        }
+        __half *dst = reinterpret_cast<__half *>(s_q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = lane + 32 * i, w = d >> 3, n = d & 7;
+            if (w >= 4 * KC) continue;
+            const int tt = VEC ? w / KC : w & 3, c = VEC ? w % KC : w >> 2;
+            const float y = ldexpf(x[i], e);
+            const __half hi = __float2half_rn(y), lo = __float2half_rn((y - __half2float(hi)) * 2048.0f);
+            // step 2c + (n & 2) / 2, register pair (n & 1), half n / 4
+            __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + r * 4 + tt) * 8 + (n & 1) * 4 + (n >> 2);
+            at[0] = hi;
+            at[2] = lo;
+        }
     }
+    __syncthreads();
+    const int limit = g < rows ? len - (p.t - 1 - (r0 + g) / rep) : 0;  // positions row g sees
+    const int least = len - (p.t - 1 - r0 / rep);                       // the smallest limit of the tile
+    const float fr = s_fr[g], qs = s_qs[g];
+
+    float acc[NBK][8][4];
+#pragma unroll
+    for (int k = 0; k < NBK; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[k][j][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f, alo = 0.0f;  // of this lane's positions of row g; m is the row's, over the quad
+    float wref = 0x1p-100f, ws = 0x1p113f;      // largest weight so far; weights are held times ws = 2^13 / 2^floor(log2 wref)
+
+    int stage = 0;
+    for (int tile0 = first; tile0 < c1; tile0 += stride) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(ATT4_STAGES - 2) : "memory");
+        __syncwarp();  // this tile has landed for every lane, and every lane is done with the stage that is filled next
+        issue(tile0 + (ATT4_STAGES - 1) * stride, stage == 0 ? ATT4_STAGES - 1 : stage - 1);
+        const uint32_t *sk = ring + stage * stage_words, *sv = sk + ATT4_TILE * W, *sp = sv + ATT4_TILE * W;
+        stage = stage + 1 == ATT4_STAGES ? 0 : stage + 1;
+
+        // ---- scores: 4 tiles of 8 positions; tile u of block h holds rows 16 h + 4 (n / 2) + 2 u + parity
+        float sc[4][4];
+        uint32_t kw[4][KC];
+        const int krow = 4 * (g >> 1) + ((g & 1) ^ ((g >> 1) & 1));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t *row = sk + (16 * (n >> 1) + 2 * (n & 1) + krow) * W;
+            if (VEC && KC == 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(row + 4 * t);
+                kw[n][0] = v.x; kw[n][1 % KC] = v.y; kw[n][2 % KC] = v.z; kw[n][3 % KC] = v.w;
+            } else if (VEC && KC == 2) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(row + 2 * t);
+                kw[n][0] = v.x; kw[n][1 % KC] = v.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kw[n][c] = k_word(t, c) < W ? row[k_word(t, c)] : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[n][i] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const uint4 a = s_q[2 * c][lane], a2 = s_q[2 * c + 1][lane];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t x = kw[n][c], y = x >> 8;
+                mma_f16(sc[n], a.x, a.y, a.z, a.w, (x << 4) & 0x00f000f0u, x & 0x00f000f0u);
+                mma_f16(sc[n], a2.x, a2.y, a2.z, a2.w, (y << 4) & 0x00f000f0u, y & 0x00f000f0u);
+            }
+        }
+        // ---- softmax weights of row g at this lane's positions: [2 u + i] of block h is position 16 h + 4 t + 2 u + (i ^ t & 1)
+        float wgt[2][4], top = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 kp = *reinterpret_cast<const uint4 *>(sp + 16 * h + 4 * t);
+            const uint32_t pr[4] = {(t & 1) ? kp.y : kp.x, (t & 1) ? kp.x : kp.y, (t & 1) ? kp.w : kp.z, (t & 1) ? kp.z : kp.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float dot = fmaf(sc[2 * h + (i >> 1)][i & 1], 0x1p20f, sc[2 * h + (i >> 1)][2 + (i & 1)] * 0x1p9f);
+                wgt[h][i] = fmaf(dot * kv4_step(pr[i]), fr, kv4_lo(pr[i]) * qs);
+            }
+        }
+        const bool tail = tile0 + ATT4_TILE > least;  // some row does not see all of the tile
+        if (tail) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (tile0 + 16 * h + 4 * t + (i & 2) + ((i ^ t) & 1) >= min(limit, c1)) wgt[h][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, wgt[h][i]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
+        const float corr = exp2_fast(m - ref);
+        l *= corr;
+        alo *= corr;
+        m = m_new;
+        float wmax = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 vp = *reinterpret_cast<const uint4 *>(sp + ATT4_TILE + 16 * h + 4 * t);
+            const uint32_t pr[4] = {(t & 1) ? vp.y : vp.x, (t & 1) ? vp.x : vp.y, (t & 1) ? vp.w : vp.z, (t & 1) ? vp.z : vp.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float pj = exp2_fast(wgt[h][i] - ref);
+                l += pj;
+                const bool seen = !tail || wgt[h][i] != -INFINITY;  // what is not seen may hold anything
+                // every second position counts down from its largest value, lo + 15 step - (15 - c) step: the sum of the
+                // products then changes sign as the values do.  With codes alone it only grows, and the instruction's
+                // truncated adds pull all of it one way (2.8e-4 of the result at 32768 positions, 8e-7 without that)
+                const float step = seen ? kv4_step(pr[i]) : 0.0f, from = seen ? kv4_lo(pr[i]) : 0.0f;
+                alo = fmaf(pj, i & 1 ? fmaf(15.0f, step, from) : from, alo);
+                wgt[h][i] = pj * (i & 1 ? -step : step);
+                wmax = fmaxf(wmax, fabsf(wgt[h][i]));
+            }
+        }
+        wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 1));
+        wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 2));
+        wref = fmaxf(fmaxf(wref * corr, wmax), 0x1p-100f);
+        // 2^13 / 2^floor(log2 wref), by exponent fields; wref is at most the largest f32
+        const float ws_new = __uint_as_float(0x85800000u - (min(__float_as_uint(wref), 0x7f7fffffu) & 0x7f800000u));
+        const float adj = corr * fminf(__fdividef(ws_new, ws), 0x1p127f);  // powers of two; corr may be 0
+        ws = ws_new;
+        if (__any_sync(0xffffffffu, adj != 1.0f)) {
+#pragma unroll
+            for (int k = 0; k < NBK; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[k][j][i] *= adj;
+        }
+        // ---- weighted sum of the codes
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            // codes of two positions, the second counted down
+            auto code = [](uint32_t x) { return (x & 0x00f000f0u) ^ 0x00f00000u; };
+            split_f16(wgt[h][0] * ws, wgt[h][1] * ws, a0, a1);
+            split_f16(wgt[h][2] * ws, wgt[h][3] * ws, a2, a3);
+            const uint32_t *rowv = sv + (16 * h + 4 * t) * W;
+            uint32_t vw[NBK][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t *row = rowv + ((i & 2) + ((i ^ t) & 1)) * W;
+                if (VEC && NBK == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(row + 2 * g);
+                    vw[0][i] = v.x;
+                    vw[NBK - 1][i] = v.y;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < NBK; ++k) vw[k][i] = g + 8 * k < W ? row[g + 8 * k] : 0u;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NBK; ++k) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {  // byte j / 2 of the four words: dims j and j + 1
+                    const uint32_t sel = 0x4400u + 0x1100u * (j / 2) + 0x11u * (j / 2);
+                    const uint32_t x = __byte_perm(vw[k][0], vw[k][1], sel), y = __byte_perm(vw[k][2], vw[k][3], sel);
+                    mma_f16(acc[k][j], a0, a1, a2, a3, code(x << 4), code(y << 4));
+                    mma_f16(acc[k][j + 1], a0, a1, a2, a3, code(x), code(y));
+                }
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // ---- join the warps: sums of row g over its four lanes, then rows over the warps through shared memory
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    alo += __shfl_xor_sync(0xffffffffu, alo, 1);
+    alo += __shfl_xor_sync(0xffffffffu, alo, 2);
+    if (t == 0) {
+        s_m[warp][g] = m;
+        s_l[warp][g] = l;
+    }
+    __syncthreads();  // every warp is done with its ring
+    constexpr int OLD = 64 * NBK + 4;  // row stride of the partial sums
+    float *so = reinterpret_cast<float *>(smem) + (size_t)warp * ATT4_ROWS * OLD + g * OLD;
+    const float inv_ws = 0x1p20f / ws;
+#pragma unroll
+    for (int k = 0; k < NBK; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int w = VEC && NBK == 2 ? 2 * (2 * t + i) + k : 2 * t + i + 8 * k;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = fmaf(acc[k][j][2 + i], 0x1p-11f, acc[k][j][i]) * inv_ws;
+                so[8 * w + j] = v + alo;
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * hd; i += ATT4_WARPS * 32) {
+        const int r = i / hd, d = i - r * hd;
+        float top = -INFINITY, sum = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ATT4_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+        for (int w = 0; w < ATT4_WARPS; ++w) {
+            const float f = s_l[w][r] == 0.0f ? 0.0f : exp2_fast(s_m[w][r] - top);  // a warp that saw nothing of the row
+            sum = fmaf(s_l[w][r], f, sum);
+            o = fmaf(reinterpret_cast<const float *>(smem)[((size_t)w * ATT4_ROWS + r) * OLD + d], f, o);
+        }
+        if (alone) {
+            p.out[q_row(r) * hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
+        } else {
+            const size_t at = q_row(r) * p.chunks + chunk_id;
+            p.part[at * hd + d] = o;
+            if (d == 0) p.part_ml[at] = make_float2(top, sum);
+        }
+    }
+}
+
+// one warp per query row that was split: the weighted mean of its chunks
+__global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnParams p, long long rows) {
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, rep = p.n_heads / p.n_kv;
+    release_and_wait();
+    if (row >= rows) return;
+    const int h = (int)(row % p.n_heads), i = (int)(row / p.n_heads % p.t);
+    const int len = min(max(p.lens[row / p.n_heads / p.t], 0), p.lmax);
+    const int r = i * rep + h % rep, tile_last = min(p.t * rep, (r / ATT4_ROWS + 1) * ATT4_ROWS) - 1;  // last row of its tile
+    const int last = len - (p.t - 1 - tile_last / rep);
+    if (last <= p.chunk) return;  // the first kernel wrote it
+    const int n = (last + p.chunk - 1) / p.chunk;
+    const float2 *ml = p.part_ml + (size_t)row * p.chunks;
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[s].x);
+    top = warp_reduce_max(top);
+    float sum = 0.0f, o[4] = {};
+    for (int s = 0; s < n; ++s) {
+        const float2 v = ml[s];
+        const float f = v.y == 0.0f ? 0.0f : exp2_fast(v.x - top);
+        sum = fmaf(v.y, f, sum);
+        const float *src = p.part + ((size_t)row * p.chunks + s) * p.hd;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (lane + 32 * k < p.hd) o[k] = fmaf(src[lane + 32 * k], f, o[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (lane + 32 * k < p.hd) p.out[(size_t)row * p.hd + lane + 32 * k] = sum == 0.0f ? 0.0f : __fdiv_rn(o[k], sum);
+}
+
+// positions per CTA.  The lengths are on the device, so the rule goes by the cache's: about four CTAs for every resident
+// one (4 per SM), so that short sequences leave room that long ones fill, and at least a tile per warp.
+static int attn_chunk(size_t units, int lmax, int sms) {
+    const size_t want = ((size_t)lmax * units + (size_t)sms * 16 - 1) / ((size_t)sms * 16);
+    const int step = ATT4_WARPS * ATT4_TILE;
+    const size_t chunk = (want + step - 1) / step * step;
+    return chunk >= (size_t)lmax ? lmax : (int)chunk;
 }
 
 static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
@@ -269,6 +594,12 @@ static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
     if (hd < 4 || hd > KV4_MAX_HD || hd % 4) return fail(KB_ERR_UNSUPPORTED, "kv4: head_dim %d must be a multiple of 4 up to %d", hd, KV4_MAX_HD);
     if (lmax < 4 || lmax % 4) return fail(KB_ERR_UNSUPPORTED, "kv4: cache length %d must be a multiple of 4", lmax);
     return KB_OK;
+}
+
+// CTAs that share nothing: (sequence, KV head, tile of query rows)
+static size_t attn_units(size_t batch, int t, int n_heads, int n_kv) {
+    const size_t rows = (size_t)t * (n_heads / n_kv);
+    return batch * n_kv * ((rows + ATT4_ROWS - 1) / ATT4_ROWS);
 }
 
 static bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, const void *d = nullptr) {
@@ -357,26 +688,71 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 read launch");
 }
 
-size_t kb_attn_kv4_workspace_bytes(size_t, int, int, int, int, int) { return 0; }
+size_t kb_attn_kv4_workspace_bytes(size_t batch, int t, int n_heads, int n_kv_heads, int head_dim, int lmax) {
+    int dev = 0;
+    if (batch == 0 || t < 1 || check_kv4(n_heads, n_kv_heads, head_dim, lmax) != KB_OK || cudaGetDevice(&dev) != cudaSuccess) return 0;
+    const size_t rows = batch * (size_t)t * n_heads;
+    const size_t chunks = (lmax - 1) / attn_chunk(attn_units(batch, t, n_heads, n_kv_heads), lmax, sm_count(dev)) + 1;
+    return chunks < 2 ? 0 : rows * chunks * ((size_t)head_dim + 2) * sizeof(float);
+}
 
 int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes, const uint32_t *v_steps,
                 const int *lens, size_t batch, int t, int n_heads, int n_kv_heads, int head_dim, int lmax, float scale, float *out,
                 void *workspace, size_t workspace_bytes, kb_stream stream) {
-    (void)workspace; (void)workspace_bytes;
     if (!q || !k_codes || !k_steps || !v_codes || !v_steps || !lens || !out) return fail(KB_ERR_INVALID, "null pointer");
     if (int rc = check_kv4(n_heads, n_kv_heads, head_dim, lmax)) return rc;
     if (t < 0) return fail(KB_ERR_INVALID, "attention: %d query tokens", t);
     if (!(fabsf(scale) < INFINITY)) return fail(KB_ERR_INVALID, "attention: scale must be finite");
-    if (!aligned16(k_codes, k_steps, v_codes, v_steps) || !aligned16(q, out)) return fail(KB_ERR_INVALID, "kv4: planes, queries and outputs must be 16-byte aligned");
+    if (!aligned16(k_codes, k_steps, v_codes, v_steps) || !aligned16(q, out, workspace))
+        return fail(KB_ERR_INVALID, "kv4: planes, queries, outputs and workspace must be 16-byte aligned");
     if (batch == 0 || t == 0) return KB_OK;
-    const size_t rows = batch * (size_t)t * n_heads;
-    if (batch > 0x7fffffffu || rows > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
+    if (batch > 0x7fffffffu || batch * (size_t)t * n_heads > 0x7fffffffu || (size_t)t * n_heads > 0x7fffffffu)
+        return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
+    int dev = 0;
+    KB_CUDA(cudaGetDevice(&dev));
+    const size_t rows = batch * (size_t)t * n_heads, units = attn_units(batch, t, n_heads, n_kv_heads);
     AttnParams p = {};
     p.q = q; p.k_codes = k_codes; p.k_steps = k_steps; p.v_codes = v_codes; p.v_steps = v_steps; p.lens = lens;
-    p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.out = out;
+    p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.words = kv4_words(head_dim); p.out = out;
     p.scale = scale != 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
-    const cudaError_t e = launch_after(attn_kv4_kernel, dim3((unsigned)rows), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
-    return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 attention launch");
+    p.row_tiles = (int)(units / (batch * n_kv_heads));
+    p.chunk = attn_chunk(units, lmax, sm_count(dev));
+    p.chunks = (lmax - 1) / p.chunk + 1;
+    if (units * p.chunks > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    void *own = nullptr;
+    if (p.chunks > 1) {
+        const size_t need = rows * p.chunks * ((size_t)head_dim + 2) * sizeof(float);
+        if (workspace && workspace_bytes < need)
+            return fail(KB_ERR_STORAGE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+        if (!workspace) {
+            KB_CUDA(cudaMallocAsync(&own, need, st));
+            workspace = own;
+        }
+        p.part_ml = static_cast<float2 *>(workspace);
+        p.part = reinterpret_cast<float *>(p.part_ml + rows * p.chunks);
+    }
+    const int W = p.words, KC = (W + 3) / 4;
+    void (*kern)(AttnParams) = KC == 1 ? attn_kv4_kernel<1, false>
+                               : KC == 2 ? (W == 8 ? attn_kv4_kernel<2, true> : attn_kv4_kernel<2, false>)
+                               : KC == 3 ? attn_kv4_kernel<3, false>
+                                         : (W == 16 ? attn_kv4_kernel<4, true> : attn_kv4_kernel<4, false>);
+    const size_t ring = (size_t)ATT4_WARPS * ATT4_STAGES * (2 * ATT4_TILE * W + 2 * ATT4_TILE) * 4;
+    const size_t joined = (size_t)ATT4_WARPS * ATT4_ROWS * (64 * ((KC + 1) / 2) + 4) * 4;
+    const size_t smem = ring > joined ? ring : joined;
+    int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, 56 * 1024, "kv4 attention smem attribute");
+    if (rc == KB_OK) {
+        cudaError_t e = launch_after(kern, dim3((unsigned)(units * p.chunks)), dim3(ATT4_WARPS * 32), smem, st, p);
+        if (e == cudaSuccess && p.chunks > 1) {
+            e = launch_after(attn_kv4_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, (long long)rows);
+        }
+        if (e != cudaSuccess) rc = cuda_fail(e, "kv4 attention launch");
+    }
+    if (own) {
+        const cudaError_t e = cudaFreeAsync(own, st);
+        if (rc == KB_OK && e != cudaSuccess) rc = cuda_fail(e, "cudaFreeAsync");
+    }
+    return rc;
 }
 
 }  // extern "C"
