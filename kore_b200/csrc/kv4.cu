@@ -209,15 +209,14 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 // instruction).  The factor goes into the end of the sums.  The bits 0x000f would do as well (code * 2^-24, two shifts fewer
 // per eight codes), but the instruction aligns its products by the operands' exponent fields, so leading zeros cost
 // bits of the sum: results were 1e-5 off that way.
-//   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo 2^-11
-// (22 bits of x relative to the largest of the row, for which rows are scaled by powers of two).  The terms sit in rows g
+//   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo
+// (2^-23 of the largest of the row, for which rows are scaled by powers of two).  The terms sit in rows g
 // and g + 8 of the 16-row tile, so a warp serves 8 query rows and the second term costs nothing while the tile is not full.
 //   Lane (g, t) = (lane / 4, lane % 4).  QK^T: the contraction runs over dims in any order as long as queries and keys
 // agree, so a lane takes whole words of key row g.  The result has query row g and two positions per 8-column tile in one
 // lane, which is exactly the operand layout of the weights in the second product: no shuffle between the two.  PV: output
 // column n = g of tile j is dim 8 word(g) + j, so a lane's words of four positions give the columns of eight tiles.
-//   Positions of a 16-block are dealt so that lane t owns rows 4t .. 4t+3 (one 128-bit load of their pairs) and the four
-// rows of a load alternate in parity (64-byte rows otherwise meet in the same banks).
+//   Positions of a 16-block are dealt so that lane t owns rows 4t .. 4t+3 (one 128-bit load of their pairs).
 //   A warp streams its own 32-position tiles through a ring of 16-byte asynchronous copies (no barrier between warps);
 // warps of a CTA deal the tiles of a chunk, chunks of a sequence go to CTAs, a second kernel joins them.
 constexpr int ATT4_WARPS = 4;
@@ -229,7 +228,7 @@ struct AttnParams {
     const float *q;
     const uint32_t *k_codes, *k_steps, *v_codes, *v_steps;
     const int *lens;
-    int t, n_heads, n_kv, hd, lmax, words;
+    int t, n_heads, n_kv, rep, hd, lmax, words;
     int row_tiles, chunk, chunks;  // chunk: positions per CTA, chunks = ceil(lmax / chunk)
     float scale;
     float *out;
@@ -242,11 +241,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two f32 numbers -> two f16 terms each: x = hi + lo 2^-11 to 22 bits (relative to 2^14, their upper end)
+// two numbers of at most 2^14 -> two f16 terms each, x = hi + lo to 2^-23 of 2^14
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn((x - f.x) * 2048.0f, (y - f.y) * 2048.0f);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
@@ -255,60 +254,95 @@ __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp over
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const uint32_t *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const uint32_t *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
 
-// KC = 32-bit words of a row per lane (4 lanes a row); VEC: rows of exactly 4 KC words, read as vectors
-template <int KC, bool VEC>
+// W = 32-bit words of a row: a constant, so that every address inside a tile is one
+template <int W>
+struct Attn4 {
+    static constexpr int KC = (W + 3) / 4;      // words of a row per lane (4 lanes a row)
+    static constexpr bool VEC = W % 4 == 0;     // lane t takes words KC t .., otherwise t, t + 4, ..
+    static constexpr int NBK = (W + 7) / 8;     // blocks of 8 words = 64 dims = 8 column tiles of the output
+    static constexpr bool SWZ = W == 16;        // 64-byte rows: 16-byte pieces of V are dealt over the banks
+    static constexpr int STAGE = 2 * ATT4_TILE * W + 2 * ATT4_TILE;  // words: K codes, V codes, K pairs, V pairs
+    static constexpr int OLD = 64 * NBK + 4;    // row stride of the partial sums in shared memory
+    static constexpr size_t RING = (size_t)ATT4_WARPS * ATT4_STAGES * STAGE * 4;
+    static constexpr size_t JOINED = (size_t)ATT4_WARPS * ATT4_ROWS * OLD * 4;
+    static constexpr size_t SMEM = RING > JOINED ? RING : JOINED;
+    __device__ static int k_word(int t, int c) { return VEC ? KC * t + c : t + 4 * c; }
+    // word of an output column n, block k
+    __device__ static int v_word(int n, int k) { return SWZ ? 2 * n + k : n + 8 * k; }
+};
+
+template <int W>
 __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams p) {
-    constexpr int NBK = (KC + 1) / 2;  // blocks of 64 dims (8 words, 8 column tiles) of the output
+    using A = Attn4<W>;
+    constexpr int KC = A::KC, NBK = A::NBK;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint4 s_q[2 * KC][32];            // query operands, in the order of the matrix instruction
+    __shared__ uint4 s_q[2 * KC][32];  // query operands, in the order of the matrix instruction
     __shared__ float s_fr[ATT4_ROWS], s_qs[ATT4_ROWS];
     __shared__ float s_m[ATT4_WARPS][ATT4_ROWS], s_l[ATT4_WARPS][ATT4_ROWS];
+    __shared__ long long s_row[ATT4_ROWS];  // index of the tile's rows in q and out
+    __shared__ int s_off[ATT4_ROWS];        // positions behind the sequence's end that a row does not see
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int chunk_id = blockIdx.x % p.chunks, rt = blockIdx.x / p.chunks % p.row_tiles;
-    const size_t unit = blockIdx.x / p.chunks / p.row_tiles;  // sequence * n_kv + KV head
-    const int b = (int)(unit / p.n_kv), kvh = (int)(unit % p.n_kv), rep = p.n_heads / p.n_kv, W = p.words, hd = p.hd;
+    const int unit = blockIdx.x, chunk_id = blockIdx.y;  // sequence * n_kv + KV head
+    const int b = unit / p.n_kv, rep = p.rep, hd = p.hd;
+    const int r0 = blockIdx.z * ATT4_ROWS, rows = min(ATT4_ROWS, p.t * rep - r0);  // rows: query token * rep + head of the group
+    if (threadIdx.x < ATT4_ROWS) {
+        const int r = r0 + min((int)threadIdx.x, rows - 1), i = r / rep;
+        s_row[threadIdx.x] = ((long long)b * p.t + i) * p.n_heads + (unit - b * p.n_kv) * rep + (r - i * rep);
+        s_off[threadIdx.x] = p.t - 1 - i;
+    }
+    __syncthreads();
     release_and_wait();
     const int len = min(max(p.lens[b], 0), p.lmax);
-    // rows of the tile: r = query token * rep + head of the group
-    const int r0 = rt * ATT4_ROWS, rows = min(ATT4_ROWS, p.t * rep - r0);
-    const int last = len - (p.t - 1 - (r0 + rows - 1) / rep);  // positions the tile's last row sees: no row sees more
+    const int last = len - s_off[rows - 1];  // positions the tile's last row sees: no row sees more
     const int c0 = chunk_id * p.chunk, c1 = min(last, c0 + p.chunk);
     const bool alone = last <= p.chunk;  // one chunk holds all that these rows see
-    if (c0 >= c1 && !(chunk_id == 0)) return;
-    auto q_row = [&](int r) { return ((size_t)b * p.t + (r0 + r) / rep) * p.n_heads + kvh * rep + (r0 + r) % rep; };
+    if (c0 >= c1 && chunk_id != 0) return;
     if (last <= 0) {  // nothing is seen by any row
-        for (int i = threadIdx.x; i < rows * hd; i += ATT4_WARPS * 32) p.out[q_row(i / hd) * hd + i % hd] = 0.0f;
+        for (int r = 0; r < rows; ++r)
+            if ((int)threadIdx.x < hd) p.out[s_row[r] * hd + threadIdx.x] = 0.0f;
         return;
     }
 
-    // the word that lane t multiplies at step c of a row
-    auto k_word = [&](int tt, int c) { return VEC ? KC * tt + c : tt + 4 * c; };
     // ---- ring of this warp
-    const int stage_words = 2 * ATT4_TILE * W + 2 * ATT4_TILE;
-    uint32_t *ring = reinterpret_cast<uint32_t *>(smem) + warp * ATT4_STAGES * stage_words;
-    const size_t base = unit * p.lmax;
-    const uint32_t *kc = p.k_codes + base * W, *vc = p.v_codes + base * W, *ks = p.k_steps + base, *vs = p.v_steps + base;
-    const int end4 = (c1 + 3) & ~3;  // rows up to here exist (lmax is a multiple of 4)
-    auto copy16 = [&](uint32_t *dst, const uint32_t *src, bool ok) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(ok ? 16 : 0)
-                     : "memory");
-    };
-    auto issue = [&](int tile0, int stage) {  // 32 positions from tile0 on; what lies behind end4 is filled with zeros
-        if (tile0 < c1) {
-            uint32_t *s = ring + stage * stage_words;
-            const int have = min(ATT4_TILE, end4 - tile0);
-            const size_t at = (size_t)tile0 * W;
-            for (int i = lane; i < 8 * W; i += 32) {
-                const bool ok = 4 * i < have * W;
-                const size_t off = ok ? at + 4 * i : 0;
-                copy16(s + 4 * i, kc + off, ok);
-                copy16(s + ATT4_TILE * W + 4 * i, vc + off, ok);
-            }
+    uint32_t *ring = reinterpret_cast<uint32_t *>(smem) + warp * ATT4_STAGES * A::STAGE;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const size_t base = (size_t)unit * p.lmax;
+    const uint32_t *kc = p.k_codes + base * W, *vc = p.v_codes + base * W, *pairs = ((lane & 8) ? p.v_steps : p.k_steps) + base;
+    // 16-byte pieces: piece i = lane + 32 j of a plane's 8 W; V's are swapped inside a row by (row / 4) % 4 where SWZ
+    const int swz[2] = {A::SWZ ? 16 * ((lane & ~3) | ((lane & 3) ^ (lane >> 4))) : 16 * lane,
+                        A::SWZ ? 16 * ((lane & ~3) | ((lane & 3) ^ (lane >> 4) ^ 2)) : 16 * lane};
+    auto issue = [&](int tile0, int stage) {
+        const uint32_t dst = ring_at + stage * (A::STAGE * 4);
+        if (tile0 + ATT4_TILE <= c1) {
+            const uint32_t *ks = kc + (size_t)tile0 * W + 4 * lane, *vs = vc + (size_t)tile0 * W + 4 * lane;
+#pragma unroll
+            for (int j = 0; j < (8 * W + 31) / 32; ++j)
+                if (32 * j + 31 < 8 * W || lane + 32 * j < 8 * W) {
+                    copy16(dst + 16 * lane + 512 * j, ks + 128 * j);
+                    copy16(dst + ATT4_TILE * W * 4 + swz[j & 1] + 512 * j, vs + 128 * j);
+                }
+            if (lane < 16) copy16(dst + 2 * ATT4_TILE * W * 4 + 16 * lane, pairs + tile0 + 4 * (lane & 7));
+        } else if (tile0 < c1) {
+            // the sequence ends inside: rows up to the next multiple of 4 exist (lmax is one), the rest is filled with zeros
+            const int have = ((c1 + 3) & ~3) - tile0;
+#pragma unroll
+            for (int j = 0; j < (8 * W + 31) / 32; ++j)
+                if (lane + 32 * j < 8 * W) {
+                    const bool ok = 4 * (lane + 32 * j) < have * W;
+                    const size_t off = (size_t)tile0 * W + (ok ? 4 * (lane + 32 * j) : 0);
+                    copy16_or_zero(dst + 16 * lane + 512 * j, kc + off, ok);
+                    copy16_or_zero(dst + ATT4_TILE * W * 4 + swz[j & 1] + 512 * j, vc + off, ok);
+                }
             if (lane < 16) {
-                const int i = lane & 7;
-                const bool ok = 4 * i < have;
-                copy16(s + 2 * ATT4_TILE * W + 4 * lane, (lane < 8 ? ks : vs) + (ok ? tile0 + 4 * i : 0), ok);
+                const bool ok = 4 * (lane & 7) < have;
+                copy16_or_zero(dst + 2 * ATT4_TILE * W * 4 + 16 * lane, pairs + tile0 + (ok ? 4 * (lane & 7) : 0), ok);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -317,33 +351,35 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
 #pragma unroll
     for (int s = 0; s < ATT4_STAGES - 1; ++s) issue(first + s * stride, s);
 
-    // ---- queries: scaled by a power of two to [2^13, 2^14), split, laid out; a warp prepares two rows
+    // ---- queries times scale log2(e), scaled by a power of two to [2^13, 2^14), split, laid out; a warp prepares two rows
     for (int r = warp; r < ATT4_ROWS; r += ATT4_WARPS) {
-        const float *src = p.q + (r < rows ? q_row(r) : q_row(0)) * hd;
+        const float *src = p.q + s_row[r] * hd;
+        const float unit2 = p.scale * 1.4426950408889634f;  // scores in units of log 2
         float x[4], amax = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = r < rows && lane + 32 * i < hd ? src[lane + 32 * i] : 0.0f;
+            x[i] = r < rows && lane + 32 * i < hd ? src[lane + 32 * i] * unit2 : 0.0f;
             amax = fmaxf(amax, fabsf(x[i]));
             sum += x[i];
         }
         amax = warp_reduce_max(amax);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const int e = amax > 0.0f && amax < INFINITY ? 13 - ilogbf(amax) : 0;
-        const float unit2 = p.scale * 1.4426950408889634f;  // scores in units of log 2
+        // by exponent fields; below 2^-113 the scores are 0 to any accuracy, from 2^120 on the row is given up (NaN)
+        const int e = max((int)(__float_as_uint(amax) >> 23), 14);
+        const float up = __int_as_float((267 - e) << 23);
         if (lane == 0) {
-            s_fr[r] = ldexpf(unit2, -e);
-            s_qs[r] = amax < INFINITY ? sum * unit2 : __uint_as_float(0x7fffffffu);  // a query with an infinity gives NaN
+            s_fr[r] = __int_as_float(min(e + 7, 254) << 23);  // 2^20 / up
+            s_qs[r] = e > 247 ? __uint_as_float(0x7fffffffu) : sum;
         }
         __half *dst = reinterpret_cast<__half *>(s_q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = lane + 32 * i, w = d >> 3, n = d & 7;
             if (w >= 4 * KC) continue;
-            const int tt = VEC ? w / KC : w & 3, c = VEC ? w % KC : w >> 2;
-            const float y = ldexpf(x[i], e);
-            const __half hi = __float2half_rn(y), lo = __float2half_rn((y - __half2float(hi)) * 2048.0f);
+            const int tt = A::VEC ? w / KC : w & 3, c = A::VEC ? w % KC : w >> 2;
+            const float y = x[i] * up;
+            const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
             // step 2c + (n & 2) / 2, register pair (n & 1), half n / 4
             __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + r * 4 + tt) * 8 + (n & 1) * 4 + (n >> 2);
             at[0] = hi;
@@ -351,8 +387,8 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
         }
     }
     __syncthreads();
-    const int limit = g < rows ? len - (p.t - 1 - (r0 + g) / rep) : 0;  // positions row g sees
-    const int least = len - (p.t - 1 - r0 / rep);                       // the smallest limit of the tile
+    const int limit = g < rows ? len - s_off[g] : 0;  // positions row g sees
+    const int least = min(c1, len - s_off[0]);        // the smallest limit of the tile's rows
     const float fr = s_fr[g], qs = s_qs[g];
 
     float acc[NBK][8][4];
@@ -370,25 +406,25 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
         asm volatile("cp.async.wait_group %0;" ::"n"(ATT4_STAGES - 2) : "memory");
         __syncwarp();  // this tile has landed for every lane, and every lane is done with the stage that is filled next
         issue(tile0 + (ATT4_STAGES - 1) * stride, stage == 0 ? ATT4_STAGES - 1 : stage - 1);
-        const uint32_t *sk = ring + stage * stage_words, *sv = sk + ATT4_TILE * W, *sp = sv + ATT4_TILE * W;
+        const uint32_t *sk = ring + stage * A::STAGE, *sv = sk + ATT4_TILE * W, *sp = sv + ATT4_TILE * W;
         stage = stage + 1 == ATT4_STAGES ? 0 : stage + 1;
 
-        // ---- scores: 4 tiles of 8 positions; tile u of block h holds rows 16 h + 4 (n / 2) + 2 u + parity
+        // ---- scores: 4 tiles of 8 positions; column n of tile u of block h is position 16 h + 4 (n / 2) + 2 u + n % 2
         float sc[4][4];
         uint32_t kw[4][KC];
-        const int krow = 4 * (g >> 1) + ((g & 1) ^ ((g >> 1) & 1));
+        const uint32_t *krow = sk + (4 * (g >> 1) + (g & 1)) * W + A::k_word(t, 0);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const uint32_t *row = sk + (16 * (n >> 1) + 2 * (n & 1) + krow) * W;
-            if (VEC && KC == 4) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(row + 4 * t);
+            const uint32_t *row = krow + (16 * (n >> 1) + 2 * (n & 1)) * W;
+            if (A::VEC && KC == 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(row);
                 kw[n][0] = v.x; kw[n][1 % KC] = v.y; kw[n][2 % KC] = v.z; kw[n][3 % KC] = v.w;
-            } else if (VEC && KC == 2) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(row + 2 * t);
+            } else if (A::VEC && KC == 2) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(row);
                 kw[n][0] = v.x; kw[n][1 % KC] = v.y;
             } else {
 #pragma unroll
-                for (int c = 0; c < KC; ++c) kw[n][c] = k_word(t, c) < W ? row[k_word(t, c)] : 0u;
+                for (int c = 0; c < KC; ++c) kw[n][c] = A::VEC || 4 * c + 3 < W || t + 4 * c < W ? row[A::VEC ? c : 4 * c] : 0u;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[n][i] = 0.0f;
@@ -403,25 +439,26 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
                 mma_f16(sc[n], a2.x, a2.y, a2.z, a2.w, (y << 4) & 0x00f000f0u, y & 0x00f000f0u);
             }
         }
-        // ---- softmax weights of row g at this lane's positions: [2 u + i] of block h is position 16 h + 4 t + 2 u + (i ^ t & 1)
+        // ---- softmax weights of row g at this lane's positions: [i] of block h is position 16 h + 4 t + i
         float wgt[2][4], top = -INFINITY;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint4 kp = *reinterpret_cast<const uint4 *>(sp + 16 * h + 4 * t);
-            const uint32_t pr[4] = {(t & 1) ? kp.y : kp.x, (t & 1) ? kp.x : kp.y, (t & 1) ? kp.w : kp.z, (t & 1) ? kp.z : kp.w};
+            const uint32_t pr[4] = {kp.x, kp.y, kp.z, kp.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float dot = fmaf(sc[2 * h + (i >> 1)][i & 1], 0x1p20f, sc[2 * h + (i >> 1)][2 + (i & 1)] * 0x1p9f);
-                wgt[h][i] = fmaf(dot * kv4_step(pr[i]), fr, kv4_lo(pr[i]) * qs);
+                const float dot = sc[2 * h + (i >> 1)][i & 1] + sc[2 * h + (i >> 1)][2 + (i & 1)];
+                wgt[h][i] = fmaf(dot, kv4_step(pr[i]) * fr, kv4_lo(pr[i]) * qs);
             }
         }
         const bool tail = tile0 + ATT4_TILE > least;  // some row does not see all of the tile
         if (tail) {
+            const int end = min(limit, c1) - tile0 - 4 * t;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (tile0 + 16 * h + 4 * t + (i & 2) + ((i ^ t) & 1) >= min(limit, c1)) wgt[h][i] = -INFINITY;
+                    if (16 * h + i >= end) wgt[h][i] = -INFINITY;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -438,16 +475,19 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint4 vp = *reinterpret_cast<const uint4 *>(sp + ATT4_TILE + 16 * h + 4 * t);
-            const uint32_t pr[4] = {(t & 1) ? vp.y : vp.x, (t & 1) ? vp.x : vp.y, (t & 1) ? vp.w : vp.z, (t & 1) ? vp.z : vp.w};
+            uint32_t pr[4] = {vp.x, vp.y, vp.z, vp.w};
+            if (tail) {  // what is not seen may hold anything, NaN too
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pr[i] = wgt[h][i] == -INFINITY ? 0u : pr[i];
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float pj = exp2_fast(wgt[h][i] - ref);
                 l += pj;
-                const bool seen = !tail || wgt[h][i] != -INFINITY;  // what is not seen may hold anything
                 // every second position counts down from its largest value, lo + 15 step - (15 - c) step: the sum of the
                 // products then changes sign as the values do.  With codes alone it only grows, and the instruction's
-                // truncated adds pull all of it one way (2.8e-4 of the result at 32768 positions, 8e-7 without that)
-                const float step = seen ? kv4_step(pr[i]) : 0.0f, from = seen ? kv4_lo(pr[i]) : 0.0f;
+                // truncated adds pull all of it one way (2.8e-4 of the result at 32768 positions, 1e-6 without that)
+                const float step = kv4_step(pr[i]), from = kv4_lo(pr[i]);
                 alo = fmaf(pj, i & 1 ? fmaf(15.0f, step, from) : from, alo);
                 wgt[h][i] = pj * (i & 1 ? -step : step);
                 wmax = fmaxf(wmax, fabsf(wgt[h][i]));
@@ -455,12 +495,11 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
         }
         wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 1));
         wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 2));
-        wref = fmaxf(fmaxf(wref * corr, wmax), 0x1p-100f);
-        // 2^13 / 2^floor(log2 wref), by exponent fields; wref is at most the largest f32
-        const float ws_new = __uint_as_float(0x85800000u - (min(__float_as_uint(wref), 0x7f7fffffu) & 0x7f800000u));
-        const float adj = corr * fminf(__fdividef(ws_new, ws), 0x1p127f);  // powers of two; corr may be 0
-        ws = ws_new;
-        if (__any_sync(0xffffffffu, adj != 1.0f)) {
+        wref = fminf(fmaxf(fmaxf(wref * corr, wmax), 0x1p-100f), 0x1p127f);
+        const float ws_new = __uint_as_float(0x85800000u - (__float_as_uint(wref) & 0x7f800000u));  // by exponent fields
+        if (__any_sync(0xffffffffu, ws_new != ws || corr != 1.0f)) {
+            const float adj = corr * fminf(__fdividef(ws_new, ws), 0x1p127f);  // a ratio of powers of two; corr may be 0
+            ws = ws_new;
 #pragma unroll
             for (int k = 0; k < NBK; ++k)
 #pragma unroll
@@ -469,29 +508,27 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
                     for (int i = 0; i < 4; ++i) acc[k][j][i] *= adj;
         }
         // ---- weighted sum of the codes
+        const uint32_t *vrow = sv + 4 * t * W + (A::SWZ ? 4 * ((g >> 1) ^ t) + 2 * (g & 1) : g);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            // codes of two positions, the second counted down
-            auto code = [](uint32_t x) { return (x & 0x00f000f0u) ^ 0x00f00000u; };
-            split_f16(wgt[h][0] * ws, wgt[h][1] * ws, a0, a1);
-            split_f16(wgt[h][2] * ws, wgt[h][3] * ws, a2, a3);
-            const uint32_t *rowv = sv + (16 * h + 4 * t) * W;
-            uint32_t vw[NBK][4];
+            uint32_t a0, a1, a2, a3, vw[NBK][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t *row = rowv + ((i & 2) + ((i ^ t) & 1)) * W;
-                if (VEC && NBK == 2) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(row + 2 * g);
+                const uint32_t *row = vrow + (16 * h + i) * W;
+                if (A::SWZ) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(row);
                     vw[0][i] = v.x;
                     vw[NBK - 1][i] = v.y;
                 } else {
 #pragma unroll
-                    for (int k = 0; k < NBK; ++k) vw[k][i] = g + 8 * k < W ? row[g + 8 * k] : 0u;
+                    for (int k = 0; k < NBK; ++k) vw[k][i] = 8 * k + 7 < W || g + 8 * k < W ? row[8 * k] : 0u;
                 }
             }
+            split_f16(wgt[h][0] * ws, wgt[h][1] * ws, a0, a1);
+            split_f16(wgt[h][2] * ws, wgt[h][3] * ws, a2, a3);
+            auto code = [](uint32_t x) { return (x & 0x00f000f0u) ^ 0x00f00000u; };  // of two positions, the second counted down
 #pragma unroll
-            for (int k = 0; k < NBK; ++k) {
+            for (int k = 0; k < NBK; ++k)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {  // byte j / 2 of the four words: dims j and j + 1
                     const uint32_t sel = 0x4400u + 0x1100u * (j / 2) + 0x11u * (j / 2);
@@ -499,7 +536,6 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
                     mma_f16(acc[k][j], a0, a1, a2, a3, code(x << 4), code(y << 4));
                     mma_f16(acc[k][j + 1], a0, a1, a2, a3, code(x), code(y));
                 }
-            }
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -513,23 +549,24 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
         s_l[warp][g] = l;
     }
     __syncthreads();  // every warp is done with its ring
-    constexpr int OLD = 64 * NBK + 4;  // row stride of the partial sums
-    float *so = reinterpret_cast<float *>(smem) + (size_t)warp * ATT4_ROWS * OLD + g * OLD;
+    float *so = reinterpret_cast<float *>(smem) + (warp * ATT4_ROWS + g) * A::OLD;
     const float inv_ws = 0x1p20f / ws;
 #pragma unroll
     for (int k = 0; k < NBK; ++k)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int w = VEC && NBK == 2 ? 2 * (2 * t + i) + k : 2 * t + i + 8 * k;
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v = fmaf(acc[k][j][2 + i], 0x1p-11f, acc[k][j][i]) * inv_ws;
-                so[8 * w + j] = v + alo;
-            }
+            for (int j = 0; j < 8; ++j) v[j] = fmaf(acc[k][j][i] + acc[k][j][2 + i], inv_ws, alo);
+            float4 *dst = reinterpret_cast<float4 *>(so + 8 * A::v_word(2 * t + i, k));
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * hd; i += ATT4_WARPS * 32) {
-        const int r = i / hd, d = i - r * hd;
+    static_assert(KV4_MAX_HD <= ATT4_WARPS * 32, "a thread takes one dim");
+    const int d = threadIdx.x;
+    if (d >= hd) return;
+    for (int r = 0; r < rows; ++r) {
         float top = -INFINITY, sum = 0.0f, o = 0.0f;
 #pragma unroll
         for (int w = 0; w < ATT4_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
@@ -537,47 +574,62 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
         for (int w = 0; w < ATT4_WARPS; ++w) {
             const float f = s_l[w][r] == 0.0f ? 0.0f : exp2_fast(s_m[w][r] - top);  // a warp that saw nothing of the row
             sum = fmaf(s_l[w][r], f, sum);
-            o = fmaf(reinterpret_cast<const float *>(smem)[((size_t)w * ATT4_ROWS + r) * OLD + d], f, o);
+            o = fmaf(reinterpret_cast<const float *>(smem)[(w * ATT4_ROWS + r) * A::OLD + d], f, o);
         }
         if (alone) {
-            p.out[q_row(r) * hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
+            p.out[s_row[r] * hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
         } else {
-            const size_t at = q_row(r) * p.chunks + chunk_id;
+            const size_t at = (size_t)s_row[r] * p.chunks + chunk_id;
             p.part[at * hd + d] = o;
             if (d == 0) p.part_ml[at] = make_float2(top, sum);
         }
     }
 }
 
-// one warp per query row that was split: the weighted mean of its chunks
-__global__ void __launch_bounds__(256) attn_kv4_join_kernel(AttnParams p, long long rows) {
-    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, rep = p.n_heads / p.n_kv;
+template <int W>
+static int launch_attn_kv4(const AttnParams &p, unsigned units, int dev, cudaStream_t stream) {
+    if (p.words != W) {
+        if constexpr (W > 1) return launch_attn_kv4<W - 1>(p, units, dev, stream);
+        return fail(KB_ERR_UNSUPPORTED, "attention: rows of %d words", p.words);
+    }
+    void (*kern)(AttnParams) = attn_kv4_kernel<W>;
+    if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, (int)Attn4<W>::SMEM, "kv4 attention smem attribute")) return rc;
+    const cudaError_t e = launch_after(kern, dim3(units, (unsigned)p.chunks, (unsigned)p.row_tiles), dim3(ATT4_WARPS * 32), Attn4<W>::SMEM, stream, p);
+    return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 attention launch");
+}
+
+// One CTA per query row that was split: the weighted mean of its chunks, a thread per dim.  Eight chunks are read at a
+// time; their factors come from the lanes of a warp, one chunk each.
+__global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p) {
+    const unsigned row = blockIdx.x, tok = row / p.n_heads;
+    const int lane = threadIdx.x & 31, d = threadIdx.x, h = row - tok * p.n_heads, b = tok / p.t, i = tok - b * p.t;
+    const int r = i * p.rep + h % p.rep, tile_last = min(p.t * p.rep, (r / ATT4_ROWS + 1) * ATT4_ROWS) - 1;  // last row of its tile
     release_and_wait();
-    if (row >= rows) return;
-    const int h = (int)(row % p.n_heads), i = (int)(row / p.n_heads % p.t);
-    const int len = min(max(p.lens[row / p.n_heads / p.t], 0), p.lmax);
-    const int r = i * rep + h % rep, tile_last = min(p.t * rep, (r / ATT4_ROWS + 1) * ATT4_ROWS) - 1;  // last row of its tile
-    const int last = len - (p.t - 1 - tile_last / rep);
+    const int len = min(max(p.lens[b], 0), p.lmax);
+    const int last = len - (p.t - 1 - tile_last / p.rep);
     if (last <= p.chunk) return;  // the first kernel wrote it
     const int n = (last + p.chunk - 1) / p.chunk;
     const float2 *ml = p.part_ml + (size_t)row * p.chunks;
-    float top = -INFINITY;
+    const float *src = p.part + (size_t)row * p.chunks * p.hd + (d < p.hd ? d : 0);
+    float top = -INFINITY, sum = 0.0f, o = 0.0f;
     for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[s].x);
     top = warp_reduce_max(top);
-    float sum = 0.0f, o[4] = {};
-    for (int s = 0; s < n; ++s) {
-        const float2 v = ml[s];
-        const float f = v.y == 0.0f ? 0.0f : exp2_fast(v.x - top);
-        sum = fmaf(v.y, f, sum);
-        const float *src = p.part + ((size_t)row * p.chunks + s) * p.hd;
+    for (int s0 = 0; s0 < n; s0 += 32) {
+        const float2 v = s0 + lane < n ? ml[s0 + lane] : make_float2(0.0f, 0.0f);
+        const float mine = v.y == 0.0f ? 0.0f : exp2_fast(v.x - top);
+        sum = fmaf(v.y, mine, sum);
+        const int m = min(32, n - s0);
+        for (int s = 0; s < m; s += 8) {
+            float x[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (lane + 32 * k < p.hd) o[k] = fmaf(src[lane + 32 * k], f, o[k]);
+            for (int k = 0; k < 8; ++k) x[k] = s + k < m ? src[(size_t)(s0 + s + k) * p.hd] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o = fmaf(x[k], __shfl_sync(0xffffffffu, mine, s + k), o);
+        }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (lane + 32 * k < p.hd) p.out[(size_t)row * p.hd + lane + 32 * k] = sum == 0.0f ? 0.0f : __fdiv_rn(o[k], sum);
+    for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (d < p.hd) p.out[(size_t)row * p.hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
 }
 
 // positions per CTA.  The lengths are on the device, so the rule goes by the cache's: about four CTAs for every resident
@@ -713,12 +765,12 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
     const size_t rows = batch * (size_t)t * n_heads, units = attn_units(batch, t, n_heads, n_kv_heads);
     AttnParams p = {};
     p.q = q; p.k_codes = k_codes; p.k_steps = k_steps; p.v_codes = v_codes; p.v_steps = v_steps; p.lens = lens;
-    p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.words = kv4_words(head_dim); p.out = out;
+    p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.rep = n_heads / n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.words = kv4_words(head_dim); p.out = out;
     p.scale = scale != 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
     p.row_tiles = (int)(units / (batch * n_kv_heads));
     p.chunk = attn_chunk(units, lmax, sm_count(dev));
     p.chunks = (lmax - 1) / p.chunk + 1;
-    if (units * p.chunks > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
+    if (batch * n_kv_heads > 0x7fffffffu || p.chunks > 65535 || p.row_tiles > 65535) return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     void *own = nullptr;
     if (p.chunks > 1) {
@@ -732,21 +784,10 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
         p.part_ml = static_cast<float2 *>(workspace);
         p.part = reinterpret_cast<float *>(p.part_ml + rows * p.chunks);
     }
-    const int W = p.words, KC = (W + 3) / 4;
-    void (*kern)(AttnParams) = KC == 1 ? attn_kv4_kernel<1, false>
-                               : KC == 2 ? (W == 8 ? attn_kv4_kernel<2, true> : attn_kv4_kernel<2, false>)
-                               : KC == 3 ? attn_kv4_kernel<3, false>
-                                         : (W == 16 ? attn_kv4_kernel<4, true> : attn_kv4_kernel<4, false>);
-    const size_t ring = (size_t)ATT4_WARPS * ATT4_STAGES * (2 * ATT4_TILE * W + 2 * ATT4_TILE) * 4;
-    const size_t joined = (size_t)ATT4_WARPS * ATT4_ROWS * (64 * ((KC + 1) / 2) + 4) * 4;
-    const size_t smem = ring > joined ? ring : joined;
-    int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, 56 * 1024, "kv4 attention smem attribute");
-    if (rc == KB_OK) {
-        cudaError_t e = launch_after(kern, dim3((unsigned)(units * p.chunks)), dim3(ATT4_WARPS * 32), smem, st, p);
-        if (e == cudaSuccess && p.chunks > 1) {
-            e = launch_after(attn_kv4_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, (long long)rows);
-        }
-        if (e != cudaSuccess) rc = cuda_fail(e, "kv4 attention launch");
+    int rc = launch_attn_kv4<KV4_MAX_HD / 8>(p, (unsigned)(batch * n_kv_heads), dev, st);
+    if (rc == KB_OK && p.chunks > 1) {
+        const cudaError_t e = launch_after(attn_kv4_join_kernel, dim3((unsigned)rows), dim3(KV4_MAX_HD), 0, st, p);
+        if (e != cudaSuccess) rc = cuda_fail(e, "kv4 attention join launch");
     }
     if (own) {
         const cudaError_t e = cudaFreeAsync(own, st);
