@@ -209,50 +209,72 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 // instruction).  The factor goes into the end of the sums.  The bits 0x000f would do as well (code * 2^-24, two shifts fewer
 // per eight codes), but the instruction aligns its products by the operands' exponent fields, so leading zeros cost
 // bits of the sum: results were 1e-5 off that way.
-//   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo
-// (2^-23 of the largest of the row, for which rows are scaled by powers of two).  The terms sit in rows g
-// and g + 8 of the 16-row tile, so a warp serves 8 query rows and the second term costs nothing while the tile is not full.
-//   Lane (g, t) = (lane / 4, lane % 4).  QK^T: the contraction runs over dims in any order as long as queries and keys
-// agree, so a lane takes whole words of key row g.  The result has query row g and two positions per 8-column tile in one
-// lane, which is exactly the operand layout of the weights in the second product: no shuffle between the two.  PV: output
-// column n = g of tile j is dim 8 word(g) + j, so a lane's words of four positions give the columns of eight tiles.
-//   Positions of a 16-block are dealt so that lane t owns rows 4t .. 4t+3 (one 128-bit load of their pairs).
+//   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo, 22
+// bits of x, for which rows are scaled by powers of two.
+//   Codes are the 16-row operand, queries and weights the 8-column one (S^T = K Q^T, O^T = V^T P^T): the two terms of four
+// query rows fill the columns, so four rows are served at the price of one, and the accumulators of 128 dims take 32
+// registers.  Up to eight rows take a second set of columns (NT = 2) over the same unpacked codes.
+//   Lane (g, t) = (lane / 4, lane % 4).  The contraction over dims runs in any order as long as queries and keys agree, so
+// a lane takes whole words of key rows 2g and 2g + 1.  It gets hi and lo of query t at these positions, adds them, and after
+// the softmax packs hi and lo of the weight in the same place; a transposition of 8 x 8 tiles (movmatrix) makes them the
+// operand of the second product, where lane t meets positions 4t .. 4t+3 and row g of tile j is dim 8 word(g) + j.
+//   The largest score is a reference only: weights up to 2^8 above it are allowed before sums are rescaled, so a tile
+// costs two votes and most tiles nothing else.
 //   A warp streams its own 32-position tiles through a ring of 16-byte asynchronous copies (no barrier between warps);
 // warps of a CTA deal the tiles of a chunk, chunks of a sequence go to CTAs, a second kernel joins them.
 constexpr int ATT4_WARPS = 4;
 constexpr int ATT4_STAGES = 3;
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
-constexpr int ATT4_ROWS = 8;   // query rows of a CTA
+constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
+constexpr float ATT4_SLACK = 8.0f;  // log2 of how far a weight may rise above the reference
 
 struct AttnParams {
     const float *q;
     const uint32_t *k_codes, *k_steps, *v_codes, *v_steps;
     const int *lens;
     int t, n_heads, n_kv, rep, hd, lmax, words;
-    int row_tiles, chunk, chunks;  // chunk: positions per CTA, chunks = ceil(lmax / chunk)
+    int row_tiles, tile_rows, chunk, chunks;  // chunk: positions per CTA, chunks = ceil(lmax / chunk)
     float scale;
     float *out;
     float *part;      // [rows][chunks][hd] unnormalised sums, where chunks > 1
     float2 *part_ml;  // [rows][chunks] (largest score, sum of weights)
 };
 
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two numbers of at most 2^14 -> two f16 terms each, x = hi + lo to 2^-23 of 2^14
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+// x -> (hi, lo), two f16 terms of it
+__device__ __forceinline__ uint32_t split_f16(float x) {
+    const __half hi = __float2half_rn(x);
+    const __half2 r = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
+    return *reinterpret_cast<const uint32_t *>(&r);
 }
-__device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp over the range used here (x <= 0)
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; a result below 2^-126 is 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_over_g(float x) {  // over the eight lanes of equal t
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
+__device__ __forceinline__ float sum_over_g(float x) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const uint32_t *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -261,38 +283,40 @@ __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const uint32_t *src
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
-// W = 32-bit words of a row: a constant, so that every address inside a tile is one
-template <int W>
+// W = 32-bit words of a row, a constant, so that every address inside a tile is one; NT = sets of four query rows
+template <int W, int NT>
 struct Attn4 {
+    static constexpr int ROWS = ATT4_ROWS * NT;
     static constexpr int KC = (W + 3) / 4;      // words of a row per lane (4 lanes a row)
     static constexpr bool VEC = W % 4 == 0;     // lane t takes words KC t .., otherwise t, t + 4, ..
-    static constexpr int NBK = (W + 7) / 8;     // blocks of 8 words = 64 dims = 8 column tiles of the output
-    static constexpr bool SWZ = W == 16;        // 64-byte rows: 16-byte pieces of V are dealt over the banks
+    static constexpr int NBK = (W + 7) / 8;     // blocks of 8 words = 64 dims = 4 tiles of 16 dims of the output
+    // 64-byte rows meet in the same banks: rows 4a+2 and 4a+3 of K change places, 16-byte pieces of V are dealt over the banks
+    static constexpr bool SWZ = W == 16;
     static constexpr int STAGE = 2 * ATT4_TILE * W + 2 * ATT4_TILE;  // words: K codes, V codes, K pairs, V pairs
     static constexpr int OLD = 64 * NBK + 4;    // row stride of the partial sums in shared memory
     static constexpr size_t RING = (size_t)ATT4_WARPS * ATT4_STAGES * STAGE * 4;
-    static constexpr size_t JOINED = (size_t)ATT4_WARPS * ATT4_ROWS * OLD * 4;
+    static constexpr size_t JOINED = (size_t)ATT4_WARPS * ROWS * OLD * 4;
     static constexpr size_t SMEM = RING > JOINED ? RING : JOINED;
     __device__ static int k_word(int t, int c) { return VEC ? KC * t + c : t + 4 * c; }
-    // word of an output column n, block k
-    __device__ static int v_word(int n, int k) { return SWZ ? 2 * n + k : n + 8 * k; }
+    // word of output row g, block k
+    __device__ static int v_word(int g, int k) { return SWZ ? 2 * g + k : g + 8 * k; }
 };
 
-template <int W>
+template <int W, int NT>
 __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams p) {
-    using A = Attn4<W>;
-    constexpr int KC = A::KC, NBK = A::NBK;
+    using A = Attn4<W, NT>;
+    constexpr int KC = A::KC, NBK = A::NBK, ROWS = A::ROWS;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint4 s_q[2 * KC][32];  // query operands, in the order of the matrix instruction
-    __shared__ float s_fr[ATT4_ROWS], s_qs[ATT4_ROWS];
-    __shared__ float s_m[ATT4_WARPS][ATT4_ROWS], s_l[ATT4_WARPS][ATT4_ROWS];
-    __shared__ long long s_row[ATT4_ROWS];  // index of the tile's rows in q and out
-    __shared__ int s_off[ATT4_ROWS];        // positions behind the sequence's end that a row does not see
+    __shared__ uint2 s_q[NT][2 * KC][32];  // query operands, in the order of the matrix instruction
+    __shared__ float s_fr[ROWS], s_qs[ROWS];
+    __shared__ float s_m[ATT4_WARPS][ROWS], s_l[ATT4_WARPS][ROWS];
+    __shared__ long long s_row[ROWS];  // index of the tile's rows in q and out
+    __shared__ int s_off[ROWS];        // positions behind the sequence's end that a row does not see
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int unit = blockIdx.x, chunk_id = blockIdx.y;  // sequence * n_kv + KV head
     const int b = unit / p.n_kv, rep = p.rep, hd = p.hd;
-    const int r0 = blockIdx.z * ATT4_ROWS, rows = min(ATT4_ROWS, p.t * rep - r0);  // rows: query token * rep + head of the group
-    if (threadIdx.x < ATT4_ROWS) {
+    const int r0 = blockIdx.z * ROWS, rows = min(ROWS, p.t * rep - r0);  // rows: query token * rep + head of the group
+    if (threadIdx.x < ROWS) {
         const int r = r0 + min((int)threadIdx.x, rows - 1), i = r / rep;
         s_row[threadIdx.x] = ((long long)b * p.t + i) * p.n_heads + (unit - b * p.n_kv) * rep + (r - i * rep);
         s_off[threadIdx.x] = p.t - 1 - i;
@@ -315,9 +339,11 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     const size_t base = (size_t)unit * p.lmax;
     const uint32_t *kc = p.k_codes + base * W, *vc = p.v_codes + base * W, *pairs = ((lane & 8) ? p.v_steps : p.k_steps) + base;
-    // 16-byte pieces: piece i = lane + 32 j of a plane's 8 W; V's are swapped inside a row by (row / 4) % 4 where SWZ
-    const int swz[2] = {A::SWZ ? 16 * ((lane & ~3) | ((lane & 3) ^ (lane >> 4))) : 16 * lane,
-                        A::SWZ ? 16 * ((lane & ~3) | ((lane & 3) ^ (lane >> 4) ^ 2)) : 16 * lane};
+    // 16-byte pieces: piece i = lane + 32 j of a plane's 8 W.  SWZ: K's go to row r ^ (r / 2) % 2, V's change places inside
+    // their row by (r / 4) % 4
+    const int kdst = A::SWZ ? 16 * (lane ^ ((lane >> 1) & 4)) : 16 * lane;
+    const int vdst[2] = {A::SWZ ? 16 * ((lane & ~3) | ((lane & 3) ^ (lane >> 4))) : 16 * lane,
+                         A::SWZ ? 16 * ((lane & ~3) | ((lane & 3) ^ (lane >> 4) ^ 2)) : 16 * lane};
     auto issue = [&](int tile0, int stage) {
         const uint32_t dst = ring_at + stage * (A::STAGE * 4);
         if (tile0 + ATT4_TILE <= c1) {
@@ -325,8 +351,8 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
 #pragma unroll
             for (int j = 0; j < (8 * W + 31) / 32; ++j)
                 if (32 * j + 31 < 8 * W || lane + 32 * j < 8 * W) {
-                    copy16(dst + 16 * lane + 512 * j, ks + 128 * j);
-                    copy16(dst + ATT4_TILE * W * 4 + swz[j & 1] + 512 * j, vs + 128 * j);
+                    copy16(dst + kdst + 512 * j, ks + 128 * j);
+                    copy16(dst + ATT4_TILE * W * 4 + vdst[j & 1] + 512 * j, vs + 128 * j);
                 }
             if (lane < 16) copy16(dst + 2 * ATT4_TILE * W * 4 + 16 * lane, pairs + tile0 + 4 * (lane & 7));
         } else if (tile0 < c1) {
@@ -337,8 +363,8 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
                 if (lane + 32 * j < 8 * W) {
                     const bool ok = 4 * (lane + 32 * j) < have * W;
                     const size_t off = (size_t)tile0 * W + (ok ? 4 * (lane + 32 * j) : 0);
-                    copy16_or_zero(dst + 16 * lane + 512 * j, kc + off, ok);
-                    copy16_or_zero(dst + ATT4_TILE * W * 4 + swz[j & 1] + 512 * j, vc + off, ok);
+                    copy16_or_zero(dst + kdst + 512 * j, kc + off, ok);
+                    copy16_or_zero(dst + ATT4_TILE * W * 4 + vdst[j & 1] + 512 * j, vc + off, ok);
                 }
             if (lane < 16) {
                 const bool ok = 4 * (lane & 7) < have;
@@ -351,8 +377,8 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
 #pragma unroll
     for (int s = 0; s < ATT4_STAGES - 1; ++s) issue(first + s * stride, s);
 
-    // ---- queries times scale log2(e), scaled by a power of two to [2^13, 2^14), split, laid out; a warp prepares two rows
-    for (int r = warp; r < ATT4_ROWS; r += ATT4_WARPS) {
+    // ---- queries times scale log2(e), scaled by a power of two to [2^13, 2^14), split, laid out; a warp takes NT rows
+    for (int r = warp; r < ROWS; r += ATT4_WARPS) {
         const float *src = p.q + s_row[r] * hd;
         const float unit2 = p.scale * 1.4426950408889634f;  // scores in units of log 2
         float x[4], amax = 0.0f, sum = 0.0f;
@@ -372,34 +398,54 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
             s_fr[r] = __int_as_float(min(e + 7, 254) << 23);  // 2^20 / up
             s_qs[r] = e > 247 ? __uint_as_float(0x7fffffffu) : sum;
         }
-        __half *dst = reinterpret_cast<__half *>(s_q);
+        __half *dst = reinterpret_cast<__half *>(s_q[r / ATT4_ROWS]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = lane + 32 * i, w = d >> 3, n = d & 7;
             if (w >= 4 * KC) continue;
             const int tt = A::VEC ? w / KC : w & 3, c = A::VEC ? w % KC : w >> 2;
-            const float y = x[i] * up;
-            const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
-            // step 2c + (n & 2) / 2, register pair (n & 1), half n / 4
-            __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + r * 4 + tt) * 8 + (n & 1) * 4 + (n >> 2);
-            at[0] = hi;
-            at[2] = lo;
+            const uint32_t y = split_f16(x[i] * up);
+            // step 2c + (n & 2) / 2, register n & 1, half n / 4; column 2 (r % 4) holds hi, the next one lo
+            __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + (r % ATT4_ROWS) * 8 + tt) * 4 + (n & 1) * 2 + (n >> 2);
+            at[0] = __ushort_as_half((unsigned short)(y & 0xffffu));
+            at[16] = __ushort_as_half((unsigned short)(y >> 16));
         }
     }
     __syncthreads();
-    const int limit = g < rows ? len - s_off[g] : 0;  // positions row g sees
-    const int least = min(c1, len - s_off[0]);        // the smallest limit of the tile's rows
-    const float fr = s_fr[g], qs = s_qs[g];
+    const int least = min(c1, len - s_off[0]);  // the smallest limit of the tile's rows
+    uint2 qf[NT][2 * KC];  // held in registers where they fit
+    if (NT == 1) {
+#pragma unroll
+        for (int c = 0; c < 2 * KC; ++c) qf[0][c] = s_q[0][c][lane];
+    }
+    int end[NT];  // positions of the chunk that this lane's row sees
+    float fr[NT], qs[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = 4 * n + t;
+        end[n] = r < rows ? min(c1, len - s_off[r]) : 0;
+        fr[n] = s_fr[r];
+        qs[n] = s_qs[r];
+    }
 
-    float acc[NBK][8][4];
+    float acc[NT][NBK][4][4];
 #pragma unroll
-    for (int k = 0; k < NBK; ++k)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int k = 0; k < NBK; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[k][j][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f, alo = 0.0f;  // of this lane's positions of row g; m is the row's, over the quad
-    float wref = 0x1p-100f, ws = 0x1p113f;      // largest weight so far; weights are held times ws = 2^13 / 2^floor(log2 wref)
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][k][j][i] = 0.0f;
+    // of row t of each set: reference, sums over this lane's positions, the largest |weight * step| at the last rescaling, and
+    // what weights are held times: 2^6 / 2^floor(log2 wref)
+    float mref[NT], l[NT], alo[NT], wref[NT], ws[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mref[n] = -INFINITY, l[n] = alo[n] = 0.0f, wref[n] = 0x1p-100f, ws[n] = 0x1p106f;
+    // every second position (odd g) counts down from its largest value, lo + 15 step - (15 - c) step: the sum of the products
+    // then changes sign as the values do.  With codes alone it only grows, and the instruction's truncated adds pull all of it
+    // one way (2.8e-4 of the result at 32768 positions, 1e-6 without that)
+    const float down = g & 1 ? 15.0f : 0.0f, sign = g & 1 ? -1.0f : 1.0f;
 
     int stage = 0;
     for (int tile0 = first; tile0 < c1; tile0 += stride) {
@@ -409,109 +455,121 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
         const uint32_t *sk = ring + stage * A::STAGE, *sv = sk + ATT4_TILE * W, *sp = sv + ATT4_TILE * W;
         stage = stage + 1 == ATT4_STAGES ? 0 : stage + 1;
 
-        // ---- scores: 4 tiles of 8 positions; column n of tile u of block h is position 16 h + 4 (n / 2) + 2 u + n % 2
-        float sc[4][4];
-        uint32_t kw[4][KC];
-        const uint32_t *krow = sk + (4 * (g >> 1) + (g & 1)) * W + A::k_word(t, 0);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const uint32_t *row = krow + (16 * (n >> 1) + 2 * (n & 1)) * W;
-            if (A::VEC && KC == 4) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(row);
-                kw[n][0] = v.x; kw[n][1 % KC] = v.y; kw[n][2 % KC] = v.z; kw[n][3 % KC] = v.w;
-            } else if (A::VEC && KC == 2) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(row);
-                kw[n][0] = v.x; kw[n][1 % KC] = v.y;
-            } else {
-#pragma unroll
-                for (int c = 0; c < KC; ++c) kw[n][c] = A::VEC || 4 * c + 3 < W || t + 4 * c < W ? row[A::VEC ? c : 4 * c] : 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[n][i] = 0.0f;
-        }
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const uint4 a = s_q[2 * c][lane], a2 = s_q[2 * c + 1][lane];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const uint32_t x = kw[n][c], y = x >> 8;
-                mma_f16(sc[n], a.x, a.y, a.z, a.w, (x << 4) & 0x00f000f0u, x & 0x00f000f0u);
-                mma_f16(sc[n], a2.x, a2.y, a2.z, a2.w, (y << 4) & 0x00f000f0u, y & 0x00f000f0u);
-            }
-        }
-        // ---- softmax weights of row g at this lane's positions: [i] of block h is position 16 h + 4 t + i
-        float wgt[2][4], top = -INFINITY;
+        // ---- scores: block h holds positions 16 h + 2 g (rows g of its tile) and 16 h + 2 g + 1 (rows g + 8)
+        float s[NT][2][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint4 kp = *reinterpret_cast<const uint4 *>(sp + 16 * h + 4 * t);
-            const uint32_t pr[4] = {kp.x, kp.y, kp.z, kp.w};
+            uint32_t kw[2][KC];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float dot = sc[2 * h + (i >> 1)][i & 1] + sc[2 * h + (i >> 1)][2 + (i & 1)];
-                wgt[h][i] = fmaf(dot, kv4_step(pr[i]) * fr, kv4_lo(pr[i]) * qs);
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t *row = sk + (16 * h + (A::SWZ ? (2 * g + i) ^ (g & 1) : 2 * g + i)) * W + A::k_word(t, 0);
+                if (A::VEC && KC == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(row);
+                    kw[i][0] = v.x; kw[i][1 % KC] = v.y; kw[i][2 % KC] = v.z; kw[i][3 % KC] = v.w;
+                } else if (A::VEC && KC == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(row);
+                    kw[i][0] = v.x; kw[i][1 % KC] = v.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) kw[i][c] = A::VEC || 4 * c + 3 < W || t + 4 * c < W ? row[A::VEC ? c : 4 * c] : 0u;
+                }
+            }
+            float sc[NT][4];
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const uint32_t x = kw[0][c], y = kw[1][c];
+                const uint32_t a[4] = {(x << 4) & 0x00f000f0u, (y << 4) & 0x00f000f0u, x & 0x00f000f0u, y & 0x00f000f0u};
+                const uint32_t x8 = x >> 8, y8 = y >> 8;
+                const uint32_t a8[4] = {(x8 << 4) & 0x00f000f0u, (y8 << 4) & 0x00f000f0u, x8 & 0x00f000f0u, y8 & 0x00f000f0u};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 q0 = NT == 1 ? qf[n][2 * c] : s_q[n][2 * c][lane], q1 = NT == 1 ? qf[n][2 * c + 1] : s_q[n][2 * c + 1][lane];
+                    if (c == 0) mma_f16_first(sc[n], a[0], a[1], a[2], a[3], q0.x, q0.y);
+                    else mma_f16(sc[n], a[0], a[1], a[2], a[3], q0.x, q0.y);
+                    mma_f16(sc[n], a8[0], a8[1], a8[2], a8[3], q1.x, q1.y);
+                }
+            }
+            const uint2 kp = *reinterpret_cast<const uint2 *>(sp + 16 * h + 2 * g);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[n][h][0] = fmaf(sc[n][0] + sc[n][1], kv4_step(kp.x) * fr[n], kv4_lo(kp.x) * qs[n]);
+                s[n][h][1] = fmaf(sc[n][2] + sc[n][3], kv4_step(kp.y) * fr[n], kv4_lo(kp.y) * qs[n]);
             }
         }
         const bool tail = tile0 + ATT4_TILE > least;  // some row does not see all of the tile
         if (tail) {
-            const int end = min(limit, c1) - tile0 - 4 * t;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (tile0 + 16 * h + 2 * g + i >= end[n]) s[n][h][i] = -INFINITY;
+        }
+        // ---- softmax weights
+        float top[NT], corr[NT];
+        bool rise = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            top[n] = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1]));
+            rise |= top[n] > mref[n] + ATT4_SLACK;
+            corr[n] = 1.0f;
+        }
+        const bool fresh = __any_sync(0xffffffffu, rise);
+        if (fresh) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float m = fmaxf(mref[n], max_over_g(top[n]));
+                corr[n] = m == -INFINITY ? 1.0f : exp2_fast(mref[n] - m);
+                mref[n] = m;
+                l[n] *= corr[n];
+                alo[n] *= corr[n];
+                wref[n] = fmaxf(wref[n] * corr[n], 0x1p-100f);
+            }
+        }
+        uint2 vp[2];
+        vp[0] = *reinterpret_cast<const uint2 *>(sp + ATT4_TILE + 2 * g);
+        vp[1] = *reinterpret_cast<const uint2 *>(sp + ATT4_TILE + 16 + 2 * g);
+        float wmax[NT];
+        bool large = fresh;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float ref = mref[n] == -INFINITY ? 0.0f : mref[n];  // nothing seen yet: every weight is 0
+            wmax[n] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (16 * h + i >= end) wgt[h][i] = -INFINITY;
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t pr = i ? vp[h].y : vp[h].x;
+                    if (tail) pr = s[n][h][i] == -INFINITY ? 0u : pr;  // what is not seen may hold anything, NaN too
+                    const float pj = exp2_fast(s[n][h][i] - ref), step = kv4_step(pr);
+                    l[n] += pj;
+                    alo[n] = fmaf(pj, fmaf(down, step, kv4_lo(pr)), alo[n]);
+                    s[n][h][i] = pj * step;
+                    wmax[n] = fmaxf(wmax[n], s[n][h][i]);
+                }
+            large |= wmax[n] * ws[n] > 0x1p15f;
         }
+        if (__any_sync(0xffffffffu, large)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int n = 0; n < NT; ++n) {
+                wref[n] = fminf(fmaxf(wref[n], max_over_g(wmax[n])), 0x1p127f);
+                const float ws_new = __uint_as_float(0x82000000u - (__float_as_uint(wref[n]) & 0x7f800000u));  // by exponent fields
+                const float adj = corr[n] * fminf(__fdividef(ws_new, ws[n]), 0x1p127f);  // a ratio of powers of two; corr may be 0
+                ws[n] = ws_new;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, wgt[h][i]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
-        const float corr = exp2_fast(m - ref);
-        l *= corr;
-        alo *= corr;
-        m = m_new;
-        float wmax = 0.0f;
+                for (int k = 0; k < NBK; ++k)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint4 vp = *reinterpret_cast<const uint4 *>(sp + ATT4_TILE + 16 * h + 4 * t);
-            uint32_t pr[4] = {vp.x, vp.y, vp.z, vp.w};
-            if (tail) {  // what is not seen may hold anything, NaN too
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pr[i] = wgt[h][i] == -INFINITY ? 0u : pr[i];
+                        for (int i = 0; i < 4; ++i) acc[n][k][j][i] *= adj;
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float pj = exp2_fast(wgt[h][i] - ref);
-                l += pj;
-                // every second position counts down from its largest value, lo + 15 step - (15 - c) step: the sum of the
-                // products then changes sign as the values do.  With codes alone it only grows, and the instruction's
-                // truncated adds pull all of it one way (2.8e-4 of the result at 32768 positions, 1e-6 without that)
-                const float step = kv4_step(pr[i]), from = kv4_lo(pr[i]);
-                alo = fmaf(pj, i & 1 ? fmaf(15.0f, step, from) : from, alo);
-                wgt[h][i] = pj * (i & 1 ? -step : step);
-                wmax = fmaxf(wmax, fabsf(wgt[h][i]));
-            }
-        }
-        wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 1));
-        wmax = fmaxf(wmax, __shfl_xor_sync(0xffffffffu, wmax, 2));
-        wref = fminf(fmaxf(fmaxf(wref * corr, wmax), 0x1p-100f), 0x1p127f);
-        const float ws_new = __uint_as_float(0x85800000u - (__float_as_uint(wref) & 0x7f800000u));  // by exponent fields
-        if (__any_sync(0xffffffffu, ws_new != ws || corr != 1.0f)) {
-            const float adj = corr * fminf(__fdividef(ws_new, ws), 0x1p127f);  // a ratio of powers of two; corr may be 0
-            ws = ws_new;
-#pragma unroll
-            for (int k = 0; k < NBK; ++k)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[k][j][i] *= adj;
         }
         // ---- weighted sum of the codes
         const uint32_t *vrow = sv + 4 * t * W + (A::SWZ ? 4 * ((g >> 1) ^ t) + 2 * (g & 1) : g);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3, vw[NBK][4];
+            uint32_t vw[NBK][4], b0[NT], b1[NT];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t *row = vrow + (16 * h + i) * W;
@@ -524,64 +582,71 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
                     for (int k = 0; k < NBK; ++k) vw[k][i] = 8 * k + 7 < W || g + 8 * k < W ? row[8 * k] : 0u;
                 }
             }
-            split_f16(wgt[h][0] * ws, wgt[h][1] * ws, a0, a1);
-            split_f16(wgt[h][2] * ws, wgt[h][3] * ws, a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float f = ws[n] * sign;
+                b0[n] = transpose_8x8(split_f16(s[n][h][0] * f));  // positions 4t and 4t + 2 of column g
+                b1[n] = transpose_8x8(split_f16(s[n][h][1] * f));  // positions 4t + 1 and 4t + 3
+            }
             auto code = [](uint32_t x) { return (x & 0x00f000f0u) ^ 0x00f00000u; };  // of two positions, the second counted down
 #pragma unroll
             for (int k = 0; k < NBK; ++k)
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {  // byte j / 2 of the four words: dims j and j + 1
-                    const uint32_t sel = 0x4400u + 0x1100u * (j / 2) + 0x11u * (j / 2);
-                    const uint32_t x = __byte_perm(vw[k][0], vw[k][1], sel), y = __byte_perm(vw[k][2], vw[k][3], sel);
-                    mma_f16(acc[k][j], a0, a1, a2, a3, code(x << 4), code(y << 4));
-                    mma_f16(acc[k][j + 1], a0, a1, a2, a3, code(x), code(y));
+                for (int j = 0; j < 4; ++j) {  // byte j of the four words: dims 2j (rows g) and 2j + 1 (rows g + 8)
+                    const uint32_t sel = 0x4400u + 0x1111u * j;
+                    const uint32_t x = __byte_perm(vw[k][0], vw[k][2], sel), y = __byte_perm(vw[k][1], vw[k][3], sel);
+                    const uint32_t a0 = code(x << 4), a1 = code(x), a2 = code(y << 4), a3 = code(y);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_f16(acc[n][k][j], a0, a1, a2, a3, b0[n], b1[n]);
                 }
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    // ---- join the warps: sums of row g over its four lanes, then rows over the warps through shared memory
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    alo += __shfl_xor_sync(0xffffffffu, alo, 1);
-    alo += __shfl_xor_sync(0xffffffffu, alo, 2);
-    if (t == 0) {
-        s_m[warp][g] = m;
-        s_l[warp][g] = l;
+    // ---- join the warps: sums of a row over its eight lanes, then rows over the warps through shared memory
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        l[n] = sum_over_g(l[n]);
+        alo[n] = sum_over_g(alo[n]);
+        if (g == 0) {
+            s_m[warp][4 * n + t] = mref[n];
+            s_l[warp][4 * n + t] = l[n];
+        }
     }
     __syncthreads();  // every warp is done with its ring
-    float *so = reinterpret_cast<float *>(smem) + (warp * ATT4_ROWS + g) * A::OLD;
-    const float inv_ws = 0x1p20f / ws;
 #pragma unroll
-    for (int k = 0; k < NBK; ++k)
+    for (int n = 0; n < NT; ++n) {
+        float *so = reinterpret_cast<float *>(smem) + (warp * ROWS + 4 * n + t) * A::OLD;
+        const float inv_ws = 0x1p20f / ws[n];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float v[8];
+        for (int k = 0; k < NBK; ++k) {
+            float4 *dst = reinterpret_cast<float4 *>(so + 8 * A::v_word(g, k));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fmaf(acc[k][j][i] + acc[k][j][2 + i], inv_ws, alo);
-            float4 *dst = reinterpret_cast<float4 *>(so + 8 * A::v_word(2 * t + i, k));
-            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            for (int j = 0; j < 4; j += 2)
+                dst[j / 2] = make_float4(fmaf(acc[n][k][j][0] + acc[n][k][j][1], inv_ws, alo[n]), fmaf(acc[n][k][j][2] + acc[n][k][j][3], inv_ws, alo[n]),
+                                         fmaf(acc[n][k][j + 1][0] + acc[n][k][j + 1][1], inv_ws, alo[n]),
+                                         fmaf(acc[n][k][j + 1][2] + acc[n][k][j + 1][3], inv_ws, alo[n]));
         }
+    }
     __syncthreads();
     static_assert(KV4_MAX_HD <= ATT4_WARPS * 32, "a thread takes one dim");
     const int d = threadIdx.x;
     if (d >= hd) return;
     for (int r = 0; r < rows; ++r) {
-        float top = -INFINITY, sum = 0.0f, o = 0.0f;
+        float m = -INFINITY, sum = 0.0f, o = 0.0f;
 #pragma unroll
-        for (int w = 0; w < ATT4_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+        for (int w = 0; w < ATT4_WARPS; ++w) m = fmaxf(m, s_m[w][r]);
 #pragma unroll
         for (int w = 0; w < ATT4_WARPS; ++w) {
-            const float f = s_l[w][r] == 0.0f ? 0.0f : exp2_fast(s_m[w][r] - top);  // a warp that saw nothing of the row
+            const float f = s_l[w][r] == 0.0f ? 0.0f : exp2_fast(s_m[w][r] - m);  // a warp that saw nothing of the row
             sum = fmaf(s_l[w][r], f, sum);
-            o = fmaf(reinterpret_cast<const float *>(smem)[(w * ATT4_ROWS + r) * A::OLD + d], f, o);
+            o = fmaf(reinterpret_cast<const float *>(smem)[(w * ROWS + r) * A::OLD + d], f, o);
         }
         if (alone) {
             p.out[s_row[r] * hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
         } else {
             const size_t at = (size_t)s_row[r] * p.chunks + chunk_id;
             p.part[at * hd + d] = o;
-            if (d == 0) p.part_ml[at] = make_float2(top, sum);
+            if (d == 0) p.part_ml[at] = make_float2(m, sum);
         }
     }
 }
@@ -592,9 +657,11 @@ static int launch_attn_kv4(const AttnParams &p, unsigned units, int dev, cudaStr
         if constexpr (W > 1) return launch_attn_kv4<W - 1>(p, units, dev, stream);
         return fail(KB_ERR_UNSUPPORTED, "attention: rows of %d words", p.words);
     }
-    void (*kern)(AttnParams) = attn_kv4_kernel<W>;
-    if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, (int)Attn4<W>::SMEM, "kv4 attention smem attribute")) return rc;
-    const cudaError_t e = launch_after(kern, dim3(units, (unsigned)p.chunks, (unsigned)p.row_tiles), dim3(ATT4_WARPS * 32), Attn4<W>::SMEM, stream, p);
+    const bool one = p.tile_rows == ATT4_ROWS;
+    void (*kern)(AttnParams) = one ? attn_kv4_kernel<W, 1> : attn_kv4_kernel<W, 2>;
+    const size_t smem = one ? Attn4<W, 1>::SMEM : Attn4<W, 2>::SMEM;
+    if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, (int)smem, "kv4 attention smem attribute")) return rc;
+    const cudaError_t e = launch_after(kern, dim3(units, (unsigned)p.chunks, (unsigned)p.row_tiles), dim3(ATT4_WARPS * 32), smem, stream, p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 attention launch");
 }
 
@@ -603,7 +670,7 @@ static int launch_attn_kv4(const AttnParams &p, unsigned units, int dev, cudaStr
 __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p) {
     const unsigned row = blockIdx.x, tok = row / p.n_heads;
     const int lane = threadIdx.x & 31, d = threadIdx.x, h = row - tok * p.n_heads, b = tok / p.t, i = tok - b * p.t;
-    const int r = i * p.rep + h % p.rep, tile_last = min(p.t * p.rep, (r / ATT4_ROWS + 1) * ATT4_ROWS) - 1;  // last row of its tile
+    const int r = i * p.rep + h % p.rep, tile_last = min(p.t * p.rep, (r / p.tile_rows + 1) * p.tile_rows) - 1;  // last row of its tile
     release_and_wait();
     const int len = min(max(p.lens[b], 0), p.lmax);
     const int last = len - (p.t - 1 - tile_last / p.rep);
@@ -648,10 +715,12 @@ static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
     return KB_OK;
 }
 
+// query rows of a CTA: one set of columns where it holds them all
+static int attn_tile_rows(int t, int n_heads, int n_kv) { return (size_t)t * (n_heads / n_kv) <= ATT4_ROWS ? ATT4_ROWS : 2 * ATT4_ROWS; }
 // CTAs that share nothing: (sequence, KV head, tile of query rows)
 static size_t attn_units(size_t batch, int t, int n_heads, int n_kv) {
     const size_t rows = (size_t)t * (n_heads / n_kv);
-    return batch * n_kv * ((rows + ATT4_ROWS - 1) / ATT4_ROWS);
+    return batch * n_kv * ((rows + attn_tile_rows(t, n_heads, n_kv) - 1) / attn_tile_rows(t, n_heads, n_kv));
 }
 
 static bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, const void *d = nullptr) {
@@ -767,6 +836,7 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
     p.q = q; p.k_codes = k_codes; p.k_steps = k_steps; p.v_codes = v_codes; p.v_steps = v_steps; p.lens = lens;
     p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.rep = n_heads / n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.words = kv4_words(head_dim); p.out = out;
     p.scale = scale != 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
+    p.tile_rows = attn_tile_rows(t, n_heads, n_kv_heads);
     p.row_tiles = (int)(units / (batch * n_kv_heads));
     p.chunk = attn_chunk(units, lmax, sm_count(dev));
     p.chunks = (lmax - 1) / p.chunk + 1;
