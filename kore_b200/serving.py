@@ -11,40 +11,50 @@ everywhere in this package.
 """
 from __future__ import annotations
 
-import ctypes as C
-from contextlib import nullcontext
+import torch
 
 from . import _cabi
 from ._cabi import KoreError
 
+_F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
 
-def _need(t, name: str, dtype, shape=None, contiguous: bool = True, device=None):
-    """t is a CUDA tensor of this type (and shape, -1 = any; and device), or a KoreError in the library's manner"""
-    import torch
 
+def _refuse(t, name, dtype, shape, dev):
+    """says which of ``_need``'s conditions t misses"""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype:
         got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise KoreError(_cabi.ERR_DTYPE, f"{name}: expected a CUDA {dtype} tensor, got {got}")
-    if shape is not None and (t.dim() != len(shape) or any(w not in (-1, g) for w, g in zip(shape, t.shape))):
+    if shape is not None and tuple(t.shape) != shape:
         raise KoreError(_cabi.ERR_SHAPE, f"{name}: shape mismatch: expected {list(shape)}, got {list(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise KoreError(_cabi.ERR_INVALID, f"{name}: expected a contiguous tensor")
-    if device is not None and t.device != device:
-        raise KoreError(_cabi.ERR_INVALID, f"{name}: on {t.device}, the other operands are on {device}")
+    if dev is not None and t.get_device() != dev:
+        raise KoreError(_cabi.ERR_INVALID, f"{name}: on {t.device}, the other operands are on cuda:{dev}")
+    raise KoreError(_cabi.ERR_INVALID, f"{name}: expected a contiguous tensor")
+
+
+def _need(t, name: str, dtype, shape=None, dev=None, contiguous: bool = True):
+    """t is a CUDA tensor of this type, shape and device index, or a KoreError in the library's manner"""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and (shape is None or t.shape == shape)
+            and (dev is None or t.get_device() == dev) and (not contiguous or t.is_contiguous())):
+        _refuse(t, name, dtype, shape, dev)
     return t
 
 
-def _on(device):
-    """the library launches on the current device"""
-    import torch
-
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _dims(t, name: str, want: str, n: int):
+    if t.dim() != n:
+        raise KoreError(_cabi.ERR_SHAPE, f"{name}: shape mismatch: expected {want}, got {list(t.shape)}")
 
 
-def _stream(device) -> int:
-    import torch
-
-    return torch.cuda.current_stream(device).cuda_stream
+def _run(dev: int, fn, *args):
+    """the entry point on the device's current stream; the library launches on the current device"""
+    # the handles themselves: torch.cuda.current_stream(dev).cuda_stream and current_device() take 2 us of a 9 us call
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc != _cabi.OK:
+        _cabi.check(rc)
 
 
 class KV4Cache:
@@ -55,14 +65,12 @@ class KV4Cache:
     [n_seqs, n_kv_heads, max_len]; a code c stands for lo + c * step.  ``max_len`` is rounded up to a multiple of 4."""
 
     def __init__(self, n_seqs: int, n_kv_heads: int, max_len: int, head_dim: int, device: int = 0):
-        import torch
-
         if min(n_seqs, n_kv_heads, max_len) < 1:
             raise KoreError(_cabi.ERR_INVALID, f"KV4Cache: {n_seqs} sequences, {n_kv_heads} KV heads, {max_len} positions")
         max_len = (max_len + 3) // 4 * 4
         dev = torch.device("cuda", device)
         words = int(_cabi.lib().kb_kv4_row_words(head_dim))
-        z = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)
+        z = lambda *shape: torch.zeros(shape, dtype=_I32, device=dev)
         self._adopt(z(n_seqs, n_kv_heads, max_len, words), z(n_seqs, n_kv_heads, max_len),
                     z(n_seqs, n_kv_heads, max_len, words), z(n_seqs, n_kv_heads, max_len), head_dim)
 
@@ -74,20 +82,22 @@ class KV4Cache:
         return self
 
     def _adopt(self, k_codes, k_steps, v_codes, v_steps, head_dim):
-        import torch
-
         if head_dim < 4 or head_dim > 128 or head_dim % 4:
             raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: head_dim {head_dim} must be a multiple of 4 up to 128")
-        _need(k_codes, "k_codes", torch.int32, (-1, -1, -1, (head_dim + 7) // 8))
-        shape = tuple(k_codes.shape)
-        for t, name, want in ((k_steps, "k_steps", shape[:3]), (v_codes, "v_codes", shape), (v_steps, "v_steps", shape[:3])):
-            _need(t, name, torch.int32, want, device=k_codes.device)
+        _need(k_codes, "k_codes", _I32)
+        _dims(k_codes, "k_codes", "[n_seqs, n_kv_heads, max_len, words]", 4)
+        shape, dev = tuple(k_codes.shape[:3]) + ((head_dim + 7) // 8,), k_codes.get_device()
+        for t, name, want in ((k_codes, "k_codes", shape), (k_steps, "k_steps", shape[:3]), (v_codes, "v_codes", shape),
+                              (v_steps, "v_steps", shape[:3])):
+            _need(t, name, _I32, want, dev)
         if shape[2] % 4 or 0 in shape:
             raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: planes of {list(shape)}: the cache length must be a multiple of 4")
         self.k_codes, self.k_steps, self.v_codes, self.v_steps = k_codes, k_steps, v_codes, v_steps
         self.n_seqs, self.n_kv_heads, self.max_len, self.head_dim = shape[0], shape[1], shape[2], int(head_dim)
         self.device = k_codes.device
+        self._dev, self._lib = dev, _cabi.lib()
         self._planes = tuple(t.data_ptr() for t in (k_codes, k_steps, v_codes, v_steps))
+        self._ws_bytes = {}  # workspace of attend by (query tokens, heads)
 
     def memory_bytes(self) -> int:
         return sum(t.numel() * 4 for t in (self.k_codes, self.k_steps, self.v_codes, self.v_steps))
@@ -95,18 +105,16 @@ class KV4Cache:
     def read(self, cache_rows, k_out=None, v_out=None):
         """The f32 values of cache rows (int64 [n], row = sequence * max_len + position; zeros for a row outside the
         cache): K and V, each [n, n_kv_heads, head_dim]."""
-        import torch
-
-        _need(cache_rows, "cache_rows", torch.int64, (-1,), device=self.device)
+        dev = self._dev
+        _need(cache_rows, "cache_rows", _I64, None, dev)
+        _dims(cache_rows, "cache_rows", "[n]", 1)
         n = cache_rows.shape[0]
         shape = (n, self.n_kv_heads, self.head_dim)
-        k_out, v_out = (torch.empty(shape, dtype=torch.float32, device=self.device) if o is None
-                        else _need(o, "out", torch.float32, shape, device=self.device) for o in (k_out, v_out))
-        if n == 0:
-            return k_out, v_out
-        with _on(self.device):
-            _cabi.check(_cabi.lib().kb_kv4_read(*self._planes, cache_rows.data_ptr(), n, self.n_kv_heads, self.head_dim,
-                                                self.n_seqs, self.max_len, k_out.data_ptr(), v_out.data_ptr(), _stream(self.device)))
+        k_out = torch.empty(shape, dtype=_F32, device=self.device) if k_out is None else _need(k_out, "k_out", _F32, shape, dev)
+        v_out = torch.empty(shape, dtype=_F32, device=self.device) if v_out is None else _need(v_out, "v_out", _F32, shape, dev)
+        if n:
+            _run(dev, self._lib.kb_kv4_read, *self._planes, cache_rows.data_ptr(), n, self.n_kv_heads, self.head_dim, self.n_seqs,
+                 self.max_len, k_out.data_ptr(), v_out.data_ptr())
         return k_out, v_out
 
 
@@ -118,42 +126,39 @@ def qknorm_rope_append(qkv, positions, cache_rows, cos, sin, cache, n_heads: int
 
     ``cache`` is a KV4Cache or a pair (k, v) of float32 caches [n_seqs, n_kv_heads, max_len, head_dim].  Returns the
     queries, float32 [n, n_heads, head_dim].  Two tokens of one call must not name the same cache row."""
-    import torch
-
-    f32 = torch.float32
     four = isinstance(cache, KV4Cache)
     if four:
-        n_seqs, n_kv, lmax, hd, dev = cache.n_seqs, cache.n_kv_heads, cache.max_len, cache.head_dim, cache.device
+        n_seqs, n_kv, lmax, hd, dev = cache.n_seqs, cache.n_kv_heads, cache.max_len, cache.head_dim, cache._dev
+        planes, fn = cache._planes, cache._lib.kb_qknorm_rope_kv4
     else:
         k, v = cache
-        _need(k, "k cache", f32, (-1, -1, -1, -1))
+        _need(k, "k cache", _F32)
+        _dims(k, "k cache", "[n_seqs, n_kv_heads, max_len, head_dim]", 4)
         n_seqs, n_kv, lmax, hd = k.shape
-        dev = k.device
-        _need(v, "v cache", f32, tuple(k.shape), device=dev)
-    _need(qkv, "qkv", f32, (-1, (n_heads + 2 * n_kv) * hd), contiguous=False, device=dev)
+        dev = k.get_device()
+        _need(v, "v cache", _F32, k.shape, dev)
+        planes, fn = (k.data_ptr(), v.data_ptr()), _cabi.lib().kb_qknorm_rope_kv
+    _need(qkv, "qkv", _F32, None, dev, False)
+    _dims(qkv, "qkv", "[n, width]", 2)
     n, width = qkv.shape
-    if width and qkv.stride(1) != 1 or (n > 1 and qkv.stride(0) < width):
+    if width != (n_heads + 2 * n_kv) * hd:
+        raise KoreError(_cabi.ERR_SHAPE, f"qkv: shape mismatch: expected [{n}, {(n_heads + 2 * n_kv) * hd}], got {list(qkv.shape)}")
+    if not qkv.is_contiguous() and (qkv.stride(1) != 1 or (n > 1 and qkv.stride(0) < width)):
         qkv = qkv.contiguous()
-    ld = qkv.stride(0) if n > 1 else width
-    _need(positions, "positions", torch.int32, (n,), device=dev)
-    _need(cache_rows, "cache_rows", torch.int64, (n,), device=dev)
-    _need(cos, "cos", f32, (-1, hd // 2), device=dev)
-    _need(sin, "sin", f32, tuple(cos.shape), device=dev)
-    for g, name in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
-        if g is not None:
-            _need(g, name, f32, (hd,), device=dev)
+    _need(positions, "positions", _I32, (n,), dev)
+    _need(cache_rows, "cache_rows", _I64, (n,), dev)
+    max_pos = cos.shape[0] if isinstance(cos, torch.Tensor) and cos.dim() == 2 else 0
+    _need(cos, "cos", _F32, (max_pos, hd // 2), dev)
+    _need(sin, "sin", _F32, (max_pos, hd // 2), dev)
+    gq = None if q_gamma is None else _need(q_gamma, "q_gamma", _F32, (hd,), dev).data_ptr()
+    gk = None if k_gamma is None else _need(k_gamma, "k_gamma", _F32, (hd,), dev).data_ptr()
     if q_out is None:
-        q_out = torch.empty((n, n_heads, hd), dtype=f32, device=dev)
+        q_out = torch.empty((n, n_heads, hd), dtype=_F32, device=qkv.device)
     else:
-        _need(q_out, "q_out", f32, (n, n_heads, hd), device=dev)
-    if n == 0:
-        return q_out
-    planes = cache._planes if four else (k.data_ptr(), v.data_ptr())
-    fn = _cabi.lib().kb_qknorm_rope_kv4 if four else _cabi.lib().kb_qknorm_rope_kv
-    with _on(dev):
-        _cabi.check(fn(qkv.data_ptr(), ld, positions.data_ptr(), cache_rows.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-                       None if q_gamma is None else q_gamma.data_ptr(), None if k_gamma is None else k_gamma.data_ptr(),
-                       C.c_float(eps), n, n_heads, n_kv, hd, n_seqs, lmax, q_out.data_ptr(), *planes, _stream(dev)))
+        _need(q_out, "q_out", _F32, (n, n_heads, hd), dev)
+    if n:
+        _run(dev, fn, qkv.data_ptr(), qkv.stride(0) if n > 1 else width, positions.data_ptr(), cache_rows.data_ptr(), cos.data_ptr(),
+             sin.data_ptr(), max_pos, gq, gk, eps, n, n_heads, n_kv, hd, n_seqs, lmax, q_out.data_ptr(), *planes)
     return q_out
 
 
@@ -162,27 +167,28 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     (or [n_seqs, n_heads, head_dim], t = 1), lens int32 [n_seqs] the cache positions up to and including the last of the t
     tokens.  Token i sees the positions below lens - (t - 1 - i); one that sees none gives zeros.  scale 0 is
     1 / sqrt(head_dim).  Returns float32 of q's shape."""
-    import torch
-
-    hd, dev = cache.head_dim, cache.device
-    _need(q, "q", torch.float32, (cache.n_seqs, -1, hd) if q.dim() == 3 else (cache.n_seqs, -1, -1, hd), contiguous=False, device=dev)
-    q = q.contiguous()
-    t, heads = (1, q.shape[1]) if q.dim() == 3 else (q.shape[1], q.shape[2])
-    _need(lens, "lens", torch.int32, (cache.n_seqs,), device=dev)
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        _need(out, "out", torch.float32, tuple(q.shape), device=dev)
-    if out.numel() == 0:
+    hd, dev, n = cache.head_dim, cache._dev, cache.n_seqs
+    _need(q, "q", _F32, None, dev, False)
+    shape = q.shape
+    if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != hd:
+        raise KoreError(_cabi.ERR_SHAPE, f"q: shape mismatch: expected [{n}, (t,) n_heads, {hd}], got {list(shape)}")
+    if not q.is_contiguous():
+        q = q.contiguous()
+    t, heads = (1, shape[1]) if len(shape) == 3 else (shape[1], shape[2])
+    _need(lens, "lens", _I32, (n,), dev)
+    out = torch.empty_like(q) if out is None else _need(out, "out", _F32, shape, dev)
+    if q.numel() == 0:
         return out
-    lib = _cabi.lib()
-    with _on(dev):
-        need = lib.kb_attn_kv4_workspace_bytes(cache.n_seqs, t, heads, cache.n_kv_heads, hd, cache.max_len)
-        # torch's allocator orders its reuse by stream and keeps a captured graph's blocks to that graph
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _cabi.check(lib.kb_attn_kv4(q.data_ptr(), *cache._planes, lens.data_ptr(), cache.n_seqs, t, heads, cache.n_kv_heads, hd,
-                                    cache.max_len, C.c_float(scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need,
-                                    _stream(dev)))
+    lib, ws = cache._lib, 0
+    need = cache._ws_bytes.get((t, heads))
+    if need is None:
+        with torch.cuda.device(dev):
+            need = cache._ws_bytes[t, heads] = lib.kb_attn_kv4_workspace_bytes(n, t, heads, cache.n_kv_heads, hd, cache.max_len)
+    if need:  # torch's allocator orders its reuse by stream and keeps a captured graph's blocks to that graph
+        block = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = block.data_ptr()
+    _run(dev, lib.kb_attn_kv4, q.data_ptr(), *cache._planes, lens.data_ptr(), n, t, heads, cache.n_kv_heads, hd, cache.max_len, scale,
+         out.data_ptr(), ws, need)
     return out
 
 
@@ -192,26 +198,22 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, r
     float32 [n], top_k int32 [n].  A temperature of 0 is greedy.  Top-k and min-p act on the tempered distribution, top-p
     on what they keep.  Returns int64 [n], with return_logprobs also float32 [n]: the log of the token's share of what was
     kept."""
-    import torch
-
-    f32 = torch.float32
-    _need(logits, "logits", f32, (-1, -1), contiguous=False)
-    dev = logits.device
-    n, vocab = logits.shape
-    if logits.stride(1) != 1 and vocab > 1 or (n > 1 and logits.stride(0) < vocab):
+    _need(logits, "logits", _F32, None, None, False)
+    _dims(logits, "logits", "[n, vocab]", 2)
+    n, vocab = shape = logits.shape
+    dev = logits.get_device()
+    if not logits.is_contiguous() and (logits.stride(1) != 1 or (n > 1 and logits.stride(0) < vocab)):
         logits = logits.contiguous()
-    _need(u, "u", f32, (n,), device=dev)
-    ptrs = []
-    for t, name, dt in ((temperature, "temperature", f32), (top_k, "top_k", torch.int32), (top_p, "top_p", f32), (min_p, "min_p", f32)):
-        ptrs.append(None if t is None else _need(t, name, dt, (n,), device=dev).data_ptr())
-    if tokens is None:
-        tokens = torch.empty(n, dtype=torch.int64, device=dev)
-    else:
-        _need(tokens, "tokens", torch.int64, (n,), device=dev)
-    logprobs = torch.empty(n, dtype=f32, device=dev) if return_logprobs else None
-    if n == 0:
-        return (tokens, logprobs) if return_logprobs else tokens
-    with _on(dev):
-        _cabi.check(_cabi.lib().kb_sample(logits.data_ptr(), n, vocab, logits.stride(0) if n > 1 else vocab, *ptrs, u.data_ptr(),
-                                          tokens.data_ptr(), None if logprobs is None else logprobs.data_ptr(), _stream(dev)))
+    row = shape[:1]
+    _need(u, "u", _F32, row, dev)
+    # the tensors stay referenced by the arguments until the launch: a freed one could be handed out again just below
+    pt = None if temperature is None else _need(temperature, "temperature", _F32, row, dev).data_ptr()
+    pk = None if top_k is None else _need(top_k, "top_k", _I32, row, dev).data_ptr()
+    pp = None if top_p is None else _need(top_p, "top_p", _F32, row, dev).data_ptr()
+    pm = None if min_p is None else _need(min_p, "min_p", _F32, row, dev).data_ptr()
+    tokens = torch.empty(row, dtype=_I64, device=logits.device) if tokens is None else _need(tokens, "tokens", _I64, row, dev)
+    logprobs = torch.empty(row, dtype=_F32, device=logits.device) if return_logprobs else None
+    if n:
+        _run(dev, _cabi.lib().kb_sample, logits.data_ptr(), n, vocab, logits.stride(0) if n > 1 else vocab, pt, pk, pp, pm,
+             u.data_ptr(), tokens.data_ptr(), logprobs.data_ptr() if return_logprobs else None)
     return (tokens, logprobs) if return_logprobs else tokens
