@@ -7,10 +7,15 @@
 //
 // Bound by the latency of the passes for a few rows and by the f64 exponentials for many (a logit is read once).  A row
 // belongs to a cluster of 1 to 8 CTAs, each with a slice of it in shared memory.  Top-k and top-p look for the element at
-// which a running measure (count, or weight) reaches a target: a histogram over 1024 steps of 1/32 in the exponent gives
-// the bin, the candidates of that bin (a few dozen of 32000 normal logits) are collected, sorted and summed by every CTA
-// alike.  A bin of more than SAMPLE_CAND candidates (ties, flat rows) is cut into 1024 parts of the order first, again and
-// again.  The draw sums the kept weights by segment and walks the one that holds the number.
+// which a running measure (count, or weight) reaches a target:
+//   1. a histogram over 1024 steps of 1/32 in the exponent.  Counts are exact.  Of a weight only its share of its bin's
+//      largest, in 16 bits, goes through an atomic (the sum of a bin is good to 2^-15), while threads add up the exact
+//      total: the bins that may hold the border are then known, one or two of them;
+//   2. their elements (a few dozen of 32000 normal logits) are collected and what lies before them is summed exactly;
+//   3. every CTA finds the element among the candidates by counting.
+// Where there are more candidates than SAMPLE_CAND (ties, flat rows), the part of the order that they span is cut into 1024
+// bins of exact 64-bit sums first, again and again.  The draw sums the kept weights by segment and walks the one that holds
+// the number.
 #include <math.h>
 #include <stdlib.h>
 
@@ -25,7 +30,7 @@ using u64 = unsigned long long;
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_BINS = 1024;
-constexpr int SAMPLE_CAND = 2048;
+constexpr int SAMPLE_CAND = 1024;
 constexpr int SAMPLE_CTAS = 8;  // of a cluster, at most
 constexpr int SAMPLE_SLICE = 40960;  // logits of a slice that shared memory holds (160 KB); a longer slice is read from L2
 constexpr size_t SAMPLE_MAX_VOCAB = (size_t)1 << 19;
@@ -42,12 +47,12 @@ struct SampleParams {
 };
 
 struct SampleShared {
-    u64 slot[8][SAMPLE_CTAS];  // one row per reduction over the cluster
+    u64 slot[8][SAMPLE_CTAS];  // one row per exchange between the CTAs
     u64 scratch[SAMPLE_WARPS];
-    uint32_t hist_lo[SAMPLE_BINS], hist_hi[SAMPLE_BINS];  // 64-bit sums in two words: 64-bit shared atomics are compare-and-swap loops
-    u64 own[SAMPLE_CAND], all[SAMPLE_CAND];
+    uint32_t hist[2][SAMPLE_BINS];  // counts or shares; 64-bit sums take both (64-bit shared atomics are compare-and-swap loops)
+    u64 own[SAMPLE_CAND], all[SAMPLE_CAND], measure[SAMPLE_CAND];
     uint32_t n_own;
-    int bin;
+    int bin[2];
     u64 before, found;
 };
 
@@ -84,9 +89,9 @@ __device__ __forceinline__ u64 exp2_fixed(double y) {
     return (u64)__double_as_longlong(v + 0x1p52) & ((1ull << 52) - 1);
 }
 
-__device__ __forceinline__ uint32_t ld_cluster(const uint32_t *p, uint32_t rank) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ptx::mapa(ptx::smem_u32(p), rank)) : "memory");
+__device__ __forceinline__ uint2 ld_cluster(const uint2 *p, uint32_t rank) {
+    uint2 v;
+    asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(ptx::mapa(ptx::smem_u32(p), rank)) : "memory");
     return v;
 }
 __device__ __forceinline__ u64 ld_cluster(const u64 *p, uint32_t rank) {
@@ -97,10 +102,13 @@ __device__ __forceinline__ u64 ld_cluster(const u64 *p, uint32_t rank) {
 __device__ __forceinline__ void st_cluster(u64 *p, uint32_t rank, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ptx::mapa(ptx::smem_u32(p), rank)), "l"(v) : "memory");
 }
+__device__ __forceinline__ u64 least(u64 a, u64 b) { return a < b ? a : b; }
+__device__ __forceinline__ u64 plus(u64 a, u64 b) { return a + b; }
 
 struct Row {
     SampleShared &sh;
-    const float *l;  // this CTA's slice: shared memory, or the logits themselves
+    const float *l;  // this CTA's slice: shared memory (filled up with -inf to a multiple of 4), or the logits themselves
+    bool held;
     int n, i0;       // its length and its first index
     uint32_t rank, ctas;
     float top;       // largest logit
@@ -111,9 +119,29 @@ struct Row {
         if (top == INFINITY) return x == top ? 1ull << 44 : 0ull;
         return exp2_fixed(((double)x - (double)top) * per);
     }
-    __device__ __forceinline__ int bin_of(float x) const {  // falls with x
-        return x == top ? 0 : (int)fminf((top - x) * bins, (float)(SAMPLE_BINS - 1));
+    __device__ __forceinline__ float bin_at(float x) const {  // falls with x
+        return x == top ? 0.0f : fminf((top - x) * bins, (float)(SAMPLE_BINS - 1));
     }
+    __device__ __forceinline__ int bin_of(float x) const { return (int)bin_at(x); }
+
+    // f(logit, index) of the slice's elements i0 + 4 i .. + 3 for i = first, first + stride, ..: whole warps where `first` is
+    // the thread's; elements behind the slice are -inf with indices behind every real one
+    template <typename F>
+    __device__ __forceinline__ void each4(int first, int stride, int end, F f) const {
+        for (int i = first; i < end; i += stride) {
+            float x[4];
+            if (held) {
+                const float4 v = reinterpret_cast<const float4 *>(l)[i];
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? l[4 * i + k] : -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f(clean(x[k]), i0 + 4 * i + k, k);
+        }
+    }
+    __device__ __forceinline__ int quads() const { return (n + 3) / 4; }
 
     template <typename F>
     __device__ __forceinline__ u64 block_reduce(u64 v, F f) const {
@@ -127,201 +155,262 @@ struct Row {
         for (int o = SAMPLE_WARPS / 2; o > 0; o >>= 1) r = f(r, __shfl_xor_sync(0xffffffffu, r, o));
         return r;
     }
-    // every CTA's value, then the join of all; `id` names a slot that no other reduction of the row still uses
-    __device__ __forceinline__ void exchange(u64 v, int id) const {
+    // this CTA's value into slot `id` of every CTA (visible behind the next cluster_sync); an id is written again only when a
+    // cluster_sync lies between its last reading and that
+    __device__ __forceinline__ void tell(u64 v, int id) const {
         if (threadIdx.x < ctas) st_cluster(&sh.slot[id][rank], threadIdx.x, v);
-        ptx::cluster_sync();
     }
     template <typename F>
-    __device__ __forceinline__ u64 cluster_reduce(u64 v, int id, F f) const {
-        exchange(block_reduce(v, f), id);
+    __device__ __forceinline__ u64 told(int id, F f) const {
         u64 r = sh.slot[id][0];
         for (uint32_t c = 1; c < ctas; ++c) r = f(r, sh.slot[id][c]);
         return r;
     }
+    template <typename F>
+    __device__ __forceinline__ u64 cluster_reduce(u64 v, int id, F f) const {
+        tell(block_reduce(v, f), id);
+        ptx::cluster_sync();
+        return told(id, f);
+    }
     // inclusive sum over the threads
-    __device__ __forceinline__ u64 block_scan(u64 v, u64 &total) const {
+    template <typename T>
+    __device__ __forceinline__ T block_scan(T v, T &total) const {
+        static_assert(sizeof(T) == 8, "");
+        T *scratch = reinterpret_cast<T *>(sh.scratch);
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+            const T up = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += up;
         }
         __syncthreads();
-        if (lane == 31) sh.scratch[warp] = v;
+        if (lane == 31) scratch[warp] = v;
         __syncthreads();
         total = 0;
-        u64 base = 0;
+        T base = 0;
 #pragma unroll
         for (int w = 0; w < SAMPLE_WARPS; ++w) {
             if (w == warp) base = total;
-            total += sh.scratch[w];
+            total += scratch[w];
         }
         return v + base;
     }
-    __device__ __forceinline__ void hist_add(int b, u64 m) const {
-        const uint32_t old = atomicAdd(sh.hist_lo + b, (uint32_t)m);
+    // a whole warp adds; -1: nothing to add
+    __device__ __forceinline__ bool same_bin(int b) const { return __all_sync(0xffffffffu, b == __shfl_sync(0xffffffffu, b, 0)); }
+    __device__ __forceinline__ void hist_add(int b, uint32_t m) const {
+        if (same_bin(b)) {  // ties and flat rows: one addition for the warp
+            m = __reduce_add_sync(0xffffffffu, m);
+            if ((threadIdx.x & 31) == 0 && b >= 0) atomicAdd(sh.hist[0] + b, m);
+        } else if (b >= 0) {
+            atomicAdd(sh.hist[0] + b, m);
+        }
+    }
+    __device__ __forceinline__ void hist_add64(int b, u64 m) const {
+        if (b < 0) return;
+        const uint32_t old = atomicAdd(sh.hist[0] + b, (uint32_t)m);
         const uint32_t hi = (uint32_t)(m >> 32) + (old + (uint32_t)m < old ? 1u : 0u);
-        if (hi) atomicAdd(sh.hist_hi + b, hi);
+        if (hi) atomicAdd(sh.hist[1] + b, hi);
+    }
+    __device__ __forceinline__ void hist_clear() const {
+        for (int b = threadIdx.x; b < 2 * SAMPLE_BINS; b += SAMPLE_THREADS) sh.hist[0][b] = 0;
+        __syncthreads();
+    }
+    // bins 2t and 2t + 1 of word array h over the whole row
+    __device__ __forceinline__ void hist_row(int h, u64 (&out)[2]) const {
+        static_assert(SAMPLE_BINS == 2 * SAMPLE_THREADS, "two bins a thread");
+        uint2 v[SAMPLE_CTAS];
+#pragma unroll
+        for (int c = 0; c < SAMPLE_CTAS; ++c)  // all loads under way before the first sum
+            if (c < (int)ctas) v[c] = ld_cluster(reinterpret_cast<const uint2 *>(sh.hist[h]) + threadIdx.x, c);
+        out[0] = out[1] = 0;
+#pragma unroll
+        for (int c = 0; c < SAMPLE_CTAS; ++c)
+            if (c < (int)ctas) {
+                out[0] += v[c].x;
+                out[1] += v[c].y;
+            }
+    }
+    // the bin of a running sum that reaches target, and the sum before it
+    __device__ __forceinline__ void find_bin(const u64 (&mine)[2], u64 target) const {
+        u64 total;
+        u64 upto = block_scan(mine[0] + mine[1], total);
+#pragma unroll
+        for (int k = 1; k >= 0; --k) {
+            if (upto - mine[k] < target && target <= upto) {
+                sh.bin[0] = sh.bin[1] = 2 * threadIdx.x + k;
+                sh.before = upto - mine[k];
+            }
+            upto -= mine[k];
+        }
     }
 
     // The element (its comp) at which the measure of the elements kept by `bound`, added up in order, reaches
     // target(measure of all); WEIGHT: measure = weight, otherwise 1.  Where that is a matter of weights of 0: ~0.
     template <bool WEIGHT, typename T>
     __device__ u64 reach(u64 bound, T target_of) const {
-        u64 lo = 0, hi = ~0ull, target = 0;
-        int shift = 0;
-        for (int level = 0;; ++level) {
-            for (int b = threadIdx.x; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.hist_lo[b] = sh.hist_hi[b] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += SAMPLE_THREADS) {  // whole warps
-                const float x = i < n ? clean(l[i]) : 0.0f;
-                const u64 c = comp_of(x, i0 + i);
-                const bool in = i < n && c <= bound && c >= lo && c <= hi;
-                const u64 m = !in ? 0ull : (WEIGHT ? weight(x) : 1ull);
-                const int b = !m ? -1 : (level == 0 ? bin_of(x) : (int)((c - lo) >> shift));
-                const int b0 = __shfl_sync(0xffffffffu, b, 0);
-                if (b0 >= 0 && __all_sync(0xffffffffu, b == b0)) {  // ties and flat rows: one addition for the warp
-                    u64 sum = m;
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if ((threadIdx.x & 31) == 0) hist_add(b0, sum);
-                } else if (b >= 0) {
-                    hist_add(b, m);
-                }
+        u64 target, sum = 0;
+        hist_clear();
+        if (threadIdx.x == 0) sh.bin[0] = sh.bin[1] = SAMPLE_BINS - 1;
+        // whole warps go around: the additions vote
+        each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](float x, int i, int) {
+            const bool in = i < i0 + n && comp_of(x, i) <= bound;
+            const float at = bin_at(x);
+            const int b = (int)at;
+            uint32_t m = 1;
+            if (WEIGHT) {
+                sum += in ? weight(x) : 0ull;
+                // share of the bin's largest weight: 2^(-fraction / 32 log2 e) in 16 bits
+                m = __float2uint_rn(65535.0f * exp2f((at - (float)b) * (-1.4426950408889634f * 32 / SAMPLE_BINS)));
             }
-            ptx::cluster_sync();
-            // thread t: bins 2t and 2t + 1 of the whole row
-            u64 mine[2] = {};
-            for (uint32_t c = 0; c < ctas; ++c)
+            hist_add(in && (!WEIGHT || b < SAMPLE_BINS - 1) ? b : -1, m);
+        });
+        if (WEIGHT) tell(block_reduce(sum, plus), 3);
+        ptx::cluster_sync();
+        u64 mine[2];
+        hist_row(0, mine);
+        if (threadIdx.x == 0) sh.n_own = 0;
+        if (WEIGHT) {
+            // sums of shares are off by less than 2^-15: the border lies in the bins that reach target - slack .. target + slack
+            const u64 all = told(3, plus);
+            target = target_of(all);
+            const double aim = (double)target * 0x1p-44, slack = (double)all * 0x1p-58;
+            double w[2], total;
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    mine[k] += (u64)ld_cluster(sh.hist_hi + 2 * threadIdx.x + k, c) << 32 | ld_cluster(sh.hist_lo + 2 * threadIdx.x + k, c);
-            u64 total;
-            u64 upto = block_scan(mine[0] + mine[1], total);
-            if (level == 0) target = target_of(total);
-            if (threadIdx.x == 0) sh.n_own = 0;
+            for (int k = 0; k < 2; ++k)
+                w[k] = (double)mine[k] * (1.0 / 65535) * (double)exp2f((float)(2 * threadIdx.x + k) * (-1.4426950408889634f * 32 / SAMPLE_BINS));
+            double upto = block_scan(w[0] + w[1], total);
 #pragma unroll
             for (int k = 1; k >= 0; --k) {
-                if (upto - mine[k] < target && target <= upto) {
-                    sh.bin = 2 * threadIdx.x + k;
-                    sh.before = upto - mine[k];
-                }
-                upto -= mine[k];
+                if (upto - w[k] < aim - slack && aim - slack <= upto) sh.bin[0] = 2 * threadIdx.x + k;
+                if (upto - w[k] < aim + slack && aim + slack <= upto) sh.bin[1] = 2 * threadIdx.x + k;
+                upto -= w[k];
             }
-            __syncthreads();
-            const int bin = sh.bin;
+            if (threadIdx.x == 0 && aim - slack <= 0.0) sh.bin[0] = 0;
+        } else {
+            target = target_of(0);
+            find_bin(mine, target);
+        }
+        __syncthreads();
+        const int b0 = sh.bin[0], b1 = sh.bin[1];
+        if (!WEIGHT) {
             target -= sh.before;
-            if (!WEIGHT && level == 0 && bin == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
-                ptx::cluster_sync();  // the histograms have been read
+            if (b0 == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
+                ptx::cluster_sync();      // the histograms have been read
                 return ~0ull;
             }
-            if (level > 0) {
-                lo += (u64)bin << shift;
-                hi = min(hi, lo + ((1ull << shift) - 1));
-            }
-            u64 first = ~0ull, last = ~0ull;
-            for (int i = threadIdx.x; i < n; i += SAMPLE_THREADS) {
-                const float x = clean(l[i]);
-                const u64 c = comp_of(x, i0 + i);
-                if (c <= bound && c >= lo && c <= hi && (level > 0 || bin_of(x) == bin)) {
-                    const uint32_t at = atomicAdd(&sh.n_own, 1u);
-                    if (at < SAMPLE_CAND) sh.own[at] = c;
-                    first = min(first, c);
-                    last = min(last, ~c);
-                }
-            }
-            ptx::cluster_sync();
-            uint32_t count = 0;
-            for (uint32_t c = 0; c < ctas; ++c) {
-                const uint32_t m = ld_cluster(&sh.n_own, c);
-                if (count + m <= SAMPLE_CAND)
-                    for (uint32_t i = threadIdx.x; i < m; i += SAMPLE_THREADS) sh.all[count + i] = ld_cluster(sh.own + i, c);
-                count = count + m <= SAMPLE_CAND ? count + m : SAMPLE_CAND + 1;
-            }
-            if (count <= SAMPLE_CAND) return pick<WEIGHT>(count, target);
-            // too many: the part of the order that they span, cut into bins
-            const auto least = [](u64 a, u64 b) { return a < b ? a : b; };
-            lo = cluster_reduce(first, 4 + 2 * (level & 1), least);
-            hi = ~cluster_reduce(last, 5 + 2 * (level & 1), least);
-            shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
         }
-    }
-    // of the candidates in sh.all the one at which their measure, added up in order, reaches target
-    template <bool WEIGHT>
-    __device__ u64 pick(uint32_t count, u64 target) const {
-        uint32_t size = 2;
-        while (size < count) size *= 2;
-        for (uint32_t i = count + threadIdx.x; i < size; i += SAMPLE_THREADS) sh.all[i] = ~0ull;
+        u64 lo = ~0ull, hi = 0;
+        sum = 0;
+        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](float x, int i, int) {
+            const u64 c = comp_of(x, i);
+            if (i >= i0 + n || c > bound) return;
+            const int b = bin_of(x);
+            if (WEIGHT && b < b0) sum += weight(x);
+            if (b >= b0 && b <= b1) {
+                const uint32_t at = atomicAdd(&sh.n_own, 1u);
+                if (at < SAMPLE_CAND) sh.own[at] = c;
+                lo = min(lo, c);
+                hi = max(hi, c);
+            }
+        });
+        if (WEIGHT) tell(block_reduce(sum, plus), 4);
         __syncthreads();
-        for (uint32_t k = 2; k <= size; k *= 2)  // bitonic sort
-            for (uint32_t j = k / 2; j > 0; j /= 2) {
-                for (uint32_t p = threadIdx.x; p < size / 2; p += SAMPLE_THREADS) {
-                    const uint32_t a = 2 * p - (p & (j - 1)), b = a + j;
-                    const u64 x = sh.all[a], y = sh.all[b];
-                    if ((x > y) == ((a & k) == 0)) {
-                        sh.all[a] = y;
-                        sh.all[b] = x;
-                    }
-                }
-                __syncthreads();
+        tell(sh.n_own, 5);
+        ptx::cluster_sync();
+        if (WEIGHT) target -= told(4, plus);
+        const u64 count = told(5, plus);
+        if (count <= SAMPLE_CAND) {
+            uint32_t c = 0;
+            u64 base = 0;
+            for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
+                while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
+                const u64 e = ld_cluster(sh.own + (i - base), c);
+                sh.all[i] = e;
+                sh.measure[i] = WEIGHT ? weight(logit_of(e)) : 1ull;
             }
-        constexpr int PER = SAMPLE_CAND / SAMPLE_THREADS;
-        u64 m[PER], mine = 0, total;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const uint32_t i = PER * threadIdx.x + k;
-            m[k] = i < count ? (WEIGHT ? weight(logit_of(sh.all[i])) : 1ull) : 0ull;
-            mine += m[k];
+            return pick((uint32_t)count, target);
         }
-        u64 upto = block_scan(mine, total) - mine;
+        // too many: the part of the order that they span, cut into bins of 64-bit sums until one element is left
+        lo = cluster_reduce(lo, 6, least);
+        hi = ~cluster_reduce(~hi, 7, least);
+        while (lo < hi) {
+            const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
+            hist_clear();
+            each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](float x, int i, int) {
+                const u64 c = comp_of(x, i);
+                const bool in = i < i0 + n && c <= bound && c >= lo && c <= hi;
+                u64 m = !in ? 0ull : (WEIGHT ? weight(x) : 1ull);
+                int b = m ? (int)((c - lo) >> shift) : -1;
+                if (same_bin(b)) {
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            if (upto < target && target <= upto + m[k]) sh.found = sh.all[PER * threadIdx.x + k];
-            upto += m[k];
+                    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+                    if (threadIdx.x & 31) b = -1;
+                }
+                hist_add64(b, m);
+            });
+            ptx::cluster_sync();
+            u64 high[2];
+            hist_row(0, mine);
+            hist_row(1, high);
+            mine[0] += high[0] << 32;
+            mine[1] += high[1] << 32;
+            find_bin(mine, target);
+            __syncthreads();
+            target -= sh.before;
+            lo += (u64)sh.bin[0] << shift;
+            hi = min(hi, lo + ((1ull << shift) - 1));
+            ptx::cluster_sync();  // the histograms have been read
+        }
+        return lo;
+    }
+    // of the candidates in sh.all the one at which their measure, added up in order, reaches target: several threads add up
+    // what lies before a candidate
+    __device__ u64 pick(uint32_t count, u64 target) const {
+        uint32_t per = 1;  // threads per candidate
+        while (per < 32 && 2 * per * count <= SAMPLE_THREADS) per *= 2;
+        __syncthreads();
+        for (uint32_t i0_ = 0; i0_ < count; i0_ += SAMPLE_THREADS / per) {
+            const uint32_t i = i0_ + threadIdx.x / per;
+            const u64 c = i < count ? sh.all[i] : 0ull;
+            u64 before = 0;
+            for (uint32_t j = threadIdx.x % per; j < count; j += per) before += sh.all[j] < c ? sh.measure[j] : 0ull;
+            for (uint32_t o = per / 2; o > 0; o /= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
+            if (i < count && before < target && target <= before + sh.measure[i]) sh.found = c;
         }
         __syncthreads();
         return sh.found;
     }
 };
 
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleParams p) {
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     uint32_t ctas;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t r = blockIdx.x / ctas;
-    Row row = {sh, nullptr, 0, 0, ptx::cluster_ctarank(), ctas, 0.0f, 0.0, 0.0f};
+    Row row = {sh, nullptr, p.slice <= SAMPLE_SLICE, 0, 0, ptx::cluster_ctarank(), ctas, 0.0f, 0.0, 0.0f};
     row.i0 = min(p.vocab, (int)row.rank * p.slice);
     row.n = min(p.slice, p.vocab - row.i0);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float *src = p.logits + r * p.ld + row.i0;
-    float *held = reinterpret_cast<float *>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
-    const bool hold = p.slice <= SAMPLE_SLICE;
-    row.l = hold ? held : src;
-    u64 best = ~0ull;
-    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        for (int i = threadIdx.x; i < row.n / 4; i += SAMPLE_THREADS) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src) + i);
-            if (hold) reinterpret_cast<float4 *>(held)[i] = v;
-            best = min(min(best, min(comp_of(clean(v.x), row.i0 + 4 * i), comp_of(clean(v.y), row.i0 + 4 * i + 1))),
-                       min(comp_of(clean(v.z), row.i0 + 4 * i + 2), comp_of(clean(v.w), row.i0 + 4 * i + 3)));
-        }
-        for (int i = (row.n & ~3) + threadIdx.x; i < row.n; i += SAMPLE_THREADS) {
-            const float v = __ldcg(src + i);
-            if (hold) held[i] = v;
-            best = min(best, comp_of(clean(v), row.i0 + i));
-        }
-    } else {
-        for (int i = threadIdx.x; i < row.n; i += SAMPLE_THREADS) {
-            const float v = __ldcg(src + i);
-            if (hold) held[i] = v;
-            best = min(best, comp_of(clean(v), row.i0 + i));
-        }
+    row.l = src;
+    if (row.held) {
+        float *held = reinterpret_cast<float *>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
+        row.l = held;
+        const int body = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? row.n / 4 : 0;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < body; i += SAMPLE_THREADS)
+            reinterpret_cast<float4 *>(held)[i] = __ldcg(reinterpret_cast<const float4 *>(src) + i);
+#pragma unroll 4
+        for (int i = 4 * body + threadIdx.x; i < 4 * row.quads(); i += SAMPLE_THREADS) held[i] = i < row.n ? __ldcg(src + i) : -INFINITY;
+        for (int i = 4 * row.quads() + threadIdx.x; i < 4 * ((row.quads() + 31) & ~31); i += SAMPLE_THREADS) held[i] = -INFINITY;
+        __syncthreads();
     }
-    const auto least = [](u64 a, u64 b) { return a < b ? a : b; };
+    // the largest logit, and of equal ones the first
+    u64 best = ~0ull;
+    row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int i, int) { best = min(best, comp_of(x, i)); });
     best = row.cluster_reduce(best, 0, least);
     row.top = logit_of(best);
     const float temp = p.temperature ? p.temperature[r] : 1.0f;
@@ -342,10 +431,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleParams p) 
     if (mp > 0.0f) {
         const double border = log((double)fminf(mp, 1.0f));
         u64 out = ~0ull;  // the first element below the border
-        for (int i = threadIdx.x; i < row.n; i += SAMPLE_THREADS) {
-            const float x = clean(row.l[i]);
-            if (x != row.top && !(((double)x - (double)row.top) * inv_t >= border)) out = min(out, comp_of(x, row.i0 + i));
-        }
+        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int i, int) {
+            if (x != row.top && !(((double)x - (double)row.top) * inv_t >= border)) out = min(out, comp_of(x, i));
+        });
         out = row.cluster_reduce(out, 1, least);
         if (out != ~0ull) bound = min(bound, out - 1);
     }
@@ -353,13 +441,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleParams p) 
     if (tp < 1.0f)
         bound = row.reach<true>(bound, [&](u64 z) { return min(max((u64)ceil((double)fmaxf(tp, 0.0f) * (double)z), 1ull), z); });
     // ---- the draw: warps sum contiguous segments, the segment that holds the number is walked in index order
-    const int seg = (row.n + SAMPLE_WARPS - 1) / SAMPLE_WARPS, s0 = min(row.n, warp * seg), s1 = min(row.n, s0 + seg);
-    auto kept = [&](int i) {
-        const float x = clean(row.l[i]);
-        return comp_of(x, row.i0 + i) <= bound ? row.weight(x) : 0ull;
-    };
+    const int seg = (row.quads() + SAMPLE_WARPS - 1) / SAMPLE_WARPS, s0 = min(row.quads(), warp * seg), s1 = min(row.quads(), s0 + seg);
     u64 s = 0;
-    for (int i = s0 + lane; i < s1; i += 32) s += kept(i);
+    row.each4(s0 + lane, 32, s1, [&](float x, int i, int) { s += comp_of(x, i) <= bound ? row.weight(x) : 0ull; });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     __syncthreads();
@@ -370,7 +454,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleParams p) 
         if (w < warp) before += sh.scratch[w];
         mine += sh.scratch[w];
     }
-    row.exchange(mine, 2);  // nothing of another CTA is read from here on
+    row.tell(mine, 2);
+    ptx::cluster_sync();  // nothing of another CTA is read from here on
     for (uint32_t c = 0; c < ctas; ++c) {
         if (c < row.rank) before += sh.slot[2][c];
         z += sh.slot[2][c];
@@ -380,8 +465,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleParams p) 
     draw = min(draw, z - 1);
     if (draw < before || draw >= before + s) return;  // one warp of the cluster goes on
     for (int i = s0; i < s1; i += 32) {
-        const u64 w = i + lane < s1 ? kept(i + lane) : 0ull;
-        u64 inc = w;
+        u64 w[4] = {}, inc = 0;
+        float x[4];
+        row.each4(i + lane, 32, min(s1, i + 32), [&](float v, int at, int k) {
+            x[k] = v;
+            w[k] = comp_of(v, at) <= bound ? row.weight(v) : 0ull;
+            inc += w[k];
+        });
+        const u64 own = inc;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 up = __shfl_up_sync(0xffffffffu, inc, o);
@@ -389,13 +480,17 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(SampleParams p) 
         }
         const u64 all = __shfl_sync(0xffffffffu, inc, 31);
         if (draw < before + all) {
-            if (draw >= before + inc - w && draw < before + inc) {
-                p.tokens[r] = row.i0 + i + lane;
-                if (p.logprobs) {
-                    const float x = clean(row.l[i + lane]);
-                    const double e = x == row.top ? 0.0 : ((double)x - (double)row.top) * inv_t;
-                    p.logprobs[r] = (float)(e - log((double)z * 0x1p-44));
+            u64 at = before + inc - own;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (draw >= at && draw < at + w[k]) {
+                    p.tokens[r] = row.i0 + 4 * (i + lane) + k;
+                    if (p.logprobs) {
+                        const double e = x[k] == row.top ? 0.0 : ((double)x[k] - (double)row.top) * inv_t;
+                        p.logprobs[r] = (float)(e - log((double)z * 0x1p-44));
+                    }
                 }
+                at += w[k];
             }
             return;
         }
@@ -425,7 +520,7 @@ extern "C" int kb_sample(const float *logits, size_t n, size_t vocab, size_t ld,
     const int slice = (int)(((vocab + ctas - 1) / ctas + 3) / 4 * 4);
     SampleParams p = {logits, ld, (int)vocab, slice, temperature, top_k, top_p, min_p, u, tokens, logprobs};
     const size_t fixed = (sizeof(SampleShared) + 15) / 16 * 16;
-    const size_t smem = fixed + (slice <= SAMPLE_SLICE ? (size_t)slice * 4 : 0);
+    const size_t smem = fixed + (slice <= SAMPLE_SLICE ? (size_t)((slice + 127) / 128 * 128) * 4 : 0);
     if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(sample_kernel), dev, (int)(fixed + SAMPLE_SLICE * 4), "sample smem attribute")) return rc;
     static const bool pdl = [] { const char *v = getenv("KB_GEMV_PDL"); return !(v && *v == '0'); }();
     cudaLaunchConfig_t cfg = {};
