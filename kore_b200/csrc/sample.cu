@@ -1,7 +1,7 @@
 // Sampling one token per row of logits from one given uniform number (sm_100a); semantics in include/kore_b200.h.
 //
 // Every filter keeps a prefix of the order (logit descending, index ascending).  As an unsigned 64-bit number that order
-// is comp = ~ordered_bits(logit) << 32 | index, so the kept set is "comp <= bound" and a filter only lowers the bound.
+// is comp = ~ordered_bits(logit) << 32 | index; the kept set is "a logit above x, or equal to it up to index i".
 // Weights are integers of 2^-44 (the largest is 2^44, 2^19 of them fit 63 bits): their sums do not depend on the order in
 // which atomics arrive, and a token's border moves by at most vocab 2^-45 of the largest weight.
 //
@@ -56,10 +56,11 @@ struct SampleShared {
     u64 before, found;
 };
 
-__device__ __forceinline__ float clean(float l) { return l == l ? l : -INFINITY; }
-// position in the order: smaller is earlier
+// NaN counts as -inf, -0 is +0
+__device__ __forceinline__ float clean(float l) { return l == l ? l + 0.0f : -INFINITY; }
+// position in the order of a clean logit: smaller is earlier
 __device__ __forceinline__ u64 comp_of(float l, int idx) {
-    uint32_t b = __float_as_uint(l == 0.0f ? 0.0f : l);  // -0 and +0 are equal logits
+    uint32_t b = __float_as_uint(l);
     b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
     return ((u64)(~b) << 32) | (uint32_t)idx;
 }
@@ -105,9 +106,20 @@ __device__ __forceinline__ void st_cluster(u64 *p, uint32_t rank, u64 v) {
 __device__ __forceinline__ u64 least(u64 a, u64 b) { return a < b ? a : b; }
 __device__ __forceinline__ u64 plus(u64 a, u64 b) { return a + b; }
 
+// what the filters keep: logits above `least`, and those equal to it up to index `last`
+struct Kept {
+    float least = -INFINITY;
+    int last = 0x7fffffff;
+    __device__ __forceinline__ bool operator()(float x, int i) const { return x >= least && (x > least || i <= last); }
+    __device__ __forceinline__ void cut(float l, int i) {
+        if (l > least) least = l, last = i;
+        else if (l == least) last = min(last, i);
+    }
+};
+
 struct Row {
     SampleShared &sh;
-    const float *l;  // this CTA's slice: shared memory (filled up with -inf to a multiple of 4), or the logits themselves
+    const float *l;  // this CTA's slice: shared memory (clean, filled up with -inf), or the logits themselves
     bool held;
     int n, i0;       // its length and its first index
     uint32_t rank, ctas;
@@ -119,10 +131,11 @@ struct Row {
         if (top == INFINITY) return x == top ? 1ull << 44 : 0ull;
         return exp2_fixed(((double)x - (double)top) * per);
     }
-    __device__ __forceinline__ float bin_at(float x) const {  // falls with x
-        return x == top ? 0.0f : fminf((top - x) * bins, (float)(SAMPLE_BINS - 1));
+    // place in the histogram, 0 .. 1023, falling with x (fminf takes the number where inf - inf or 0 * inf give none)
+    __device__ __forceinline__ float bin_at(float x) const {
+        const float at = fminf((top - x) * bins, (float)(SAMPLE_BINS - 1));
+        return x == top ? 0.0f : at;
     }
-    __device__ __forceinline__ int bin_of(float x) const { return (int)bin_at(x); }
 
     // f(logit, index) of the slice's elements i0 + 4 i .. + 3 for i = first, first + stride, ..: whole warps where `first` is
     // the thread's; elements behind the slice are -inf with indices behind every real one
@@ -138,7 +151,7 @@ struct Row {
                 for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? l[4 * i + k] : -INFINITY;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f(clean(x[k]), i0 + 4 * i + k, k);
+            for (int k = 0; k < 4; ++k) f(held ? x[k] : clean(x[k]), i0 + 4 * i + k, k);
         }
     }
     __device__ __forceinline__ int quads() const { return (n + 3) / 4; }
@@ -195,16 +208,7 @@ struct Row {
         }
         return v + base;
     }
-    // a whole warp adds; -1: nothing to add
     __device__ __forceinline__ bool same_bin(int b) const { return __all_sync(0xffffffffu, b == __shfl_sync(0xffffffffu, b, 0)); }
-    __device__ __forceinline__ void hist_add(int b, uint32_t m) const {
-        if (same_bin(b)) {  // ties and flat rows: one addition for the warp
-            m = __reduce_add_sync(0xffffffffu, m);
-            if ((threadIdx.x & 31) == 0 && b >= 0) atomicAdd(sh.hist[0] + b, m);
-        } else if (b >= 0) {
-            atomicAdd(sh.hist[0] + b, m);
-        }
-    }
     __device__ __forceinline__ void hist_add64(int b, u64 m) const {
         if (b < 0) return;
         const uint32_t old = atomicAdd(sh.hist[0] + b, (uint32_t)m);
@@ -244,25 +248,25 @@ struct Row {
         }
     }
 
-    // The element (its comp) at which the measure of the elements kept by `bound`, added up in order, reaches
-    // target(measure of all); WEIGHT: measure = weight, otherwise 1.  Where that is a matter of weights of 0: ~0.
+    // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
+    // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.
     template <bool WEIGHT, typename T>
-    __device__ u64 reach(u64 bound, T target_of) const {
+    __device__ void cut(Kept &kept, T target_of) const {
         u64 target, sum = 0;
         hist_clear();
         if (threadIdx.x == 0) sh.bin[0] = sh.bin[1] = SAMPLE_BINS - 1;
-        // whole warps go around: the additions vote
-        each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](float x, int i, int) {
-            const bool in = i < i0 + n && comp_of(x, i) <= bound;
-            const float at = bin_at(x);
-            const int b = (int)at;
+        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](float x, int i, int) {
+            const bool in = kept(x, i) && i < i0 + n;
+            if (WEIGHT && in) sum += weight(x);
+            const float at = bin_at(x), magic = __fadd_rd(at, 0x1p23f);  // the floor, in the low bits
+            const int b = __float_as_int(magic) & (SAMPLE_BINS - 1);
             uint32_t m = 1;
             if (WEIGHT) {
-                sum += in ? weight(x) : 0ull;
-                // share of the bin's largest weight: 2^(-fraction / 32 log2 e) in 16 bits
-                m = __float2uint_rn(65535.0f * exp2f((at - (float)b) * (-1.4426950408889634f * 32 / SAMPLE_BINS)));
+                // share of the bin's largest weight in 16 bits: e^-z for z = fraction / 32, to z^3 / 6 < 2^-17
+                const float z = (at - (magic - 0x1p23f)) * (32.0f / SAMPLE_BINS);
+                m = __float_as_uint(fmaf(fmaf(z, fmaf(z, 0.5f, -1.0f), 1.0f), 65535.0f, 0x1p23f)) & 0xffffu;
             }
-            hist_add(in && (!WEIGHT || b < SAMPLE_BINS - 1) ? b : -1, m);
+            if (in && !(WEIGHT && b == SAMPLE_BINS - 1)) atomicAdd(sh.hist[0] + b, m);
         });
         if (WEIGHT) tell(block_reduce(sum, plus), 3);
         ptx::cluster_sync();
@@ -296,21 +300,23 @@ struct Row {
             target -= sh.before;
             if (b0 == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
                 ptx::cluster_sync();      // the histograms have been read
-                return ~0ull;
+                return;
             }
         }
         u64 lo = ~0ull, hi = 0;
         sum = 0;
+        const float from = (float)b0, to = (float)(b1 + 1);
         each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](float x, int i, int) {
-            const u64 c = comp_of(x, i);
-            if (i >= i0 + n || c > bound) return;
-            const int b = bin_of(x);
-            if (WEIGHT && b < b0) sum += weight(x);
-            if (b >= b0 && b <= b1) {
-                const uint32_t at = atomicAdd(&sh.n_own, 1u);
-                if (at < SAMPLE_CAND) sh.own[at] = c;
+            const float at = bin_at(x);
+            if (at >= to || !kept(x, i) || i >= i0 + n) return;
+            if (at >= from) {
+                const u64 c = comp_of(x, i);
+                const uint32_t slot = atomicAdd(&sh.n_own, 1u);
+                if (slot < SAMPLE_CAND) sh.own[slot] = c;
                 lo = min(lo, c);
                 hi = max(hi, c);
+            } else if (WEIGHT) {
+                sum += weight(x);
             }
         });
         if (WEIGHT) tell(block_reduce(sum, plus), 4);
@@ -328,7 +334,9 @@ struct Row {
                 sh.all[i] = e;
                 sh.measure[i] = WEIGHT ? weight(logit_of(e)) : 1ull;
             }
-            return pick((uint32_t)count, target);
+            const u64 found = pick((uint32_t)count, target);
+            kept.cut(logit_of(found), (int)(uint32_t)found);
+            return;
         }
         // too many: the part of the order that they span, cut into bins of 64-bit sums until one element is left
         lo = cluster_reduce(lo, 6, least);
@@ -338,7 +346,7 @@ struct Row {
             hist_clear();
             each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](float x, int i, int) {
                 const u64 c = comp_of(x, i);
-                const bool in = i < i0 + n && c <= bound && c >= lo && c <= hi;
+                const bool in = i < i0 + n && kept(x, i) && c >= lo && c <= hi;
                 u64 m = !in ? 0ull : (WEIGHT ? weight(x) : 1ull);
                 int b = m ? (int)((c - lo) >> shift) : -1;
                 if (same_bin(b)) {
@@ -361,7 +369,7 @@ struct Row {
             hi = min(hi, lo + ((1ull << shift) - 1));
             ptx::cluster_sync();  // the histograms have been read
         }
-        return lo;
+        kept.cut(logit_of(lo), (int)(uint32_t)lo);
     }
     // of the candidates in sh.all the one at which their measure, added up in order, reaches target: several threads add up
     // what lies before a candidate
@@ -396,27 +404,34 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float *src = p.logits + r * p.ld + row.i0;
     row.l = src;
+    float top = -INFINITY;
     if (row.held) {
         float *held = reinterpret_cast<float *>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
         row.l = held;
         const int body = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? row.n / 4 : 0;
 #pragma unroll 4
-        for (int i = threadIdx.x; i < body; i += SAMPLE_THREADS)
-            reinterpret_cast<float4 *>(held)[i] = __ldcg(reinterpret_cast<const float4 *>(src) + i);
+        for (int i = threadIdx.x; i < body; i += SAMPLE_THREADS) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src) + i);
+            reinterpret_cast<float4 *>(held)[i] = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+            top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));  // passes over NaN
+        }
 #pragma unroll 4
-        for (int i = 4 * body + threadIdx.x; i < 4 * row.quads(); i += SAMPLE_THREADS) held[i] = i < row.n ? __ldcg(src + i) : -INFINITY;
-        for (int i = 4 * row.quads() + threadIdx.x; i < 4 * ((row.quads() + 31) & ~31); i += SAMPLE_THREADS) held[i] = -INFINITY;
+        for (int i = 4 * body + threadIdx.x; i < 4 * ((row.quads() + 31) & ~31); i += SAMPLE_THREADS) {
+            held[i] = i < row.n ? clean(__ldcg(src + i)) : -INFINITY;
+            top = fmaxf(top, held[i]);
+        }
         __syncthreads();
+    } else {
+        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int, int) { top = fmaxf(top, x); });
     }
-    // the largest logit, and of equal ones the first
-    u64 best = ~0ull;
-    row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int i, int) { best = min(best, comp_of(x, i)); });
-    best = row.cluster_reduce(best, 0, least);
-    row.top = logit_of(best);
+    row.top = logit_of(row.cluster_reduce(comp_of(top + 0.0f, 0), 0, least));
     const float temp = p.temperature ? p.temperature[r] : 1.0f;
-    if (row.top == -INFINITY || !(temp > 0.0f)) {
+    if (row.top == -INFINITY || !(temp > 0.0f)) {  // the first of the largest
+        u64 best = 0xffffffffull;
+        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int i, int) { if (x == row.top) best = min(best, (u64)i); });
+        best = row.cluster_reduce(best, 1, least);
         if (row.rank == 0 && threadIdx.x == 0) {
-            p.tokens[r] = row.top == -INFINITY ? 0 : (long long)(uint32_t)best;
+            p.tokens[r] = row.top == -INFINITY ? 0 : (long long)best;
             if (p.logprobs) p.logprobs[r] = row.top == -INFINITY ? __uint_as_float(0x7fffffffu) : 0.0f;
         }
         return;
@@ -424,26 +439,28 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     const double inv_t = 1.0 / (double)temp;
     row.per = inv_t * 1.4426950408889634074;
     row.bins = (float)(inv_t * (SAMPLE_BINS / 32));
-    u64 bound = ~0ull;
+    Kept kept;
     const int k = p.top_k ? p.top_k[r] : 0;
-    if (k > 0 && k < p.vocab) bound = row.reach<false>(bound, [&](u64) { return (u64)k; });
+    if (k > 0 && k < p.vocab) row.cut<false>(kept, [&](u64) { return (u64)k; });
     const float mp = p.min_p ? p.min_p[r] : 0.0f;
     if (mp > 0.0f) {
+        // the smallest f32 logit that passes: the border in f64 is within a rounding of it
         const double border = log((double)fminf(mp, 1.0f));
-        u64 out = ~0ull;  // the first element below the border
-        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int i, int) {
-            if (x != row.top && !(((double)x - (double)row.top) * inv_t >= border)) out = min(out, comp_of(x, i));
-        });
-        out = row.cluster_reduce(out, 1, least);
-        if (out != ~0ull) bound = min(bound, out - 1);
+        const auto passes = [&](float x) { return x == row.top || ((double)x - (double)row.top) * inv_t >= border; };
+        float x = fminf((float)((double)row.top + border * (double)temp), row.top);
+        for (int i = 0; i < 4 && !passes(x); ++i) x = nextafterf(x, INFINITY);
+        for (int i = 0; i < 4 && x > -INFINITY && passes(nextafterf(x, -INFINITY)); ++i) x = nextafterf(x, -INFINITY);
+        kept.cut(x, 0x7fffffff);
     }
     const float tp = p.top_p ? p.top_p[r] : 1.0f;
     if (tp < 1.0f)
-        bound = row.reach<true>(bound, [&](u64 z) { return min(max((u64)ceil((double)fmaxf(tp, 0.0f) * (double)z), 1ull), z); });
+        row.cut<true>(kept, [&](u64 z) { return min(max((u64)ceil((double)fmaxf(tp, 0.0f) * (double)z), 1ull), z); });
     // ---- the draw: warps sum contiguous segments, the segment that holds the number is walked in index order
     const int seg = (row.quads() + SAMPLE_WARPS - 1) / SAMPLE_WARPS, s0 = min(row.quads(), warp * seg), s1 = min(row.quads(), s0 + seg);
     u64 s = 0;
-    row.each4(s0 + lane, 32, s1, [&](float x, int i, int) { s += comp_of(x, i) <= bound ? row.weight(x) : 0ull; });
+    row.each4(s0 + lane, 32, s1, [&](float x, int i, int) {
+        if (kept(x, i)) s += row.weight(x);  // what lies behind the slice has weight 0
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     __syncthreads();
@@ -469,7 +486,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         float x[4];
         row.each4(i + lane, 32, min(s1, i + 32), [&](float v, int at, int k) {
             x[k] = v;
-            w[k] = comp_of(v, at) <= bound ? row.weight(v) : 0ull;
+            w[k] = kept(v, at) ? row.weight(v) : 0ull;
             inc += w[k];
         });
         const u64 own = inc;
