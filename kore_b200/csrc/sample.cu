@@ -13,7 +13,9 @@
 //      total: the bins that may hold the border are then known, one or two of them;
 //   2. their elements (a few dozen of 32000 normal logits) are collected and what lies before them is summed exactly;
 //   3. every CTA finds the element among the candidates by counting.
-// Where there are more candidates than SAMPLE_CAND (ties, flat rows), the part of the order that they span is cut into 1024
+// Where all that is kept down to there is a short list (top-k, most nuclei), the whole of it is collected in step 2 and the
+// rest, the draw included, happens on the list without another exchange.
+//   Where there are more candidates than SAMPLE_CAND (ties, flat rows), the part of the order that they span is cut into 1024
 // bins of exact 64-bit sums first, again and again.  The draw sums the kept weights by segment and walks the one that holds
 // the number.
 #include <math.h>
@@ -31,6 +33,7 @@ constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_BINS = 1024;
 constexpr int SAMPLE_CAND = 1024;
+constexpr int SAMPLE_LIST = 256;  // a kept set of at most so many is collected and finished as a list
 constexpr int SAMPLE_CTAS = 8;  // of a cluster, at most
 constexpr int SAMPLE_SLICE = 40960;  // logits of a slice that shared memory holds (160 KB); a longer slice is read from L2
 constexpr size_t SAMPLE_MAX_VOCAB = (size_t)1 << 19;
@@ -53,7 +56,7 @@ struct SampleShared {
     u64 own[SAMPLE_CAND], all[SAMPLE_CAND], measure[SAMPLE_CAND];
     uint32_t n_own;
     int bin[2];
-    u64 before, found;
+    u64 before, upto, found;
 };
 
 // NaN counts as -inf, -0 is +0
@@ -69,10 +72,10 @@ __device__ __forceinline__ float logit_of(u64 comp) {
     return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
 
-// 2^44 2^y rounded to an integer, y <= 0: 2^f on [-1/2, 1/2] by its Taylor series to the 11th power (the next term is below
+// 2^44 2^y rounded to an integer, y <= 0 or NaN (0): 2^f on [-1/2, 1/2] by its Taylor series to the 11th power (the next term is below
 // 7e-15, 2^-47), times 2^n by the exponent field, rounded by adding 2^52
 __device__ __forceinline__ u64 exp2_fixed(double y) {
-    if (!(y > -46.0)) return 0ull;
+    y = fmax(y, -64.0);  // 0 from -46 on; no branch, so that several can be under way in a thread
     const double shift = 0x1.8p52, n = y + shift, f = y - (n - shift);
     double r = 4.44553827187081162491e-10;  // ln(2)^k / k!, k = 11 .. 0
     r = fma(r, f, 7.05491162080112335899e-09);
@@ -128,8 +131,8 @@ struct Row {
     float bins;      // bins per unit of logit
 
     __device__ __forceinline__ u64 weight(float x) const {
-        if (top == INFINITY) return x == top ? 1ull << 44 : 0ull;
-        return exp2_fixed(((double)x - (double)top) * per);
+        const double y = ((double)x - (double)top) * per;
+        return exp2_fixed(x == top ? 0.0 : y);
     }
     // place in the histogram, 0 .. 1023, falling with x (fminf takes the number where inf - inf or 0 * inf give none)
     __device__ __forceinline__ float bin_at(float x) const {
@@ -137,8 +140,8 @@ struct Row {
         return x == top ? 0.0f : at;
     }
 
-    // f(logit, index) of the slice's elements i0 + 4 i .. + 3 for i = first, first + stride, ..: whole warps where `first` is
-    // the thread's; elements behind the slice are -inf with indices behind every real one
+    // f(four logits, index of the first) of the slice's quads first, first + stride, .. below end; elements behind the slice
+    // are -inf with indices behind every real one
     template <typename F>
     __device__ __forceinline__ void each4(int first, int stride, int end, F f) const {
         for (int i = first; i < end; i += stride) {
@@ -148,10 +151,20 @@ struct Row {
                 x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
             } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? l[4 * i + k] : -INFINITY;
+                for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? clean(l[4 * i + k]) : -INFINITY;
             }
+            f(x, i0 + 4 * i);
+        }
+    }
+    // weights of the four where `in`, all under way at once; nothing where the warp has none
+    __device__ __forceinline__ void weigh(const float (&x)[4], const bool (&in)[4], u64 (&w)[4]) const {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f(held ? x[k] : clean(x[k]), i0 + 4 * i + k, k);
+        for (int k = 0; k < 4; ++k) w[k] = 0;
+        if (__any_sync(__activemask(), in[0] || in[1] || in[2] || in[3])) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = weight(x[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = in[k] ? w[k] : 0ull;
         }
     }
     __device__ __forceinline__ int quads() const { return (n + 3) / 4; }
@@ -243,30 +256,41 @@ struct Row {
             if (upto - mine[k] < target && target <= upto) {
                 sh.bin[0] = sh.bin[1] = 2 * threadIdx.x + k;
                 sh.before = upto - mine[k];
+                sh.upto = upto;
             }
             upto -= mine[k];
         }
     }
 
     // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
-    // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.
+    // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.  Returns the
+    // length of the list in sh.all that holds all that is kept, or 0 where there is none.
     template <bool WEIGHT, typename T>
-    __device__ void cut(Kept &kept, T target_of) const {
+    __device__ int cut(Kept &kept, T target_of) const {
         u64 target, sum = 0;
         hist_clear();
         if (threadIdx.x == 0) sh.bin[0] = sh.bin[1] = SAMPLE_BINS - 1;
-        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](float x, int i, int) {
-            const bool in = kept(x, i) && i < i0 + n;
-            if (WEIGHT && in) sum += weight(x);
-            const float at = bin_at(x), magic = __fadd_rd(at, 0x1p23f);  // the floor, in the low bits
-            const int b = __float_as_int(magic) & (SAMPLE_BINS - 1);
-            uint32_t m = 1;
+        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](const float (&x)[4], int i) {
+            bool in[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) in[k] = kept(x[k], i + k) && i + k < i0 + n;
             if (WEIGHT) {
-                // share of the bin's largest weight in 16 bits: e^-z for z = fraction / 32, to z^3 / 6 < 2^-17
-                const float z = (at - (magic - 0x1p23f)) * (32.0f / SAMPLE_BINS);
-                m = __float_as_uint(fmaf(fmaf(z, fmaf(z, 0.5f, -1.0f), 1.0f), 65535.0f, 0x1p23f)) & 0xffffu;
+                u64 w[4];
+                weigh(x, in, w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
-            if (in && !(WEIGHT && b == SAMPLE_BINS - 1)) atomicAdd(sh.hist[0] + b, m);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float at = bin_at(x[k]), magic = __fadd_rd(at, 0x1p23f);  // the floor, in the low bits
+                const int b = __float_as_int(magic) & (SAMPLE_BINS - 1);
+                uint32_t m = 1;
+                if (WEIGHT) {
+                    // share of the bin's largest weight in 16 bits: e^-z for z = fraction / 32, to z^3 / 6 < 2^-17
+                    const float z = (at - (magic - 0x1p23f)) * (32.0f / SAMPLE_BINS);
+                    m = __float_as_uint(fmaf(fmaf(z, fmaf(z, 0.5f, -1.0f), 1.0f), 65535.0f, 0x1p23f)) & 0xffffu;
+                }
+                if (in[k] && !(WEIGHT && b == SAMPLE_BINS - 1)) atomicAdd(sh.hist[0] + b, m);
+            }
         });
         if (WEIGHT) tell(block_reduce(sum, plus), 3);
         ptx::cluster_sync();
@@ -290,33 +314,48 @@ struct Row {
                 upto -= w[k];
             }
             if (threadIdx.x == 0 && aim - slack <= 0.0) sh.bin[0] = 0;
+            // elements of a bin: its shares are 0.969 to 1 of 65535
+            u64 total_shares;
+            u64 shares = block_scan(mine[0] + mine[1], total_shares);
+            __syncthreads();
+            if (sh.bin[1] / 2 == (int)threadIdx.x) sh.before = sh.bin[1] & 1 ? shares : shares - mine[1];
         } else {
             target = target_of(0);
             find_bin(mine, target);
         }
         __syncthreads();
-        const int b0 = sh.bin[0], b1 = sh.bin[1];
+        const int b1 = sh.bin[1];
+        const bool list = WEIGHT ? sh.before <= (u64)(SAMPLE_LIST * 0.96 * 65535) : sh.upto <= SAMPLE_LIST;
+        const int b0 = list ? 0 : sh.bin[0];
         if (!WEIGHT) {
-            target -= sh.before;
-            if (b0 == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
+            if (!list) target -= sh.before;
+            if (b1 == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
                 ptx::cluster_sync();      // the histograms have been read
-                return;
+                return 0;
             }
         }
         u64 lo = ~0ull, hi = 0;
         sum = 0;
         const float from = (float)b0, to = (float)(b1 + 1);
-        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](float x, int i, int) {
-            const float at = bin_at(x);
-            if (at >= to || !kept(x, i) || i >= i0 + n) return;
-            if (at >= from) {
-                const u64 c = comp_of(x, i);
-                const uint32_t slot = atomicAdd(&sh.n_own, 1u);
-                if (slot < SAMPLE_CAND) sh.own[slot] = c;
-                lo = min(lo, c);
-                hi = max(hi, c);
-            } else if (WEIGHT) {
-                sum += weight(x);
+        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](const float (&x)[4], int i) {
+            bool above[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float at = bin_at(x[k]);
+                const bool in = at < to && kept(x[k], i + k) && i + k < i0 + n;
+                above[k] = in && at < from;
+                if (in && at >= from) {
+                    const u64 c = comp_of(x[k], i + k);
+                    const uint32_t slot = atomicAdd(&sh.n_own, 1u);
+                    if (slot < SAMPLE_CAND) sh.own[slot] = c;
+                    lo = min(lo, c);
+                    hi = max(hi, c);
+                }
+            }
+            if (WEIGHT) {
+                u64 w[4];
+                weigh(x, above, w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
         });
         if (WEIGHT) tell(block_reduce(sum, plus), 4);
@@ -332,11 +371,10 @@ struct Row {
                 while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
                 const u64 e = ld_cluster(sh.own + (i - base), c);
                 sh.all[i] = e;
-                sh.measure[i] = WEIGHT ? weight(logit_of(e)) : 1ull;
+                sh.measure[i] = weight(logit_of(e));
             }
-            const u64 found = pick((uint32_t)count, target);
-            kept.cut(logit_of(found), (int)(uint32_t)found);
-            return;
+            cut_list<WEIGHT>(kept, (uint32_t)count, target);
+            return list ? (int)count : 0;
         }
         // too many: the part of the order that they span, cut into bins of 64-bit sums until one element is left
         lo = cluster_reduce(lo, 6, least);
@@ -344,17 +382,21 @@ struct Row {
         while (lo < hi) {
             const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
             hist_clear();
-            each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](float x, int i, int) {
-                const u64 c = comp_of(x, i);
-                const bool in = i < i0 + n && kept(x, i) && c >= lo && c <= hi;
-                u64 m = !in ? 0ull : (WEIGHT ? weight(x) : 1ull);
-                int b = m ? (int)((c - lo) >> shift) : -1;
-                if (same_bin(b)) {
+            // whole warps go around: they vote
+            each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](const float (&x)[4], int i) {
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-                    if (threadIdx.x & 31) b = -1;
+                for (int k = 0; k < 4; ++k) {
+                    const u64 c = comp_of(x[k], i + k);
+                    const bool in = i + k < i0 + n && kept(x[k], i + k) && c >= lo && c <= hi;
+                    u64 m = !in ? 0ull : (WEIGHT ? weight(x[k]) : 1ull);
+                    int b = m ? (int)((c - lo) >> shift) : -1;
+                    if (same_bin(b)) {  // ties and flat rows: one addition for the warp
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+                        if (threadIdx.x & 31) b = -1;
+                    }
+                    hist_add64(b, m);
                 }
-                hist_add64(b, m);
             });
             ptx::cluster_sync();
             u64 high[2];
@@ -370,25 +412,50 @@ struct Row {
             ptx::cluster_sync();  // the histograms have been read
         }
         kept.cut(logit_of(lo), (int)(uint32_t)lo);
+        return 0;
     }
-    // of the candidates in sh.all the one at which their measure, added up in order, reaches target: several threads add up
-    // what lies before a candidate
-    __device__ u64 pick(uint32_t count, u64 target) const {
-        uint32_t per = 1;  // threads per candidate
+    // Calls f(i, measure before it) for the elements of the list in sh.all, in the order that key(comp) gives; several threads
+    // add up what lies before an element, and the first of them calls.
+    template <bool WEIGHT, typename K, typename F>
+    __device__ __forceinline__ void in_order(uint32_t count, K key, F f) const {
+        uint32_t per = 1;  // threads per element
         while (per < 32 && 2 * per * count <= SAMPLE_THREADS) per *= 2;
         __syncthreads();
-        for (uint32_t i0_ = 0; i0_ < count; i0_ += SAMPLE_THREADS / per) {
-            const uint32_t i = i0_ + threadIdx.x / per;
-            const u64 c = i < count ? sh.all[i] : 0ull;
+        for (uint32_t start = 0; start < count; start += SAMPLE_THREADS / per) {
+            const uint32_t i = start + threadIdx.x / per;
+            const auto c = i < count ? key(sh.all[i]) : key(0);
             u64 before = 0;
-            for (uint32_t j = threadIdx.x % per; j < count; j += per) before += sh.all[j] < c ? sh.measure[j] : 0ull;
+            for (uint32_t j = threadIdx.x % per; j < count; j += per) before += key(sh.all[j]) < c ? (WEIGHT ? sh.measure[j] : 1ull) : 0ull;
             for (uint32_t o = per / 2; o > 0; o /= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
-            if (i < count && before < target && target <= before + sh.measure[i]) sh.found = c;
+            if (i < count && threadIdx.x % per == 0) f(i, before);
         }
         __syncthreads();
-        return sh.found;
+    }
+    // cuts behind the element of the list at which the measure reaches target
+    template <bool WEIGHT>
+    __device__ void cut_list(Kept &kept, uint32_t count, u64 target) const {
+        in_order<WEIGHT>(count, [](u64 c) { return c; }, [&](uint32_t i, u64 before) {
+            if (before < target && target <= before + (WEIGHT ? sh.measure[i] : 1ull)) sh.found = sh.all[i];
+        });
+        kept.cut(logit_of(sh.found), (int)(uint32_t)sh.found);
+    }
+    // measure 0 for what is not kept any more; returns the sum of the others
+    __device__ u64 keep_list(const Kept &kept, uint32_t count) const {
+        u64 sum = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
+            const u64 c = sh.all[i];
+            if (!kept(logit_of(c), (int)(uint32_t)c)) sh.measure[i] = 0;
+            sum += sh.measure[i];
+        }
+        return block_reduce(sum, plus);
     }
 };
+
+__device__ __forceinline__ u64 drawn(float u, u64 z) {  // u of z, below z
+    const u64 d = u > 0.0f ? (u64)((double)fminf(u, 1.0f) * (double)z) : 0ull;
+    return min(d, z - 1);
+}
 
 __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -422,13 +489,26 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         }
         __syncthreads();
     } else {
-        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int, int) { top = fmaxf(top, x); });
+        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](const float (&x)[4], int) { top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))); });
     }
-    row.top = logit_of(row.cluster_reduce(comp_of(top + 0.0f, 0), 0, least));
+    {
+        // the smallest of ~ordered bits: one instruction a warp
+        const uint32_t warp_top = __reduce_min_sync(0xffffffffu, (uint32_t)(comp_of(top + 0.0f, 0) >> 32));
+        if (lane == 0) sh.scratch[warp] = warp_top;
+        __syncthreads();
+        const uint32_t all = __reduce_min_sync(0xffffffffu, (uint32_t)sh.scratch[lane % SAMPLE_WARPS]);
+        row.tell((u64)all << 32, 0);
+        ptx::cluster_sync();
+        row.top = logit_of(row.told(0, least));
+    }
     const float temp = p.temperature ? p.temperature[r] : 1.0f;
     if (row.top == -INFINITY || !(temp > 0.0f)) {  // the first of the largest
         u64 best = 0xffffffffull;
-        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](float x, int i, int) { if (x == row.top) best = min(best, (u64)i); });
+        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](const float (&x)[4], int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (x[k] == row.top) best = min(best, (u64)(i + k));
+        });
         best = row.cluster_reduce(best, 1, least);
         if (row.rank == 0 && threadIdx.x == 0) {
             p.tokens[r] = row.top == -INFINITY ? 0 : (long long)best;
@@ -441,9 +521,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     row.bins = (float)(inv_t * (SAMPLE_BINS / 32));
     Kept kept;
     const int k = p.top_k ? p.top_k[r] : 0;
-    if (k > 0 && k < p.vocab) row.cut<false>(kept, [&](u64) { return (u64)k; });
+    int list = 0;
+    if (k > 0 && k < p.vocab) list = row.cut<false>(kept, [&](u64) { return (u64)k; });
     const float mp = p.min_p ? p.min_p[r] : 0.0f;
-    if (mp > 0.0f) {
+    if (mp > 0.0f && temp < INFINITY) {  // an infinite temperature makes all finite logits equal
         // the smallest f32 logit that passes: the border in f64 is within a rounding of it
         const double border = log((double)fminf(mp, 1.0f));
         const auto passes = [&](float x) { return x == row.top || ((double)x - (double)row.top) * inv_t >= border; };
@@ -453,13 +534,40 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         kept.cut(x, 0x7fffffff);
     }
     const float tp = p.top_p ? p.top_p[r] : 1.0f;
-    if (tp < 1.0f)
-        row.cut<true>(kept, [&](u64 z) { return min(max((u64)ceil((double)fmaxf(tp, 0.0f) * (double)z), 1ull), z); });
+    const auto nucleus = [&](u64 all) { return min(max((u64)ceil((double)fmaxf(tp, 0.0f) * (double)all), 1ull), all); };
+    if (tp < 1.0f) {
+        if (list) row.cut_list<true>(kept, list, nucleus(row.keep_list(kept, list)));
+        else list = row.cut<true>(kept, nucleus);
+    }
+    const float u = p.u[r];
+    const auto chosen = [&](float x, int i, u64 all) {
+        p.tokens[r] = i;
+        if (p.logprobs) {
+            const double e = x == row.top ? 0.0 : ((double)x - (double)row.top) * inv_t;
+            p.logprobs[r] = (float)(e - log((double)all * 0x1p-44));
+        }
+    };
+    if (list) {  // every CTA knows the answer, the first one writes it
+        const u64 all = row.keep_list(kept, list), draw = drawn(u, all);
+        row.in_order<true>(list, [](u64 c) { return (uint32_t)c; }, [&](uint32_t i, u64 before) {
+            if (row.rank == 0 && draw >= before && draw < before + sh.measure[i]) chosen(logit_of(sh.all[i]), (int)(uint32_t)sh.all[i], all);
+        });
+        ptx::cluster_sync();  // the others have read this CTA's candidates
+        return;
+    }
     // ---- the draw: warps sum contiguous segments, the segment that holds the number is walked in index order
     const int seg = (row.quads() + SAMPLE_WARPS - 1) / SAMPLE_WARPS, s0 = min(row.quads(), warp * seg), s1 = min(row.quads(), s0 + seg);
     u64 s = 0;
-    row.each4(s0 + lane, 32, s1, [&](float x, int i, int) {
-        if (kept(x, i)) s += row.weight(x);  // what lies behind the slice has weight 0
+    const auto weigh = [&](const float (&x)[4], int i, u64 (&w)[4]) {  // what lies behind the slice has weight 0
+        bool in[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) in[k] = kept(x[k], i + k);
+        row.weigh(x, in, w);
+    };
+    row.each4(s0 + lane, 32, s1, [&](const float (&x)[4], int i) {
+        u64 w[4];
+        weigh(x, i, w);
+        s += (w[0] + w[1]) + (w[2] + w[3]);
     });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -477,17 +585,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         if (c < row.rank) before += sh.slot[2][c];
         z += sh.slot[2][c];
     }
-    const float u = p.u[r];
-    u64 draw = u > 0.0f ? (u64)((double)fminf(u, 1.0f) * (double)z) : 0ull;
-    draw = min(draw, z - 1);
+    const u64 draw = drawn(u, z);
     if (draw < before || draw >= before + s) return;  // one warp of the cluster goes on
     for (int i = s0; i < s1; i += 32) {
         u64 w[4] = {}, inc = 0;
         float x[4];
-        row.each4(i + lane, 32, min(s1, i + 32), [&](float v, int at, int k) {
-            x[k] = v;
-            w[k] = kept(v, at) ? row.weight(v) : 0ull;
-            inc += w[k];
+        row.each4(i + lane, 32, min(s1, i + 32), [&](const float (&v)[4], int at) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = v[k];
+            weigh(v, at, w);
+            inc = (w[0] + w[1]) + (w[2] + w[3]);
         });
         const u64 own = inc;
 #pragma unroll
@@ -500,13 +607,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
             u64 at = before + inc - own;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (draw >= at && draw < at + w[k]) {
-                    p.tokens[r] = row.i0 + 4 * (i + lane) + k;
-                    if (p.logprobs) {
-                        const double e = x[k] == row.top ? 0.0 : ((double)x[k] - (double)row.top) * inv_t;
-                        p.logprobs[r] = (float)(e - log((double)z * 0x1p-44));
-                    }
-                }
+                if (draw >= at && draw < at + w[k]) chosen(x[k], row.i0 + 4 * (i + lane) + k, z);
                 at += w[k];
             }
             return;
