@@ -5,19 +5,20 @@
 // Weights are integers of 2^-44 (the largest is 2^44, 2^19 of them fit 63 bits): their sums do not depend on the order in
 // which atomics arrive, and a token's border moves by at most vocab 2^-45 of the largest weight.
 //
-// Bound by the latency of the passes for a few rows and by the f64 exponentials for many (a logit is read once).  A row
-// belongs to a cluster of 1 to 8 CTAs, each with a slice of it in shared memory.  Top-k and top-p look for the element at
-// which a running measure (count, or weight) reaches a target:
+// Bound by the latency of the passes for a few rows and by the f64 exponentials for many (13 f64 operations each).  A row
+// belongs to a cluster of 1 to 8 CTAs; each has a slice of the row, in shared memory where it fits, otherwise in L2.  Top-k and top-p look for the element at which a running measure (count, or weight)
+// reaches a target:
 //   1. a histogram over 1024 steps of 1/32 in the exponent.  Counts are exact.  Of a weight only its share of its bin's
 //      largest, in 16 bits, goes through an atomic (the sum of a bin is good to 2^-15), while threads add up the exact
 //      total: the bins that may hold the border are then known, one or two of them;
-//   2. their elements (a few dozen of 32000 normal logits) are collected and what lies before them is summed exactly;
+//   2. their elements (a few dozen of 32000 normal logits) are collected and what lies before them is summed exactly.  While
+//      there are more than SAMPLE_CAND of them (flat distributions, ties), the part of the order that they span is cut into
+//      1024 bins of exact 64-bit sums;
 //   3. every CTA finds the element among the candidates by counting.
 // Where all that is kept down to there is a short list (top-k, most nuclei), the whole of it is collected in step 2 and the
-// rest, the draw included, happens on the list without another exchange.
-//   Where there are more candidates than SAMPLE_CAND (ties, flat rows), the part of the order that they span is cut into 1024
-// bins of exact 64-bit sums first, again and again.  The draw sums the kept weights by segment and walks the one that holds
-// the number.
+// rest, the draw included, happens on the list without another exchange.  Otherwise step 2 has the sums of the kept weights
+// by segment already, and the draw walks the segment that holds the number.
+#include <float.h>
 #include <math.h>
 #include <stdlib.h>
 
@@ -32,16 +33,15 @@ using u64 = unsigned long long;
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_BINS = 1024;
-constexpr int SAMPLE_CAND = 1024;
-constexpr int SAMPLE_LIST = 256;  // a kept set of at most so many is collected and finished as a list
-constexpr int SAMPLE_CTAS = 8;  // of a cluster, at most
-constexpr int SAMPLE_SLICE = 40960;  // logits of a slice that shared memory holds (160 KB); a longer slice is read from L2
+constexpr int SAMPLE_CAND = 256;  // counting what lies before each of c elements takes c^2 / 512 steps of a thread
+constexpr int SAMPLE_CTAS = 8;    // of a cluster, at most
 constexpr size_t SAMPLE_MAX_VOCAB = (size_t)1 << 19;
 
 struct SampleParams {
     const float *logits;
     size_t ld;
     int vocab, slice;
+    bool held;  // slices in shared memory
     const float *temperature;
     const int *top_k;
     const float *top_p, *min_p, *u;
@@ -51,13 +51,15 @@ struct SampleParams {
 
 struct SampleShared {
     u64 slot[8][SAMPLE_CTAS];  // one row per exchange between the CTAs
-    u64 scratch[SAMPLE_WARPS];
+    u64 scratch[SAMPLE_WARPS], segment[SAMPLE_WARPS];
+    double scale[32];               // see exp2_fixed
     uint32_t hist[2][SAMPLE_BINS];  // counts or shares; 64-bit sums take both (64-bit shared atomics are compare-and-swap loops)
     u64 own[SAMPLE_CAND], all[SAMPLE_CAND], measure[SAMPLE_CAND];
     uint32_t n_own;
     int bin[2];
     u64 before, upto, found;
 };
+constexpr size_t SAMPLE_FIXED = (sizeof(SampleShared) + 15) / 16 * 16;
 
 // NaN counts as -inf, -0 is +0
 __device__ __forceinline__ float clean(float l) { return l == l ? l + 0.0f : -INFINITY; }
@@ -72,25 +74,24 @@ __device__ __forceinline__ float logit_of(u64 comp) {
     return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
 
-// 2^44 2^y rounded to an integer, y <= 0 or NaN (0): 2^f on [-1/2, 1/2] by its Taylor series to the 11th power (the next term is below
-// 7e-15, 2^-47), times 2^n by the exponent field, rounded by adding 2^52
-__device__ __forceinline__ u64 exp2_fixed(double y) {
-    y = fmax(y, -64.0);  // 0 from -46 on; no branch, so that several can be under way in a thread
-    const double shift = 0x1.8p52, n = y + shift, f = y - (n - shift);
-    double r = 4.44553827187081162491e-10;  // ln(2)^k / k!, k = 11 .. 0
-    r = fma(r, f, 7.05491162080112335899e-09);
-    r = fma(r, f, 1.01780860092396999224e-07);
-    r = fma(r, f, 1.32154867901443095086e-06);
-    r = fma(r, f, 1.52527338040598410828e-05);
-    r = fma(r, f, 1.54035303933816087761e-04);
-    r = fma(r, f, 1.33335581464284432841e-03);
-    r = fma(r, f, 9.61812910762847687873e-03);
-    r = fma(r, f, 5.55041086648215831190e-02);
-    r = fma(r, f, 2.40226506959100721827e-01);
-    r = fma(r, f, 6.93147180559945286227e-01);
+// The bits of 2^52 + (2^44 2^y rounded to an integer), y <= 0; 2^52 + 0 where not `in`.  y = e + j / 32 + f: 2^f on [-1/64,
+// 1/64] by its Taylor series to the 5th power (the next term is below 2.3e-15, 2^-48) times 2^(44 + e + j/32), which comes
+// from the table entry scale[j] = 2^(44 + j/32) with j << 15 taken off its upper word: adding (32 e + j) << 15 puts e into the
+// exponent field.  Adding 2^52 rounds.  No branch, so that several can be under way in a thread.
+constexpr u64 FIXED_ZERO = 0x433ull << 52;
+__device__ __forceinline__ u64 exp2_fixed(double y, bool in, const double *scale) {
+    // below -64 (0 from -46 on) by the sign and exponent bits
+    y = __hiloint2double(in && (uint32_t)__double2hiint(y) <= 0xc0500000u ? __double2hiint(y) : (int)0xc0500000u, __double2loint(y));
+    const double shift = 0x1.8p47, n = y + shift, f = y - (n - shift);
+    double r = 1.33335581464284434234e-03;  // ln(2)^k / k!, k = 5 .. 0
+    r = fma(r, f, 9.61812910762847716198e-03);
+    r = fma(r, f, 5.55041086648215799531e-02);
+    r = fma(r, f, 2.40226506959100712334e-01);
+    r = fma(r, f, 6.93147180559945309417e-01);
     r = fma(r, f, 1.0);
-    const double v = __hiloint2double(__double2hiint(r) + ((__double2loint(n) + 44) << 20), __double2loint(r));
-    return (u64)__double_as_longlong(v + 0x1p52) & ((1ull << 52) - 1);
+    const int k = __double2loint(n);
+    const double s = scale[k & 31];
+    return (u64)__double_as_longlong(r * __hiloint2double(__double2hiint(s) + (k << 15), __double2loint(s)) + 0x1p52);
 }
 
 __device__ __forceinline__ uint2 ld_cluster(const uint2 *p, uint32_t rank) {
@@ -108,66 +109,85 @@ __device__ __forceinline__ void st_cluster(u64 *p, uint32_t rank, u64 v) {
 }
 __device__ __forceinline__ u64 least(u64 a, u64 b) { return a < b ? a : b; }
 __device__ __forceinline__ u64 plus(u64 a, u64 b) { return a + b; }
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T up = __shfl_up_sync(0xffffffffu, v, o);
+        if ((int)(threadIdx.x & 31) >= o) v += up;
+    }
+    return v;
+}
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
-// what the filters keep: logits above `least`, and those equal to it up to index `last`
+// what the filters keep: logits above `least`, and those equal to it up to index `last`; never a logit of -inf
 struct Kept {
-    float least = -INFINITY;
-    int last = 0x7fffffff;
-    __device__ __forceinline__ bool operator()(float x, int i) const { return x >= least && (x > least || i <= last); }
+    float least;
+    int last;
+    __device__ __forceinline__ bool operator()(float x, int i) const { return x > least || (x == least && i <= last); }
     __device__ __forceinline__ void cut(float l, int i) {
         if (l > least) least = l, last = i;
         else if (l == least) last = min(last, i);
     }
+    __device__ __forceinline__ void cut(u64 comp) { cut(logit_of(comp), (int)(uint32_t)comp); }
 };
 
 struct Row {
     SampleShared &sh;
-    const float *l;  // this CTA's slice: shared memory (clean, filled up with -inf), or the logits themselves
-    bool held;
-    int n, i0;       // its length and its first index
+    const float *l;     // this CTA's slice: shared memory (clean, filled up with -inf), or the logits themselves
+    bool held, wide;    // wide: the logits are 16-byte aligned
+    int n, i0;          // its length and its first index
+    int q0, q1;         // this warp's segment of it, in quads
     uint32_t rank, ctas;
-    float top;       // largest logit
-    double per;      // log2(e) / temperature
-    float bins;      // bins per unit of logit
+    float top;          // largest logit, at most FLT_MAX
+    double per;         // log2(e) / temperature
+    float bins;         // bins per unit of logit
 
-    __device__ __forceinline__ u64 weight(float x) const {
-        const double y = ((double)x - (double)top) * per;
-        return exp2_fixed(x == top ? 0.0 : y);
-    }
-    // place in the histogram, 0 .. 1023, falling with x (fminf takes the number where inf - inf or 0 * inf give none)
-    __device__ __forceinline__ float bin_at(float x) const {
-        const float at = fminf((top - x) * bins, (float)(SAMPLE_BINS - 1));
-        return x == top ? 0.0f : at;
-    }
+    // exponent of a kept logit; infinite logits are all that is kept where there are any
+    __device__ __forceinline__ double exponent(float x) const { return ((double)fminf(x, FLT_MAX) - (double)top) * per; }
+    __device__ __forceinline__ u64 weight(float x) const { return exp2_fixed(exponent(x), true, sh.scale) - FIXED_ZERO; }
+    // place in the histogram, 0 .. 1023, falling with x
+    __device__ __forceinline__ float bin_at(float x) const { return fminf((top - fminf(x, FLT_MAX)) * bins, (float)(SAMPLE_BINS - 1)); }
 
-    // f(four logits, index of the first) of the slice's quads first, first + stride, .. below end; elements behind the slice
-    // are -inf with indices behind every real one
-    template <typename F>
-    __device__ __forceinline__ void each4(int first, int stride, int end, F f) const {
-        for (int i = first; i < end; i += stride) {
-            float x[4];
-            if (held) {
-                const float4 v = reinterpret_cast<const float4 *>(l)[i];
-                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-            } else {
+    __device__ __forceinline__ void load4(int i, float (&x)[4]) const {
+        if (held || (wide && 4 * i + 3 < n)) {
+            const float4 v = reinterpret_cast<const float4 *>(l)[i];
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? clean(l[4 * i + k]) : -INFINITY;
-            }
-            f(x, i0 + 4 * i);
+            for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? l[4 * i + k] : -INFINITY;
         }
     }
-    // weights of the four where `in`, all under way at once; nothing where the warp has none
-    __device__ __forceinline__ void weigh(const float (&x)[4], const bool (&in)[4], u64 (&w)[4]) const {
+    // f(four logits, index of the first) for the quads of this warp's segment, in index order; elements behind the slice are
+    // -inf.  The next quad is loaded before this one is used.  WHOLE: all lanes go around.
+    template <bool WHOLE, typename F>
+    __device__ __forceinline__ void each4(F f) const {
+        const int lane = threadIdx.x & 31;
+        float x[4], y[4];
+        if (q0 + lane < q1) load4(q0 + lane, x);
+        for (int i = q0 + lane; WHOLE ? i - lane < q1 : i < q1; i += 32) {
+            if (i + 32 < q1) load4(i + 32, y);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = 0;
+            for (int k = 0; k < 4; ++k) x[k] = WHOLE && i >= q1 ? -INFINITY : held ? x[k] : clean(x[k]);
+            f(x, i0 + 4 * i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = y[k];
+        }
+    }
+    // sum of the weights of the four where `in`, all under way at once; nothing is done where the warp has none
+    __device__ __forceinline__ u64 weigh(const float (&x)[4], const bool (&in)[4]) const {
+        u64 sum = 0;
         if (__any_sync(__activemask(), in[0] || in[1] || in[2] || in[3])) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = weight(x[k]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = in[k] ? w[k] : 0ull;
+            for (int k = 0; k < 4; ++k) sum += exp2_fixed(exponent(x[k]), in[k], sh.scale);
+            sum -= 4 * FIXED_ZERO;
         }
+        return sum;
     }
-    __device__ __forceinline__ int quads() const { return (n + 3) / 4; }
 
     template <typename F>
     __device__ __forceinline__ u64 block_reduce(u64 v, F f) const {
@@ -200,28 +220,17 @@ struct Row {
     }
     // inclusive sum over the threads
     template <typename T>
-    __device__ __forceinline__ T block_scan(T v, T &total) const {
+    __device__ __forceinline__ T block_scan(T v) const {
         static_assert(sizeof(T) == 8, "");
         T *scratch = reinterpret_cast<T *>(sh.scratch);
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const T up = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += up;
-        }
+        v = warp_scan(v);
         __syncthreads();
-        if (lane == 31) scratch[warp] = v;
+        if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = v;
         __syncthreads();
-        total = 0;
         T base = 0;
-#pragma unroll
-        for (int w = 0; w < SAMPLE_WARPS; ++w) {
-            if (w == warp) base = total;
-            total += scratch[w];
-        }
+        for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) base += scratch[w];
         return v + base;
     }
-    __device__ __forceinline__ bool same_bin(int b) const { return __all_sync(0xffffffffu, b == __shfl_sync(0xffffffffu, b, 0)); }
     __device__ __forceinline__ void hist_add64(int b, u64 m) const {
         if (b < 0) return;
         const uint32_t old = atomicAdd(sh.hist[0] + b, (uint32_t)m);
@@ -229,7 +238,7 @@ struct Row {
         if (hi) atomicAdd(sh.hist[1] + b, hi);
     }
     __device__ __forceinline__ void hist_clear() const {
-        for (int b = threadIdx.x; b < 2 * SAMPLE_BINS; b += SAMPLE_THREADS) sh.hist[0][b] = 0;
+        for (int b = threadIdx.x; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.hist[0][b] = sh.hist[1][b] = 0;
         __syncthreads();
     }
     // bins 2t and 2t + 1 of word array h over the whole row
@@ -247,10 +256,9 @@ struct Row {
                 out[1] += v[c].y;
             }
     }
-    // the bin of a running sum that reaches target, and the sum before it
+    // the bin in which the running sum reaches target, the sum before it and with it
     __device__ __forceinline__ void find_bin(const u64 (&mine)[2], u64 target) const {
-        u64 total;
-        u64 upto = block_scan(mine[0] + mine[1], total);
+        u64 upto = block_scan(mine[0] + mine[1]);
 #pragma unroll
         for (int k = 1; k >= 0; --k) {
             if (upto - mine[k] < target && target <= upto) {
@@ -261,24 +269,27 @@ struct Row {
             upto -= mine[k];
         }
     }
+    __device__ __forceinline__ void collect(u64 c, u64 &lo, u64 &hi) const {
+        const uint32_t slot = atomicAdd(&sh.n_own, 1u);
+        if (slot < SAMPLE_CAND) sh.own[slot] = c;
+        lo = min(lo, c);
+        hi = max(hi, c);
+    }
 
     // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
     // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.  Returns the
-    // length of the list in sh.all that holds all that is kept, or 0 where there is none.
+    // length of the list in sh.all that holds all that is kept, or 0 where there is none; WEIGHT without a list: sh.segment
+    // has the warps' sums of the kept weights.
     template <bool WEIGHT, typename T>
     __device__ int cut(Kept &kept, T target_of) const {
         u64 target, sum = 0;
         hist_clear();
         if (threadIdx.x == 0) sh.bin[0] = sh.bin[1] = SAMPLE_BINS - 1;
-        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](const float (&x)[4], int i) {
+        each4<false>([&](const float (&x)[4], int i) {
             bool in[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) in[k] = kept(x[k], i + k) && i + k < i0 + n;
-            if (WEIGHT) {
-                u64 w[4];
-                weigh(x, in, w);
-                sum += (w[0] + w[1]) + (w[2] + w[3]);
-            }
+            for (int k = 0; k < 4; ++k) in[k] = kept(x[k], i + k);
+            if (WEIGHT) sum += weigh(x, in);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float at = bin_at(x[k]), magic = __fadd_rd(at, 0x1p23f);  // the floor, in the low bits
@@ -302,11 +313,11 @@ struct Row {
             const u64 all = told(3, plus);
             target = target_of(all);
             const double aim = (double)target * 0x1p-44, slack = (double)all * 0x1p-58;
-            double w[2], total;
+            double w[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 w[k] = (double)mine[k] * (1.0 / 65535) * (double)exp2f((float)(2 * threadIdx.x + k) * (-1.4426950408889634f * 32 / SAMPLE_BINS));
-            double upto = block_scan(w[0] + w[1], total);
+            double upto = block_scan(w[0] + w[1]);
 #pragma unroll
             for (int k = 1; k >= 0; --k) {
                 if (upto - w[k] < aim - slack && aim - slack <= upto) sh.bin[0] = 2 * threadIdx.x + k;
@@ -314,85 +325,60 @@ struct Row {
                 upto -= w[k];
             }
             if (threadIdx.x == 0 && aim - slack <= 0.0) sh.bin[0] = 0;
-            // elements of a bin: its shares are 0.969 to 1 of 65535
-            u64 total_shares;
-            u64 shares = block_scan(mine[0] + mine[1], total_shares);
+            // shares up to bin[1]: 0.969 to 1 of 65535 for every element
+            const u64 shares = block_scan(mine[0] + mine[1]);
             __syncthreads();
-            if (sh.bin[1] / 2 == (int)threadIdx.x) sh.before = sh.bin[1] & 1 ? shares : shares - mine[1];
+            if (sh.bin[1] / 2 == (int)threadIdx.x) sh.upto = sh.bin[1] & 1 ? shares : shares - mine[1];
         } else {
             target = target_of(0);
             find_bin(mine, target);
         }
         __syncthreads();
         const int b1 = sh.bin[1];
-        const bool list = WEIGHT ? sh.before <= (u64)(SAMPLE_LIST * 0.96 * 65535) : sh.upto <= SAMPLE_LIST;
-        const int b0 = list ? 0 : sh.bin[0];
-        if (!WEIGHT) {
-            if (!list) target -= sh.before;
-            if (b1 == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
-                ptx::cluster_sync();      // the histograms have been read
-                return 0;
-            }
+        if (!WEIGHT && b1 == SAMPLE_BINS - 1) {  // from 31.9 on in the exponent weights are 0: who is kept does not matter
+            ptx::cluster_sync();                 // the histograms have been read
+            return 0;
         }
+        const bool list = WEIGHT ? sh.upto <= (u64)(SAMPLE_CAND * 0.96 * 65535) : sh.upto <= SAMPLE_CAND;
+        const int b0 = list ? 0 : sh.bin[0];
+        if (!WEIGHT && !list) target -= sh.before;
+
+        // ---- the elements of bins b0 .. b1, and the sum of what lies before
         u64 lo = ~0ull, hi = 0;
         sum = 0;
         const float from = (float)b0, to = (float)(b1 + 1);
-        each4(threadIdx.x, SAMPLE_THREADS, quads(), [&](const float (&x)[4], int i) {
+        each4<false>([&](const float (&x)[4], int i) {
             bool above[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float at = bin_at(x[k]);
-                const bool in = at < to && kept(x[k], i + k) && i + k < i0 + n;
+                const bool in = at < to && kept(x[k], i + k);
                 above[k] = in && at < from;
-                if (in && at >= from) {
-                    const u64 c = comp_of(x[k], i + k);
-                    const uint32_t slot = atomicAdd(&sh.n_own, 1u);
-                    if (slot < SAMPLE_CAND) sh.own[slot] = c;
-                    lo = min(lo, c);
-                    hi = max(hi, c);
-                }
+                if (in && at >= from) collect(comp_of(x[k], i + k), lo, hi);
             }
-            if (WEIGHT) {
-                u64 w[4];
-                weigh(x, above, w);
-                sum += (w[0] + w[1]) + (w[2] + w[3]);
-            }
+            if (WEIGHT) sum += weigh(x, above);
         });
         if (WEIGHT) tell(block_reduce(sum, plus), 4);
         __syncthreads();
         tell(sh.n_own, 5);
         ptx::cluster_sync();
         if (WEIGHT) target -= told(4, plus);
-        const u64 count = told(5, plus);
-        if (count <= SAMPLE_CAND) {
-            uint32_t c = 0;
-            u64 base = 0;
-            for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
-                while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
-                const u64 e = ld_cluster(sh.own + (i - base), c);
-                sh.all[i] = e;
-                sh.measure[i] = weight(logit_of(e));
-            }
-            cut_list<WEIGHT>(kept, (uint32_t)count, target);
-            return list ? (int)count : 0;
-        }
-        // too many: the part of the order that they span, cut into bins of 64-bit sums until one element is left
-        lo = cluster_reduce(lo, 6, least);
-        hi = ~cluster_reduce(~hi, 7, least);
-        while (lo < hi) {
+        u64 count = told(5, plus);
+        while (count > SAMPLE_CAND) {  // the part of the order that they span, cut into bins of 64-bit sums
+            lo = cluster_reduce(lo, 6, least);
+            hi = ~cluster_reduce(~hi, 7, least);
             const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
             hist_clear();
-            // whole warps go around: they vote
-            each4(threadIdx.x, SAMPLE_THREADS, (quads() + 31) & ~31, [&](const float (&x)[4], int i) {
+            each4<true>([&](const float (&x)[4], int i) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const u64 c = comp_of(x[k], i + k);
-                    const bool in = i + k < i0 + n && kept(x[k], i + k) && c >= lo && c <= hi;
+                    const bool in = kept(x[k], i + k) && c >= lo && c <= hi;
+                    if (!__any_sync(0xffffffffu, in)) continue;
                     u64 m = !in ? 0ull : (WEIGHT ? weight(x[k]) : 1ull);
                     int b = m ? (int)((c - lo) >> shift) : -1;
-                    if (same_bin(b)) {  // ties and flat rows: one addition for the warp
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+                    if (__all_sync(0xffffffffu, b == __shfl_sync(0xffffffffu, b, 0))) {  // ties and flat rows: one addition for the warp
+                        m = warp_sum(m);
                         if (threadIdx.x & 31) b = -1;
                     }
                     hist_add64(b, m);
@@ -405,15 +391,56 @@ struct Row {
             mine[0] += high[0] << 32;
             mine[1] += high[1] << 32;
             find_bin(mine, target);
+            if (threadIdx.x == 0) sh.n_own = 0;
             __syncthreads();
             target -= sh.before;
+            const u64 first = lo;
             lo += (u64)sh.bin[0] << shift;
             hi = min(hi, lo + ((1ull << shift) - 1));
-            ptx::cluster_sync();  // the histograms have been read
+            u64 new_lo = ~0ull, new_hi = 0;
+            each4<false>([&](const float (&x)[4], int i) {
+                bool above[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const u64 c = comp_of(x[k], i + k);
+                    const bool in = kept(x[k], i + k);
+                    above[k] = in && c >= first && c < lo;
+                    if (in && c >= lo && c <= hi) collect(c, new_lo, new_hi);
+                }
+                if (WEIGHT) sum += weigh(x, above);
+            });
+            lo = new_lo;
+            hi = new_hi;
+            __syncthreads();
+            tell(sh.n_own, 5);
+            ptx::cluster_sync();
+            count = told(5, plus);
         }
-        kept.cut(logit_of(lo), (int)(uint32_t)lo);
+        uint32_t c = 0;
+        u64 base = 0;
+        for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
+            while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
+            const u64 e = ld_cluster(sh.own + (i - base), c);
+            sh.all[i] = e;
+            sh.measure[i] = weight(logit_of(e));
+        }
+        cut_list<WEIGHT>(kept, (uint32_t)count, target);
+        if (list) return (int)count;
+        if (WEIGHT) {  // the kept candidates of this CTA go to their segments
+            sum = warp_sum(sum);
+            if ((threadIdx.x & 31) == 0) sh.segment[threadIdx.x >> 5] = sum;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < (uint32_t)count; i += SAMPLE_THREADS) {
+                const u64 e = sh.all[i];
+                const int at = (int)(uint32_t)e - i0;
+                if (at >= 0 && at < n && kept(logit_of(e), (int)(uint32_t)e)) atomicAdd(sh.segment + at / 4 / quads_per_warp(), sh.measure[i]);
+            }
+            __syncthreads();
+        }
         return 0;
     }
+    __device__ __forceinline__ int quads_per_warp() const { return max(1, ((n + 3) / 4 + SAMPLE_WARPS - 1) / SAMPLE_WARPS); }
+
     // Calls f(i, measure before it) for the elements of the list in sh.all, in the order that key(comp) gives; several threads
     // add up what lies before an element, and the first of them calls.
     template <bool WEIGHT, typename K, typename F>
@@ -437,7 +464,7 @@ struct Row {
         in_order<WEIGHT>(count, [](u64 c) { return c; }, [&](uint32_t i, u64 before) {
             if (before < target && target <= before + (WEIGHT ? sh.measure[i] : 1ull)) sh.found = sh.all[i];
         });
-        kept.cut(logit_of(sh.found), (int)(uint32_t)sh.found);
+        kept.cut(sh.found);
     }
     // measure 0 for what is not kept any more; returns the sum of the others
     __device__ u64 keep_list(const Kept &kept, uint32_t count) const {
@@ -464,18 +491,29 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t r = blockIdx.x / ctas;
-    Row row = {sh, nullptr, p.slice <= SAMPLE_SLICE, 0, 0, ptx::cluster_ctarank(), ctas, 0.0f, 0.0, 0.0f};
+    Row row = {sh};
+    row.held = p.held;
+    row.rank = ptx::cluster_ctarank();
+    row.ctas = ctas;
     row.i0 = min(p.vocab, (int)row.rank * p.slice);
     row.n = min(p.slice, p.vocab - row.i0);
+    const int quads = (row.n + 3) / 4;
+    row.q0 = min(quads, warp * row.quads_per_warp());
+    row.q1 = min(quads, row.q0 + row.quads_per_warp());
+    if (threadIdx.x < 32) {
+        const double s = exp2(44.0 + (double)threadIdx.x * (1.0 / 32));
+        sh.scale[threadIdx.x] = __hiloint2double(__double2hiint(s) - ((int)threadIdx.x << 15), __double2loint(s));
+    }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float *src = p.logits + r * p.ld + row.i0;
     row.l = src;
+    row.wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     float top = -INFINITY;
     if (row.held) {
-        float *held = reinterpret_cast<float *>(smem + (sizeof(SampleShared) + 15) / 16 * 16);
+        float *held = reinterpret_cast<float *>(smem + SAMPLE_FIXED);
         row.l = held;
-        const int body = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? row.n / 4 : 0;
+        const int body = row.wide ? row.n / 4 : 0;
 #pragma unroll 4
         for (int i = threadIdx.x; i < body; i += SAMPLE_THREADS) {
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(src) + i);
@@ -483,43 +521,50 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
             top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));  // passes over NaN
         }
 #pragma unroll 4
-        for (int i = 4 * body + threadIdx.x; i < 4 * ((row.quads() + 31) & ~31); i += SAMPLE_THREADS) {
-            held[i] = i < row.n ? clean(__ldcg(src + i)) : -INFINITY;
-            top = fmaxf(top, held[i]);
+        for (int i = 4 * body + threadIdx.x; i < 4 * quads; i += SAMPLE_THREADS) {
+            const float v = i < row.n ? clean(__ldcg(src + i)) : -INFINITY;
+            held[i] = v;
+            top = fmaxf(top, v);
         }
-        __syncthreads();
     } else {
-        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](const float (&x)[4], int) { top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))); });
-    }
-    {
-        // the smallest of ~ordered bits: one instruction a warp
-        const uint32_t warp_top = __reduce_min_sync(0xffffffffu, (uint32_t)(comp_of(top + 0.0f, 0) >> 32));
-        if (lane == 0) sh.scratch[warp] = warp_top;
-        __syncthreads();
-        const uint32_t all = __reduce_min_sync(0xffffffffu, (uint32_t)sh.scratch[lane % SAMPLE_WARPS]);
-        row.tell((u64)all << 32, 0);
-        ptx::cluster_sync();
-        row.top = logit_of(row.told(0, least));
+        row.each4<false>([&](const float (&x)[4], int) { top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))); });
     }
     const float temp = p.temperature ? p.temperature[r] : 1.0f;
-    if (row.top == -INFINITY || !(temp > 0.0f)) {  // the first of the largest
-        u64 best = 0xffffffffull;
-        row.each4(threadIdx.x, SAMPLE_THREADS, row.quads(), [&](const float (&x)[4], int i) {
+    // the smallest of ~ordered bits: one instruction a warp
+    const uint32_t warp_top = __reduce_min_sync(0xffffffffu, (uint32_t)(comp_of(top + 0.0f, 0) >> 32));
+    if (lane == 0) sh.scratch[warp] = warp_top;
+    __syncthreads();  // the slice and the table are there, too
+    top = logit_of((u64)__reduce_min_sync(0xffffffffu, (uint32_t)sh.scratch[lane % SAMPLE_WARPS]) << 32);
+    if (!(temp > 0.0f)) {  // the first of the largest: of the slice, then of all
+        u64 best = ~0ull;
+        row.each4<false>([&](const float (&x)[4], int i) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (x[k] == row.top) best = min(best, (u64)(i + k));
+                if (x[k] == top) best = min(best, comp_of(top, i + k));
         });
-        best = row.cluster_reduce(best, 1, least);
+        best = row.cluster_reduce(best, 0, least);
+        row.top = logit_of(best);
         if (row.rank == 0 && threadIdx.x == 0) {
-            p.tokens[r] = row.top == -INFINITY ? 0 : (long long)best;
+            p.tokens[r] = row.top == -INFINITY ? 0 : (long long)(uint32_t)best;
             if (p.logprobs) p.logprobs[r] = row.top == -INFINITY ? __uint_as_float(0x7fffffffu) : 0.0f;
+        }
+        return;
+    }
+    row.tell(comp_of(top, 0), 0);
+    ptx::cluster_sync();
+    top = logit_of(row.told(0, least));
+    row.top = fminf(top, FLT_MAX);
+    if (top == -INFINITY) {
+        if (row.rank == 0 && threadIdx.x == 0) {
+            p.tokens[r] = 0;
+            if (p.logprobs) p.logprobs[r] = __uint_as_float(0x7fffffffu);
         }
         return;
     }
     const double inv_t = 1.0 / (double)temp;
     row.per = inv_t * 1.4426950408889634074;
-    row.bins = (float)(inv_t * (SAMPLE_BINS / 32));
-    Kept kept;
+    row.bins = fminf((float)(inv_t * (SAMPLE_BINS / 32)), FLT_MAX);  // 0 times it is 0
+    Kept kept = {top == INFINITY ? INFINITY : -FLT_MAX, 0x7fffffff};
     const int k = p.top_k ? p.top_k[r] : 0;
     int list = 0;
     if (k > 0 && k < p.vocab) list = row.cut<false>(kept, [&](u64) { return (u64)k; });
@@ -527,7 +572,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     if (mp > 0.0f && temp < INFINITY) {  // an infinite temperature makes all finite logits equal
         // the smallest f32 logit that passes: the border in f64 is within a rounding of it
         const double border = log((double)fminf(mp, 1.0f));
-        const auto passes = [&](float x) { return x == row.top || ((double)x - (double)row.top) * inv_t >= border; };
+        const auto passes = [&](float x) { return x >= row.top || ((double)x - (double)row.top) * inv_t >= border; };
         float x = fminf((float)((double)row.top + border * (double)temp), row.top);
         for (int i = 0; i < 4 && !passes(x); ++i) x = nextafterf(x, INFINITY);
         for (int i = 0; i < 4 && x > -INFINITY && passes(nextafterf(x, -INFINITY)); ++i) x = nextafterf(x, -INFINITY);
@@ -535,15 +580,20 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     }
     const float tp = p.top_p ? p.top_p[r] : 1.0f;
     const auto nucleus = [&](u64 all) { return min(max((u64)ceil((double)fmaxf(tp, 0.0f) * (double)all), 1ull), all); };
+    bool summed = false;
     if (tp < 1.0f) {
-        if (list) row.cut_list<true>(kept, list, nucleus(row.keep_list(kept, list)));
-        else list = row.cut<true>(kept, nucleus);
+        if (list) {
+            row.cut_list<true>(kept, list, nucleus(row.keep_list(kept, list)));
+        } else {
+            list = row.cut<true>(kept, nucleus);
+            summed = true;
+        }
     }
     const float u = p.u[r];
     const auto chosen = [&](float x, int i, u64 all) {
         p.tokens[r] = i;
         if (p.logprobs) {
-            const double e = x == row.top ? 0.0 : ((double)x - (double)row.top) * inv_t;
+            const double e = ((double)fminf(x, FLT_MAX) - (double)row.top) * inv_t;
             p.logprobs[r] = (float)(e - log((double)all * 0x1p-44));
         }
     };
@@ -555,29 +605,26 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         ptx::cluster_sync();  // the others have read this CTA's candidates
         return;
     }
-    // ---- the draw: warps sum contiguous segments, the segment that holds the number is walked in index order
-    const int seg = (row.quads() + SAMPLE_WARPS - 1) / SAMPLE_WARPS, s0 = min(row.quads(), warp * seg), s1 = min(row.quads(), s0 + seg);
-    u64 s = 0;
-    const auto weigh = [&](const float (&x)[4], int i, u64 (&w)[4]) {  // what lies behind the slice has weight 0
-        bool in[4];
+    // ---- the draw: the warps' sums of kept weights, then the segment that holds the number is walked in index order
+    const auto kept4 = [&](const float (&x)[4], int i, bool (&in)[4]) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) in[k] = kept(x[k], i + k);
-        row.weigh(x, in, w);
+        for (int j = 0; j < 4; ++j) in[j] = kept(x[j], i + j);
     };
-    row.each4(s0 + lane, 32, s1, [&](const float (&x)[4], int i) {
-        u64 w[4];
-        weigh(x, i, w);
-        s += (w[0] + w[1]) + (w[2] + w[3]);
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    __syncthreads();
-    if (lane == 0) sh.scratch[warp] = s;
-    __syncthreads();
+    if (!summed) {
+        u64 s = 0;
+        row.each4<false>([&](const float (&x)[4], int i) {
+            bool in[4];
+            kept4(x, i, in);
+            s += row.weigh(x, in);
+        });
+        s = warp_sum(s);
+        if (lane == 0) sh.segment[warp] = s;
+        __syncthreads();
+    }
     u64 before = 0, mine = 0, z = 0;
     for (int w = 0; w < SAMPLE_WARPS; ++w) {
-        if (w < warp) before += sh.scratch[w];
-        mine += sh.scratch[w];
+        if (w < warp) before += sh.segment[w];
+        mine += sh.segment[w];
     }
     row.tell(mine, 2);
     ptx::cluster_sync();  // nothing of another CTA is read from here on
@@ -586,34 +633,29 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         z += sh.slot[2][c];
     }
     const u64 draw = drawn(u, z);
-    if (draw < before || draw >= before + s) return;  // one warp of the cluster goes on
-    for (int i = s0; i < s1; i += 32) {
-        u64 w[4] = {}, inc = 0;
-        float x[4];
-        row.each4(i + lane, 32, min(s1, i + 32), [&](const float (&v)[4], int at) {
+    if (draw < before || draw >= before + sh.segment[warp]) return;  // one warp of the cluster goes on
+    bool done = false;
+    row.each4<true>([&](const float (&x)[4], int i) {
+        bool in[4];
+        kept4(x, i, in);
+        u64 w[4], own = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = v[k];
-            weigh(v, at, w);
-            inc = (w[0] + w[1]) + (w[2] + w[3]);
-        });
-        const u64 own = inc;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 up = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += up;
+        for (int j = 0; j < 4; ++j) {
+            w[j] = in[j] ? row.weight(x[j]) : 0ull;
+            own += w[j];
         }
-        const u64 all = __shfl_sync(0xffffffffu, inc, 31);
-        if (draw < before + all) {
+        const u64 inc = warp_scan(own), all = __shfl_sync(0xffffffffu, inc, 31);
+        if (!done && draw < before + all) {
             u64 at = before + inc - own;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (draw >= at && draw < at + w[k]) chosen(x[k], row.i0 + 4 * (i + lane) + k, z);
-                at += w[k];
+            for (int j = 0; j < 4; ++j) {
+                if (draw >= at && draw < at + w[j]) chosen(x[j], i + j, z);
+                at += w[j];
             }
-            return;
+            done = true;
         }
         before += all;
-    }
+    });
 }
 
 }  // namespace kb
@@ -631,15 +673,19 @@ extern "C" int kb_sample(const float *logits, size_t n, size_t vocab, size_t ld,
     if (n > 0x7fffffffu / SAMPLE_CTAS) return fail(KB_ERR_UNSUPPORTED, "sample: %zu rows", n);
     int dev = 0;
     KB_CUDA(cudaGetDevice(&dev));
-    // CTAs per row: all eight for the few rows that leave SMs idle, otherwise slices of up to 16384 logits; at least 1024 each
-    const size_t per = n * SAMPLE_CTAS <= (size_t)sm_count(dev) * 2 ? 1024 : 16384;
+    // CTAs per row: slices of at least 1024 logits, and as many CTAs as there are: a batch of unlike rows (greedy ones next to
+    // flat nuclei) fills the SMs better in many short CTAs than in one round of long ones (128 mixed rows of 131072: 115 us with
+    // eight, 140 with four, 190 with two)
+    const size_t sms = (size_t)sm_count(dev);
     int ctas = 1;
-    while (ctas < SAMPLE_CTAS && vocab > per * ctas) ctas *= 2;
+    while (ctas < SAMPLE_CTAS && vocab > (size_t)1024 * ctas) ctas *= 2;
     const int slice = (int)(((vocab + ctas - 1) / ctas + 3) / 4 * 4);
-    SampleParams p = {logits, ld, (int)vocab, slice, temperature, top_k, top_p, min_p, u, tokens, logprobs};
-    const size_t fixed = (sizeof(SampleShared) + 15) / 16 * 16;
-    const size_t smem = fixed + (slice <= SAMPLE_SLICE ? (size_t)((slice + 127) / 128 * 128) * 4 : 0);
-    if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(sample_kernel), dev, (int)(fixed + SAMPLE_SLICE * 4), "sample smem attribute")) return rc;
+    // the slice in shared memory where one CTA per SM (few rows), or two, have the room
+    const size_t room = n * ctas <= sms ? 200 * 1024 : 100 * 1024;
+    const bool held = SAMPLE_FIXED + (size_t)slice * 4 <= room;
+    SampleParams p = {logits, ld, (int)vocab, slice, held, temperature, top_k, top_p, min_p, u, tokens, logprobs};
+    const size_t smem = SAMPLE_FIXED + (held ? (size_t)slice * 4 : 0);
+    if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(sample_kernel), dev, 200 * 1024, "sample smem attribute")) return rc;
     static const bool pdl = [] { const char *v = getenv("KB_GEMV_PDL"); return !(v && *v == '0'); }();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ctas));
