@@ -161,21 +161,21 @@ struct Row {
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[k] = 4 * i + k < n ? l[4 * i + k] : -INFINITY;
         }
+        if (!held) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = clean(x[k]);
+        }
     }
     // f(four logits, index of the first) for the quads of this warp's segment, in index order; elements behind the slice are
-    // -inf.  The next quad is loaded before this one is used.  WHOLE: all lanes go around.
+    // -inf.  WHOLE: all lanes go around.
     template <bool WHOLE, typename F>
     __device__ __forceinline__ void each4(F f) const {
         const int lane = threadIdx.x & 31;
-        float x[4], y[4];
-        if (q0 + lane < q1) load4(q0 + lane, x);
+#pragma unroll 1
         for (int i = q0 + lane; WHOLE ? i - lane < q1 : i < q1; i += 32) {
-            if (i + 32 < q1) load4(i + 32, y);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = WHOLE && i >= q1 ? -INFINITY : held ? x[k] : clean(x[k]);
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (!WHOLE || i < q1) load4(i, x);
             f(x, i0 + 4 * i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = y[k];
         }
     }
     // sum of the weights of the four where `in`, all under way at once; nothing is done where the warp has none
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         float *held = reinterpret_cast<float *>(smem + SAMPLE_FIXED);
         row.l = held;
         const int body = row.wide ? row.n / 4 : 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = threadIdx.x; i < body; i += SAMPLE_THREADS) {
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(src) + i);
             reinterpret_cast<float4 *>(held)[i] = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
