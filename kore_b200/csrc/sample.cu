@@ -276,6 +276,49 @@ struct Row {
         hi = max(hi, c);
     }
 
+    // Top-k for a k that is small against the number of threads: a histogram of the threads' own largest logits (mine_top) is
+    // enough.  k of them lie in the bins up to some b, so the k largest of all do, and hardly more than k others with them.
+    // Returns the length of the list, or 0 where it would be too long or the maxima too few.
+    __device__ int cut_few(Kept &kept, float mine_top, int k) const {
+        hist_clear();
+        if (threadIdx.x == 0) sh.bin[1] = SAMPLE_BINS - 1;
+        if (mine_top >= -FLT_MAX) atomicAdd(sh.hist[0] + (int)bin_at(mine_top), 1u);
+        ptx::cluster_sync();
+        u64 mine[2];
+        hist_row(0, mine);
+        find_bin(mine, (u64)k);
+        if (threadIdx.x == 0) sh.n_own = 0;
+        __syncthreads();
+        const int b1 = sh.bin[1];
+        u64 lo = ~0ull, hi = 0;
+        if (b1 < SAMPLE_BINS - 1) {
+            const float to = (float)(b1 + 1);
+            each4<false>([&](const float (&x)[4], int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (bin_at(x[j]) < to && kept(x[j], i + j)) collect(comp_of(x[j], i + j), lo, hi);
+            });
+        }
+        __syncthreads();
+        tell(sh.n_own, 5);
+        ptx::cluster_sync();
+        const u64 count = told(5, plus);
+        if (count == 0 || count > SAMPLE_CAND) return 0;
+        fetch_list(count);
+        cut_list<false>(kept, (uint32_t)count, (u64)k);
+        return (int)count;
+    }
+    // the candidates of all CTAs (their numbers in slot 5) into sh.all, and their weights
+    __device__ void fetch_list(u64 count) const {
+        uint32_t c = 0;
+        u64 base = 0;
+        for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
+            while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
+            const u64 e = ld_cluster(sh.own + (i - base), c);
+            sh.all[i] = e;
+            sh.measure[i] = weight(logit_of(e));
+        }
+    }
     // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
     // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.  Returns the
     // length of the list in sh.all that holds all that is kept, or 0 where there is none; WEIGHT without a list: sh.segment
@@ -416,14 +459,7 @@ struct Row {
             ptx::cluster_sync();
             count = told(5, plus);
         }
-        uint32_t c = 0;
-        u64 base = 0;
-        for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
-            while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
-            const u64 e = ld_cluster(sh.own + (i - base), c);
-            sh.all[i] = e;
-            sh.measure[i] = weight(logit_of(e));
-        }
+        fetch_list(count);
         cut_list<WEIGHT>(kept, (uint32_t)count, target);
         if (list) return (int)count;
         if (WEIGHT) {  // the kept candidates of this CTA go to their segments
@@ -529,7 +565,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     } else {
         row.each4<false>([&](const float (&x)[4], int) { top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))); });
     }
-    const float temp = p.temperature ? p.temperature[r] : 1.0f;
+    const float mine_top = top, temp = p.temperature ? p.temperature[r] : 1.0f;
     // the smallest of ~ordered bits: one instruction a warp
     const uint32_t warp_top = __reduce_min_sync(0xffffffffu, (uint32_t)(comp_of(top + 0.0f, 0) >> 32));
     if (lane == 0) sh.scratch[warp] = warp_top;
@@ -567,7 +603,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     Kept kept = {top == INFINITY ? INFINITY : -FLT_MAX, 0x7fffffff};
     const int k = p.top_k ? p.top_k[r] : 0;
     int list = 0;
-    if (k > 0 && k < p.vocab) list = row.cut<false>(kept, [&](u64) { return (u64)k; });
+    if (k > 0 && k < p.vocab) {
+        if (k <= SAMPLE_CAND / 2) list = row.cut_few(kept, mine_top, k);
+        if (!list) list = row.cut<false>(kept, [&](u64) { return (u64)k; });
+    }
     const float mp = p.min_p ? p.min_p[r] : 0.0f;
     if (mp > 0.0f && temp < INFINITY) {  // an infinite temperature makes all finite logits equal
         // the smallest f32 logit that passes: the border in f64 is within a rounding of it
