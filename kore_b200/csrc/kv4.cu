@@ -52,18 +52,19 @@ struct AppendParams {
     const int *positions;
     const long long *cache_rows;
     const float *cos_t, *sin_t;
-    long long max_pos;
+    int max_pos;
     const float *q_gamma, *k_gamma;
     float eps;
-    long long tasks;  // tokens * (n_heads + 2 n_kv)
+    unsigned tasks, groups;  // tokens * groups of heads
     int n_heads, n_kv, hd;
     long long cache_len;  // n_seqs * lmax
     int lmax;
+    bool pairs;  // rows and tables are 8-byte aligned: a lane's two neighbours come in one load
     float *q_out, *k_cache, *v_cache;
     uint32_t *k_codes, *k_steps, *v_codes, *v_steps;
 };
 
-// x >= 0 or x < 0, finite: the bfloat16 at or below x, and (x >= 0) the one at or above it
+// the bfloat16 at or below x (finite), and the one at or above x >= 0
 __device__ __forceinline__ float bf16_below(float x) {
     const uint32_t i = __float_as_uint(x), cut = i & 0xffff0000u;
     return __uint_as_float(x < 0.0f && i != cut ? cut + 0x10000u : cut);
@@ -72,133 +73,243 @@ __device__ __forceinline__ float bf16_above_nonneg(float x) {
     const uint32_t i = __float_as_uint(x), cut = i & 0xffff0000u;
     return __uint_as_float(i != cut ? cut + 0x10000u : cut);
 }
+__device__ __forceinline__ float warp_min(float x) {
+    float y;
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float warp_absmax_or_nan(float x) {
+    float y;
+    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+// sequence and position of a cache row
+__device__ __forceinline__ void split_row(long long row, int lmax, size_t &seq, size_t &pos) {
+    if (row >> 32) {
+        seq = (size_t)(row / lmax);
+        pos = (size_t)(row - (long long)seq * lmax);
+    } else {
+        seq = (uint32_t)row / (uint32_t)lmax;
+        pos = (uint32_t)row - (uint32_t)seq * (uint32_t)lmax;
+    }
+}
+// 1 / sqrt(x) to 2^-52: an f32 estimate and two Newton steps, 9 f64 operations where division and root take ten times as many
+__device__ __forceinline__ double rsqrt_f64(double x) {
+    if (!(x > 1e-30 && x < 1e30)) return 1.0 / sqrt(x);
+    double y = (double)rsqrtf((float)x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return y;
+}
+// sums over the warp, of HPW values at once: while a lane holds several it passes on half of them
+template <int HPW>
+__device__ __forceinline__ void warp_sums(double (&v)[HPW]) {
+    const int lane = threadIdx.x & 31;
+    if (HPW == 4) {
+        const bool up16 = lane & 16, up8 = lane & 8;
+        double a[2], b;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            a[i] = (up16 ? v[(2 + i) % HPW] : v[i % HPW]) + __shfl_xor_sync(0xffffffffu, up16 ? v[i % HPW] : v[(2 + i) % HPW], 16);
+        b = (up8 ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, up8 ? a[0] : a[1], 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
+#pragma unroll
+        for (int i = 0; i < HPW; ++i) v[i] = __shfl_sync(0xffffffffu, b, 8 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < HPW; ++i)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+}
 
-// A warp takes one head of one token.  Lane l owns the rotation pairs 2l and 2l + 1, dims {2l, 2l + 1} of each half:
-// its codes are then whole bytes of the row, and a row needs no shared memory.
-template <bool Q4>
+// Bound by the bytes of the rows for many tokens, by one memory round trip for a few.  A warp takes HPW heads of one token:
+// its lane l owns the rotation pairs 2l and 2l + 1, dims {2l, 2l + 1} of each half, so that its codes are whole bytes of the
+// row, a row needs no shared memory, and the token's angles are read once for all heads.
+template <bool Q4, int HPW>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     const int lane = threadIdx.x & 31;
-    const long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const unsigned task = blockIdx.x * 8u + (threadIdx.x >> 5);
     release_and_wait();
     if (task >= p.tasks) return;
     const int heads = p.n_heads + 2 * p.n_kv, hd = p.hd, half = hd / 2;
-    const long long t = task / heads;
-    const int head = (int)(task - t * heads);
-    const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.n_kv;
-    const long long pos = p.positions[t];
-    const bool pos_ok = pos >= 0 && pos < p.max_pos;
-    const long long crow = p.cache_rows[t];
-    if (!is_q && (!pos_ok || crow < 0 || crow >= p.cache_len)) return;  // not appended
-    const float *row = p.qkv + (size_t)t * p.ld + (size_t)head * hd;
+    const unsigned t = task / p.groups;
+    const int head0 = (int)(task - t * p.groups) * HPW;
     const int i0 = 2 * lane;
     const bool own0 = i0 < half, own1 = i0 + 1 < half;
-    float a[2] = {own0 ? row[i0] : 0.0f, own1 ? row[i0 + 1] : 0.0f};
-    float b[2] = {own0 ? row[half + i0] : 0.0f, own1 ? row[half + i0 + 1] : 0.0f};
-    const float *gamma = is_q ? p.q_gamma : p.k_gamma;
-    if (!is_v && gamma) {
-        double ss = 0.0;  // f64: the order of the sum then cannot move a rounding of inv, so codes do not depend on it
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ss += (double)a[i] * a[i] + (double)b[i] * b[i];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = (float)(1.0 / sqrt(ss / hd + (double)p.eps));
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i0 + i < half) {
-                a[i] = __fmul_rn(__fmul_rn(a[i], inv), gamma[i0 + i]);
-                b[i] = __fmul_rn(__fmul_rn(b[i], inv), gamma[half + i0 + i]);
-            }
-    }
-    if (!is_v && pos_ok) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i0 + i < half) {
-                const float c = p.cos_t[(size_t)pos * half + i0 + i], s = p.sin_t[(size_t)pos * half + i0 + i];
-                const float x = a[i], y = b[i];
-                a[i] = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
-                b[i] = __fadd_rn(__fmul_rn(x, s), __fmul_rn(y, c));
-            }
-    }
-    if (is_q) {
-        float *q = p.q_out + ((size_t)t * p.n_heads + head) * hd;
-        const float bad = __uint_as_float(0x7fffffffu);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i0 + i < half) {
-                q[i0 + i] = pos_ok ? a[i] : bad;
-                q[half + i0 + i] = pos_ok ? b[i] : bad;
-            }
-        return;
-    }
-    const int kvh = is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
-    const size_t crow_head = ((size_t)(crow / p.lmax) * p.n_kv + kvh) * p.lmax + (size_t)(crow % p.lmax);
-    if (!Q4) {
-        float *dst = (is_v ? p.v_cache : p.k_cache) + crow_head * hd;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i0 + i < half) {
-                dst[i0 + i] = a[i];
-                dst[half + i0 + i] = b[i];
-            }
-        return;
-    }
-    // hd is a multiple of 4 here, so a lane owns both of its pairs or none
-    float mn = own0 ? fminf(fminf(a[0], a[1]), fminf(b[0], b[1])) : INFINITY;
-    float mx = own0 ? fmaxf(fmaxf(a[0], a[1]), fmaxf(b[0], b[1])) : -INFINITY;
-    const float big = fmaxf(fmaxf(fabsf(a[0]), fabsf(a[1])), fmaxf(fabsf(b[0]), fabsf(b[1])));
-    const bool nan = a[0] != a[0] || a[1] != a[1] || b[0] != b[0] || b[1] != b[1];  // fmaxf passes over them
-    const bool broken = __any_sync(0xffffffffu, own0 && (nan || big == INFINITY));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    const float lo = bf16_below(mn);
-    const float step = bf16_above_nonneg(fmaxf(__fdiv_rn(__fsub_rn(mx, lo), 15.0f), 0x1p-100f));
-    const bool ok = !broken && fabsf(lo) < INFINITY && step < INFINITY;
-    const float inv = __frcp_rn(step);
-    auto code = [&](float x) {
-        const int c = ok ? __float2int_rn(__fmul_rn(__fsub_rn(x, lo), inv)) : 0;
-        return (uint32_t)max(0, min(15, c));
+    float a[HPW][2], b[HPW][2];
+    const float *row = p.qkv + (size_t)t * p.ld + (size_t)head0 * hd;
+    auto load2 = [&](const float *src, float (&x)[2]) {
+        if (p.pairs) {  // half is even then
+            const float2 v = own0 ? *reinterpret_cast<const float2 *>(src + i0) : make_float2(0.0f, 0.0f);
+            x[0] = v.x; x[1] = v.y;
+        } else {
+            x[0] = own0 ? src[i0] : 0.0f;
+            x[1] = own1 ? src[i0 + 1] : 0.0f;
+        }
     };
-    const int words = kv4_words(hd);
-    uint8_t *bytes = reinterpret_cast<uint8_t *>((is_v ? p.v_codes : p.k_codes) + crow_head * words);
-    if (own0) {
-        bytes[lane] = (uint8_t)(code(a[0]) | code(a[1]) << 4);
-        bytes[half / 2 + lane] = (uint8_t)(code(b[0]) | code(b[1]) << 4);
+#pragma unroll
+    for (int j = 0; j < HPW; ++j) {
+        a[j][0] = a[j][1] = b[j][0] = b[j][1] = 0.0f;
+        if (head0 + j < heads) {
+            load2(row + j * hd, a[j]);
+            load2(row + j * hd + half, b[j]);
+        }
     }
-    if (lane < 4 * words - half) bytes[half + lane] = 0;  // tail of the last word
-    if (lane == 0)
-        (is_v ? p.v_steps : p.k_steps)[crow_head] = ok ? (__float_as_uint(lo) | __float_as_uint(step) >> 16) : 0x7fc07fc0u;
+    const int pos = p.positions[t];
+    const bool pos_ok = pos >= 0 && pos < p.max_pos;
+    const long long crow = p.cache_rows[t];
+    const bool stored = pos_ok && crow >= 0 && crow < p.cache_len;
+    float c[2] = {}, s[2] = {};
+    if (head0 < p.n_heads + p.n_kv && pos_ok) {
+        load2(p.cos_t + (size_t)pos * half, c);
+        load2(p.sin_t + (size_t)pos * half, s);
+    }
+    if (p.q_gamma || p.k_gamma) {
+        double ss[HPW];  // f64: the order of the sum then cannot move a rounding of inv, so codes do not depend on it
+#pragma unroll
+        for (int j = 0; j < HPW; ++j) {
+            ss[j] = 0.0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) ss[j] = fma((double)a[j][i], (double)a[j][i], fma((double)b[j][i], (double)b[j][i], ss[j]));
+        }
+        warp_sums<HPW>(ss);
+        const double per = 1.0 / hd;
+        float g[2][4] = {};
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const float *gamma = side ? p.k_gamma : p.q_gamma;
+            if (gamma) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (i0 + i < half) {
+                        g[side][i] = gamma[i0 + i];
+                        g[side][2 + i] = gamma[half + i0 + i];
+                    }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < HPW; ++j) {
+            const bool is_k = head0 + j >= p.n_heads;
+            if (head0 + j >= p.n_heads + p.n_kv || !(is_k ? p.k_gamma : p.q_gamma)) continue;
+            const float inv = (float)rsqrt_f64(ss[j] * per + (double)p.eps);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), is_k ? g[1][i] : g[0][i]);
+                b[j][i] = __fmul_rn(__fmul_rn(b[j][i], inv), is_k ? g[1][2 + i] : g[0][2 + i]);
+            }
+        }
+    }
+    size_t seq = 0, cpos = 0;
+    if (stored) split_row(crow, p.lmax, seq, cpos);
+#pragma unroll
+    for (int j = 0; j < HPW; ++j) {
+        const int head = head0 + j;
+        if (head >= heads) break;
+        const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.n_kv;
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float x = a[j][i], y = b[j][i];
+                a[j][i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+                b[j][i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
+            }
+        }
+        if (!is_q && !stored) continue;
+        const int kvh = is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
+        const size_t at = (seq * p.n_kv + kvh) * p.lmax + cpos;
+        if (is_q || !Q4) {
+            float *dst = is_q ? p.q_out + ((size_t)t * p.n_heads + head) * hd : (is_v ? p.v_cache : p.k_cache) + at * hd;
+            const float bad = __uint_as_float(0x7fffffffu);
+            if (is_q && !pos_ok) a[j][0] = a[j][1] = b[j][0] = b[j][1] = bad;
+            if (p.pairs) {
+                if (own0) {
+                    *reinterpret_cast<float2 *>(dst + i0) = make_float2(a[j][0], a[j][1]);
+                    *reinterpret_cast<float2 *>(dst + half + i0) = make_float2(b[j][0], b[j][1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (i0 + i < half) {
+                        dst[i0 + i] = a[j][i];
+                        dst[half + i0 + i] = b[j][i];
+                    }
+            }
+            continue;
+        }
+        // hd is a multiple of 4 here, so a lane owns both of its pairs or none
+        const float mn = warp_min(own0 ? fminf(fminf(a[j][0], a[j][1]), fminf(b[j][0], b[j][1])) : INFINITY);
+        const float mx = warp_max(own0 ? fmaxf(fmaxf(a[j][0], a[j][1]), fmaxf(b[j][0], b[j][1])) : -INFINITY);
+        // fmaxf passes over NaN, a difference of infinities or with a NaN does not
+        const float any = warp_absmax_or_nan(own0 ? (a[j][0] - a[j][0]) + (a[j][1] - a[j][1]) + (b[j][0] - b[j][0]) + (b[j][1] - b[j][1]) : 0.0f);
+        const float lo = bf16_below(mn);
+        const float step = bf16_above_nonneg(fmaxf(__fdiv_rn(__fsub_rn(mx, lo), 15.0f), 0x1p-100f));
+        const bool ok = any == 0.0f && fabsf(lo) < INFINITY && step < INFINITY;
+        const float inv = __frcp_rn(step);
+        auto code = [&](float x) {  // rounded to even in the low bits by adding 1.5 2^23
+            const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x, lo), inv), 0.0f), 15.0f);
+            return ok ? __float_as_uint(y + 12582912.0f) & 15u : 0u;
+        };
+        const int words = kv4_words(hd);
+        uint8_t *bytes = reinterpret_cast<uint8_t *>((is_v ? p.v_codes : p.k_codes) + at * words);
+        if (own0) {
+            bytes[lane] = (uint8_t)(code(a[j][0]) | code(a[j][1]) << 4);
+            bytes[half / 2 + lane] = (uint8_t)(code(b[j][0]) | code(b[j][1]) << 4);
+        }
+        if (lane < 4 * words - half) bytes[half + lane] = 0;  // tail of the last word
+        if (lane == 0) (is_v ? p.v_steps : p.k_steps)[at] = ok ? (__float_as_uint(lo) | __float_as_uint(step) >> 16) : 0x7fc07fc0u;
+    }
 }
 
 // ---- read-back ---------------------------------------------------------------------------------
-// A warp takes one head of one row: lanes 0..15 the words of K, lanes 16..31 those of V, eight values (32 bytes) a lane.
+// Bound by the bytes written.  A warp takes one row and up to four heads of it; a lane writes 16 bytes of K and of V, so a
+// store covers whole lines, and reads its 16 bits of codes from a word that it shares with its neighbour.
+constexpr int READ_HEADS = 4;
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes,
-                                                       const uint32_t *v_steps, const long long *cache_rows, long long tasks, int n_kv,
-                                                       int hd, long long cache_len, int lmax, float *k_out, float *v_out) {
-    const int lane = threadIdx.x & 31, w = lane & 15;
-    const long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+                                                       const uint32_t *v_steps, const long long *cache_rows, unsigned tasks, unsigned groups,
+                                                       int n_kv, int hd, long long cache_len, int lmax, float *k_out, float *v_out) {
+    const int lane = threadIdx.x & 31;
+    const unsigned task = blockIdx.x * 8u + (threadIdx.x >> 5);
     release_and_wait();
-    if (task >= tasks) return;
-    const bool is_v = lane >= 16;
-    const int words = kv4_words(hd);
-    float *out = is_v ? v_out : k_out;
-    if (!out || w >= words) return;
-    const long long i = task / n_kv;
-    const int head = (int)(task - i * n_kv);
+    if (task >= tasks || 4 * lane >= hd) return;
+    const unsigned i = task / groups;
+    const int head0 = (int)(task - i * groups) * READ_HEADS, words = kv4_words(hd);
     const long long crow = cache_rows[i];
-    float v[8] = {};
-    if (crow >= 0 && crow < cache_len) {
-        const size_t at = ((size_t)(crow / lmax) * n_kv + head) * lmax + (size_t)(crow % lmax);
-        const uint32_t c = (is_v ? v_codes : k_codes)[at * words + w], s = (is_v ? v_steps : k_steps)[at];
-        const float step = kv4_step(s), lo = kv4_lo(s);
+    const bool ok = crow >= 0 && crow < cache_len;
+    size_t seq = 0, pos = 0;
+    if (ok) split_row(crow, lmax, seq, pos);
+    uint32_t c[2][READ_HEADS], s[2][READ_HEADS];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf((float)((c >> (4 * j)) & 15u), step, lo);
+    for (int j = 0; j < READ_HEADS; ++j) {
+        const bool live = ok && head0 + j < n_kv;
+        const size_t at = (seq * n_kv + (live ? head0 + j : 0)) * lmax + pos;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const bool get = live && (side ? v_out : k_out);
+            c[side][j] = get ? (side ? v_codes : k_codes)[at * words + (lane >> 1)] >> (16 * (lane & 1)) : 0u;
+            s[side][j] = get ? (side ? v_steps : k_steps)[at] : 0u;  // a row outside the cache: lo + 0 * 0 = 0
+        }
     }
-    float4 *dst = reinterpret_cast<float4 *>(out + (size_t)task * hd + 8 * w);
-    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-    if (8 * w + 4 < hd) dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+    for (int j = 0; j < READ_HEADS; ++j) {
+        if (head0 + j >= n_kv) return;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            float *out = side ? v_out : k_out;
+            if (!out) continue;
+            const float step = kv4_step(s[side][j]), lo = kv4_lo(s[side][j]);
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = fmaf(__uint_as_float(0x4b000000u | (c[side][j] >> (4 * k) & 15u)) - 8388608.0f, step, lo);
+            *reinterpret_cast<float4 *>(out + ((size_t)i * n_kv + head0 + j) * hd + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
 }
 
 // ---- attention ---------------------------------------------------------------------------------
@@ -727,11 +838,11 @@ static bool aligned16(const void *a, const void *b = nullptr, const void *c = nu
     return !((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d)) & 15);
 }
 
-// blocks of 8 warps for `tasks` warps
-static int warp_grid(long long tasks, unsigned *grid) {
-    const long long g = (tasks + 7) / 8;
-    if (g > 0x7fffffffLL) return fail(KB_ERR_UNSUPPORTED, "%lld rows in one call", tasks);
-    *grid = (unsigned)g;
+// blocks of 8 warps for `rows * groups` warps
+static int warp_grid(size_t rows, size_t groups, unsigned *tasks, unsigned *grid) {
+    if (rows > 0x7fffffffu || groups > 0x7fffffffu || rows * groups > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "%zu rows of %zu head groups in one call", rows, groups);
+    *tasks = (unsigned)(rows * groups);
+    *grid = (*tasks + 7) / 8;
     return KB_OK;
 }
 
@@ -741,13 +852,22 @@ static int append(AppendParams &p, bool q4, size_t n, size_t max_pos, size_t n_s
     if (p.ld < heads * p.hd) return fail(KB_ERR_INVALID, "append: row stride %zu below %zu", p.ld, heads * p.hd);
     if (!(p.eps >= 0.0f)) return fail(KB_ERR_INVALID, "append: eps must not be negative");
     if (n == 0) return KB_OK;
-    if (n > 0x7fffffffu || heads > 0xffffffu || max_pos > 0x7fffffffu || n_seqs > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "append: %zu tokens of %zu heads", n, heads);
-    p.tasks = (long long)n * (long long)heads;
-    p.max_pos = (long long)max_pos;
+    if (n > 0x7fffffffu || heads > 0xffffffu || max_pos > 0x7fffffffu || n_seqs > 0x7fffffffu)
+        return fail(KB_ERR_UNSUPPORTED, "append: %zu tokens of %zu heads, %zu sequences", n, heads, n_seqs);
+    p.max_pos = (int)max_pos;
     p.cache_len = (long long)n_seqs * p.lmax;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.qkv) | reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t) |
+                          reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache);
+    p.pairs = p.hd % 4 == 0 && p.ld % 2 == 0 && all % 8 == 0;
+    // one head per warp while that leaves warps to spare (16 per SM), four for many tokens
+    int dev = 0;
+    KB_CUDA(cudaGetDevice(&dev));
+    const bool many = n * heads > (size_t)sm_count(dev) * 16;
+    p.groups = (unsigned)(many ? (heads + 3) / 4 : heads);
     unsigned grid = 0;
-    if (int rc = warp_grid(p.tasks, &grid)) return rc;
-    const cudaError_t e = launch_after(q4 ? append_kernel<true> : append_kernel<false>, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
+    if (int rc = warp_grid(n, p.groups, &p.tasks, &grid)) return rc;
+    void (*kern)(AppendParams) = q4 ? (many ? append_kernel<true, 4> : append_kernel<true, 1>) : (many ? append_kernel<false, 4> : append_kernel<false, 1>);
+    const cudaError_t e = launch_after(kern, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "append launch");
 }
 
@@ -800,12 +920,12 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
     if (!aligned16(k_codes, k_steps, v_codes, v_steps) || !aligned16(k_out, v_out))
         return fail(KB_ERR_INVALID, "kv4: planes and outputs must be 16-byte aligned");
     if (n == 0) return KB_OK;
-    if (n > 0x7fffffffu || n_seqs > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "kv4: %zu rows of %zu sequences", n, n_seqs);
-    const long long tasks = (long long)n * n_kv_heads;
-    unsigned grid = 0;
-    if (int rc = warp_grid(tasks, &grid)) return rc;
+    if (n_seqs > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "kv4: %zu sequences", n_seqs);
+    unsigned tasks = 0, grid = 0;
+    const unsigned groups = (unsigned)(n_kv_heads + READ_HEADS - 1) / READ_HEADS;
+    if (int rc = warp_grid(n, groups, &tasks, &grid)) return rc;
     const cudaError_t e = launch_after(kv4_read_kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), k_codes, k_steps, v_codes,
-                                       v_steps, cache_rows, tasks, n_kv_heads, head_dim, (long long)n_seqs * lmax, lmax, k_out, v_out);
+                                       v_steps, cache_rows, tasks, groups, n_kv_heads, head_dim, (long long)n_seqs * lmax, lmax, k_out, v_out);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 read launch");
 }
 
