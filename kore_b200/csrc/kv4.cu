@@ -106,27 +106,26 @@ __device__ __forceinline__ double rsqrt_f64(double x) {
     for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
     return y;
 }
-// sums over the warp, of HPW values at once: while a lane holds several it passes on half of them
+// Sum over the warp of one of HPW values: that of index lane / 8 (HPW = 4: while a lane holds several it passes on half of
+// them), or the only one.  What follows on it is then done for all of them at once.
 template <int HPW>
-__device__ __forceinline__ void warp_sums(double (&v)[HPW]) {
+__device__ __forceinline__ double warp_sum_of(const double (&v)[HPW]) {
     const int lane = threadIdx.x & 31;
+    double x = v[0];
     if (HPW == 4) {
         const bool up16 = lane & 16, up8 = lane & 8;
-        double a[2], b;
+        double a[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             a[i] = (up16 ? v[(2 + i) % HPW] : v[i % HPW]) + __shfl_xor_sync(0xffffffffu, up16 ? v[i % HPW] : v[(2 + i) % HPW], 16);
-        b = (up8 ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, up8 ? a[0] : a[1], 8);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
-#pragma unroll
-        for (int i = 0; i < HPW; ++i) v[i] = __shfl_sync(0xffffffffu, b, 8 * i);
+        x = (up8 ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, up8 ? a[0] : a[1], 8);
     } else {
-#pragma unroll
-        for (int i = 0; i < HPW; ++i)
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
     }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
 }
 
 // Bound by the bytes of the rows for many tokens, by one memory round trip for a few.  A warp takes HPW heads of one token:
@@ -179,8 +178,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) ss[j] = fma((double)a[j][i], (double)a[j][i], fma((double)b[j][i], (double)b[j][i], ss[j]));
         }
-        warp_sums<HPW>(ss);
-        const double per = 1.0 / hd;
+        const float inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);  // of head lane / 8
         float g[2][4] = {};
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
@@ -198,7 +196,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
         for (int j = 0; j < HPW; ++j) {
             const bool is_k = head0 + j >= p.n_heads;
             if (head0 + j >= p.n_heads + p.n_kv || !(is_k ? p.k_gamma : p.q_gamma)) continue;
-            const float inv = (float)rsqrt_f64(ss[j] * per + (double)p.eps);
+            const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 8 * j);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), is_k ? g[1][i] : g[0][i]);
@@ -208,6 +206,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     }
     size_t seq = 0, cpos = 0;
     if (stored) split_row(crow, p.lmax, seq, cpos);
+    const size_t at0 = seq * p.n_kv * p.lmax + cpos;
+    float mn_of = 0.0f, mx_of = 0.0f, any_of = 0.0f;  // lane j: of head j
 #pragma unroll
     for (int j = 0; j < HPW; ++j) {
         const int head = head0 + j;
@@ -222,10 +222,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
             }
         }
         if (!is_q && !stored) continue;
-        const int kvh = is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
-        const size_t at = (seq * p.n_kv + kvh) * p.lmax + cpos;
         if (is_q || !Q4) {
-            float *dst = is_q ? p.q_out + ((size_t)t * p.n_heads + head) * hd : (is_v ? p.v_cache : p.k_cache) + at * hd;
+            const int kvh = is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
+            float *dst = is_q ? p.q_out + ((size_t)t * p.n_heads + head) * hd : (is_v ? p.v_cache : p.k_cache) + (at0 + (size_t)kvh * p.lmax) * hd;
             const float bad = __uint_as_float(0x7fffffffu);
             if (is_q && !pos_ok) a[j][0] = a[j][1] = b[j][0] = b[j][1] = bad;
             if (p.pairs) {
@@ -246,24 +245,37 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
         // hd is a multiple of 4 here, so a lane owns both of its pairs or none
         const float mn = warp_min(own0 ? fminf(fminf(a[j][0], a[j][1]), fminf(b[j][0], b[j][1])) : INFINITY);
         const float mx = warp_max(own0 ? fmaxf(fmaxf(a[j][0], a[j][1]), fmaxf(b[j][0], b[j][1])) : -INFINITY);
-        // fmaxf passes over NaN, a difference of infinities or with a NaN does not
-        const float any = warp_absmax_or_nan(own0 ? (a[j][0] - a[j][0]) + (a[j][1] - a[j][1]) + (b[j][0] - b[j][0]) + (b[j][1] - b[j][1]) : 0.0f);
-        const float lo = bf16_below(mn);
-        const float step = bf16_above_nonneg(fmaxf(__fdiv_rn(__fsub_rn(mx, lo), 15.0f), 0x1p-100f));
-        const bool ok = any == 0.0f && fabsf(lo) < INFINITY && step < INFINITY;
-        const float inv = __frcp_rn(step);
+        // fminf and fmaxf pass over NaN; 0 times a NaN or an infinity is NaN
+        const float any = warp_absmax_or_nan(own0 ? fmaf(a[j][0], 0.0f, fmaf(a[j][1], 0.0f, fmaf(b[j][0], 0.0f, b[j][1] * 0.0f))) : 0.0f);
+        if (HPW == 1 || lane == j) mn_of = mn, mx_of = mx, any_of = any;
+    }
+    if (!Q4 || !stored || head0 + HPW <= p.n_heads) return;
+    // the pair of each head, in lane j for head j
+    const float lo_of = bf16_below(mn_of);
+    const float step_of = bf16_above_nonneg(fmaxf(__fdiv_rn(__fsub_rn(mx_of, lo_of), 15.0f), 0x1p-100f));
+    const bool ok_of = any_of == 0.0f && fabsf(lo_of) < INFINITY && step_of < INFINITY;
+    const float inv_of = ok_of ? __frcp_rn(step_of) : 0.0f;  // 0: no row
+    const int words = kv4_words(hd);
+#pragma unroll
+    for (int j = 0; j < HPW; ++j) {
+        const int head = head0 + j;
+        if (head >= heads) break;
+        const float lo = HPW == 1 ? lo_of : __shfl_sync(0xffffffffu, lo_of, j), inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, j);
+        if (head < p.n_heads) continue;
+        const bool is_v = head >= p.n_heads + p.n_kv;
+        const size_t at = at0 + (size_t)(is_v ? head - p.n_heads - p.n_kv : head - p.n_heads) * p.lmax;
         auto code = [&](float x) {  // rounded to even in the low bits by adding 1.5 2^23
-            const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(x, lo), inv), 0.0f), 15.0f);
-            return ok ? __float_as_uint(y + 12582912.0f) & 15u : 0u;
+            return __float_as_uint(fminf(fmaxf(__fmul_rn(__fsub_rn(x, lo), inv), 0.0f), 15.0f) + 12582912.0f) & 15u;
         };
-        const int words = kv4_words(hd);
         uint8_t *bytes = reinterpret_cast<uint8_t *>((is_v ? p.v_codes : p.k_codes) + at * words);
         if (own0) {
-            bytes[lane] = (uint8_t)(code(a[j][0]) | code(a[j][1]) << 4);
-            bytes[half / 2 + lane] = (uint8_t)(code(b[j][0]) | code(b[j][1]) << 4);
+            const bool ok = inv != 0.0f;
+            bytes[lane] = ok ? (uint8_t)(code(a[j][0]) | code(a[j][1]) << 4) : 0;
+            bytes[half / 2 + lane] = ok ? (uint8_t)(code(b[j][0]) | code(b[j][1]) << 4) : 0;
         }
         if (lane < 4 * words - half) bytes[half + lane] = 0;  // tail of the last word
-        if (lane == 0) (is_v ? p.v_steps : p.k_steps)[at] = ok ? (__float_as_uint(lo) | __float_as_uint(step) >> 16) : 0x7fc07fc0u;
+        if (lane == (HPW == 1 ? 0 : j))
+            (is_v ? p.v_steps : p.k_steps)[at] = ok_of ? (__float_as_uint(lo_of) | __float_as_uint(step_of) >> 16) : 0x7fc07fc0u;
     }
 }
 
