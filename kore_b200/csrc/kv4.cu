@@ -73,19 +73,20 @@ __device__ __forceinline__ float bf16_above_nonneg(float x) {
     const uint32_t i = __float_as_uint(x), cut = i & 0xffff0000u;
     return __uint_as_float(i != cut ? cut + 0x10000u : cut);
 }
-__device__ __forceinline__ float warp_min(float x) {
+// minima and maxima that a NaN passes through
+__device__ __forceinline__ float min_nan(float x, float y) {
+    float z;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+__device__ __forceinline__ float warp_min_nan(float x) {
     float y;
-    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    asm volatile("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float warp_max(float x) {
     float y;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float warp_absmax_or_nan(float x) {
-    float y;
-    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
     return y;
 }
 // sequence and position of a cache row
@@ -179,35 +180,33 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
             for (int i = 0; i < 2; ++i) ss[j] = fma((double)a[j][i], (double)a[j][i], fma((double)b[j][i], (double)b[j][i], ss[j]));
         }
         const float inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);  // of head lane / 8
-        float g[2][4] = {};
+        const float *held = nullptr;  // the gamma in g
+        float g[4] = {};
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const float *gamma = side ? p.k_gamma : p.q_gamma;
-            if (gamma) {
+        for (int j = 0; j < HPW; ++j) {
+            const float *gamma = head0 + j < p.n_heads ? p.q_gamma : (head0 + j < p.n_heads + p.n_kv ? p.k_gamma : nullptr);
+            if (!gamma) continue;
+            if (gamma != held) {
+                held = gamma;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     if (i0 + i < half) {
-                        g[side][i] = gamma[i0 + i];
-                        g[side][2 + i] = gamma[half + i0 + i];
+                        g[i] = gamma[i0 + i];
+                        g[2 + i] = gamma[half + i0 + i];
                     }
             }
-        }
-#pragma unroll
-        for (int j = 0; j < HPW; ++j) {
-            const bool is_k = head0 + j >= p.n_heads;
-            if (head0 + j >= p.n_heads + p.n_kv || !(is_k ? p.k_gamma : p.q_gamma)) continue;
             const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 8 * j);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), is_k ? g[1][i] : g[0][i]);
-                b[j][i] = __fmul_rn(__fmul_rn(b[j][i], inv), is_k ? g[1][2 + i] : g[0][2 + i]);
+                a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), g[i]);
+                b[j][i] = __fmul_rn(__fmul_rn(b[j][i], inv), g[2 + i]);
             }
         }
     }
     size_t seq = 0, cpos = 0;
-    if (stored) split_row(crow, p.lmax, seq, cpos);
+    if (stored && head0 + HPW > p.n_heads) split_row(crow, p.lmax, seq, cpos);
     const size_t at0 = seq * p.n_kv * p.lmax + cpos;
-    float mn_of = 0.0f, mx_of = 0.0f, any_of = 0.0f;  // lane j: of head j
+    float mn_of = 0.0f, mx_of = 0.0f;  // lane j: of head j
 #pragma unroll
     for (int j = 0; j < HPW; ++j) {
         const int head = head0 + j;
@@ -243,39 +242,40 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
             continue;
         }
         // hd is a multiple of 4 here, so a lane owns both of its pairs or none
-        const float mn = warp_min(own0 ? fminf(fminf(a[j][0], a[j][1]), fminf(b[j][0], b[j][1])) : INFINITY);
+        const float mn = warp_min_nan(own0 ? min_nan(min_nan(a[j][0], a[j][1]), min_nan(b[j][0], b[j][1])) : INFINITY);
         const float mx = warp_max(own0 ? fmaxf(fmaxf(a[j][0], a[j][1]), fmaxf(b[j][0], b[j][1])) : -INFINITY);
-        // fminf and fmaxf pass over NaN; 0 times a NaN or an infinity is NaN
-        const float any = warp_absmax_or_nan(own0 ? fmaf(a[j][0], 0.0f, fmaf(a[j][1], 0.0f, fmaf(b[j][0], 0.0f, b[j][1] * 0.0f))) : 0.0f);
-        if (HPW == 1 || lane == j) mn_of = mn, mx_of = mx, any_of = any;
+        if (HPW == 1 || lane == j) mn_of = mn, mx_of = mx;
     }
     if (!Q4 || !stored || head0 + HPW <= p.n_heads) return;
-    // the pair of each head, in lane j for head j
+    // the pair of each head, in lane j for head j; an infinity or a NaN in the row makes one of the two no number
     const float lo_of = bf16_below(mn_of);
     const float step_of = bf16_above_nonneg(fmaxf(__fdiv_rn(__fsub_rn(mx_of, lo_of), 15.0f), 0x1p-100f));
-    const bool ok_of = any_of == 0.0f && fabsf(lo_of) < INFINITY && step_of < INFINITY;
+    const bool ok_of = fabsf(lo_of) < INFINITY && step_of < INFINITY;
     const float inv_of = ok_of ? __frcp_rn(step_of) : 0.0f;  // 0: no row
     const int words = kv4_words(hd);
+    if (lane < HPW && head0 + lane >= p.n_heads && head0 + lane < heads) {
+        const int kvh = head0 + lane - p.n_heads;
+        const size_t at = at0 + (size_t)(kvh >= p.n_kv ? kvh - p.n_kv : kvh) * p.lmax;
+        (kvh >= p.n_kv ? p.v_steps : p.k_steps)[at] = ok_of ? (__float_as_uint(lo_of) | __float_as_uint(step_of) >> 16) : 0x7fc07fc0u;
+    }
 #pragma unroll
     for (int j = 0; j < HPW; ++j) {
         const int head = head0 + j;
         if (head >= heads) break;
-        const float lo = HPW == 1 ? lo_of : __shfl_sync(0xffffffffu, lo_of, j), inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, j);
+        const float lo = __shfl_sync(0xffffffffu, lo_of, j), inv = __shfl_sync(0xffffffffu, inv_of, j);
         if (head < p.n_heads) continue;
         const bool is_v = head >= p.n_heads + p.n_kv;
         const size_t at = at0 + (size_t)(is_v ? head - p.n_heads - p.n_kv : head - p.n_heads) * p.lmax;
-        auto code = [&](float x) {  // rounded to even in the low bits by adding 1.5 2^23
-            return __float_as_uint(fminf(fmaxf(__fmul_rn(__fsub_rn(x, lo), inv), 0.0f), 15.0f) + 12582912.0f) & 15u;
-        };
+        // a code lies in 0 .. 15 already: x >= lo, and step is not below (max - lo) / 15.  Adding 1.5 2^23 rounds to even; two
+        // of them make a byte of the sum's low bits
+        auto whole = [&](float x) { return __fadd_rn(__fmul_rn(__fsub_rn(x, lo), inv), 12582912.0f); };
+        auto byte_of = [&](const float (&x)[2]) { return inv == 0.0f ? (uint8_t)0 : (uint8_t)__float_as_uint(fmaf(whole(x[1]) - 12582912.0f, 16.0f, whole(x[0]))); };
         uint8_t *bytes = reinterpret_cast<uint8_t *>((is_v ? p.v_codes : p.k_codes) + at * words);
         if (own0) {
-            const bool ok = inv != 0.0f;
-            bytes[lane] = ok ? (uint8_t)(code(a[j][0]) | code(a[j][1]) << 4) : 0;
-            bytes[half / 2 + lane] = ok ? (uint8_t)(code(b[j][0]) | code(b[j][1]) << 4) : 0;
+            bytes[lane] = byte_of(a[j]);
+            bytes[half / 2 + lane] = byte_of(b[j]);
         }
         if (lane < 4 * words - half) bytes[half + lane] = 0;  // tail of the last word
-        if (lane == (HPW == 1 ? 0 : j))
-            (is_v ? p.v_steps : p.k_steps)[at] = ok_of ? (__float_as_uint(lo_of) | __float_as_uint(step_of) >> 16) : 0x7fc07fc0u;
     }
 }
 
