@@ -107,26 +107,22 @@ __device__ __forceinline__ double rsqrt_f64(double x) {
     for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
     return y;
 }
-// Sum over the warp of one of HPW values: that of index lane / 8 (HPW = 4: while a lane holds several it passes on half of
-// them), or the only one.  What follows on it is then done for all of them at once.
+// Sum over the warp of one of HPW values, that of index lane / (32 / HPW): while a lane holds several it passes on half of
+// them.  What follows on the sums is then done for all of them at once.
 template <int HPW>
-__device__ __forceinline__ double warp_sum_of(const double (&v)[HPW]) {
+__device__ __forceinline__ double warp_sum_of(double (&v)[HPW]) {
     const int lane = threadIdx.x & 31;
-    double x = v[0];
-    if (HPW == 4) {
-        const bool up16 = lane & 16, up8 = lane & 8;
-        double a[2];
+    int o = 16;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            a[i] = (up16 ? v[(2 + i) % HPW] : v[i % HPW]) + __shfl_xor_sync(0xffffffffu, up16 ? v[i % HPW] : v[(2 + i) % HPW], 16);
-        x = (up8 ? a[1] : a[0]) + __shfl_xor_sync(0xffffffffu, up8 ? a[0] : a[1], 8);
-    } else {
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-    }
+    for (int left = HPW / 2; left > 0; left /= 2, o /= 2)
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
+        for (int i = 0; i < left; ++i) {
+            const double mine = lane & o ? v[left + i] : v[i], other = lane & o ? v[i] : v[left + i];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+        }
+#pragma unroll
+    for (int k = 16 / HPW; k > 0; k /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], k);
+    return v[0];
 }
 
 // Bound by the bytes of the rows for many tokens, by one memory round trip for a few.  A warp takes HPW heads of one token:
@@ -179,7 +175,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) ss[j] = fma((double)a[j][i], (double)a[j][i], fma((double)b[j][i], (double)b[j][i], ss[j]));
         }
-        const float inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);  // of head lane / 8
+        const float inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);  // of head lane / (32 / HPW)
         const float *held = nullptr;  // the gamma in g
         float g[4] = {};
 #pragma unroll
@@ -195,7 +191,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
                         g[2 + i] = gamma[half + i0 + i];
                     }
             }
-            const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 8 * j);
+            const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 32 / HPW * j);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), g[i]);
@@ -280,9 +276,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
 }
 
 // ---- read-back ---------------------------------------------------------------------------------
-// Bound by the bytes written.  A warp takes one row and up to four heads of it; a lane writes 16 bytes of K and of V, so a
+// Bound by the bytes written.  A warp takes one row and two heads of it; a lane writes 16 bytes of K and of V, so a
 // store covers whole lines, and reads its 16 bits of codes from a word that it shares with its neighbour.
-constexpr int READ_HEADS = 4;
+constexpr int READ_HEADS = 2;  // 4 x 8192 rows of 8 heads: 53 us with two, 59 with four, 71 with one
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes,
                                                        const uint32_t *v_steps, const long long *cache_rows, unsigned tasks, unsigned groups,
                                                        int n_kv, int hd, long long cache_len, int lmax, float *k_out, float *v_out) {
