@@ -339,12 +339,16 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 // operand of the second product, where lane t meets positions 4t .. 4t+3 and row g of tile j is dim 8 word(g) + j.
 //   The largest score is a reference only: weights up to 2^8 above it are allowed before sums are rescaled, so a tile
 // costs two votes and most tiles nothing else.
-//   A warp streams its own 32-position tiles through a ring of 16-byte asynchronous copies (no barrier between warps);
-// warps of a CTA deal the tiles of a chunk, chunks of a sequence go to CTAs, a second kernel joins them.
+//   A warp streams its own 32-position tiles through a ring of 16-byte asynchronous copies (no barrier between warps) and
+// the warps of a CTA deal the tiles of a chunk.  A CTA costs about three tiles of a warp before and behind its loop, so long
+// caches are cut into as few chunks as fill the GPU once, of one size for all sequences: the CTAs work that out from the
+// lengths, and a second kernel joins the chunks.
 constexpr int ATT4_WARPS = 4;
-constexpr int ATT4_STAGES = 3;
+constexpr int ATT4_STAGES = 2;
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
 constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
+constexpr int ATT4_GRAIN = ATT4_WARPS * ATT4_TILE;  // positions that give every warp a tile
+constexpr int ATT4_LEAST = 5;  // grains of a chunk at least: 640 positions of one sequence take 6.5 us whole, 7.0 us in five chunks
 constexpr float ATT4_SLACK = 8.0f;  // log2 of how far a weight may rise above the reference
 
 struct AttnParams {
@@ -352,12 +356,59 @@ struct AttnParams {
     const uint32_t *k_codes, *k_steps, *v_codes, *v_steps;
     const int *lens;
     int t, n_heads, n_kv, rep, hd, lmax, words;
-    int row_tiles, tile_rows, chunk, chunks;  // chunk: positions per CTA, chunks = ceil(lmax / chunk)
+    int batch, row_tiles, tile_rows;
+    int slots;  // CTAs that the GPU holds; 0: nothing is split, a CTA per unit (sequence, KV head, tile of query rows)
     float scale;
     float *out;
-    float *part;      // [rows][chunks][hd] unnormalised sums, where chunks > 1
-    float2 *part_ml;  // [rows][chunks] (largest score, sum of weights)
+    float *part;      // [CTAs][tile_rows][hd] unnormalised sums
+    float2 *part_ml;  // [CTAs][tile_rows] (largest score, sum of weights)
+    int2 *part_of;    // [units] (first CTA, CTAs) of a unit
 };
+
+__device__ __forceinline__ int kv4_len(const AttnParams &p, int b) { return min(max(p.lens[b], 0), p.lmax); }
+
+// What a CTA of a split launch works on: every unit of sequence b is cut into ceil(grains of b / size) chunks, at least one,
+// with the smallest size for which the CTAs fit the GPU.  Every warp works it out alike from the lengths.
+struct AttnWork {
+    int b, unit, chunk, chunks, size;  // unit: of the sequence; size in grains
+};
+__device__ inline bool find_attn_work(const AttnParams &p, AttnWork &w) {
+    const int lane = threadIdx.x & 31, units = p.n_kv * p.row_tiles;
+    auto grains = [&](int b) { return b < p.batch ? (kv4_len(p, b) + ATT4_GRAIN - 1) / ATT4_GRAIN : 0; };
+    const int mine = grains(lane);
+    auto sum_over = [&](auto f) {
+        long long s = 0;
+        for (int b = lane; b < p.batch; b += 32) s += f(b < 32 ? mine : grains(b));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        return s;
+    };
+    const long long total = sum_over([](int g) { return (long long)g; }) * units;
+    int size = (int)max((total + p.slots - 1) / p.slots, (long long)ATT4_LEAST);
+    if ((long long)p.batch * units <= p.slots)
+        while (sum_over([&](int g) { return (long long)max((g + size - 1) / size, 1); }) * units > p.slots) size += max(size / 16, 1);
+    // the sequence of this CTA: running sum of CTAs over the sequences
+    long long first = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int b = b0 + lane, c = b < p.batch ? max(((b0 ? grains(b) : mine) + size - 1) / size, 1) : 0;
+        long long upto = (long long)c * units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += up;
+        }
+        const unsigned in = __ballot_sync(0xffffffffu, first + upto > (long long)blockIdx.x);
+        if (in) {
+            const int at = __ffs(in) - 1, chunks = __shfl_sync(0xffffffffu, c, at);
+            const int r = (int)((long long)blockIdx.x - first - __shfl_sync(0xffffffffu, upto, at)) + chunks * units;
+            w.b = b0 + at; w.chunks = chunks; w.unit = r / chunks; w.chunk = r - w.unit * chunks; w.size = size;
+            return true;
+        }
+        first += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;  // more CTAs than work
+}
+
 
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -422,7 +473,7 @@ struct Attn4 {
 };
 
 template <int W, int NT>
-__global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams p) {
+__global__ void __launch_bounds__(ATT4_WARPS * 32, NT == 1 ? 5 : 4) attn_kv4_kernel(AttnParams p) {
     using A = Attn4<W, NT>;
     constexpr int KC = A::KC, NBK = A::NBK, ROWS = A::ROWS;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -432,31 +483,32 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
     __shared__ long long s_row[ROWS];  // index of the tile's rows in q and out
     __shared__ int s_off[ROWS];        // positions behind the sequence's end that a row does not see
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int unit = blockIdx.x, chunk_id = blockIdx.y;  // sequence * n_kv + KV head
-    const int b = unit / p.n_kv, rep = p.rep, hd = p.hd;
-    const int r0 = blockIdx.z * ROWS, rows = min(ROWS, p.t * rep - r0);  // rows: query token * rep + head of the group
+    const int rep = p.rep, hd = p.hd;
+    release_and_wait();
+    AttnWork work;
+    if (p.slots == 0) {
+        const int per = p.n_kv * p.row_tiles;
+        work.b = blockIdx.x / per; work.unit = blockIdx.x - work.b * per; work.chunk = 0; work.chunks = 1; work.size = (p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN;
+    } else if (!find_attn_work(p, work)) {
+        return;
+    }
+    const int b = work.b, kvh = work.unit / p.row_tiles;
+    const int r0 = (work.unit - kvh * p.row_tiles) * ROWS, rows = min(ROWS, p.t * rep - r0);  // rows: query token * rep + head of the group
     if (threadIdx.x < ROWS) {
         const int r = r0 + min((int)threadIdx.x, rows - 1), i = r / rep;
-        s_row[threadIdx.x] = ((long long)b * p.t + i) * p.n_heads + (unit - b * p.n_kv) * rep + (r - i * rep);
+        s_row[threadIdx.x] = ((long long)b * p.t + i) * p.n_heads + kvh * rep + (r - i * rep);
         s_off[threadIdx.x] = p.t - 1 - i;
     }
     __syncthreads();
-    release_and_wait();
-    const int len = min(max(p.lens[b], 0), p.lmax);
+    const int len = kv4_len(p, b);
     const int last = len - s_off[rows - 1];  // positions the tile's last row sees: no row sees more
-    const int c0 = chunk_id * p.chunk, c1 = min(last, c0 + p.chunk);
-    const bool alone = last <= p.chunk;  // one chunk holds all that these rows see
-    if (c0 >= c1 && chunk_id != 0) return;
-    if (last <= 0) {  // nothing is seen by any row
-        for (int r = 0; r < rows; ++r)
-            if ((int)threadIdx.x < hd) p.out[s_row[r] * hd + threadIdx.x] = 0.0f;
-        return;
-    }
+    const int c0 = work.chunk * work.size * ATT4_GRAIN, c1 = min(last, c0 + work.size * ATT4_GRAIN);
+    if (p.slots && work.chunk == 0 && threadIdx.x == 0) p.part_of[((size_t)b * p.n_kv + kvh) * p.row_tiles + r0 / ROWS] = make_int2(blockIdx.x, work.chunks);
 
     // ---- ring of this warp
     uint32_t *ring = reinterpret_cast<uint32_t *>(smem) + warp * ATT4_STAGES * A::STAGE;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    const size_t base = (size_t)unit * p.lmax;
+    const size_t base = ((size_t)b * p.n_kv + kvh) * p.lmax;
     const uint32_t *kc = p.k_codes + base * W, *vc = p.v_codes + base * W, *pairs = ((lane & 8) ? p.v_steps : p.k_steps) + base;
     // 16-byte pieces: piece i = lane + 32 j of a plane's 8 W.  SWZ: K's go to row r ^ (r / 2) % 2, V's change places inside
     // their row by (r / 4) % 4
@@ -760,10 +812,10 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
             sum = fmaf(s_l[w][r], f, sum);
             o = fmaf(reinterpret_cast<const float *>(smem)[(w * ROWS + r) * A::OLD + d], f, o);
         }
-        if (alone) {
+        if (work.chunks == 1) {
             p.out[s_row[r] * hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
         } else {
-            const size_t at = (size_t)s_row[r] * p.chunks + chunk_id;
+            const size_t at = (size_t)blockIdx.x * ROWS + r;
             p.part[at * hd + d] = o;
             if (d == 0) p.part_ml[at] = make_float2(m, sum);
         }
@@ -771,44 +823,44 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, 4) attn_kv4_kernel(AttnParams
 }
 
 template <int W>
-static int launch_attn_kv4(const AttnParams &p, unsigned units, int dev, cudaStream_t stream) {
+static int launch_attn_kv4(const AttnParams &p, unsigned ctas, int dev, cudaStream_t stream) {
     if (p.words != W) {
-        if constexpr (W > 1) return launch_attn_kv4<W - 1>(p, units, dev, stream);
+        if constexpr (W > 1) return launch_attn_kv4<W - 1>(p, ctas, dev, stream);
         return fail(KB_ERR_UNSUPPORTED, "attention: rows of %d words", p.words);
     }
     const bool one = p.tile_rows == ATT4_ROWS;
     void (*kern)(AttnParams) = one ? attn_kv4_kernel<W, 1> : attn_kv4_kernel<W, 2>;
     const size_t smem = one ? Attn4<W, 1>::SMEM : Attn4<W, 2>::SMEM;
     if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, (int)smem, "kv4 attention smem attribute")) return rc;
-    const cudaError_t e = launch_after(kern, dim3(units, (unsigned)p.chunks, (unsigned)p.row_tiles), dim3(ATT4_WARPS * 32), smem, stream, p);
+    const cudaError_t e = launch_after(kern, dim3(ctas), dim3(ATT4_WARPS * 32), smem, stream, p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 attention launch");
 }
 
-// One CTA per query row that was split: the weighted mean of its chunks, a thread per dim.  Eight chunks are read at a
-// time; their factors come from the lanes of a warp, one chunk each.
+// One CTA per query row: the weighted mean of its chunks where there are several, a thread per dim.  Eight chunks are read
+// at a time; their factors come from the lanes of a warp, one chunk each.
 __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p) {
     const unsigned row = blockIdx.x, tok = row / p.n_heads;
     const int lane = threadIdx.x & 31, d = threadIdx.x, h = row - tok * p.n_heads, b = tok / p.t, i = tok - b * p.t;
-    const int r = i * p.rep + h % p.rep, tile_last = min(p.t * p.rep, (r / p.tile_rows + 1) * p.tile_rows) - 1;  // last row of its tile
+    const int kvh = h / p.rep, r = i * p.rep + h - kvh * p.rep, tile = r / p.tile_rows;
     release_and_wait();
-    const int len = min(max(p.lens[b], 0), p.lmax);
-    const int last = len - (p.t - 1 - tile_last / p.rep);
-    if (last <= p.chunk) return;  // the first kernel wrote it
-    const int n = (last + p.chunk - 1) / p.chunk;
-    const float2 *ml = p.part_ml + (size_t)row * p.chunks;
-    const float *src = p.part + (size_t)row * p.chunks * p.hd + (d < p.hd ? d : 0);
+    const int2 of = p.part_of[((size_t)b * p.n_kv + kvh) * p.row_tiles + tile];
+    const int n = of.y;
+    if (n == 1) return;  // the first kernel wrote it
+    const size_t stride = p.tile_rows, at = (size_t)of.x * stride + (r - tile * p.tile_rows);
+    const float2 *ml = p.part_ml + at;
+    const float *src = p.part + at * p.hd + (d < p.hd ? d : 0);
     float top = -INFINITY, sum = 0.0f, o = 0.0f;
-    for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[s].x);
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[s * stride].x);
     top = warp_reduce_max(top);
     for (int s0 = 0; s0 < n; s0 += 32) {
-        const float2 v = s0 + lane < n ? ml[s0 + lane] : make_float2(0.0f, 0.0f);
+        const float2 v = s0 + lane < n ? ml[(s0 + lane) * stride] : make_float2(0.0f, 0.0f);
         const float mine = v.y == 0.0f ? 0.0f : exp2_fast(v.x - top);
         sum = fmaf(v.y, mine, sum);
         const int m = min(32, n - s0);
         for (int s = 0; s < m; s += 8) {
             float x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = s + k < m ? src[(size_t)(s0 + s + k) * p.hd] : 0.0f;
+            for (int k = 0; k < 8; ++k) x[k] = s + k < m ? src[(s0 + s + k) * stride * p.hd] : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) o = fmaf(x[k], __shfl_sync(0xffffffffu, mine, s + k), o);
         }
@@ -816,15 +868,6 @@ __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p)
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
     if (d < p.hd) p.out[(size_t)row * p.hd + d] = sum == 0.0f ? 0.0f : __fdiv_rn(o, sum);
-}
-
-// positions per CTA.  The lengths are on the device, so the rule goes by the cache's: about four CTAs for every resident
-// one (4 per SM), so that short sequences leave room that long ones fill, and at least a tile per warp.
-static int attn_chunk(size_t units, int lmax, int sms) {
-    const size_t want = ((size_t)lmax * units + (size_t)sms * 16 - 1) / ((size_t)sms * 16);
-    const int step = ATT4_WARPS * ATT4_TILE;
-    const size_t chunk = (want + step - 1) / step * step;
-    return chunk >= (size_t)lmax ? lmax : (int)chunk;
 }
 
 static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
@@ -836,10 +879,30 @@ static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
 
 // query rows of a CTA: one set of columns where it holds them all
 static int attn_tile_rows(int t, int n_heads, int n_kv) { return (size_t)t * (n_heads / n_kv) <= ATT4_ROWS ? ATT4_ROWS : 2 * ATT4_ROWS; }
-// CTAs that share nothing: (sequence, KV head, tile of query rows)
-static size_t attn_units(size_t batch, int t, int n_heads, int n_kv) {
-    const size_t rows = (size_t)t * (n_heads / n_kv);
-    return batch * n_kv * ((rows + attn_tile_rows(t, n_heads, n_kv) - 1) / attn_tile_rows(t, n_heads, n_kv));
+
+// How a call is launched: CTAs, and the workspace of its chunks.  The lengths are on the device; a cache that could not make
+// two chunks of a sequence is not split.
+struct AttnPlan {
+    int tile_rows, row_tiles, slots;
+    size_t units, ctas;
+    size_t of_bytes, ml_bytes, part_bytes;
+    size_t bytes() const { return of_bytes + ml_bytes + part_bytes; }
+};
+static AttnPlan attn_plan(size_t batch, int t, int n_heads, int n_kv, int hd, int lmax, int sms) {
+    AttnPlan a = {};
+    a.tile_rows = attn_tile_rows(t, n_heads, n_kv);
+    a.row_tiles = (int)(((size_t)t * (n_heads / n_kv) + a.tile_rows - 1) / a.tile_rows);
+    a.units = batch * n_kv * a.row_tiles;
+    a.slots = lmax <= ATT4_LEAST * ATT4_GRAIN ? 0 : sms * (a.tile_rows == ATT4_ROWS ? 5 : 4);
+    // chunks of one size: less than one CTA per unit more than the GPU holds, and exactly what it holds where the units fit
+    a.ctas = a.slots == 0 ? a.units : a.units <= (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;
+    if (a.slots) {
+        auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+        a.of_bytes = up(a.units * sizeof(int2));
+        a.ml_bytes = up(a.ctas * a.tile_rows * sizeof(float2));
+        a.part_bytes = a.ctas * a.tile_rows * (size_t)hd * sizeof(float);
+    }
+    return a;
 }
 
 static bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, const void *d = nullptr) {
@@ -940,9 +1003,7 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
 size_t kb_attn_kv4_workspace_bytes(size_t batch, int t, int n_heads, int n_kv_heads, int head_dim, int lmax) {
     int dev = 0;
     if (batch == 0 || t < 1 || check_kv4(n_heads, n_kv_heads, head_dim, lmax) != KB_OK || cudaGetDevice(&dev) != cudaSuccess) return 0;
-    const size_t rows = batch * (size_t)t * n_heads;
-    const size_t chunks = (lmax - 1) / attn_chunk(attn_units(batch, t, n_heads, n_kv_heads), lmax, sm_count(dev)) + 1;
-    return chunks < 2 ? 0 : rows * chunks * ((size_t)head_dim + 2) * sizeof(float);
+    return attn_plan(batch, t, n_heads, n_kv_heads, head_dim, lmax, sm_count(dev)).bytes();
 }
 
 int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes, const uint32_t *v_steps,
@@ -959,31 +1020,30 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
         return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
     int dev = 0;
     KB_CUDA(cudaGetDevice(&dev));
-    const size_t rows = batch * (size_t)t * n_heads, units = attn_units(batch, t, n_heads, n_kv_heads);
+    const AttnPlan plan = attn_plan(batch, t, n_heads, n_kv_heads, head_dim, lmax, sm_count(dev));
+    if (plan.ctas > 0x7fffffffu) return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
+    const size_t rows = batch * (size_t)t * n_heads;
     AttnParams p = {};
     p.q = q; p.k_codes = k_codes; p.k_steps = k_steps; p.v_codes = v_codes; p.v_steps = v_steps; p.lens = lens;
     p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.rep = n_heads / n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.words = kv4_words(head_dim); p.out = out;
     p.scale = scale != 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
-    p.tile_rows = attn_tile_rows(t, n_heads, n_kv_heads);
-    p.row_tiles = (int)(units / (batch * n_kv_heads));
-    p.chunk = attn_chunk(units, lmax, sm_count(dev));
-    p.chunks = (lmax - 1) / p.chunk + 1;
-    if (batch * n_kv_heads > 0x7fffffffu || p.chunks > 65535 || p.row_tiles > 65535) return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);
+    p.batch = (int)batch; p.row_tiles = plan.row_tiles; p.tile_rows = plan.tile_rows; p.slots = plan.slots;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     void *own = nullptr;
-    if (p.chunks > 1) {
-        const size_t need = rows * p.chunks * ((size_t)head_dim + 2) * sizeof(float);
-        if (workspace && workspace_bytes < need)
-            return fail(KB_ERR_STORAGE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    if (plan.slots) {
+        if (workspace && workspace_bytes < plan.bytes())
+            return fail(KB_ERR_STORAGE, "workspace too small: need %zu bytes, got %zu", plan.bytes(), workspace_bytes);
         if (!workspace) {
-            KB_CUDA(cudaMallocAsync(&own, need, st));
+            KB_CUDA(cudaMallocAsync(&own, plan.bytes(), st));
             workspace = own;
         }
-        p.part_ml = static_cast<float2 *>(workspace);
-        p.part = reinterpret_cast<float *>(p.part_ml + rows * p.chunks);
+        uint8_t *ws = static_cast<uint8_t *>(workspace);
+        p.part_of = reinterpret_cast<int2 *>(ws);
+        p.part_ml = reinterpret_cast<float2 *>(ws + plan.of_bytes);
+        p.part = reinterpret_cast<float *>(ws + plan.of_bytes + plan.ml_bytes);
     }
-    int rc = launch_attn_kv4<KV4_MAX_HD / 8>(p, (unsigned)(batch * n_kv_heads), dev, st);
-    if (rc == KB_OK && p.chunks > 1) {
+    int rc = launch_attn_kv4<KV4_MAX_HD / 8>(p, (unsigned)plan.ctas, dev, st);
+    if (rc == KB_OK && plan.slots) {
         const cudaError_t e = launch_after(attn_kv4_join_kernel, dim3((unsigned)rows), dim3(KV4_MAX_HD), 0, st, p);
         if (e != cudaSuccess) rc = cuda_fail(e, "kv4 attention join launch");
     }

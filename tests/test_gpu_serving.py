@@ -201,6 +201,18 @@ def test_attention(env, seqs, t, heads, kv, hd, lmax, lens):
     check_attention(env, q, filled_cache(env, seqs, kv, lmax, hd, 11), lens)
 
 
+@pytest.mark.parametrize("seqs,t,heads,kv,hd,lmax,longest", [(40, 1, 4, 2, 8, 1500, 1500), (50, 1, 16, 16, 8, 2000, 2000), (33, 4, 6, 2, 16, 800, 790),
+                                                             (3, 2, 4, 4, 64, 20000, 20000)])
+def test_attention_splits_of_many_unlike_sequences(env, seqs, t, heads, kv, hd, lmax, longest):
+    """chunks are dealt over more sequences than a warp has lanes, over more units than the GPU holds CTAs, over one long among short"""
+    rng = np.random.default_rng(seqs)
+    lens = rng.integers(0, 60, seqs)
+    lens[rng.choice(seqs, max(1, seqs // 8), replace=False)] = rng.integers(longest // 2, longest, max(1, seqs // 8))
+    lens[seqs // 2] = longest
+    q = cases.gaussian(seqs + t, (seqs, t, heads, hd), 1.0)
+    check_attention(env, q, filled_cache(env, seqs, kv, lmax, hd, 15), list(lens))
+
+
 def test_attention_scale_lens_and_squeezed_queries(env):
     """scale is used, lens beyond the cache or below zero are clamped, [seqs, heads, hd] is one token, strided queries"""
     t = env.torch
