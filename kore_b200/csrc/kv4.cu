@@ -357,6 +357,7 @@ struct AttnParams {
     const int *lens;
     int t, n_heads, n_kv, rep, hd, lmax, words;
     int batch, row_tiles, tile_rows;
+    int least_ctas;  // sequences * units, where slots > 0 and that is below it; otherwise slots
     int slots;  // CTAs that the GPU holds; 0: nothing is split, a CTA per unit (sequence, KV head, tile of query rows)
     float scale;
     float *out;
@@ -367,48 +368,51 @@ struct AttnParams {
 
 __device__ __forceinline__ int kv4_len(const AttnParams &p, int b) { return min(max(p.lens[b], 0), p.lmax); }
 
-// What a CTA of a split launch works on: every unit of sequence b is cut into ceil(grains of b / size) chunks, at least one,
-// with the smallest size for which the CTAs fit the GPU.  Every warp works it out alike from the lengths.
+// What a CTA works on.  In a split launch every unit (KV head, tile of query rows) of sequence b is cut into ceil(grains of
+// b / size) chunks, at least one; every warp works that out alike from the lengths.
 struct AttnWork {
-    int b, unit, chunk, chunks, size;  // unit: of the sequence; size in grains
+    int b, len, unit, chunk, chunks, size;  // unit: of the sequence; size in grains
 };
-__device__ inline bool find_attn_work(const AttnParams &p, AttnWork &w) {
+__device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w) {
     const int lane = threadIdx.x & 31, units = p.n_kv * p.row_tiles;
-    auto grains = [&](int b) { return b < p.batch ? (kv4_len(p, b) + ATT4_GRAIN - 1) / ATT4_GRAIN : 0; };
-    const int mine = grains(lane);
-    auto sum_over = [&](auto f) {
-        long long s = 0;
-        for (int b = lane; b < p.batch; b += 32) s += f(b < 32 ? mine : grains(b));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        return s;
-    };
-    const long long total = sum_over([](int g) { return (long long)g; }) * units;
-    int size = (int)max((total + p.slots - 1) / p.slots, (long long)ATT4_LEAST);
-    if ((long long)p.batch * units <= p.slots)
-        while (sum_over([&](int g) { return (long long)max((g + size - 1) / size, 1); }) * units > p.slots) size += max(size / 16, 1);
-    // the sequence of this CTA: running sum of CTAs over the sequences
-    long long first = 0;
+    if (p.slots == 0) {
+        w.b = blockIdx.x / units;
+        w.unit = blockIdx.x - w.b * units;
+        w.len = kv4_len(p, w.b);
+        w.chunk = 0; w.chunks = 1; w.size = (p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN;
+        return true;
+    }
+    const int len0 = lane < p.batch ? kv4_len(p, lane) : 0;
+    unsigned grains = (len0 + ATT4_GRAIN - 1) / ATT4_GRAIN;
+    for (int b = lane + 32; b < p.batch; b += 32) grains += (kv4_len(p, b) + ATT4_GRAIN - 1) / ATT4_GRAIN;
+    const unsigned long long total = (unsigned long long)__reduce_add_sync(0xffffffffu, grains) * units;
+    // sum of ceil(g / size) <= total / size + sequences * units, which is at most `slots` for the first size.  Where the
+    // units alone take most of the slots the second one is used, and up to a CTA per unit more than the GPU holds
+    const unsigned share = p.slots - p.least_ctas > p.slots / 2 ? p.slots - p.least_ctas : p.slots;
+    const unsigned even = total >> 32 ? (unsigned)((total + share - 1) / share) : ((unsigned)total + share - 1) / share;
+    w.size = max((int)even, ATT4_LEAST);
+    int first = 0;  // running sum of CTAs over the sequences
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int b = b0 + lane, c = b < p.batch ? max(((b0 ? grains(b) : mine) + size - 1) / size, 1) : 0;
-        long long upto = (long long)c * units;
+        const int b = b0 + lane, len = b0 == 0 ? len0 : b < p.batch ? kv4_len(p, b) : 0;
+        const int c = b < p.batch ? max((int)((unsigned)(len + w.size * ATT4_GRAIN - 1) / (unsigned)(w.size * ATT4_GRAIN)), 1) : 0;
+        int upto = c * units;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+            const int up = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += up;
         }
-        const unsigned in = __ballot_sync(0xffffffffu, first + upto > (long long)blockIdx.x);
+        const unsigned in = __ballot_sync(0xffffffffu, first + upto > (int)blockIdx.x);
         if (in) {
-            const int at = __ffs(in) - 1, chunks = __shfl_sync(0xffffffffu, c, at);
-            const int r = (int)((long long)blockIdx.x - first - __shfl_sync(0xffffffffu, upto, at)) + chunks * units;
-            w.b = b0 + at; w.chunks = chunks; w.unit = r / chunks; w.chunk = r - w.unit * chunks; w.size = size;
+            const int at = __ffs(in) - 1, r = (int)blockIdx.x - first - __shfl_sync(0xffffffffu, upto, at) + __shfl_sync(0xffffffffu, c, at) * units;
+            w.chunks = __shfl_sync(0xffffffffu, c, at);
+            w.len = __shfl_sync(0xffffffffu, len, at);
+            w.b = b0 + at; w.unit = r / w.chunks; w.chunk = r - w.unit * w.chunks;
             return true;
         }
         first += __shfl_sync(0xffffffffu, upto, 31);
     }
     return false;  // more CTAs than work
 }
-
 
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -486,22 +490,32 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, NT == 1 ? 5 : 4) attn_kv4_ker
     const int rep = p.rep, hd = p.hd;
     release_and_wait();
     AttnWork work;
-    if (p.slots == 0) {
-        const int per = p.n_kv * p.row_tiles;
-        work.b = blockIdx.x / per; work.unit = blockIdx.x - work.b * per; work.chunk = 0; work.chunks = 1; work.size = (p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN;
-    } else if (!find_attn_work(p, work)) {
-        return;
-    }
-    const int b = work.b, kvh = work.unit / p.row_tiles;
+    if (!find_attn_work(p, work)) return;
+    const int b = work.b, kvh = work.unit / p.row_tiles, len = work.len;
     const int r0 = (work.unit - kvh * p.row_tiles) * ROWS, rows = min(ROWS, p.t * rep - r0);  // rows: query token * rep + head of the group
-    if (threadIdx.x < ROWS) {
-        const int r = r0 + min((int)threadIdx.x, rows - 1), i = r / rep;
-        s_row[threadIdx.x] = ((long long)b * p.t + i) * p.n_heads + kvh * rep + (r - i * rep);
-        s_off[threadIdx.x] = p.t - 1 - i;
+    // index of a row in q and out, and the positions behind the sequence's end that it does not see
+    auto row_of = [&](int r, int &off) {
+        const int i = (r0 + r) / rep;
+        off = p.t - 1 - i;
+        return ((long long)b * p.t + i) * p.n_heads + kvh * rep + (r0 + r - i * rep);
+    };
+    // a warp takes NT query rows; their loads are under way first
+    float x[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = warp + n * ATT4_WARPS;
+        int off;
+        const long long row = row_of(min(r, rows - 1), off);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = r < rows && lane + 32 * i < hd ? p.q[row * hd + lane + 32 * i] : 0.0f;
+        if (lane == 0) {
+            s_row[r] = row;
+            s_off[r] = off;
+        }
     }
-    __syncthreads();
-    const int len = kv4_len(p, b);
-    const int last = len - s_off[rows - 1];  // positions the tile's last row sees: no row sees more
+    int last_off;
+    row_of(rows - 1, last_off);
+    const int last = len - last_off;  // positions the tile's last row sees: no row sees more
     const int c0 = work.chunk * work.size * ATT4_GRAIN, c1 = min(last, c0 + work.size * ATT4_GRAIN);
     if (p.slots && work.chunk == 0 && threadIdx.x == 0) p.part_of[((size_t)b * p.n_kv + kvh) * p.row_tiles + r0 / ROWS] = make_int2(blockIdx.x, work.chunks);
 
@@ -548,18 +562,20 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, NT == 1 ? 5 : 4) attn_kv4_ker
 #pragma unroll
     for (int s = 0; s < ATT4_STAGES - 1; ++s) issue(first + s * stride, s);
 
-    // ---- queries times scale log2(e), scaled by a power of two to [2^13, 2^14), split, laid out; a warp takes NT rows
-    for (int r = warp; r < ROWS; r += ATT4_WARPS) {
-        const float *src = p.q + s_row[r] * hd;
+    // ---- queries times scale log2(e), scaled by a power of two to [2^13, 2^14), split, laid out
+    static_assert(ATT4_ROWS == ATT4_WARPS, "a warp takes one row of each set");
+#pragma unroll
+    for (int m = 0; m < NT; ++m) {
+        const int r = warp + m * ATT4_WARPS;
         const float unit2 = p.scale * 1.4426950408889634f;  // scores in units of log 2
-        float x[4], amax = 0.0f, sum = 0.0f;
+        float amax = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = r < rows && lane + 32 * i < hd ? src[lane + 32 * i] * unit2 : 0.0f;
-            amax = fmaxf(amax, fabsf(x[i]));
-            sum += x[i];
+            x[m][i] *= unit2;
+            amax = fmaxf(amax, fabsf(x[m][i]));
+            sum += x[m][i];
         }
-        amax = warp_reduce_max(amax);
+        amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));  // not negative: ordered as integers
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         // by exponent fields; below 2^-113 the scores are 0 to any accuracy, from 2^120 on the row is given up (NaN)
@@ -569,15 +585,15 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, NT == 1 ? 5 : 4) attn_kv4_ker
             s_fr[r] = __int_as_float(min(e + 7, 254) << 23);  // 2^20 / up
             s_qs[r] = e > 247 ? __uint_as_float(0x7fffffffu) : sum;
         }
-        __half *dst = reinterpret_cast<__half *>(s_q[r / ATT4_ROWS]);
+        __half *dst = reinterpret_cast<__half *>(s_q[m]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = lane + 32 * i, w = d >> 3, n = d & 7;
             if (w >= 4 * KC) continue;
             const int tt = A::VEC ? w / KC : w & 3, c = A::VEC ? w % KC : w >> 2;
-            const uint32_t y = split_f16(x[i] * up);
-            // step 2c + (n & 2) / 2, register n & 1, half n / 4; column 2 (r % 4) holds hi, the next one lo
-            __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + (r % ATT4_ROWS) * 8 + tt) * 4 + (n & 1) * 2 + (n >> 2);
+            const uint32_t y = split_f16(x[m][i] * up);
+            // step 2c + (n & 2) / 2, register n & 1, half n / 4; column 2 warp holds hi, the next one lo
+            __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + warp * 8 + tt) * 4 + (n & 1) * 2 + (n >> 2);
             at[0] = __ushort_as_half((unsigned short)(y & 0xffffu));
             at[16] = __ushort_as_half((unsigned short)(y >> 16));
         }
@@ -894,8 +910,7 @@ static AttnPlan attn_plan(size_t batch, int t, int n_heads, int n_kv, int hd, in
     a.row_tiles = (int)(((size_t)t * (n_heads / n_kv) + a.tile_rows - 1) / a.tile_rows);
     a.units = batch * n_kv * a.row_tiles;
     a.slots = lmax <= ATT4_LEAST * ATT4_GRAIN ? 0 : sms * (a.tile_rows == ATT4_ROWS ? 5 : 4);
-    // chunks of one size: less than one CTA per unit more than the GPU holds, and exactly what it holds where the units fit
-    a.ctas = a.slots == 0 ? a.units : a.units <= (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;
+    a.ctas = a.slots == 0 ? a.units : a.units * 2 < (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;  // see find_attn_work
     if (a.slots) {
         auto up = [](size_t v) { return (v + 255) / 256 * 256; };
         a.of_bytes = up(a.units * sizeof(int2));
@@ -1027,6 +1042,7 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
     p.q = q; p.k_codes = k_codes; p.k_steps = k_steps; p.v_codes = v_codes; p.v_steps = v_steps; p.lens = lens;
     p.t = t; p.n_heads = n_heads; p.n_kv = n_kv_heads; p.rep = n_heads / n_kv_heads; p.hd = head_dim; p.lmax = lmax; p.words = kv4_words(head_dim); p.out = out;
     p.scale = scale != 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
+    p.least_ctas = plan.units < (size_t)plan.slots ? (int)plan.units : plan.slots;
     p.batch = (int)batch; p.row_tiles = plan.row_tiles; p.tile_rows = plan.tile_rows; p.slots = plan.slots;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     void *own = nullptr;
