@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 // caches are cut into as few chunks as fill the GPU once, of one size for all sequences: the CTAs work that out from the
 // lengths, and a second kernel joins the chunks.
 constexpr int ATT4_WARPS = 4;
-constexpr int ATT4_STAGES = 2;
+constexpr int ATT4_STAGES = 2;   // with 16 warps on an SM a second tile in flight each is enough
+constexpr int ATT4_PER_SM = 4;   // resident CTAs: 128 registers a thread (five with 96 take 2.3 us longer for 16 sequences of 640)
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
 constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
 constexpr int ATT4_GRAIN = ATT4_WARPS * ATT4_TILE;  // positions that give every warp a tile
@@ -477,7 +478,7 @@ struct Attn4 {
 };
 
 template <int W, int NT>
-__global__ void __launch_bounds__(ATT4_WARPS * 32, NT == 1 ? 5 : 4) attn_kv4_kernel(AttnParams p) {
+__global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(AttnParams p) {
     using A = Attn4<W, NT>;
     constexpr int KC = A::KC, NBK = A::NBK, ROWS = A::ROWS;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -775,7 +776,11 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, NT == 1 ? 5 : 4) attn_kv4_ker
                 b0[n] = transpose_8x8(split_f16(s[n][h][0] * f));  // positions 4t and 4t + 2 of column g
                 b1[n] = transpose_8x8(split_f16(s[n][h][1] * f));  // positions 4t + 1 and 4t + 3
             }
-            auto code = [](uint32_t x) { return (x & 0x00f000f0u) ^ 0x00f00000u; };  // of two positions, the second counted down
+            auto code = [](uint32_t x) {  // of two positions, the second counted down: (x & 0x00f000f0) ^ 0x00f00000 in one instruction
+                uint32_t y;
+                asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0x00f000f0u), "r"(0x00f00000u));
+                return y;
+            };
 #pragma unroll
             for (int k = 0; k < NBK; ++k)
 #pragma unroll
@@ -909,7 +914,7 @@ static AttnPlan attn_plan(size_t batch, int t, int n_heads, int n_kv, int hd, in
     a.tile_rows = attn_tile_rows(t, n_heads, n_kv);
     a.row_tiles = (int)(((size_t)t * (n_heads / n_kv) + a.tile_rows - 1) / a.tile_rows);
     a.units = batch * n_kv * a.row_tiles;
-    a.slots = lmax <= ATT4_LEAST * ATT4_GRAIN ? 0 : sms * (a.tile_rows == ATT4_ROWS ? 5 : 4);
+    a.slots = lmax <= ATT4_LEAST * ATT4_GRAIN ? 0 : sms * ATT4_PER_SM;
     a.ctas = a.slots == 0 ? a.units : a.units * 2 < (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;  // see find_attn_work
     if (a.slots) {
         auto up = [](size_t v) { return (v + 255) / 256 * 256; };
