@@ -630,10 +630,11 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
     float mref[NT], l[NT], alo[NT], wref[NT], ws[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) mref[n] = -INFINITY, l[n] = alo[n] = 0.0f, wref[n] = 0x1p-100f, ws[n] = 0x1p106f;
-    // every second position (odd g) counts down from its largest value, lo + 15 step - (15 - c) step: the sum of the products
-    // then changes sign as the values do.  With codes alone it only grows, and the instruction's truncated adds pull all of it
-    // one way (2.8e-4 of the result at 32768 positions, 1e-6 without that)
-    const float down = g & 1 ? 15.0f : 0.0f, sign = g & 1 ? -1.0f : 1.0f;
+    // every second position counts down from its largest value, lo + 15 step - (15 - c) step: the sums of the products and of
+    // the constant parts then change sign as the values do.  With codes alone they only grow, and the instruction's truncated
+    // adds pull all of it one way (2.8e-4 of the result at 32768 positions).  Odd lanes g count down in block 0, even ones in
+    // block 1, so that every lane does both
+    const float down[2] = {g & 1 ? 15.0f : 0.0f, g & 1 ? 0.0f : 15.0f}, sign = g & 1 ? -1.0f : 1.0f;
 
     int stage = 0;
     for (int tile0 = first; tile0 < c1; tile0 += stride) {
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
                     if (tail) pr = s[n][h][i] == -INFINITY ? 0u : pr;  // what is not seen may hold anything, NaN too
                     const float pj = exp2_fast(s[n][h][i] - ref), step = kv4_step(pr);
                     l[n] += pj;
-                    alo[n] = fmaf(pj, fmaf(down, step, kv4_lo(pr)), alo[n]);
+                    alo[n] = fmaf(pj, fmaf(down[h], step, kv4_lo(pr)), alo[n]);
                     s[n][h][i] = pj * step;
                     wmax[n] = fmaxf(wmax[n], s[n][h][i]);
                 }
@@ -772,13 +773,13 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float f = ws[n] * sign;
+                const float f = h == 0 ? ws[n] * sign : -(ws[n] * sign);
                 b0[n] = transpose_8x8(split_f16(s[n][h][0] * f));  // positions 4t and 4t + 2 of column g
                 b1[n] = transpose_8x8(split_f16(s[n][h][1] * f));  // positions 4t + 1 and 4t + 3
             }
-            auto code = [](uint32_t x) {  // of two positions, the second counted down: (x & 0x00f000f0) ^ 0x00f00000 in one instruction
+            auto code = [&](uint32_t x) {  // of two positions, one counted down: (x & mask) ^ half of it in one instruction
                 uint32_t y;
-                asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0x00f000f0u), "r"(0x00f00000u));
+                asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0x00f000f0u), "r"(h == 0 ? 0x00f00000u : 0x000000f0u));
                 return y;
             };
 #pragma unroll
