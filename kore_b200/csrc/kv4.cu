@@ -756,43 +756,56 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
         }
         // ---- weighted sum of the codes
         const uint32_t *vrow = sv + 4 * t * W + (A::SWZ ? 4 * ((g >> 1) ^ t) + 2 * (g & 1) : g);
+        uint32_t vw[2][NBK][4], b0[2][NT], b1[2][NT];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t vw[NBK][4], b0[NT], b1[NT];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t *row = vrow + (16 * h + i) * W;
                 if (A::SWZ) {
                     const uint2 v = *reinterpret_cast<const uint2 *>(row);
-                    vw[0][i] = v.x;
-                    vw[NBK - 1][i] = v.y;
+                    vw[h][0][i] = v.x;
+                    vw[h][NBK - 1][i] = v.y;
                 } else {
 #pragma unroll
-                    for (int k = 0; k < NBK; ++k) vw[k][i] = 8 * k + 7 < W || g + 8 * k < W ? row[8 * k] : 0u;
+                    for (int k = 0; k < NBK; ++k) vw[h][k][i] = 8 * k + 7 < W || g + 8 * k < W ? row[8 * k] : 0u;
                 }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float f = h == 0 ? ws[n] * sign : -(ws[n] * sign);
-                b0[n] = transpose_8x8(split_f16(s[n][h][0] * f));  // positions 4t and 4t + 2 of column g
-                b1[n] = transpose_8x8(split_f16(s[n][h][1] * f));  // positions 4t + 1 and 4t + 3
+                b0[h][n] = transpose_8x8(split_f16(s[n][h][0] * f));  // positions 4t and 4t + 2 of column g
+                b1[h][n] = transpose_8x8(split_f16(s[n][h][1] * f));  // positions 4t + 1 and 4t + 3
             }
-            auto code = [&](uint32_t x) {  // of two positions, one counted down: (x & mask) ^ half of it in one instruction
-                uint32_t y;
-                asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0x00f000f0u), "r"(h == 0 ? 0x00f00000u : 0x000000f0u));
-                return y;
-            };
+        }
+        // a tile's sums start from zero and are added by rounding: left in the instruction's accumulators they would shrink
+        // by up to 2^-23 with every step
 #pragma unroll
-            for (int k = 0; k < NBK; ++k)
+        for (int k = 0; k < NBK; ++k)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {  // byte j of the four words: dims 2j (rows g) and 2j + 1 (rows g + 8)
-                    const uint32_t sel = 0x4400u + 0x1111u * j;
-                    const uint32_t x = __byte_perm(vw[k][0], vw[k][2], sel), y = __byte_perm(vw[k][1], vw[k][3], sel);
+            for (int j = 0; j < 4; ++j) {  // byte j of the words: dims 2j (rows g) and 2j + 1 (rows g + 8)
+                const uint32_t sel = 0x4400u + 0x1111u * j;
+                float part[NT][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    auto code = [&](uint32_t x) {  // of two positions, one counted down: (x & mask) ^ half of it in one instruction
+                        uint32_t y;
+                        asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0x00f000f0u), "r"(h == 0 ? 0x00f00000u : 0x000000f0u));
+                        return y;
+                    };
+                    const uint32_t x = __byte_perm(vw[h][k][0], vw[h][k][2], sel), y = __byte_perm(vw[h][k][1], vw[h][k][3], sel);
                     const uint32_t a0 = code(x << 4), a1 = code(x), a2 = code(y << 4), a3 = code(y);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(acc[n][k][j], a0, a1, a2, a3, b0[n], b1[n]);
+                    for (int n = 0; n < NT; ++n) {
+                        if (h == 0) mma_f16_first(part[n], a0, a1, a2, a3, b0[h][n], b1[h][n]);
+                        else mma_f16(part[n], a0, a1, a2, a3, b0[h][n], b1[h][n]);
+                    }
                 }
-        }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][k][j][i] += part[n][i];
+            }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     // ---- join the warps: sums of a row over its eight lanes, then rows over the warps through shared memory
@@ -903,7 +916,7 @@ static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
 static int attn_tile_rows(int t, int n_heads, int n_kv) { return (size_t)t * (n_heads / n_kv) <= ATT4_ROWS ? ATT4_ROWS : 2 * ATT4_ROWS; }
 
 // How a call is launched: CTAs, and the workspace of its chunks.  The lengths are on the device; a cache that could not make
-// two chunks of a sequence is not split.
+// two chunks of a sequence is not split, nor a call of so many units that a long one among short ones hardly shows.
 struct AttnPlan {
     int tile_rows, row_tiles, slots;
     size_t units, ctas;
@@ -915,7 +928,8 @@ static AttnPlan attn_plan(size_t batch, int t, int n_heads, int n_kv, int hd, in
     a.tile_rows = attn_tile_rows(t, n_heads, n_kv);
     a.row_tiles = (int)(((size_t)t * (n_heads / n_kv) + a.tile_rows - 1) / a.tile_rows);
     a.units = batch * n_kv * a.row_tiles;
-    a.slots = lmax <= ATT4_LEAST * ATT4_GRAIN ? 0 : sms * ATT4_PER_SM;
+    a.slots = sms * ATT4_PER_SM;
+    if (lmax <= ATT4_LEAST * ATT4_GRAIN || a.units > (size_t)16 * a.slots) a.slots = 0;
     a.ctas = a.slots == 0 ? a.units : a.units * 2 < (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;  // see find_attn_work
     if (a.slots) {
         auto up = [](size_t v) { return (v + 255) / 256 * 256; };
@@ -1034,8 +1048,8 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
     if (int rc = check_kv4(n_heads, n_kv_heads, head_dim, lmax)) return rc;
     if (t < 0) return fail(KB_ERR_INVALID, "attention: %d query tokens", t);
     if (!(fabsf(scale) < INFINITY)) return fail(KB_ERR_INVALID, "attention: scale must be finite");
-    if (!aligned16(k_codes, k_steps, v_codes, v_steps) || !aligned16(q, out, workspace))
-        return fail(KB_ERR_INVALID, "kv4: planes, queries, outputs and workspace must be 16-byte aligned");
+    if (!aligned16(k_codes, k_steps, v_codes, v_steps) || !aligned16(workspace))
+        return fail(KB_ERR_INVALID, "kv4: planes and workspace must be 16-byte aligned");
     if (batch == 0 || t == 0) return KB_OK;
     if (batch > 0x7fffffffu || batch * (size_t)t * n_heads > 0x7fffffffu || (size_t)t * n_heads > 0x7fffffffu)
         return fail(KB_ERR_UNSUPPORTED, "attention: %zu sequences of %d tokens", batch, t);

@@ -114,7 +114,7 @@ def test_empty_calls_do_nothing(lib):
     (_read, dict(rows=None), E_INVALID), (_read, dict(k=None, v=None), E_INVALID), (_read, dict(kc=None), E_INVALID),
     (_read, dict(hd=6), E_UNSUPPORTED), (_read, dict(lmax=2), E_UNSUPPORTED), (_read, dict(v=P + 8), E_INVALID),
     (_attn, dict(lens=None), E_INVALID), (_attn, dict(heads=5), E_INVALID), (_attn, dict(hd=256), E_UNSUPPORTED),
-    (_attn, dict(t=-1), E_INVALID), (_attn, dict(q=P + 4), E_INVALID), (_attn, dict(lmax=7), E_UNSUPPORTED),
+    (_attn, dict(t=-1), E_INVALID), (_attn, dict(ws=P + 4), E_INVALID), (_attn, dict(lmax=7), E_UNSUPPORTED),
     (_attn, dict(batch=1 << 40), E_UNSUPPORTED), (_attn, dict(scale=float("inf")), E_INVALID),
     (_sample, dict(u=None), E_INVALID), (_sample, dict(vocab=0), E_INVALID), (_sample, dict(vocab=(1 << 19) + 1), E_UNSUPPORTED),
     (_sample, dict(ld=9), E_INVALID), (_sample, dict(n=1 << 40), E_UNSUPPORTED),
