@@ -297,7 +297,7 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
  * zeros; positions it does not see have no influence, whatever they hold.  scale multiplies the scores, 0 means
  * 1 / sqrt(head_dim).  Statistics and sums are f32; queries and softmax weights enter the products with 22 bits (results
  * within 1e-6 .. 2e-6 of 64-bit ones).  A query with an infinity or a NaN, or one that scale * log2(e) takes to 2^120 and
- * beyond, gives NaN.  The answer depends neither on the launch nor on other calls.  workspace:
+ * beyond, gives NaN.  The same call gives the same bits.  workspace:
  * kb_attn_kv4_workspace_bytes bytes (for the current device), 16-byte aligned, no initial contents needed, not shared by
  * calls that overlap; NULL takes it from the stream-ordered allocator. */
 int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes,

@@ -12,8 +12,8 @@
 //      largest, in 16 bits, goes through an atomic (the sum of a bin is good to 2^-15), while threads add up the exact
 //      total: the bins that may hold the border are then known, one or two of them;
 //   2. their elements (a few dozen of 32000 normal logits) are collected and what lies before them is summed exactly.  While
-//      there are more than SAMPLE_CAND of them (flat distributions, ties), the part of the order that they span is cut into
-//      1024 bins of exact 64-bit sums;
+//      there are more than SAMPLE_CAND of them (flat distributions), the part of the order that they span is cut into 1024
+//      bins of exact 64-bit sums; where a CTA has more than SAMPLE_OWN of them (ties) by going over its logits again;
 //   3. every CTA finds the element among the candidates by counting.
 // Where all that is kept down to there is a short list (top-k, most nuclei), the whole of it is collected in step 2 and the
 // rest, the draw included, happens on the list without another exchange.  Otherwise step 2 has the sums of the kept weights
@@ -33,6 +33,7 @@ using u64 = unsigned long long;
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_BINS = 1024;
+constexpr int SAMPLE_OWN = 1024;  // elements that a CTA collects
 constexpr int SAMPLE_CAND = 256;  // counting what lies before each of c elements takes c^2 / 512 steps of a thread
 constexpr int SAMPLE_CTAS = 8;    // of a cluster, at most
 constexpr size_t SAMPLE_MAX_VOCAB = (size_t)1 << 19;
@@ -49,13 +50,19 @@ struct SampleParams {
     float *logprobs;
 };
 
+struct __align__(16) Candidate {
+    u64 comp;
+    double weight;  // a whole number; the sum of SAMPLE_CAND of them has 52 bits
+};
+
 struct SampleShared {
     u64 slot[8][SAMPLE_CTAS];  // one row per exchange between the CTAs
     u64 scratch[SAMPLE_WARPS], segment[SAMPLE_WARPS];
     double scale[32];               // see exp2_fixed
     uint32_t hist[2][SAMPLE_BINS];  // counts or shares; 64-bit sums take both (64-bit shared atomics are compare-and-swap loops)
-    u64 own[SAMPLE_CAND], all[SAMPLE_CAND], measure[SAMPLE_CAND];
-    uint32_t n_own;
+    u64 own[SAMPLE_OWN], chosen[SAMPLE_CAND];  // collected by this CTA, and what is left of them in a part of the order
+    Candidate all[SAMPLE_CAND];                // of the whole row
+    uint32_t n_own, n_chosen;
     int bin[2];
     u64 before, upto, found;
 };
@@ -271,9 +278,15 @@ struct Row {
     }
     __device__ __forceinline__ void collect(u64 c, u64 &lo, u64 &hi) const {
         const uint32_t slot = atomicAdd(&sh.n_own, 1u);
-        if (slot < SAMPLE_CAND) sh.own[slot] = c;
+        if (slot < SAMPLE_OWN) sh.own[slot] = c;
         lo = min(lo, c);
         hi = max(hi, c);
+    }
+    // CTAs that collected more than they have room for
+    __device__ __forceinline__ bool overflown(int id) const {
+        bool over = false;
+        for (uint32_t c = 0; c < ctas; ++c) over |= sh.slot[id][c] > SAMPLE_OWN;
+        return over;
     }
 
     // Top-k for a k that is small against the number of threads: a histogram of the threads' own largest logits (mine_top) is
@@ -304,19 +317,18 @@ struct Row {
         ptx::cluster_sync();
         const u64 count = told(5, plus);
         if (count == 0 || count > SAMPLE_CAND) return 0;
-        fetch_list(count);
+        fetch_list(sh.own, count);
         cut_list<false>(kept, (uint32_t)count, (u64)k);
         return (int)count;
     }
-    // the candidates of all CTAs (their numbers in slot 5) into sh.all, and their weights
-    __device__ void fetch_list(u64 count) const {
+    // the candidates of all CTAs (their numbers in slot 5) into sh.all, with their weights
+    __device__ void fetch_list(const u64 *from, u64 count) const {
         uint32_t c = 0;
         u64 base = 0;
         for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
             while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
-            const u64 e = ld_cluster(sh.own + (i - base), c);
-            sh.all[i] = e;
-            sh.measure[i] = weight(logit_of(e));
+            const u64 e = ld_cluster(from + (i - base), c);
+            sh.all[i] = {e, (double)weight(logit_of(e))};
         }
     }
     // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
@@ -361,17 +373,21 @@ struct Row {
             for (int k = 0; k < 2; ++k)
                 w[k] = (double)mine[k] * (1.0 / 65535) * (double)exp2f((float)(2 * threadIdx.x + k) * (-1.4426950408889634f * 32 / SAMPLE_BINS));
             double upto = block_scan(w[0] + w[1]);
+            // shares up to bin[1]: 0.969 to 1 of 65535 for every element
+            u64 shares = block_scan(mine[0] + mine[1]);
+            if (threadIdx.x == SAMPLE_THREADS - 1) sh.upto = shares;
+            __syncthreads();
 #pragma unroll
             for (int k = 1; k >= 0; --k) {
                 if (upto - w[k] < aim - slack && aim - slack <= upto) sh.bin[0] = 2 * threadIdx.x + k;
-                if (upto - w[k] < aim + slack && aim + slack <= upto) sh.bin[1] = 2 * threadIdx.x + k;
+                if (upto - w[k] < aim + slack && aim + slack <= upto) {
+                    sh.bin[1] = 2 * threadIdx.x + k;
+                    sh.upto = shares;
+                }
                 upto -= w[k];
+                shares -= mine[k];
             }
             if (threadIdx.x == 0 && aim - slack <= 0.0) sh.bin[0] = 0;
-            // shares up to bin[1]: 0.969 to 1 of 65535 for every element
-            const u64 shares = block_scan(mine[0] + mine[1]);
-            __syncthreads();
-            if (sh.bin[1] / 2 == (int)threadIdx.x) sh.upto = sh.bin[1] & 1 ? shares : shares - mine[1];
         } else {
             target = target_of(0);
             find_bin(mine, target);
@@ -407,26 +423,36 @@ struct Row {
         ptx::cluster_sync();
         if (WEIGHT) target -= told(4, plus);
         u64 count = told(5, plus);
+        const bool over = overflown(5);  // then the logits are gone over again, otherwise what was collected
+        const uint32_t n_own = min(sh.n_own, (uint32_t)SAMPLE_OWN);
+        const u64 *from_list = sh.own;
         while (count > SAMPLE_CAND) {  // the part of the order that they span, cut into bins of 64-bit sums
             lo = cluster_reduce(lo, 6, least);
             hi = ~cluster_reduce(~hi, 7, least);
             const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
             hist_clear();
-            each4<true>([&](const float (&x)[4], int i) {
+            if (over) {
+                each4<true>([&](const float (&x)[4], int i) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const u64 c = comp_of(x[k], i + k);
-                    const bool in = kept(x[k], i + k) && c >= lo && c <= hi;
-                    if (!__any_sync(0xffffffffu, in)) continue;
-                    u64 m = !in ? 0ull : (WEIGHT ? weight(x[k]) : 1ull);
-                    int b = m ? (int)((c - lo) >> shift) : -1;
-                    if (__all_sync(0xffffffffu, b == __shfl_sync(0xffffffffu, b, 0))) {  // ties and flat rows: one addition for the warp
-                        m = warp_sum(m);
-                        if (threadIdx.x & 31) b = -1;
+                    for (int k = 0; k < 4; ++k) {
+                        const u64 c = comp_of(x[k], i + k);
+                        const bool in = kept(x[k], i + k) && c >= lo && c <= hi;
+                        if (!__any_sync(0xffffffffu, in)) continue;
+                        u64 m = !in ? 0ull : (WEIGHT ? weight(x[k]) : 1ull);
+                        int b = m ? (int)((c - lo) >> shift) : -1;
+                        if (__all_sync(0xffffffffu, b == __shfl_sync(0xffffffffu, b, 0))) {  // ties: one addition for the warp
+                            m = warp_sum(m);
+                            if (threadIdx.x & 31) b = -1;
+                        }
+                        hist_add64(b, m);
                     }
-                    hist_add64(b, m);
+                });
+            } else {
+                for (uint32_t i = threadIdx.x; i < n_own; i += SAMPLE_THREADS) {
+                    const u64 c = sh.own[i];
+                    if (c >= lo && c <= hi) hist_add64((int)((c - lo) >> shift), WEIGHT ? weight(logit_of(c)) : 1ull);
                 }
-            });
+            }
             ptx::cluster_sync();
             u64 high[2];
             hist_row(0, mine);
@@ -434,42 +460,58 @@ struct Row {
             mine[0] += high[0] << 32;
             mine[1] += high[1] << 32;
             find_bin(mine, target);
-            if (threadIdx.x == 0) sh.n_own = 0;
+            if (threadIdx.x == 0) sh.n_chosen = 0;
             __syncthreads();
             target -= sh.before;
             const u64 first = lo;
             lo += (u64)sh.bin[0] << shift;
             hi = min(hi, lo + ((1ull << shift) - 1));
             u64 new_lo = ~0ull, new_hi = 0;
-            each4<false>([&](const float (&x)[4], int i) {
-                bool above[4];
+            auto choose = [&](u64 c) {
+                const uint32_t slot = atomicAdd(&sh.n_chosen, 1u);
+                if (slot < SAMPLE_CAND) sh.chosen[slot] = c;
+                new_lo = min(new_lo, c);
+                new_hi = max(new_hi, c);
+            };
+            if (over) {
+                each4<false>([&](const float (&x)[4], int i) {
+                    bool above[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const u64 c = comp_of(x[k], i + k);
-                    const bool in = kept(x[k], i + k);
-                    above[k] = in && c >= first && c < lo;
-                    if (in && c >= lo && c <= hi) collect(c, new_lo, new_hi);
-                }
-                if (WEIGHT) sum += weigh(x, above);
-            });
+                    for (int k = 0; k < 4; ++k) {
+                        const u64 c = comp_of(x[k], i + k);
+                        const bool in = kept(x[k], i + k);
+                        above[k] = in && c >= first && c < lo;
+                        if (in && c >= lo && c <= hi) choose(c);
+                    }
+                    if (WEIGHT) sum += weigh(x, above);
+                });
+            } else {
+                for (uint32_t i = threadIdx.x; i < n_own; i += SAMPLE_THREADS)
+                    if (sh.own[i] >= lo && sh.own[i] <= hi) choose(sh.own[i]);
+            }
             lo = new_lo;
             hi = new_hi;
             __syncthreads();
-            tell(sh.n_own, 5);
+            tell(sh.n_chosen, 5);
             ptx::cluster_sync();
             count = told(5, plus);
+            from_list = sh.chosen;
         }
-        fetch_list(count);
+        fetch_list(from_list, count);
         cut_list<WEIGHT>(kept, (uint32_t)count, target);
         if (list) return (int)count;
-        if (WEIGHT) {  // the kept candidates of this CTA go to their segments
+        if (WEIGHT) {  // what is kept of this CTA's candidates goes to its segment
             sum = warp_sum(sum);
             if ((threadIdx.x & 31) == 0) sh.segment[threadIdx.x >> 5] = sum;
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < (uint32_t)count; i += SAMPLE_THREADS) {
-                const u64 e = sh.all[i];
-                const int at = (int)(uint32_t)e - i0;
-                if (at >= 0 && at < n && kept(logit_of(e), (int)(uint32_t)e)) atomicAdd(sh.segment + at / 4 / quads_per_warp(), sh.measure[i]);
+            auto put = [&](u64 e) {
+                if (kept(logit_of(e), (int)(uint32_t)e))
+                    atomicAdd(sh.segment + ((int)(uint32_t)e - i0) / 4 / quads_per_warp(), weight(logit_of(e)));
+            };
+            if (over) {
+                for (uint32_t i = threadIdx.x; i < min(sh.n_chosen, (uint32_t)SAMPLE_CAND); i += SAMPLE_THREADS) put(sh.chosen[i]);
+            } else {
+                for (uint32_t i = threadIdx.x; i < n_own; i += SAMPLE_THREADS) put(sh.own[i]);
             }
             __syncthreads();
         }
@@ -486,9 +528,13 @@ struct Row {
         __syncthreads();
         for (uint32_t start = 0; start < count; start += SAMPLE_THREADS / per) {
             const uint32_t i = start + threadIdx.x / per;
-            const auto c = i < count ? key(sh.all[i]) : key(0);
-            u64 before = 0;
-            for (uint32_t j = threadIdx.x % per; j < count; j += per) before += key(sh.all[j]) < c ? (WEIGHT ? sh.measure[j] : 1ull) : 0ull;
+            const auto c = i < count ? key(sh.all[i].comp) : key(0);
+            double before = 0.0;  // whole numbers of at most 52 bits
+#pragma unroll 4
+            for (uint32_t j = threadIdx.x % per; j < count; j += per) {
+                const Candidate e = sh.all[j];
+                if (key(e.comp) < c) before += WEIGHT ? e.weight : 1.0;
+            }
             for (uint32_t o = per / 2; o > 0; o /= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
             if (i < count && threadIdx.x % per == 0) f(i, before);
         }
@@ -497,19 +543,20 @@ struct Row {
     // cuts behind the element of the list at which the measure reaches target
     template <bool WEIGHT>
     __device__ void cut_list(Kept &kept, uint32_t count, u64 target) const {
-        in_order<WEIGHT>(count, [](u64 c) { return c; }, [&](uint32_t i, u64 before) {
-            if (before < target && target <= before + (WEIGHT ? sh.measure[i] : 1ull)) sh.found = sh.all[i];
+        const double at = (double)target;
+        in_order<WEIGHT>(count, [](u64 c) { return c; }, [&](uint32_t i, double before) {
+            if (before < at && at <= before + (WEIGHT ? sh.all[i].weight : 1.0)) sh.found = sh.all[i].comp;
         });
         kept.cut(sh.found);
     }
-    // measure 0 for what is not kept any more; returns the sum of the others
+    // weight 0 for what is not kept any more; returns the sum of the others
     __device__ u64 keep_list(const Kept &kept, uint32_t count) const {
         u64 sum = 0;
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
-            const u64 c = sh.all[i];
-            if (!kept(logit_of(c), (int)(uint32_t)c)) sh.measure[i] = 0;
-            sum += sh.measure[i];
+            const u64 c = sh.all[i].comp;
+            if (!kept(logit_of(c), (int)(uint32_t)c)) sh.all[i].weight = 0.0;
+            sum += (u64)sh.all[i].weight;
         }
         return block_reduce(sum, plus);
     }
@@ -637,9 +684,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         }
     };
     if (list) {  // every CTA knows the answer, the first one writes it
-        const u64 all = row.keep_list(kept, list), draw = drawn(u, all);
-        row.in_order<true>(list, [](u64 c) { return (uint32_t)c; }, [&](uint32_t i, u64 before) {
-            if (row.rank == 0 && draw >= before && draw < before + sh.measure[i]) chosen(logit_of(sh.all[i]), (int)(uint32_t)sh.all[i], all);
+        const u64 all = row.keep_list(kept, list);
+        const double draw = (double)drawn(u, all);
+        row.in_order<true>(list, [](u64 c) { return (uint32_t)c; }, [&](uint32_t i, double before) {
+            const Candidate e = sh.all[i];
+            if (row.rank == 0 && draw >= before && draw < before + e.weight) chosen(logit_of(e.comp), (int)(uint32_t)e.comp, all);
         });
         ptx::cluster_sync();  // the others have read this CTA's candidates
         return;

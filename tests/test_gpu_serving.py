@@ -18,7 +18,7 @@ def env():
     from kore_b200 import KoreError, decoder, serving
 
     assert torch.cuda.is_available()
-    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    dev = lambda a: torch.from_numpy(np.array(a)).cuda()
     return type("E", (), {"torch": torch, "serving": serving, "decoder": decoder, "KoreError": KoreError, "dev": staticmethod(dev)})
 
 
@@ -349,6 +349,18 @@ def test_sample_ties_and_flat_rows(env):
     steps = np.round(cases.gaussian(3, (n, v), 2.0))  # a few dozen different logits
     check_sample(env, steps, u, top_k=[1, 2, 3, 5, 50, 500, 1000, 4000])
     check_sample(env, steps, u, top_p=[0.01, 0.1, 0.3, 0.5, 0.7, 0.9, 0.99, 0.999])
+
+
+@pytest.mark.parametrize("vocab,spread", [(60000, 0.05), (131072, 1.0), (40000, 0.0), (9000, 0.2), (200003, 4.0)])
+def test_sample_many_candidates(env, vocab, spread):
+    """borders inside bins of hundreds to tens of thousands of elements, of unlike and of equal logits"""
+    n = 6
+    logits = cases.gaussian(vocab, (n, vocab), spread)
+    u = ((np.arange(n) + 0.37) / n).astype(f32)
+    check_sample(env, logits, u, top_p=[0.1, 0.5, 0.9, 0.99, 0.99999, 0.3])
+    check_sample(env, logits, u, top_k=[300, 2999, 127, 129, vocab - 1, 20000 if vocab > 20000 else 5000])
+    check_sample(env, logits, u, top_k=5000, top_p=0.7, temperature=1.7)
+    check_sample(env, logits, u, temperature=[0.05, 0.3, 1.0, 3.0, 30.0, 1000.0], top_p=0.95, min_p=0.001)
 
 
 def test_sample_special_rows_and_settings(env):
