@@ -871,8 +871,8 @@ static int launch_attn_kv4(const AttnParams &p, unsigned ctas, int dev, cudaStre
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 attention launch");
 }
 
-// One CTA per query row: the weighted mean of its chunks where there are several, a thread per dim.  Eight chunks are read
-// at a time; their factors come from the lanes of a warp, one chunk each.
+// One CTA per query row: the weighted mean of its chunks where there are several, a thread per dim.  A round takes 32 chunks,
+// a lane's factor each; the first sums are on their way while the factors are worked out.
 __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p) {
     const unsigned row = blockIdx.x, tok = row / p.n_heads;
     const int lane = threadIdx.x & 31, d = threadIdx.x, h = row - tok * p.n_heads, b = tok / p.t, i = tok - b * p.t;
@@ -884,20 +884,26 @@ __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p)
     const size_t stride = p.tile_rows, at = (size_t)of.x * stride + (r - tile * p.tile_rows);
     const float2 *ml = p.part_ml + at;
     const float *src = p.part + at * p.hd + (d < p.hd ? d : 0);
-    float top = -INFINITY, sum = 0.0f, o = 0.0f;
-    for (int s = lane; s < n; s += 32) top = fmaxf(top, ml[s * stride].x);
+    constexpr int FIRST = 16;
+    float x[FIRST];
+    float2 v = lane < n ? ml[lane * stride] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int k = 0; k < FIRST; ++k) x[k] = k < n ? src[k * stride * p.hd] : 0.0f;
+    float top = v.x, sum = 0.0f, o = 0.0f;
+    for (int s = 32 + lane; s < n; s += 32) top = fmaxf(top, ml[s * stride].x);
     top = warp_reduce_max(top);
     for (int s0 = 0; s0 < n; s0 += 32) {
-        const float2 v = s0 + lane < n ? ml[(s0 + lane) * stride] : make_float2(0.0f, 0.0f);
+        if (s0) v = s0 + lane < n ? ml[(s0 + lane) * stride] : make_float2(0.0f, 0.0f);
         const float mine = v.y == 0.0f ? 0.0f : exp2_fast(v.x - top);
         sum = fmaf(v.y, mine, sum);
         const int m = min(32, n - s0);
-        for (int s = 0; s < m; s += 8) {
-            float x[8];
+        for (int s = 0; s < m; s += FIRST) {
+            if (s0 + s) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = s + k < m ? src[(s0 + s + k) * stride * p.hd] : 0.0f;
+                for (int k = 0; k < FIRST; ++k) x[k] = s + k < m ? src[(s0 + s + k) * stride * p.hd] : 0.0f;
+            }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o = fmaf(x[k], __shfl_sync(0xffffffffu, mine, s + k), o);
+            for (int k = 0; k < FIRST; ++k) o = fmaf(x[k], __shfl_sync(0xffffffffu, mine, s + k), o);
         }
     }
 #pragma unroll
