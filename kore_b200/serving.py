@@ -31,17 +31,26 @@ def _refuse(t, name, dtype, shape, dev):
     raise KoreError(_cabi.ERR_INVALID, f"{name}: expected a contiguous tensor")
 
 
-def _need(t, name: str, dtype, shape=None, dev=None, contiguous: bool = True):
-    """t is a CUDA tensor of this type, shape and device index, or a KoreError in the library's manner"""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and (shape is None or t.shape == shape)
-            and (dev is None or t.get_device() == dev) and (not contiguous or t.is_contiguous())):
-        _refuse(t, name, dtype, shape, dev)
-    return t
+def _need(t, name: str, dtype, shape, dev: int):
+    """t is a contiguous tensor of this type and shape on this GPU, or a KoreError in the library's manner"""
+    try:
+        if t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous():
+            return t
+    except AttributeError:
+        pass
+    _refuse(t, name, dtype, shape, dev)
 
 
-def _dims(t, name: str, want: str, n: int):
-    if t.dim() != n:
+def _rows(t, name: str, dtype, want: str, dims: int, dev=None):
+    """t is a tensor of this type and number of dimensions on this (or any) GPU, strided as it may be; its device index"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not dtype:
+        _refuse(t, name, dtype, None, dev)
+    if t.dim() != dims:
         raise KoreError(_cabi.ERR_SHAPE, f"{name}: shape mismatch: expected {want}, got {list(t.shape)}")
+    at = t.get_device()
+    if dev is not None and at != dev:
+        _refuse(t, name, dtype, None, dev)
+    return at
 
 
 def _run(dev: int, fn, *args):
@@ -84,9 +93,8 @@ class KV4Cache:
     def _adopt(self, k_codes, k_steps, v_codes, v_steps, head_dim):
         if head_dim < 4 or head_dim > 128 or head_dim % 4:
             raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: head_dim {head_dim} must be a multiple of 4 up to 128")
-        _need(k_codes, "k_codes", _I32)
-        _dims(k_codes, "k_codes", "[n_seqs, n_kv_heads, max_len, words]", 4)
-        shape, dev = tuple(k_codes.shape[:3]) + ((head_dim + 7) // 8,), k_codes.get_device()
+        dev = _rows(k_codes, "k_codes", _I32, "[n_seqs, n_kv_heads, max_len, words]", 4)
+        shape = tuple(k_codes.shape[:3]) + ((head_dim + 7) // 8,)
         for t, name, want in ((k_codes, "k_codes", shape), (k_steps, "k_steps", shape[:3]), (v_codes, "v_codes", shape),
                               (v_steps, "v_steps", shape[:3])):
             _need(t, name, _I32, want, dev)
@@ -106,12 +114,12 @@ class KV4Cache:
         """The f32 values of cache rows (int64 [n], row = sequence * max_len + position; zeros for a row outside the
         cache): K and V, each [n, n_kv_heads, head_dim]."""
         dev = self._dev
-        _need(cache_rows, "cache_rows", _I64, None, dev)
-        _dims(cache_rows, "cache_rows", "[n]", 1)
+        _rows(cache_rows, "cache_rows", _I64, "[n]", 1, dev)
         n = cache_rows.shape[0]
+        _need(cache_rows, "cache_rows", _I64, (n,), dev)
         shape = (n, self.n_kv_heads, self.head_dim)
-        k_out = torch.empty(shape, dtype=_F32, device=self.device) if k_out is None else _need(k_out, "k_out", _F32, shape, dev)
-        v_out = torch.empty(shape, dtype=_F32, device=self.device) if v_out is None else _need(v_out, "v_out", _F32, shape, dev)
+        k_out = self.k_steps.new_empty(shape, dtype=_F32) if k_out is None else _need(k_out, "k_out", _F32, shape, dev)
+        v_out = self.k_steps.new_empty(shape, dtype=_F32) if v_out is None else _need(v_out, "v_out", _F32, shape, dev)
         if n:
             _run(dev, self._lib.kb_kv4_read, *self._planes, cache_rows.data_ptr(), n, self.n_kv_heads, self.head_dim, self.n_seqs,
                  self.max_len, k_out.data_ptr(), v_out.data_ptr())
@@ -132,14 +140,12 @@ def qknorm_rope_append(qkv, positions, cache_rows, cos, sin, cache, n_heads: int
         planes, fn = cache._planes, cache._lib.kb_qknorm_rope_kv4
     else:
         k, v = cache
-        _need(k, "k cache", _F32)
-        _dims(k, "k cache", "[n_seqs, n_kv_heads, max_len, head_dim]", 4)
-        n_seqs, n_kv, lmax, hd = k.shape
-        dev = k.get_device()
-        _need(v, "v cache", _F32, k.shape, dev)
+        dev = _rows(k, "k cache", _F32, "[n_seqs, n_kv_heads, max_len, head_dim]", 4)
+        n_seqs, n_kv, lmax, hd = shape = k.shape
+        _need(k, "k cache", _F32, shape, dev)
+        _need(v, "v cache", _F32, shape, dev)
         planes, fn = (k.data_ptr(), v.data_ptr()), _cabi.lib().kb_qknorm_rope_kv
-    _need(qkv, "qkv", _F32, None, dev, False)
-    _dims(qkv, "qkv", "[n, width]", 2)
+    _rows(qkv, "qkv", _F32, "[n, width]", 2, dev)
     n, width = qkv.shape
     if width != (n_heads + 2 * n_kv) * hd:
         raise KoreError(_cabi.ERR_SHAPE, f"qkv: shape mismatch: expected [{n}, {(n_heads + 2 * n_kv) * hd}], got {list(qkv.shape)}")
@@ -153,7 +159,7 @@ def qknorm_rope_append(qkv, positions, cache_rows, cos, sin, cache, n_heads: int
     gq = None if q_gamma is None else _need(q_gamma, "q_gamma", _F32, (hd,), dev).data_ptr()
     gk = None if k_gamma is None else _need(k_gamma, "k_gamma", _F32, (hd,), dev).data_ptr()
     if q_out is None:
-        q_out = torch.empty((n, n_heads, hd), dtype=_F32, device=qkv.device)
+        q_out = qkv.new_empty((n, n_heads, hd))
     else:
         _need(q_out, "q_out", _F32, (n, n_heads, hd), dev)
     if n:
@@ -168,9 +174,9 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     tokens.  Token i sees the positions below lens - (t - 1 - i); one that sees none gives zeros.  scale 0 is
     1 / sqrt(head_dim).  Returns float32 of q's shape."""
     hd, dev, n = cache.head_dim, cache._dev, cache.n_seqs
-    _need(q, "q", _F32, None, dev, False)
+    _rows(q, "q", _F32, f"[{n}, (t,) n_heads, {hd}]", 3 if isinstance(q, torch.Tensor) and q.dim() == 3 else 4, dev)
     shape = q.shape
-    if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != hd:
+    if shape[0] != n or shape[-1] != hd:
         raise KoreError(_cabi.ERR_SHAPE, f"q: shape mismatch: expected [{n}, (t,) n_heads, {hd}], got {list(shape)}")
     if not q.is_contiguous():
         q = q.contiguous()
@@ -185,7 +191,7 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
         with torch.cuda.device(dev):
             need = cache._ws_bytes[t, heads] = lib.kb_attn_kv4_workspace_bytes(n, t, heads, cache.n_kv_heads, hd, cache.max_len)
     if need:  # torch's allocator orders its reuse by stream and keeps a captured graph's blocks to that graph
-        block = torch.empty(need, dtype=torch.uint8, device=q.device)
+        block = q.new_empty(need // 4)
         ws = block.data_ptr()
     _run(dev, lib.kb_attn_kv4, q.data_ptr(), *cache._planes, lens.data_ptr(), n, t, heads, cache.n_kv_heads, hd, cache.max_len, scale,
          out.data_ptr(), ws, need)
@@ -198,10 +204,8 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, r
     float32 [n], top_k int32 [n].  A temperature of 0 is greedy.  Top-k and min-p act on the tempered distribution, top-p
     on what they keep.  Returns int64 [n], with return_logprobs also float32 [n]: the log of the token's share of what was
     kept."""
-    _need(logits, "logits", _F32, None, None, False)
-    _dims(logits, "logits", "[n, vocab]", 2)
+    dev = _rows(logits, "logits", _F32, "[n, vocab]", 2)
     n, vocab = shape = logits.shape
-    dev = logits.get_device()
     if not logits.is_contiguous() and (logits.stride(1) != 1 or (n > 1 and logits.stride(0) < vocab)):
         logits = logits.contiguous()
     row = shape[:1]
@@ -211,8 +215,8 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, r
     pk = None if top_k is None else _need(top_k, "top_k", _I32, row, dev).data_ptr()
     pp = None if top_p is None else _need(top_p, "top_p", _F32, row, dev).data_ptr()
     pm = None if min_p is None else _need(min_p, "min_p", _F32, row, dev).data_ptr()
-    tokens = torch.empty(row, dtype=_I64, device=logits.device) if tokens is None else _need(tokens, "tokens", _I64, row, dev)
-    logprobs = torch.empty(row, dtype=_F32, device=logits.device) if return_logprobs else None
+    tokens = logits.new_empty(row, dtype=_I64) if tokens is None else _need(tokens, "tokens", _I64, row, dev)
+    logprobs = logits.new_empty(row) if return_logprobs else None
     if n:
         _run(dev, _cabi.lib().kb_sample, logits.data_ptr(), n, vocab, logits.stride(0) if n > 1 else vocab, pt, pk, pp, pm,
              u.data_ptr(), tokens.data_ptr(), logprobs.data_ptr() if return_logprobs else None)
