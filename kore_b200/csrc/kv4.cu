@@ -59,7 +59,6 @@ struct AppendParams {
     int n_heads, n_kv, hd;
     long long cache_len;  // n_seqs * lmax
     int lmax;
-    bool pairs;  // rows and tables are 8-byte aligned: a lane's two neighbours come in one load
     float *q_out, *k_cache, *v_cache;
     uint32_t *k_codes, *k_steps, *v_codes, *v_steps;
 };
@@ -128,7 +127,8 @@ __device__ __forceinline__ double warp_sum_of(double (&v)[HPW]) {
 // Bound by the bytes of the rows for many tokens, by one memory round trip for a few.  A warp takes HPW heads of one token:
 // its lane l owns the rotation pairs 2l and 2l + 1, dims {2l, 2l + 1} of each half, so that its codes are whole bytes of the
 // row, a row needs no shared memory, and the token's angles are read once for all heads.
-template <bool Q4, int HPW>
+// PAIRS: rows and tables are 8-byte aligned and half is even, a lane's two neighbours come and go in one access.
+template <bool Q4, int HPW, bool PAIRS>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 8u + (threadIdx.x >> 5);
@@ -142,12 +142,20 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     float a[HPW][2], b[HPW][2];
     const float *row = p.qkv + (size_t)t * p.ld + (size_t)head0 * hd;
     auto load2 = [&](const float *src, float (&x)[2]) {
-        if (p.pairs) {  // half is even then
+        if (PAIRS) {
             const float2 v = own0 ? *reinterpret_cast<const float2 *>(src + i0) : make_float2(0.0f, 0.0f);
             x[0] = v.x; x[1] = v.y;
         } else {
             x[0] = own0 ? src[i0] : 0.0f;
             x[1] = own1 ? src[i0 + 1] : 0.0f;
+        }
+    };
+    auto store2 = [&](float *dst, const float (&x)[2]) {
+        if (PAIRS) {
+            if (own0) *reinterpret_cast<float2 *>(dst + i0) = make_float2(x[0], x[1]);
+        } else {
+            if (own0) dst[i0] = x[0];
+            if (own1) dst[i0 + 1] = x[1];
         }
     };
 #pragma unroll
@@ -167,7 +175,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
         load2(p.cos_t + (size_t)pos * half, c);
         load2(p.sin_t + (size_t)pos * half, s);
     }
-    if (p.q_gamma || p.k_gamma) {
+    const bool normed = p.q_gamma || p.k_gamma;
+    float inv_of = 0.0f;  // of head lane / (32 / HPW)
+    if (normed) {
         double ss[HPW];  // f64: the order of the sum then cannot move a rounding of inv, so codes do not depend on it
 #pragma unroll
         for (int j = 0; j < HPW; ++j) {
@@ -175,28 +185,55 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) ss[j] = fma((double)a[j][i], (double)a[j][i], fma((double)b[j][i], (double)b[j][i], ss[j]));
         }
-        const float inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);  // of head lane / (32 / HPW)
-        const float *held = nullptr;  // the gamma in g
-        float g[4] = {};
+        inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);
+    }
+    auto scale = [&](int j, const float (&ga)[2], const float (&gb)[2]) {
+        const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 32 / HPW * j);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), ga[i]);
+            b[j][i] = __fmul_rn(__fmul_rn(b[j][i], inv), gb[i]);
+        }
+    };
+    auto rotate = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float x = a[j][i], y = b[j][i];
+            a[j][i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+            b[j][i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
+        }
+    };
+    const float bad = __uint_as_float(0x7fffffffu);
+    float ga[2] = {}, gb[2] = {};
+    if (HPW > 1 && head0 + HPW <= p.n_heads) {  // queries only
+        if (p.q_gamma) {
+            load2(p.q_gamma, ga);
+            load2(p.q_gamma + half, gb);
+#pragma unroll
+            for (int j = 0; j < HPW; ++j) scale(j, ga, gb);
+        }
+        float *dst = p.q_out + ((size_t)t * p.n_heads + head0) * hd;
+#pragma unroll
+        for (int j = 0; j < HPW; ++j) {
+            rotate(j);
+            if (!pos_ok) a[j][0] = a[j][1] = b[j][0] = b[j][1] = bad;
+            store2(dst + j * hd, a[j]);
+            store2(dst + j * hd + half, b[j]);
+        }
+        return;
+    }
+    if (normed) {
+        const float *held = nullptr;  // the gamma in ga and gb
 #pragma unroll
         for (int j = 0; j < HPW; ++j) {
             const float *gamma = head0 + j < p.n_heads ? p.q_gamma : (head0 + j < p.n_heads + p.n_kv ? p.k_gamma : nullptr);
             if (!gamma) continue;
             if (gamma != held) {
                 held = gamma;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (i0 + i < half) {
-                        g[i] = gamma[i0 + i];
-                        g[2 + i] = gamma[half + i0 + i];
-                    }
+                load2(gamma, ga);
+                load2(gamma + half, gb);
             }
-            const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 32 / HPW * j);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[j][i] = __fmul_rn(__fmul_rn(a[j][i], inv), g[i]);
-                b[j][i] = __fmul_rn(__fmul_rn(b[j][i], inv), g[2 + i]);
-            }
+            scale(j, ga, gb);
         }
     }
     size_t seq = 0, cpos = 0;
@@ -208,33 +245,14 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
         const int head = head0 + j;
         if (head >= heads) break;
         const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.n_kv;
-        if (!is_v) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float x = a[j][i], y = b[j][i];
-                a[j][i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
-                b[j][i] = __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i]));
-            }
-        }
+        if (!is_v) rotate(j);
         if (!is_q && !stored) continue;
         if (is_q || !Q4) {
             const int kvh = is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
             float *dst = is_q ? p.q_out + ((size_t)t * p.n_heads + head) * hd : (is_v ? p.v_cache : p.k_cache) + (at0 + (size_t)kvh * p.lmax) * hd;
-            const float bad = __uint_as_float(0x7fffffffu);
             if (is_q && !pos_ok) a[j][0] = a[j][1] = b[j][0] = b[j][1] = bad;
-            if (p.pairs) {
-                if (own0) {
-                    *reinterpret_cast<float2 *>(dst + i0) = make_float2(a[j][0], a[j][1]);
-                    *reinterpret_cast<float2 *>(dst + half + i0) = make_float2(b[j][0], b[j][1]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (i0 + i < half) {
-                        dst[i0 + i] = a[j][i];
-                        dst[half + i0 + i] = b[j][i];
-                    }
-            }
+            store2(dst, a[j]);
+            store2(dst + half, b[j]);
             continue;
         }
         // hd is a multiple of 4 here, so a lane owns both of its pairs or none
@@ -247,7 +265,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     const float lo_of = bf16_below(mn_of);
     const float step_of = bf16_above_nonneg(fmaxf(__fdiv_rn(__fsub_rn(mx_of, lo_of), 15.0f), 0x1p-100f));
     const bool ok_of = fabsf(lo_of) < INFINITY && step_of < INFINITY;
-    const float inv_of = ok_of ? __frcp_rn(step_of) : 0.0f;  // 0: no row
+    const float per_of = ok_of ? __frcp_rn(step_of) : 0.0f;  // 0: no row
     const int words = kv4_words(hd);
     if (lane < HPW && head0 + lane >= p.n_heads && head0 + lane < heads) {
         const int kvh = head0 + lane - p.n_heads;
@@ -258,14 +276,14 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     for (int j = 0; j < HPW; ++j) {
         const int head = head0 + j;
         if (head >= heads) break;
-        const float lo = __shfl_sync(0xffffffffu, lo_of, j), inv = __shfl_sync(0xffffffffu, inv_of, j);
+        const float lo = __shfl_sync(0xffffffffu, lo_of, j), per = __shfl_sync(0xffffffffu, per_of, j);
         if (head < p.n_heads) continue;
         const bool is_v = head >= p.n_heads + p.n_kv;
         const size_t at = at0 + (size_t)(is_v ? head - p.n_heads - p.n_kv : head - p.n_heads) * p.lmax;
         // a code lies in 0 .. 15 already: x >= lo, and step is not below (max - lo) / 15.  Adding 1.5 2^23 rounds to even; two
         // of them make a byte of the sum's low bits
-        auto whole = [&](float x) { return __fadd_rn(__fmul_rn(__fsub_rn(x, lo), inv), 12582912.0f); };
-        auto byte_of = [&](const float (&x)[2]) { return inv == 0.0f ? (uint8_t)0 : (uint8_t)__float_as_uint(fmaf(whole(x[1]) - 12582912.0f, 16.0f, whole(x[0]))); };
+        auto whole = [&](float x) { return __fadd_rn(__fmul_rn(__fsub_rn(x, lo), per), 12582912.0f); };
+        auto byte_of = [&](const float (&x)[2]) { return per == 0.0f ? (uint8_t)0 : (uint8_t)__float_as_uint(fmaf(whole(x[1]) - 12582912.0f, 16.0f, whole(x[0]))); };
         uint8_t *bytes = reinterpret_cast<uint8_t *>((is_v ? p.v_codes : p.k_codes) + at * words);
         if (own0) {
             bytes[lane] = byte_of(a[j]);
@@ -969,8 +987,9 @@ static int append(AppendParams &p, bool q4, size_t n, size_t max_pos, size_t n_s
     p.max_pos = (int)max_pos;
     p.cache_len = (long long)n_seqs * p.lmax;
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.qkv) | reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t) |
-                          reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache);
-    p.pairs = p.hd % 4 == 0 && p.ld % 2 == 0 && all % 8 == 0;
+                          reinterpret_cast<uintptr_t>(p.q_gamma) | reinterpret_cast<uintptr_t>(p.k_gamma) | reinterpret_cast<uintptr_t>(p.q_out) |
+                          reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache);
+    const bool pairs = p.hd % 4 == 0 && p.ld % 2 == 0 && all % 8 == 0;
     // one head per warp while that leaves warps to spare (16 per SM), four for many tokens
     int dev = 0;
     KB_CUDA(cudaGetDevice(&dev));
@@ -978,7 +997,9 @@ static int append(AppendParams &p, bool q4, size_t n, size_t max_pos, size_t n_s
     p.groups = (unsigned)(many ? (heads + 3) / 4 : heads);
     unsigned grid = 0;
     if (int rc = warp_grid(n, p.groups, &p.tasks, &grid)) return rc;
-    void (*kern)(AppendParams) = q4 ? (many ? append_kernel<true, 4> : append_kernel<true, 1>) : (many ? append_kernel<false, 4> : append_kernel<false, 1>);
+    void (*kern)(AppendParams) =
+        q4 ? (many ? (pairs ? append_kernel<true, 4, true> : append_kernel<true, 4, false>) : (pairs ? append_kernel<true, 1, true> : append_kernel<true, 1, false>))
+           : (many ? (pairs ? append_kernel<false, 4, true> : append_kernel<false, 4, false>) : (pairs ? append_kernel<false, 1, true> : append_kernel<false, 1, false>));
     const cudaError_t e = launch_after(kern, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "append launch");
 }
