@@ -574,6 +574,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t r = blockIdx.x / ctas;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA runs: the others may write to its slots
     Row row = {sh};
     row.held = p.held;
     row.rank = ptx::cluster_ctarank();
@@ -617,6 +618,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     const uint32_t warp_top = __reduce_min_sync(0xffffffffu, (uint32_t)(comp_of(top + 0.0f, 0) >> 32));
     if (lane == 0) sh.scratch[warp] = warp_top;
     __syncthreads();  // the slice and the table are there, too
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     top = logit_of((u64)__reduce_min_sync(0xffffffffu, (uint32_t)sh.scratch[lane % SAMPLE_WARPS]) << 32);
     if (!(temp > 0.0f)) {  // the first of the largest: of the slice, then of all
         u64 best = ~0ull;
