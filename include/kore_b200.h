@@ -261,8 +261,8 @@ int kb_decoder_status(kb_decoder *h, kb_stream stream, int *status);
  *   codes  uint32 [n_seqs][n_kv_heads][lmax][kb_kv4_row_words(head_dim)]: dim 8w + i in bits 4i .. 4i+3 of word w, the tail
  *          of the last word zero;
  *   steps  uint32 [n_seqs][n_kv_heads][lmax]: two bfloat16 numbers, the step in the low half and lo in the high half.
- * A code c stands for lo + c * step (one f32 rounding).  head_dim is a multiple of 4 up to 128, lmax a multiple of 4, the
- * planes are 16-byte aligned.  A row is quantised from its own f32 values x:
+ * A code c stands for lo + c * step (one f32 rounding).  head_dim is a multiple of 4 up to 128, lmax a multiple of 4 up
+ * to 2^30, the planes are 16-byte aligned.  A row is quantised from its own f32 values x:
  *   lo = bfloat16 at or below min(x);  step = bfloat16 at or above max((max(x) - lo) / 15, 2^-100);
  *   code = clamp(rne((x - lo) * (1 / step)), 0, 15)
  * with every f32 operation rounded once.  A row that holds an infinity or a NaN, or whose range overflows f32, is stored
@@ -287,7 +287,7 @@ int kb_qknorm_rope_kv4(const float *qkv, size_t ld, const int *positions, const 
                        int n_heads, int n_kv_heads, int head_dim, size_t n_seqs, int lmax, float *q_out, uint32_t *k_codes,
                        uint32_t *k_steps, uint32_t *v_codes, uint32_t *v_steps, kb_stream stream);
 /* Rows read back as f32: out[i][n_kv_heads][head_dim] = the values of cache row cache_rows[i] (zeros where it lies outside
- * the cache), for K and V in one launch; k_out or v_out may be NULL. */
+ * the cache), for K and V in one launch; k_out or v_out may be NULL, and are 16-byte aligned. */
 int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes, const uint32_t *v_steps,
                 const long long *cache_rows, size_t n, int n_kv_heads, int head_dim, size_t n_seqs, int lmax, float *k_out,
                 float *v_out, kb_stream stream);
@@ -297,9 +297,10 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
  * zeros; positions it does not see have no influence, whatever they hold.  scale multiplies the scores, 0 means
  * 1 / sqrt(head_dim).  Statistics and sums are f32; queries and softmax weights enter the products with 22 bits (results
  * within 1e-6 .. 2e-6 of 64-bit ones).  A query with an infinity or a NaN, or one that scale * log2(e) takes to 2^120 and
- * beyond, gives NaN.  The same call gives the same bits.  workspace:
- * kb_attn_kv4_workspace_bytes bytes (for the current device), 16-byte aligned, no initial contents needed, not shared by
- * calls that overlap; NULL takes it from the stream-ordered allocator. */
+ * beyond, gives NaN.  Sums are held up to 2^8 times the weights and divided last, so values of V from 2^119 / lens on may
+ * overflow.  The same call gives the same bits.  out may be q.  workspace: kb_attn_kv4_workspace_bytes bytes (for the
+ * current device), 16-byte aligned, no initial contents needed, not shared by calls that overlap; NULL takes it from the
+ * stream-ordered allocator. */
 int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes,
                 const uint32_t *v_steps, const int *lens, size_t batch, int t, int n_heads, int n_kv_heads, int head_dim,
                 int lmax, float scale, float *out, void *workspace, size_t workspace_bytes, kb_stream stream);

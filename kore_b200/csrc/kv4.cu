@@ -14,6 +14,7 @@
 namespace kb {
 
 constexpr int KV4_MAX_HD = 128;
+constexpr int KV4_MAX_LEN = 1 << 30;  // positions are 32-bit numbers, with room for a chunk behind the last one
 
 __host__ __device__ inline int kv4_words(int hd) { return (hd + 7) / 8; }
 
@@ -408,8 +409,9 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
     // sum of ceil(g / size) <= total / size + sequences * units, which is at most `slots` for the first size.  Where the
     // units alone take most of the slots the second one is used, and up to a CTA per unit more than the GPU holds
     const unsigned share = p.slots - p.least_ctas > p.slots / 2 ? p.slots - p.least_ctas : p.slots;
-    const unsigned even = total >> 32 ? (unsigned)((total + share - 1) / share) : ((unsigned)total + share - 1) / share;
-    w.size = max((int)even, ATT4_LEAST);
+    const unsigned even = total >> 31 ? (unsigned)((total + share - 1) / share) : ((unsigned)total + share - 1) / share;
+    // no larger than the cache: many units over a long one would take the products below past 32 bits
+    w.size = min(max((int)even, ATT4_LEAST), (p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
     int first = 0;  // running sum of CTAs over the sequences
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
         const int b = b0 + lane, len = b0 == 0 ? len0 : b < p.batch ? kv4_len(p, b) : 0;
@@ -932,7 +934,7 @@ __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p)
 static int check_kv4(int n_heads, int n_kv, int hd, int lmax) {
     if (n_heads < 1 || n_kv < 1 || n_heads % n_kv) return fail(KB_ERR_INVALID, "kv4: %d heads over %d KV heads", n_heads, n_kv);
     if (hd < 4 || hd > KV4_MAX_HD || hd % 4) return fail(KB_ERR_UNSUPPORTED, "kv4: head_dim %d must be a multiple of 4 up to %d", hd, KV4_MAX_HD);
-    if (lmax < 4 || lmax % 4) return fail(KB_ERR_UNSUPPORTED, "kv4: cache length %d must be a multiple of 4", lmax);
+    if (lmax < 4 || lmax % 4 || lmax > KV4_MAX_LEN) return fail(KB_ERR_UNSUPPORTED, "kv4: cache length %d must be a multiple of 4 up to %d", lmax, KV4_MAX_LEN);
     return KB_OK;
 }
 

@@ -71,11 +71,13 @@ class KV4Cache:
     of bfloat16 numbers, 4.25 bits a value for heads of 128 (f32 caches take 32).
 
     ``k_codes`` / ``v_codes``: int32 [n_seqs, n_kv_heads, max_len, ceil(head_dim / 8)], ``k_steps`` / ``v_steps``: int32
-    [n_seqs, n_kv_heads, max_len]; a code c stands for lo + c * step.  ``max_len`` is rounded up to a multiple of 4."""
+    [n_seqs, n_kv_heads, max_len]; a code c stands for lo + c * step.  ``max_len`` is rounded up to a multiple of 4, at most 2^30."""
 
     def __init__(self, n_seqs: int, n_kv_heads: int, max_len: int, head_dim: int, device: int = 0):
         if min(n_seqs, n_kv_heads, max_len) < 1:
             raise KoreError(_cabi.ERR_INVALID, f"KV4Cache: {n_seqs} sequences, {n_kv_heads} KV heads, {max_len} positions")
+        if max_len > 1 << 30:
+            raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: {max_len} positions, at most {1 << 30}")
         max_len = (max_len + 3) // 4 * 4
         dev = torch.device("cuda", device)
         words = int(_cabi.lib().kb_kv4_row_words(head_dim))

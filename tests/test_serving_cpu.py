@@ -124,6 +124,13 @@ def test_refusals(lib, call, changes, code):
     assert lib.kb_last_error()
 
 
+@pytest.mark.parametrize("call", [_append4, _read, _attn])
+def test_the_longest_cache(lib, call):
+    """positions are 32-bit numbers with room for a chunk behind the last"""
+    assert call(lib, lmax=1 << 30) == 0
+    assert call(lib, lmax=(1 << 30) + 4) == E_UNSUPPORTED and call(lib, lmax=(1 << 31) - 4) == E_UNSUPPORTED
+
+
 def test_row_words(lib):
     assert [int(lib.kb_kv4_row_words(h)) for h in (-1, 0, 4, 8, 100, 128)] == [0, 0, 1, 1, 13, 16]
 
@@ -138,6 +145,8 @@ def test_python_layer_refuses_host_tensors():
     assert "logits" in e.value.message
     with pytest.raises(KoreError):
         serving.KV4Cache(1, 1, 0, 32)
+    with pytest.raises(KoreError):
+        serving.KV4Cache(1, 1, (1 << 30) + 1, 32)
     z = torch.zeros((1, 1, 4, 4), dtype=torch.int32)
     with pytest.raises(KoreError):
         serving.KV4Cache.from_planes(z, z, z, z, 32)
