@@ -102,15 +102,24 @@ class KV4Cache:
             _need(t, name, _I32, want, dev)
         if shape[2] % 4 or 0 in shape:
             raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: planes of {list(shape)}: the cache length must be a multiple of 4")
-        self.k_codes, self.k_steps, self.v_codes, self.v_steps = k_codes, k_steps, v_codes, v_steps
+        self._held = (k_codes, k_steps, v_codes, v_steps)
         self.n_seqs, self.n_kv_heads, self.max_len, self.head_dim = shape[0], shape[1], shape[2], int(head_dim)
         self.device = k_codes.device
-        self._dev, self._lib = dev, _cabi.lib()
-        self._planes = tuple(t.data_ptr() for t in (k_codes, k_steps, v_codes, v_steps))
+        self._dev = dev
         self._ws_bytes = {}  # workspace of attend by (query tokens, heads)
 
+    # the planes were checked once and stay: they may be written, not replaced
+    k_codes = property(lambda self: self._held[0])
+    k_steps = property(lambda self: self._held[1])
+    v_codes = property(lambda self: self._held[2])
+    v_steps = property(lambda self: self._held[3])
+
+    def _planes(self):
+        a, b, c, d = self._held
+        return a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr()
+
     def memory_bytes(self) -> int:
-        return sum(t.numel() * 4 for t in (self.k_codes, self.k_steps, self.v_codes, self.v_steps))
+        return sum(t.numel() * 4 for t in self._held)
 
     def read(self, cache_rows, k_out=None, v_out=None):
         """The f32 values of cache rows (int64 [n], row = sequence * max_len + position; zeros for a row outside the
@@ -123,7 +132,7 @@ class KV4Cache:
         k_out = self.k_steps.new_empty(shape, dtype=_F32) if k_out is None else _need(k_out, "k_out", _F32, shape, dev)
         v_out = self.k_steps.new_empty(shape, dtype=_F32) if v_out is None else _need(v_out, "v_out", _F32, shape, dev)
         if n:
-            _run(dev, self._lib.kb_kv4_read, *self._planes, cache_rows.data_ptr(), n, self.n_kv_heads, self.head_dim, self.n_seqs,
+            _run(dev, _cabi.lib().kb_kv4_read, *self._planes(), cache_rows.data_ptr(), n, self.n_kv_heads, self.head_dim, self.n_seqs,
                  self.max_len, k_out.data_ptr(), v_out.data_ptr())
         return k_out, v_out
 
@@ -139,7 +148,7 @@ def qknorm_rope_append(qkv, positions, cache_rows, cos, sin, cache, n_heads: int
     four = isinstance(cache, KV4Cache)
     if four:
         n_seqs, n_kv, lmax, hd, dev = cache.n_seqs, cache.n_kv_heads, cache.max_len, cache.head_dim, cache._dev
-        planes, fn = cache._planes, cache._lib.kb_qknorm_rope_kv4
+        planes, fn = cache._planes(), _cabi.lib().kb_qknorm_rope_kv4
     else:
         k, v = cache
         dev = _rows(k, "k cache", _F32, "[n_seqs, n_kv_heads, max_len, head_dim]", 4)
@@ -187,7 +196,7 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     out = torch.empty_like(q) if out is None else _need(out, "out", _F32, shape, dev)
     if q.numel() == 0:
         return out
-    lib, ws = cache._lib, 0
+    lib, ws = _cabi.lib(), 0
     need = cache._ws_bytes.get((t, heads))
     if need is None:
         with torch.cuda.device(dev):
@@ -195,7 +204,7 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     if need:  # torch's allocator orders its reuse by stream and keeps a captured graph's blocks to that graph
         block = q.new_empty(need // 4)
         ws = block.data_ptr()
-    _run(dev, lib.kb_attn_kv4, q.data_ptr(), *cache._planes, lens.data_ptr(), n, t, heads, cache.n_kv_heads, hd, cache.max_len, scale,
+    _run(dev, lib.kb_attn_kv4, q.data_ptr(), *cache._planes(), lens.data_ptr(), n, t, heads, cache.n_kv_heads, hd, cache.max_len, scale,
          out.data_ptr(), ws, need)
     return out
 
