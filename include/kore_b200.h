@@ -307,7 +307,8 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
 size_t kb_attn_kv4_workspace_bytes(size_t batch, int t, int n_heads, int n_kv_heads, int head_dim, int lmax);
 /* One token per row of logits [n][vocab] (row stride ld, 0 = vocab) from one given uniform number u[i] in [0, 1) per row.
  * Settings are device arrays of one value per row, each nullable (NULL: temperature 1, the filter off):
- *   weights  exp((logit - max) / temperature); a temperature of 0 (or below, or NaN) takes the largest logit;
+ *   weights  exp((logit - max) / temperature); a temperature of 0 (or below, or NaN) takes the largest logit, others below
+ *            2^-100 count as 2^-100;
  *   top_k    the k largest logits (<= 0: off);  min_p  weights of at least min_p times the largest (<= 0: off; above 1 is 1);
  *   top_p    of what those two keep, the shortest run from the largest on whose weights reach top_p of the sum (>= 1: off).
  * Runs go by logit, equal logits by index, lowest first; the largest is always kept.  The token is the first, in index

@@ -152,13 +152,15 @@ struct Row {
     uint32_t rank, ctas;
     float top;          // largest logit, at most FLT_MAX
     double per;         // log2(e) / temperature
-    float bins;         // bins per unit of logit
+    float bins;         // bins per two units of logit
 
     // exponent of a kept logit; infinite logits are all that is kept where there are any
     __device__ __forceinline__ double exponent(float x) const { return ((double)fminf(x, FLT_MAX) - (double)top) * per; }
     __device__ __forceinline__ u64 weight(float x) const { return exp2_fixed(exponent(x), true, sh.scale) - FIXED_ZERO; }
-    // place in the histogram, 0 .. 1023, falling with x
-    __device__ __forceinline__ float bin_at(float x) const { return fminf((top - fminf(x, FLT_MAX)) * bins, (float)(SAMPLE_BINS - 1)); }
+    // place in the histogram, 0 .. 1023, falling with x; half the difference, which the ends of the type do not take to infinity
+    __device__ __forceinline__ float bin_at(float x) const {
+        return fminf(fmaf(-0.5f, fminf(x, FLT_MAX), 0.5f * top) * bins, (float)(SAMPLE_BINS - 1));
+    }
 
     __device__ __forceinline__ void load4(int i, float (&x)[4]) const {
         if (held || (wide && 4 * i + 3 < n)) {
@@ -646,9 +648,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         }
         return;
     }
-    const double inv_t = 1.0 / (double)temp;
+    const float temp_used = fmaxf(temp, 0x1p-100f);  // below that `bins` could leave f32
+    const double inv_t = 1.0 / (double)temp_used;
     row.per = inv_t * 1.4426950408889634074;
-    row.bins = fminf((float)(inv_t * (SAMPLE_BINS / 32)), FLT_MAX);  // 0 times it is 0
+    row.bins = (float)(inv_t * (SAMPLE_BINS / 16));
     Kept kept = {top == INFINITY ? INFINITY : -FLT_MAX, 0x7fffffff};
     const int k = p.top_k ? p.top_k[r] : 0;
     int list = 0;
@@ -661,7 +664,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         // the smallest f32 logit that passes: the border in f64 is within a rounding of it
         const double border = log((double)fminf(mp, 1.0f));
         const auto passes = [&](float x) { return x >= row.top || ((double)x - (double)row.top) * inv_t >= border; };
-        float x = fminf((float)((double)row.top + border * (double)temp), row.top);
+        float x = fminf((float)((double)row.top + border * (double)temp_used), row.top);
         for (int i = 0; i < 4 && !passes(x); ++i) x = nextafterf(x, INFINITY);
         for (int i = 0; i < 4 && x > -INFINITY && passes(nextafterf(x, -INFINITY)); ++i) x = nextafterf(x, -INFINITY);
         kept.cut(x, 0x7fffffff);

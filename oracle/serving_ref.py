@@ -113,7 +113,7 @@ def sample_row(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not temperature > 0:
         return int(order[0]), 0.0, np.inf
     with np.errstate(invalid="ignore", divide="ignore"):
-        x = np.where(l == top, 0.0, np.where(np.isinf(l) | np.isinf(top), -np.inf, (l - top) / np.float64(temperature)))
+        x = np.where(l == top, 0.0, np.where(np.isinf(l) | np.isinf(top), -np.inf, (l - top) / max(np.float64(temperature), 2.0 ** -100)))
     x = x[order]
     n = len(l) if top_k <= 0 else min(int(top_k), len(l))
     if min_p > 0:

@@ -301,6 +301,126 @@ def test_attention_repeats_bit_for_bit_on_streams_and_in_graphs(env):
     assert all((o == ref).all() for o in outs)
 
 
+def test_attention_workspaces_and_places_of_a_c_caller(env):
+    """no workspace (eager and captured), one too small, queries and results at odd addresses, results over the queries"""
+    from kore_b200 import _cabi
+
+    t, lib = env.torch, _cabi.lib()
+    seqs, heads, kv, hd, lmax = 3, 8, 2, 100, 4000
+    cache = filled_cache(env, seqs, kv, lmax, hd, 16)
+    q = env.dev(cases.gaussian(7, (seqs, 1, heads, hd), 1.0))
+    lens = env.dev(np.array([4000, 17, 2600], np.int32))
+    ref = env.serving.attend(q, cache, lens)
+    need = int(lib.kb_attn_kv4_workspace_bytes(seqs, 1, heads, kv, hd, lmax))
+    assert need > 0
+    planes = [x.data_ptr() for x in (cache.k_codes, cache.k_steps, cache.v_codes, cache.v_steps)]
+    ws = t.empty(need, dtype=t.uint8, device="cuda")
+
+    def call(src, dst, space, size):
+        return lib.kb_attn_kv4(src.data_ptr(), *planes, lens.data_ptr(), seqs, 1, heads, kv, hd, lmax, 0.0, dst.data_ptr(), space, size,
+                               t.cuda.current_stream().cuda_stream)
+    out = t.zeros_like(q)
+    assert call(q, out, None, 0) == 0
+    t.cuda.synchronize()
+    assert (out == ref).all()
+    out.zero_()
+    assert call(q, out, ws.data_ptr(), need - 1) == _cabi.ERR_STORAGE
+    t.cuda.synchronize()
+    assert (out == 0).all()
+    src, dst = (t.zeros(q.numel() + 3, device="cuda")[o:o + q.numel()] for o in (1, 3))
+    src.copy_(q.view(-1))
+    assert call(src, dst, ws.data_ptr(), need) == 0
+    t.cuda.synchronize()
+    assert (dst.view_as(ref) == ref).all()
+    assert env.serving.attend(src.view_as(q), cache, lens, out=src.view_as(q)).data_ptr() == src.data_ptr()
+    assert (src.view_as(ref) == ref).all()
+    out.zero_()
+    g = t.cuda.CUDAGraph()
+    with t.cuda.graph(g):
+        assert call(q, out, None, 0) == 0
+    for _ in range(3):
+        g.replay()
+    t.cuda.synchronize()
+    assert (out == ref).all()
+
+
+def test_attention_of_more_units_than_are_split(env):
+    """1300 sequences of 8 KV heads: a CTA takes a unit whole, however long"""
+    rng = np.random.default_rng(8)
+    lens = rng.integers(0, 9, 1300)
+    lens[[0, 700, 1299]] = 700, 671, 1
+    check_attention(env, cases.gaussian(10, (1300, 1, 8, 4), 1.0), filled_cache(env, 1300, 8, 700, 4, 17), list(lens))
+
+
+def test_a_cache_of_more_than_2_31_words(env):
+    """the last rows of one sequence of 2^27 + 64 positions: appended, read back, attended to"""
+    t, hd, lmax = env.torch, 128, (1 << 27) + 64
+    if t.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 20 GB")
+    cache = env.serving.KV4Cache(1, 1, lmax, hd)
+    rows = np.array([0, (1 << 27) - 1, 1 << 27, lmax - 1], np.int64)
+    x = cases.gaussian(18, (4, 3 * hd), 1.0)
+    x[3, hd:2 * hd] = 4.0  # the last key
+    one, zero = np.ones((1, hd // 2), f32), np.zeros((1, hd // 2), f32)
+    q = env.serving.qknorm_rope_append(env.dev(x), t.zeros(4, dtype=t.int32, device="cuda"), env.dev(rows), env.dev(one), env.dev(zero), cache, 1)
+    assert (q.cpu().numpy()[:, 0] == x[:, :hd]).all()
+    k, v = (a.cpu().numpy()[:, 0] for a in cache.read(env.dev(rows)))
+    for got, at in ((k, hd), (v, 2 * hd)):
+        assert (got == sr.values(*sr.quantise(x[:, at:at + hd]), hd)).all()
+    ask = np.full((1, 1, 1, hd), 0.5, f32)  # 256 times the scale with the last key: 22.6; 0 with the empty rows
+    got = env.serving.attend(env.dev(ask), cache, env.dev(np.array([lmax], np.int32))).cpu().numpy()[0, 0, 0]
+    w = np.exp(k.astype(np.float64) @ ask[0, 0, 0].astype(np.float64) / np.sqrt(hd))
+    ref = (w @ v.astype(np.float64)) / (w.sum() + lmax - 4)
+    # a weight of e^22.6 next to 2^27 of 1: scores to 2^-18 of 22.6, sums as in check_attention
+    assert np.abs(got - ref).max() <= (2.0 ** -18 * 22.7 + 2.0 ** -16) * np.abs(v).max()
+    del cache
+    t.cuda.empty_cache()
+
+
+# ---- the cache object --------------------------------------------------------------------------
+def test_planes_stay_and_copies_are_their_own(env):
+    """planes are written, not replaced; a deep copy has its own memory"""
+    import copy
+
+    t = env.torch
+    cache = filled_cache(env, 2, 2, 8, 16, 19)
+    with pytest.raises(AttributeError):
+        cache.k_codes = t.zeros_like(cache.k_codes)
+    other, before = copy.deepcopy(cache), planes_of(cache)
+    x = env.dev(cases.gaussian(20, (1, 6 * 16), 1.0))
+    i = lambda v, dt: t.full((1,), v, dtype=dt, device="cuda")
+    cos, sin = tables(4, 16)
+    env.serving.qknorm_rope_append(x, i(3, t.int32), i(3, t.int64), env.dev(cos), env.dev(sin), other, 2)
+    assert all((a == b).all() for a, b in zip(planes_of(cache), before))
+    assert any((a != b).any() for a, b in zip(planes_of(other), before))
+    view = env.serving.KV4Cache.from_planes(cache.k_codes, cache.k_steps, cache.v_codes, cache.v_steps, 16)
+    env.serving.qknorm_rope_append(x, i(3, t.int32), i(3, t.int64), env.dev(cos), env.dev(sin), view, 2)
+    assert all((a == b).all() for a, b in zip(planes_of(cache), planes_of(other)))
+
+
+def test_append_in_graphs_with_positions_moved_in_place(env):
+    """what a decode step does: one captured append, replayed as the positions and rows advance"""
+    t, heads, kv, hd, lmax = env.torch, 4, 2, 64, 16
+    cos, sin = (env.dev(a) for a in tables(lmax, hd))
+    xs = env.dev(cases.gaussian(21, (6, 3, (heads + 2 * kv) * hd), 1.0))
+    eager, replayed = (env.serving.KV4Cache(3, kv, lmax, hd) for _ in range(2))
+    pos, rows = t.zeros(3, dtype=t.int32, device="cuda"), t.arange(3, device="cuda") * lmax
+    x, q = t.zeros_like(xs[0]), t.zeros((3, heads, hd), device="cuda")
+    g = t.cuda.CUDAGraph()
+    t.cuda.synchronize()
+    with t.cuda.graph(g):
+        env.serving.qknorm_rope_append(x, pos, rows, cos, sin, replayed, heads, q_out=q)
+        pos.add_(1)
+        rows.add_(1)
+    for i in range(6):
+        x.copy_(xs[i])
+        g.replay()
+        ref = env.serving.qknorm_rope_append(xs[i], t.full((3,), i, dtype=t.int32, device="cuda"), t.arange(3, device="cuda") * lmax + i, cos, sin,
+                                             eager, heads)
+        assert (q == ref).all()
+    assert all((a == b).all() for a, b in zip(planes_of(eager), planes_of(replayed)))
+
+
 # ---- sampling ----------------------------------------------------------------------------------
 def check_sample(env, logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     n = len(logits)
@@ -384,6 +504,55 @@ def test_sample_special_rows_and_settings(env):
         assert got[0] == 0 and got[1] == 0 and got[5] == 123 and got[4] != 7 and (got[2] % 2 == 1)
     assert check_sample(env, l, u, temperature=0.0)[7] == 10
     assert set(check_sample(env, l, u)[3:4]) <= {5, 9}
+
+
+def test_sample_logits_further_apart_than_f32_reaches(env):
+    """differences above the largest f32 number under large and infinite temperatures; the smallest numbers under the smallest ones"""
+    n, v = 8, 2000
+    u = ((np.arange(n) + 0.3) / n).astype(f32)
+    far = (np.random.default_rng(5).uniform(-1, 1, (n, v)) * 3.4e38).astype(f32)
+    far[:, 7], far[:, 9] = -np.inf, np.nan
+    for temp in (1e38, 3e38, 3e37, np.inf):
+        for kw in ({}, {"top_k": 5}, {"top_k": 700}, {"top_p": 0.5}, {"top_p": 0.02}, {"min_p": 0.2}, {"top_k": 1000, "top_p": 0.7}):
+            check_sample(env, far, u, temperature=temp, **kw)
+    near = (np.random.default_rng(6).integers(0, 40, (n, v)) * 1e-44).astype(f32)
+    for temp in (1e-45, 1e-40, 1e-38, 1e-31):
+        for kw in ({}, {"top_k": 5}, {"top_p": 0.5}, {"min_p": 0.2}, {"top_k": 1000, "top_p": 0.7}):
+            assert (check_sample(env, near, u, temperature=temp, **kw) < v).all()
+
+
+def test_sample_on_streams_and_in_graphs(env):
+    """two streams at once and captured calls give the eager tokens; settings changed in place take effect at the next replay"""
+    t, n, v = env.torch, 40, 20000
+    logits = env.dev(cases.gaussian(12, (n, v), 2.0))
+    u = t.rand(n, device="cuda")
+    kw = {"temperature": t.full((n,), 0.8, device="cuda"), "top_p": t.full((n,), 0.9, device="cuda"),
+          "top_k": t.full((n,), 300, dtype=t.int32, device="cuda"), "min_p": t.zeros(n, device="cuda")}
+    ref = env.serving.sample(logits, u, **kw)
+    t.cuda.synchronize()
+    streams, graphs, outs, captured = [t.cuda.Stream() for _ in range(2)], [], [], []
+    for s in streams:
+        with t.cuda.stream(s):
+            outs += [env.serving.sample(logits, u, **kw) for _ in range(5)]
+    t.cuda.synchronize()
+    for s in streams:
+        g = t.cuda.CUDAGraph()
+        with t.cuda.graph(g, stream=s):
+            captured.append(env.serving.sample(logits, u, **kw))
+        graphs.append(g)
+
+    def replay():
+        for _ in range(3):
+            for s, g in zip(streams, graphs):
+                with t.cuda.stream(s):
+                    g.replay()
+        t.cuda.synchronize()
+    replay()
+    assert all((o == ref).all() for o in outs + captured)
+    kw["temperature"].zero_()
+    t.cuda.synchronize()
+    replay()
+    assert all((o == logits.argmax(1)).all() for o in captured)
 
 
 def test_sample_strided_rows_and_largest_vocabulary(env):
