@@ -22,6 +22,8 @@
 #include <math.h>
 #include <stdlib.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "device_utils.cuh"
 #include "tc_ptx.cuh"
@@ -227,18 +229,23 @@ struct Row {
         ptx::cluster_sync();
         return told(id, f);
     }
-    // inclusive sum over the threads
-    template <typename T>
-    __device__ __forceinline__ T block_scan(T v) const {
-        static_assert(sizeof(T) == 8, "");
-        T *scratch = reinterpret_cast<T *>(sh.scratch);
-        v = warp_scan(v);
+    // inclusive sums over the threads
+    template <typename... T>
+    __device__ __forceinline__ void block_scan(T &...v) const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        ((v = warp_scan(v)), ...);
         __syncthreads();
-        if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = v;
+        int at = 0;
+        if (lane == 31) ((reinterpret_cast<T *>(at++ ? sh.segment : sh.scratch)[warp] = v), ...);
         __syncthreads();
-        T base = 0;
-        for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) base += scratch[w];
-        return v + base;
+        at = 0;
+        auto add = [&](auto &x) {
+            using V = std::remove_reference_t<decltype(x)>;
+            const V upto = warp_scan(reinterpret_cast<V *>(at++ ? sh.segment : sh.scratch)[lane % SAMPLE_WARPS]);
+            const V base = __shfl_sync(0xffffffffu, upto, warp ? warp - 1 : 0);
+            if (warp) x += base;
+        };
+        (add(v), ...);
     }
     __device__ __forceinline__ void hist_add64(int b, u64 m) const {
         if (b < 0) return;
@@ -267,7 +274,8 @@ struct Row {
     }
     // the bin in which the running sum reaches target, the sum before it and with it
     __device__ __forceinline__ void find_bin(const u64 (&mine)[2], u64 target) const {
-        u64 upto = block_scan(mine[0] + mine[1]);
+        u64 upto = mine[0] + mine[1];
+        block_scan(upto);
 #pragma unroll
         for (int k = 1; k >= 0; --k) {
             if (upto - mine[k] < target && target <= upto) {
@@ -278,11 +286,9 @@ struct Row {
             upto -= mine[k];
         }
     }
-    __device__ __forceinline__ void collect(u64 c, u64 &lo, u64 &hi) const {
+    __device__ __forceinline__ void collect(u64 c) const {
         const uint32_t slot = atomicAdd(&sh.n_own, 1u);
         if (slot < SAMPLE_OWN) sh.own[slot] = c;
-        lo = min(lo, c);
-        hi = max(hi, c);
     }
     // CTAs that collected more than they have room for
     __device__ __forceinline__ bool overflown(int id) const {
@@ -305,13 +311,12 @@ struct Row {
         if (threadIdx.x == 0) sh.n_own = 0;
         __syncthreads();
         const int b1 = sh.bin[1];
-        u64 lo = ~0ull, hi = 0;
         if (b1 < SAMPLE_BINS - 1) {
             const float to = (float)(b1 + 1);
             each4<false>([&](const float (&x)[4], int i) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (bin_at(x[j]) < to && kept(x[j], i + j)) collect(comp_of(x[j], i + j), lo, hi);
+                    if (bin_at(x[j]) < to && kept(x[j], i + j)) collect(comp_of(x[j], i + j));
             });
         }
         __syncthreads();
@@ -374,9 +379,9 @@ struct Row {
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 w[k] = (double)mine[k] * (1.0 / 65535) * (double)exp2f((float)(2 * threadIdx.x + k) * (-1.4426950408889634f * 32 / SAMPLE_BINS));
-            double upto = block_scan(w[0] + w[1]);
-            // shares up to bin[1]: 0.969 to 1 of 65535 for every element
-            u64 shares = block_scan(mine[0] + mine[1]);
+            double upto = w[0] + w[1];
+            u64 shares = mine[0] + mine[1];  // up to bin[1]: 0.969 to 1 of 65535 for every element
+            block_scan(upto, shares);
             if (threadIdx.x == SAMPLE_THREADS - 1) sh.upto = shares;
             __syncthreads();
 #pragma unroll
@@ -405,7 +410,6 @@ struct Row {
         if (!WEIGHT && !list) target -= sh.before;
 
         // ---- the elements of bins b0 .. b1, and the sum of what lies before
-        u64 lo = ~0ull, hi = 0;
         sum = 0;
         const float from = (float)b0, to = (float)(b1 + 1);
         each4<false>([&](const float (&x)[4], int i) {
@@ -415,7 +419,7 @@ struct Row {
                 const float at = bin_at(x[k]);
                 const bool in = at < to && kept(x[k], i + k);
                 above[k] = in && at < from;
-                if (in && at >= from) collect(comp_of(x[k], i + k), lo, hi);
+                if (in && at >= from) collect(comp_of(x[k], i + k));
             }
             if (WEIGHT) sum += weigh(x, above);
         });
@@ -428,9 +432,15 @@ struct Row {
         const bool over = overflown(5);  // then the logits are gone over again, otherwise what was collected
         const uint32_t n_own = min(sh.n_own, (uint32_t)SAMPLE_OWN);
         const u64 *from_list = sh.own;
-        while (count > SAMPLE_CAND) {  // the part of the order that they span, cut into bins of 64-bit sums
-            lo = cluster_reduce(lo, 6, least);
-            hi = ~cluster_reduce(~hi, 7, least);
+        // the part of the order that they span: by the bins' ends, and a little more than their rounding on either side
+        const double wide_bin = 2.0 / (double)bins;
+        u64 lo = comp_of(nextafterf((float)((double)top - (b0 ? b0 * wide_bin * (1.0 - 0x1p-20) : 0.0)), INFINITY) + 0.0f, 0);
+        u64 hi = b1 < SAMPLE_BINS - 1 ? comp_of(nextafterf((float)((double)top - (b1 + 1) * wide_bin * (1.0 + 0x1p-20)), -INFINITY) + 0.0f, -1) : ~0ull;
+        const auto candidate = [&](float x, int i) {
+            const float at = bin_at(x);
+            return at >= from && at < to && kept(x, i);
+        };
+        while (count > SAMPLE_CAND) {  // that part is cut into bins of 64-bit sums
             const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
             hist_clear();
             if (over) {
@@ -438,7 +448,7 @@ struct Row {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const u64 c = comp_of(x[k], i + k);
-                        const bool in = kept(x[k], i + k) && c >= lo && c <= hi;
+                        const bool in = candidate(x[k], i + k) && c >= lo && c <= hi;
                         if (!__any_sync(0xffffffffu, in)) continue;
                         u64 m = !in ? 0ull : (WEIGHT ? weight(x[k]) : 1ull);
                         int b = m ? (int)((c - lo) >> shift) : -1;
@@ -481,7 +491,7 @@ struct Row {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const u64 c = comp_of(x[k], i + k);
-                        const bool in = kept(x[k], i + k);
+                        const bool in = candidate(x[k], i + k);
                         above[k] = in && c >= first && c < lo;
                         if (in && c >= lo && c <= hi) choose(c);
                     }
@@ -491,13 +501,15 @@ struct Row {
                 for (uint32_t i = threadIdx.x; i < n_own; i += SAMPLE_THREADS)
                     if (sh.own[i] >= lo && sh.own[i] <= hi) choose(sh.own[i]);
             }
-            lo = new_lo;
-            hi = new_hi;
             __syncthreads();
             tell(sh.n_chosen, 5);
             ptx::cluster_sync();
             count = told(5, plus);
             from_list = sh.chosen;
+            if (count > SAMPLE_CAND) {
+                lo = cluster_reduce(new_lo, 6, least);
+                hi = ~cluster_reduce(~new_hi, 7, least);
+            }
         }
         fetch_list(from_list, count);
         cut_list<WEIGHT>(kept, (uint32_t)count, target);
@@ -596,6 +608,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     row.l = src;
     row.wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     float top = -INFINITY;
+    int top_at = 0;  // the first quad of this thread that holds its largest
+    const auto rise = [&](float m, int i) {
+        if (m > top) top = m, top_at = i;
+    };
     if (row.held) {
         float *held = reinterpret_cast<float *>(smem + SAMPLE_FIXED);
         row.l = held;
@@ -604,16 +620,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         for (int i = threadIdx.x; i < body; i += SAMPLE_THREADS) {
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(src) + i);
             reinterpret_cast<float4 *>(held)[i] = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
-            top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));  // passes over NaN
+            rise(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), i);  // passes over NaN
         }
 #pragma unroll 4
         for (int i = 4 * body + threadIdx.x; i < 4 * quads; i += SAMPLE_THREADS) {
             const float v = i < row.n ? clean(__ldcg(src + i)) : -INFINITY;
             held[i] = v;
-            top = fmaxf(top, v);
+            rise(v, i / 4);
         }
     } else {
-        row.each4<false>([&](const float (&x)[4], int) { top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))); });
+        row.each4<false>([&](const float (&x)[4], int i) { rise(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), (i - row.i0) / 4); });
     }
     const float mine_top = top, temp = p.temperature ? p.temperature[r] : 1.0f;
     // the smallest of ~ordered bits: one instruction a warp
@@ -624,11 +640,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     top = logit_of((u64)__reduce_min_sync(0xffffffffu, (uint32_t)sh.scratch[lane % SAMPLE_WARPS]) << 32);
     if (!(temp > 0.0f)) {  // the first of the largest: of the slice, then of all
         u64 best = ~0ull;
-        row.each4<false>([&](const float (&x)[4], int i) {
+        if (mine_top + 0.0f == top && row.n > 0) {
+            float x[4];
+            row.load4(top_at, x);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (x[k] == top) best = min(best, comp_of(top, i + k));
-        });
+            for (int k = 3; k >= 0; --k)
+                if (x[k] == top) best = comp_of(top, row.i0 + 4 * top_at + k);
+        }
         best = row.cluster_reduce(best, 0, least);
         row.top = logit_of(best);
         if (row.rank == 0 && threadIdx.x == 0) {
