@@ -732,41 +732,43 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         if (lane == 0) sh.segment[warp] = s;
         __syncthreads();
     }
-    u64 before = 0, mine = 0, z = 0;
-    for (int w = 0; w < SAMPLE_WARPS; ++w) {
-        if (w < warp) before += sh.segment[w];
-        mine += sh.segment[w];
-    }
+    // this CTA's sums up to each of its segments
+    const u64 upto = warp_scan(lane < SAMPLE_WARPS ? sh.segment[lane] : 0ull), mine = __shfl_sync(0xffffffffu, upto, SAMPLE_WARPS - 1);
     row.tell(mine, 2);
     ptx::cluster_sync();  // nothing of another CTA is read from here on
+    u64 before = 0, z = 0;
     for (uint32_t c = 0; c < ctas; ++c) {
         if (c < row.rank) before += sh.slot[2][c];
         z += sh.slot[2][c];
     }
     const u64 draw = drawn(u, z);
-    if (draw < before || draw >= before + sh.segment[warp]) return;  // one warp of the cluster goes on
-    bool done = false;
-    row.each4<true>([&](const float (&x)[4], int i) {
-        bool in[4];
-        kept4(x, i, in);
+    if (draw < before || draw >= before + mine) return;  // one CTA of the cluster goes on, with one of its segments
+    const int seg = __ffs(__ballot_sync(0xffffffffu, draw < before + upto)) - 1;
+    if (seg > 0) before += __shfl_sync(0xffffffffu, upto, seg - 1);
+    const int end = min(quads, (seg + 1) * row.quads_per_warp());
+    for (int i0 = seg * row.quads_per_warp(); i0 < end; i0 += SAMPLE_THREADS) {
+        const int i = i0 + threadIdx.x;
+        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i < end) row.load4(i, x);
         u64 w[4], own = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            w[j] = in[j] ? row.weight(x[j]) : 0ull;
+            w[j] = kept(x[j], row.i0 + 4 * i + j) ? row.weight(x[j]) : 0ull;
             own += w[j];
         }
-        const u64 inc = warp_scan(own), all = __shfl_sync(0xffffffffu, inc, 31);
-        if (!done && draw < before + all) {
-            u64 at = before + inc - own;
+        u64 at = own;
+        row.block_scan(at);
+        if (threadIdx.x == SAMPLE_THREADS - 1) sh.upto = at;
+        at += before - own;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (draw >= at && draw < at + w[j]) chosen(x[j], i + j, z);
-                at += w[j];
-            }
-            done = true;
+        for (int j = 0; j < 4; ++j) {
+            if (draw >= at && draw < at + w[j]) chosen(x[j], row.i0 + 4 * i + j, z);
+            at += w[j];
         }
-        before += all;
-    });
+        __syncthreads();
+        before += sh.upto;
+        if (draw < before) return;
+    }
 }
 
 }  // namespace kb
