@@ -324,8 +324,7 @@ struct Row {
         ptx::cluster_sync();
         const u64 count = told(5, plus);
         if (count == 0 || count > SAMPLE_CAND) return 0;
-        fetch_list(sh.own, count);
-        cut_list<false>(kept, (uint32_t)count, (u64)k);
+        if (take_list(sh.own, count)) cut_list<false>(kept, (uint32_t)count, (u64)k);
         return (int)count;
     }
     // the candidates of all CTAs (their numbers in slot 5) into sh.all, with their weights
@@ -337,6 +336,12 @@ struct Row {
             const u64 e = ld_cluster(from + (i - base), c);
             sh.all[i] = {e, (double)weight(logit_of(e))};
         }
+    }
+    // the list of all that is kept, by the first CTA; the others have nothing left to do
+    __device__ bool take_list(const u64 *from, u64 count) const {
+        if (rank == 0) fetch_list(from, count);
+        ptx::cluster_sync();  // the others' candidates have been read
+        return rank == 0;
     }
     // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
     // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.  Returns the
@@ -511,9 +516,12 @@ struct Row {
                 hi = ~cluster_reduce(~new_hi, 7, least);
             }
         }
+        if (list) {
+            if (take_list(from_list, count)) cut_list<WEIGHT>(kept, (uint32_t)count, target);
+            return (int)count;
+        }
         fetch_list(from_list, count);
         cut_list<WEIGHT>(kept, (uint32_t)count, target);
-        if (list) return (int)count;
         if (WEIGHT) {  // what is kept of this CTA's candidates goes to its segment
             sum = warp_sum(sum);
             if ((threadIdx.x & 31) == 0) sh.segment[threadIdx.x >> 5] = sum;
@@ -676,6 +684,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     if (k > 0 && k < p.vocab) {
         if (k <= SAMPLE_CAND / 2) list = row.cut_few(kept, mine_top, k);
         if (!list) list = row.cut<false>(kept, [&](u64) { return (u64)k; });
+        if (list && row.rank) return;
     }
     const float mp = p.min_p ? p.min_p[r] : 0.0f;
     if (mp > 0.0f && temp < INFINITY) {  // an infinite temperature makes all finite logits equal
@@ -695,6 +704,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
             row.cut_list<true>(kept, list, nucleus(row.keep_list(kept, list)));
         } else {
             list = row.cut<true>(kept, nucleus);
+            if (list && row.rank) return;
             summed = true;
         }
     }
@@ -706,14 +716,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
             p.logprobs[r] = (float)(e - log((double)all * 0x1p-44));
         }
     };
-    if (list) {  // every CTA knows the answer, the first one writes it
+    if (list) {
         const u64 all = row.keep_list(kept, list);
         const double draw = (double)drawn(u, all);
         row.in_order<true>(list, [](u64 c) { return (uint32_t)c; }, [&](uint32_t i, double before) {
             const Candidate e = sh.all[i];
-            if (row.rank == 0 && draw >= before && draw < before + e.weight) chosen(logit_of(e.comp), (int)(uint32_t)e.comp, all);
+            if (draw >= before && draw < before + e.weight) chosen(logit_of(e.comp), (int)(uint32_t)e.comp, all);
         });
-        ptx::cluster_sync();  // the others have read this CTA's candidates
         return;
     }
     // ---- the draw: the warps' sums of kept weights, then the segment that holds the number is walked in index order
