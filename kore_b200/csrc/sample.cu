@@ -416,7 +416,8 @@ struct Row {
 
         // ---- the elements of bins b0 .. b1, and the sum of what lies before
         sum = 0;
-        const float from = (float)b0, to = (float)(b1 + 1);
+        // the last bin's weights are 0 and its shares not counted: no border there, and no place in a list
+        const float from = (float)b0, to = (float)(WEIGHT ? min(b1 + 1, SAMPLE_BINS - 1) : b1 + 1);
         each4<false>([&](const float (&x)[4], int i) {
             bool above[4];
 #pragma unroll

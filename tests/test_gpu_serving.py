@@ -521,6 +521,20 @@ def test_sample_logits_further_apart_than_f32_reaches(env):
             assert (check_sample(env, near, u, temperature=temp, **kw) < v).all()
 
 
+@pytest.mark.parametrize("temp,top", [(0.04, None), (0.02, None), (0.3, None), (0.03, 4.05), (0.02, 4.05), (0.03, 0.1)])
+def test_sample_nuclei_next_to_the_whole(env, temp, top):
+    """top_p so close to 1 that the border may be any of the last weights, among thousands of logits whose weight is 0"""
+    n, v = 8, 60000
+    logits = cases.gaussian(31, (n, v), 1.0)
+    if top is not None:  # the largest just above a power of two, most of the others below it
+        logits += f32(top) - logits.max(1, keepdims=True)
+    u = np.array([0.0, 0.2, 0.5, 0.9, 0.99, 0.999, 0.9999, 0.99999], f32)
+    for top_p in (0.9999, 0.99995, 0.99999, 0.9999999):
+        check_sample(env, logits, u, temperature=temp, top_p=top_p)
+        check_sample(env, logits, u, temperature=temp, top_p=top_p, min_p=1e-12)
+        check_sample(env, logits, u, temperature=temp, top_p=top_p, top_k=30000)
+
+
 def test_sample_on_streams_and_in_graphs(env):
     """two streams at once and captured calls give the eager tokens; settings changed in place take effect at the next replay"""
     t, n, v = env.torch, 40, 20000
