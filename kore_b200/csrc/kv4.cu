@@ -368,7 +368,8 @@ constexpr int ATT4_PER_SM = 4;   // resident CTAs: 128 registers a thread (five 
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
 constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
 constexpr int ATT4_GRAIN = ATT4_WARPS * ATT4_TILE;  // positions that give every warp a tile
-constexpr int ATT4_LEAST = 5;  // grains of a chunk at least: 640 positions of one sequence take 6.5 us whole, 7.0 us in five chunks
+constexpr int ATT4_WHOLE = 5;  // grains of a cache that is not split: 577 positions of 32 KV heads take 6.7 us whole, 7.5 us in five chunks
+constexpr int ATT4_ROUND = 32;  // chunks that the second kernel takes in a round
 constexpr float ATT4_SLACK = 8.0f;  // log2 of how far a weight may rise above the reference
 
 struct AttnParams {
@@ -403,15 +404,22 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
         return true;
     }
     const int len0 = lane < p.batch ? kv4_len(p, lane) : 0;
-    unsigned grains = (len0 + ATT4_GRAIN - 1) / ATT4_GRAIN;
-    for (int b = lane + 32; b < p.batch; b += 32) grains += (kv4_len(p, b) + ATT4_GRAIN - 1) / ATT4_GRAIN;
+    unsigned grains = (len0 + ATT4_GRAIN - 1) / ATT4_GRAIN, longest = grains;
+    for (int b = lane + 32; b < p.batch; b += 32) {
+        const unsigned g = (kv4_len(p, b) + ATT4_GRAIN - 1) / ATT4_GRAIN;
+        grains += g;
+        longest = max(longest, g);
+    }
     const unsigned long long total = (unsigned long long)__reduce_add_sync(0xffffffffu, grains) * units;
     // sum of ceil(g / size) <= total / size + sequences * units, which is at most `slots` for the first size.  Where the
     // units alone take most of the slots the second one is used, and up to a CTA per unit more than the GPU holds
     const unsigned share = p.slots - p.least_ctas > p.slots / 2 ? p.slots - p.least_ctas : p.slots;
     const unsigned even = total >> 31 ? (unsigned)((total + share - 1) / share) : ((unsigned)total + share - 1) / share;
-    // no larger than the cache: many units over a long one would take the products below past 32 bits
-    w.size = min(max((int)even, ATT4_LEAST), (p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
+    // A tile per warp is enough for a chunk (16 sequences of 641 positions and 8 KV heads: 13.1 us, in chunks of five 18.0); more
+    // than a round of them costs more than a second tile does (one sequence of 8000: 12.4 and 11.4 us).  No larger than the
+    // cache: many units over a long one would take the products below past 32 bits
+    const unsigned least = __reduce_max_sync(0xffffffffu, longest) > ATT4_ROUND ? 2 : 1;
+    w.size = min(max(even, least), (unsigned)(p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
     int first = 0;  // running sum of CTAs over the sequences
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
         const int b = b0 + lane, len = b0 == 0 ? len0 : b < p.batch ? kv4_len(p, b) : 0;
@@ -955,7 +963,7 @@ static AttnPlan attn_plan(size_t batch, int t, int n_heads, int n_kv, int hd, in
     a.row_tiles = (int)(((size_t)t * (n_heads / n_kv) + a.tile_rows - 1) / a.tile_rows);
     a.units = batch * n_kv * a.row_tiles;
     a.slots = sms * ATT4_PER_SM;
-    if (lmax <= ATT4_LEAST * ATT4_GRAIN || a.units > (size_t)16 * a.slots) a.slots = 0;
+    if (lmax <= ATT4_WHOLE * ATT4_GRAIN || a.units > (size_t)16 * a.slots) a.slots = 0;
     a.ctas = a.slots == 0 ? a.units : a.units * 2 < (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;  // see find_attn_work
     if (a.slots) {
         auto up = [](size_t v) { return (v + 255) / 256 * 256; };
