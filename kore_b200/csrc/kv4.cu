@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 // costs two votes and most tiles nothing else.
 //   A warp streams its own 32-position tiles through a ring of 16-byte asynchronous copies (no barrier between warps) and
 // the warps of a CTA deal the tiles of a chunk.  A CTA costs about three tiles of a warp before and behind its loop, so long
-// caches are cut into as few chunks as fill the GPU once, of one size for all sequences: the CTAs work that out from the
+// caches are cut into as many chunks as fill the GPU once, of one size for all sequences: the CTAs work that out from the
 // lengths, and a second kernel joins the chunks.
 constexpr int ATT4_WARPS = 4;
 constexpr int ATT4_STAGES = 2;   // with 16 warps on an SM a second tile in flight each is enough
@@ -368,7 +368,12 @@ constexpr int ATT4_PER_SM = 4;   // resident CTAs: 128 registers a thread (five 
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
 constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
 constexpr int ATT4_GRAIN = ATT4_WARPS * ATT4_TILE;  // positions that give every warp a tile
-constexpr int ATT4_WHOLE = 5;  // grains of a cache that is not split: 577 positions of 32 KV heads take 6.7 us whole, 7.5 us in five chunks
+// A cache of so many grains is not split: 577 positions of one sequence and 32 KV heads take 6.8 us whole, 7.5 us in five chunks;
+// from ATT4_MANY units on two grains more (4 sequences of 760 positions, 8 KV heads, five tokens: 12.1 us whole, 15.1 split)
+constexpr int ATT4_WHOLE = 5, ATT4_MANY = 32;
+// nor, among that many units, is the longest sequence that has so many grains more than an even share: 16 sequences of 1020
+// positions and 32 KV heads, 8 grains of 7, take 23.6 us and 32.1 us with a second chunk of one grain
+constexpr int ATT4_EXTRA = 4;
 constexpr int ATT4_ROUND = 32;  // chunks that the second kernel takes in a round
 constexpr float ATT4_SLACK = 8.0f;  // log2 of how far a weight may rise above the reference
 
@@ -418,8 +423,9 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
     // A tile per warp is enough for a chunk (16 sequences of 641 positions and 8 KV heads: 13.1 us, in chunks of five 18.0); more
     // than a round of them costs more than a second tile does (one sequence of 8000: 12.4 and 11.4 us).  No larger than the
     // cache: many units over a long one would take the products below past 32 bits
-    const unsigned least = __reduce_max_sync(0xffffffffu, longest) > ATT4_ROUND ? 2 : 1;
-    w.size = min(max(even, least), (unsigned)(p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const unsigned least = longest <= even + ATT4_EXTRA && p.batch * units >= ATT4_MANY ? longest : longest > ATT4_ROUND ? 2 : 1;
+    w.size = min(max(max(even, least), 1u), (unsigned)(p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
     int first = 0;  // running sum of CTAs over the sequences
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
         const int b = b0 + lane, len = b0 == 0 ? len0 : b < p.batch ? kv4_len(p, b) : 0;
@@ -963,7 +969,7 @@ static AttnPlan attn_plan(size_t batch, int t, int n_heads, int n_kv, int hd, in
     a.row_tiles = (int)(((size_t)t * (n_heads / n_kv) + a.tile_rows - 1) / a.tile_rows);
     a.units = batch * n_kv * a.row_tiles;
     a.slots = sms * ATT4_PER_SM;
-    if (lmax <= ATT4_WHOLE * ATT4_GRAIN || a.units > (size_t)16 * a.slots) a.slots = 0;
+    if (lmax <= (a.units < ATT4_MANY ? ATT4_WHOLE : ATT4_WHOLE + 2) * ATT4_GRAIN || a.units > (size_t)16 * a.slots) a.slots = 0;
     a.ctas = a.slots == 0 ? a.units : a.units * 2 < (size_t)a.slots ? (size_t)a.slots : a.units + a.slots;  // see find_attn_work
     if (a.slots) {
         auto up = [](size_t v) { return (v + 255) / 256 * 256; };
