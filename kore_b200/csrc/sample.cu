@@ -5,9 +5,11 @@
 // Weights are integers of 2^-44 (the largest is 2^44, 2^19 of them fit 63 bits): their sums do not depend on the order in
 // which atomics arrive, and a token's border moves by at most vocab 2^-45 of the largest weight.
 //
-// Bound by the latency of the passes for a few rows and by the f64 exponentials for many (13 f64 operations each).  A row
-// belongs to a cluster of 1 to 8 CTAs; each has a slice of the row, in shared memory where it fits, otherwise in L2.  Top-k and top-p look for the element at which a running measure (count, or weight)
-// reaches a target:
+// Bound by the latency of the passes and of the exchanges between CTAs (one row of 32000: 6.6 us without filters, 9.7 with
+// top-k, 16 with top-p), for many rows by how many clusters fit next to the f64 exponentials (13 f64 operations each): 128 rows
+// of 131072 with unlike settings take 76 us, the logits alone 10 us.  A row belongs to a cluster of 1 to 8 CTAs; each has a
+// slice of the row, in shared memory where it fits, otherwise in L2.  Top-k and top-p look for the element at which a running
+// measure (count, or weight) reaches a target:
 //   1. a histogram over 1024 steps of 1/32 in the exponent.  Counts are exact.  Of a weight only its share of its bin's
 //      largest, in 16 bits, goes through an atomic (the sum of a bin is good to 2^-15), while threads add up the exact
 //      total: the bins that may hold the border are then known, one or two of them;
@@ -16,8 +18,8 @@
 //      bins of exact 64-bit sums; where a CTA has more than SAMPLE_OWN of them (ties) by going over its logits again;
 //   3. every CTA finds the element among the candidates by counting.
 // Where all that is kept down to there is a short list (top-k, most nuclei), the whole of it is collected in step 2 and the
-// rest, the draw included, happens on the list without another exchange.  Otherwise step 2 has the sums of the kept weights
-// by segment already, and the draw walks the segment that holds the number.
+// first CTA does the rest, the draw included, on the list; the others are done.  Otherwise step 2 has the sums of the kept
+// weights by segment already, and the CTA that holds the number walks the segment that does.
 #include <float.h>
 #include <math.h>
 #include <stdlib.h>
@@ -797,8 +799,8 @@ extern "C" int kb_sample(const float *logits, size_t n, size_t vocab, size_t ld,
     int dev = 0;
     KB_CUDA(cudaGetDevice(&dev));
     // CTAs per row: slices of at least 1024 logits, and as many CTAs as there are: a batch of unlike rows (greedy ones next to
-    // flat nuclei) fills the SMs better in many short CTAs than in one round of long ones (128 mixed rows of 131072: 115 us with
-    // eight, 140 with four, 190 with two)
+    // flat nuclei) fills the SMs better in many short CTAs than in one round of long ones (128 mixed rows of 131072: 76 us with
+    // eight, 86 with four, 108 with two)
     const size_t sms = (size_t)sm_count(dev);
     int ctas = 1;
     while (ctas < SAMPLE_CTAS && vocab > (size_t)1024 * ctas) ctas *= 2;
