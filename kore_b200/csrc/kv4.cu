@@ -343,13 +343,13 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 
 // ---- attention ---------------------------------------------------------------------------------
 // Bound by the bytes of the cache as long as the unpacking keeps up (8 sequences of 8191 .. 32768 positions, 8 KV heads of 128:
-// 49.6 us, 3.6 TB/s; 16 sequences of 513 .. 640, 32 of 100: 14.1 us, of which five tiles a warp are 6.5): at the copy bandwidth an SM receives a position (K
-// and V, 136 bytes for heads of 128) every 6 clocks, too few for a multiply-add per value on the FP32 lanes.  So both
-// products run on the matrix instruction m16n8k16 with f16 operands and f32 sums, and a 4-bit code becomes an operand by
-// masking alone: the bits 0x00f0 of a 16-bit lane ARE the f16 number code * 2^-20 (subnormal, exact, taken as such by the
-// instruction).  The factor goes into the end of the sums.  The bits 0x000f would do as well (code * 2^-24, two shifts fewer
-// per eight codes), but the instruction aligns its products by the operands' exponent fields, so leading zeros cost
-// bits of the sum: results were 1e-5 off that way.
+// 49.6 us, 3.6 TB/s; 16 sequences of 513 .. 640, 32 KV heads of 100: 14.1 us, 6.5 of them in the five tiles of a warp): at the
+// copy bandwidth an SM receives a position (K and V, 136 bytes for heads of 128) every 6 clocks, too few for a multiply-add per
+// value on the FP32 lanes.  So both products run on the matrix instruction m16n8k16 with f16 operands and f32 sums, and a 4-bit
+// code becomes an operand by masking alone: the bits 0x00f0 of a 16-bit lane ARE the f16 number code * 2^-20 (subnormal, exact,
+// taken as such by the instruction).  The factor goes into the end of the sums.  The bits 0x000f would do as well (code *
+// 2^-24, two shifts fewer per eight codes), but the instruction aligns its products by the operands' exponent fields, so
+// leading zeros cost bits of the sum: results were 1e-5 off that way.
 //   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo, 22
 // bits of x, for which rows are scaled by powers of two.
 //   Codes are the 16-row operand, queries and weights the 8-column one (S^T = K Q^T, O^T = V^T P^T): the two terms of four

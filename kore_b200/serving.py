@@ -7,7 +7,7 @@
 The reference's decoder loop has an f32 cache, one KV head per query head and a greedy head
 (``crates/kore-edge/src/runtime.rs:106-294``).  All arithmetic runs in the CUDA library (``include/kore_b200.h`` states
 it down to the roundings); this file checks shapes and moves pointers.  Activations and logits are float32, as
-everywhere in this package.
+everywhere in this package.  Results carry no gradient.
 """
 from __future__ import annotations
 
