@@ -1,4 +1,4 @@
-"""Ahead-of-time build of libkore_b200.so with nvcc for sm_100a (in-tree, no JIT cache)."""
+"""Ahead-of-time build (in-tree, no JIT cache): libkore_b200.so with nvcc for sm_100a, and the Python module of the serving calls."""
 from __future__ import annotations
 
 import os
@@ -11,6 +11,9 @@ LIB_DIR = os.path.join(_PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libkore_b200.so")
 SOURCES = ["api.cu", "quant.cu", "gemv.cu", "gemv_group.cu", "gemv_mma.cu", "gemv_stream.cu", "gemm_tc.cu", "gemm_tcs.cu", "gemm_tc2.cu", "static_scratch.cu", "shard.cu", "decoder_ops.cu", "decode_step.cu", "kv4.cu", "sample.cu"]
 HEADERS = ["common.cuh", "device_utils.cuh", "tc_ptx.cuh", os.path.join("..", "..", "include", "kore_b200.h")]
+
+MODULE_PATH = os.path.join(LIB_DIR, "kore_b200_serving.so")  # a Python module against torch's C++ headers; loads without a GPU
+MODULE_SOURCE = "serving_py.cpp"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -52,7 +55,31 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+def build_module(force: bool = False) -> str:
+    """Compile the Python module of kore_b200.serving; returns its path."""
+    import sysconfig
+
+    import torch
+
+    deps = [os.path.join(CSRC, MODULE_SOURCE), os.path.join(CSRC, HEADERS[-1])]
+    if not force and os.path.exists(MODULE_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(MODULE_PATH) for d in deps):
+        return MODULE_PATH
+    os.makedirs(LIB_DIR, exist_ok=True)
+    base = os.path.dirname(torch.__file__)
+    includes = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+                os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"), sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for path in includes:
+        cmd += ["-isystem", path]
+    cmd += ["-o", MODULE_PATH, deps[0], "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
+    return MODULE_PATH
+
+
 if __name__ == "__main__":
     import sys
 
     print(build(force=True, verbose="-v" in sys.argv))
+    print(build_module(force=True))

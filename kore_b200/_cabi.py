@@ -139,6 +139,11 @@ def lib() -> C.CDLL:
     return _lib
 
 
+def address(fn) -> int:
+    """Address of one of the library's functions, for native callers."""
+    return C.cast(fn, C.c_void_p).value
+
+
 def check(rc: int) -> None:
     if rc != OK:
         raise KoreError(rc, lib().kb_last_error().decode("utf-8", "replace"))

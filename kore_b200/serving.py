@@ -6,17 +6,42 @@
 
 The reference's decoder loop has an f32 cache, one KV head per query head and a greedy head
 (``crates/kore-edge/src/runtime.rs:106-294``).  All arithmetic runs in the CUDA library (``include/kore_b200.h`` states
-it down to the roundings); this file checks shapes and moves pointers.  Activations and logits are float32, as
+it down to the roundings); this file checks shapes and moves pointers.  Calls whose arguments need nothing else go through a
+small native module (``csrc/serving_py.cpp``: checks, results and launch in 5 us); it declines every other one, and what
+follows here copies strided operands, changes the device or says what is wrong.  Activations and logits are float32, as
 everywhere in this package.  Results carry no gradient.
 """
 from __future__ import annotations
 
+import importlib.machinery
+import importlib.util
+import os
+
 import torch
 
-from . import _cabi
+from . import _build, _cabi
 from ._cabi import KoreError
 
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+
+
+_native = None
+
+
+def native():
+    """The module of the calls (raises if it has not been built)."""
+    global _native
+    if _native is None:
+        lib, name, path = _cabi.lib(), "kore_b200_serving", _build.MODULE_PATH
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: the module has not been built (run `python -m kore_b200._build`)")
+        loader = importlib.machinery.ExtensionFileLoader(name, path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location(name, path, loader=loader))
+        loader.exec_module(module)
+        module.setup(*(_cabi.address(f) for f in (lib.kb_qknorm_rope_kv, lib.kb_qknorm_rope_kv4, lib.kb_kv4_read, lib.kb_attn_kv4,
+                                                   lib.kb_attn_kv4_workspace_bytes, lib.kb_sample)))
+        _native = module
+    return _native
 
 
 def _refuse(t, name, dtype, shape, dev):
@@ -124,6 +149,9 @@ class KV4Cache:
     def read(self, cache_rows, k_out=None, v_out=None):
         """The f32 values of cache rows (int64 [n], row = sequence * max_len + position; zeros for a row outside the
         cache): K and V, each [n, n_kv_heads, head_dim]."""
+        done = (_native or native()).read(self._held, self.head_dim, cache_rows, k_out, v_out)
+        if done is not None:
+            return done
         dev = self._dev
         _rows(cache_rows, "cache_rows", _I64, "[n]", 1, dev)
         n = cache_rows.shape[0]
@@ -146,6 +174,10 @@ def qknorm_rope_append(qkv, positions, cache_rows, cos, sin, cache, n_heads: int
     ``cache`` is a KV4Cache or a pair (k, v) of float32 caches [n_seqs, n_kv_heads, max_len, head_dim].  Returns the
     queries, float32 [n, n_heads, head_dim].  Two tokens of one call must not name the same cache row."""
     four = isinstance(cache, KV4Cache)
+    done = (_native or native()).append(qkv, positions, cache_rows, cos, sin, cache._held if four else cache, cache.head_dim if four else 0,
+                                        n_heads, q_gamma, k_gamma, eps, q_out)
+    if done is not None:
+        return done
     if four:
         n_seqs, n_kv, lmax, hd, dev = cache.n_seqs, cache.n_kv_heads, cache.max_len, cache.head_dim, cache._dev
         planes, fn = cache._planes(), _cabi.lib().kb_qknorm_rope_kv4
@@ -184,6 +216,9 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     (or [n_seqs, n_heads, head_dim], t = 1), lens int32 [n_seqs] the cache positions up to and including the last of the t
     tokens.  Token i sees the positions below lens - (t - 1 - i); one that sees none gives zeros.  scale 0 is
     1 / sqrt(head_dim).  Returns float32 of q's shape."""
+    done = (_native or native()).attend(cache._held, cache.head_dim, q, lens, scale, out)
+    if done is not None:
+        return done
     hd, dev, n = cache.head_dim, cache._dev, cache.n_seqs
     _rows(q, "q", _F32, f"[{n}, (t,) n_heads, {hd}]", 3 if isinstance(q, torch.Tensor) and q.dim() == 3 else 4, dev)
     shape = q.shape
@@ -215,6 +250,9 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, r
     float32 [n], top_k int32 [n].  A temperature of 0 is greedy.  Top-k and min-p act on the tempered distribution, top-p
     on what they keep.  Returns int64 [n], with return_logprobs also float32 [n]: the log of the token's share of what was
     kept."""
+    done = (_native or native()).sample(logits, u, temperature, top_k, top_p, min_p, return_logprobs, tokens)
+    if done is not None:
+        return done
     dev = _rows(logits, "logits", _F32, "[n, vocab]", 2)
     n, vocab = shape = logits.shape
     if not logits.is_contiguous() and (logits.stride(1) != 1 or (n > 1 and logits.stride(0) < vocab)):

@@ -616,6 +616,68 @@ def test_python_refusals(env):
             call()
 
 
+def test_native_calls_and_what_they_decline(env):
+    """plain arguments are answered by the native module, with the results of the way around it; others are declined, whatever they are"""
+    t, s = env.torch, env.serving
+    nat, f, i32 = s.native(), t.float32, t.int32
+    cache = filled_cache(env, 2, 2, 12, 16, 40)
+    z = lambda *shape, dt=f: t.zeros(shape, dtype=dt, device="cuda")
+    q, lens = env.dev(cases.gaussian(41, (2, 3, 4, 16), 1.0)), env.dev(np.array([12, 5], np.int32))
+    held = cache._held
+    around = s.attend(t.cat([q, q], -1)[..., :16], cache, lens, scale=1)  # strided, an integer scale
+    out = z(2, 3, 4, 16)
+    got = nat.attend(held, 16, q, lens, 1.0, out)
+    assert got is out and (out == around).all() and (nat.attend(held, 16, q, lens, 1.0, None) == around).all()
+    rows = t.arange(24, device="cuda")
+    k, v = nat.read(held, 16, rows, None, None)
+    k2, v2 = z(24, 2, 16), z(24, 2, 16)
+    assert nat.read(held, 16, rows, k2, v2)[1] is v2 and (k == k2).all() and (v == v2).all()
+    logits, u = env.dev(cases.gaussian(42, (5, 90), 2.0)), t.rand(5, device="cuda")
+    kw = dict(temperature=z(5) + 0.5, top_k=z(5, dt=i32) + 9, top_p=z(5) + 0.9, min_p=z(5) + 0.01)
+    a = nat.sample(logits, u, *kw.values(), True, None)
+    b = s.sample(t.nn.functional.pad(logits, (0, 7))[:, :90].t().contiguous().t(), u, return_logprobs=True, **kw)
+    assert (a[0] == b[0]).all() and (a[1] == b[1]).all() and nat.sample(logits[:, 3:50], u, None, None, None, None, False, None) is not None
+    x, pos, at = env.dev(cases.gaussian(43, (3, 8 * 16), 1.0)), z(3, dt=i32), t.arange(3, device="cuda")
+    cos, sin = (env.dev(c) for c in tables(4, 16))
+    pair = (z(2, 2, 12, 16), z(2, 2, 12, 16))
+    for caches, hd in ((filled_cache(env, 2, 2, 12, 16, 44)._held, 16), (pair, 0)):
+        good = [x, pos, at, cos, sin, caches, hd, 4, z(16) + 1, None, 1e-5, None]
+        assert nat.append(*good).shape == (3, 4, 16)
+        # arguments changed one at a time: types, shapes, orders, devices, kinds
+        for i, bads in ((0, [x.double(), x[:, 1:], x.cpu(), x[0], None, x.t().contiguous().t()]), (1, [pos.long(), pos[:2], pos.cpu(), 7]),
+                        (2, [at.int(), at[None], None]), (3, [cos[:, :3], cos.half(), cos.cpu(), z(0, 8)]), (4, [sin[:2], sin.t()]),
+                        (5, [list(caches), caches[:1], (1, 2), None]), (7, [3, 4.0, -1, 1 << 70, "4"]), (8, [z(15), z(16, dt=t.float16)]),
+                        (10, [1, None, -1.0]), (11, [z(3, 4, 15), x])):
+            for bad in bads:
+                assert nat.append(*good[:i], bad, *good[i + 1:]) is None, (i, bad)
+        assert nat.append(*good[:-1]) is None and nat.append() is None
+    assert nat.attend(held, 16, q[:1], lens, 1.0, None) is None and nat.attend(held, 16, q, lens.long(), 1.0, None) is None
+    assert nat.attend(held, 16, q[:, :, :3].contiguous(), lens, 1.0, None) is None and nat.attend(held, 16, q, lens, float("nan"), None) is None
+    assert nat.attend(held, 16, q[:, :0], lens, 1.0, None) is None and nat.attend(held[:3], 16, q, lens, 1.0, None) is None
+    assert nat.read(held, 16, rows.int(), None, None) is None and nat.read(held, 16, rows, z(24, 2, 15), None) is None and nat.read(held, 16, rows[:0], None, None) is None
+    assert nat.sample(logits, u[:4], None, None, None, None, False, None) is None and nat.sample(logits, u, None, z(5), None, None, False, None) is None
+    assert nat.sample(logits, u, None, None, None, None, 0, None) is None and nat.sample(z(5, 0), u, None, None, None, None, False, None) is None
+    # on another stream, and from several threads at once
+    side = t.cuda.Stream()
+    side.wait_stream(t.cuda.current_stream())
+    with t.cuda.stream(side):
+        assert (s.attend(q, cache, lens, scale=1.0) == around).all()
+    import threading
+
+    results = []
+
+    def work():
+        with t.cuda.stream(t.cuda.Stream()):
+            r = [s.attend(q, cache, lens, scale=1.0) for _ in range(50)]
+            t.cuda.current_stream().synchronize()
+            results.append(all((y == around).all() for y in r))
+    t.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    [th.start() for th in threads]
+    [th.join() for th in threads]
+    assert results == [True] * 4
+
+
 # ---- together: the decoder ------------------------------------------------------------------------
 class Ref4(dr.DecoderRef):
     """the decoder's restatement with grouped heads, norms of queries and keys, and keys and values as the 4-bit cache stores them"""

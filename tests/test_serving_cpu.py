@@ -135,11 +135,33 @@ def test_row_words(lib):
     assert [int(lib.kb_kv4_row_words(h)) for h in (-1, 0, 4, 8, 100, 128)] == [0, 0, 1, 1, 13, 16]
 
 
+def test_native_module_declines_without_a_gpu():
+    """host tensors, wrong kinds and wrong numbers of arguments are left to the Python layer, nothing is touched"""
+    import torch
+
+    from kore_b200 import _build, serving
+
+    _build.build_module()
+    nat = serving.native()
+    z = torch.zeros
+    i32, i64 = torch.int32, torch.int64
+    held = tuple(z(s, dtype=i32) for s in ((1, 1, 4, 2), (1, 1, 4), (1, 1, 4, 2), (1, 1, 4)))
+    assert nat.sample(z(2, 5), z(2), None, None, None, None, False, None) is None
+    assert nat.sample(None, None, None, None, None, None, None, None) is None and nat.sample() is None
+    assert nat.read(held, 16, z(3, dtype=i64), None, None) is None and nat.read(1, 16, z(3, dtype=i64), None, None) is None
+    assert nat.attend(held, 16, z(1, 2, 16), z(1, dtype=i32), 0.0, None) is None
+    for caches in (held, (z(1, 1, 4, 16), z(1, 1, 4, 16)), (1, 2), "ab"):
+        assert nat.append(z(1, 64), z(1, dtype=i32), z(1, dtype=i64), z(4, 8), z(4, 8), caches, 16, 2, None, None, 1e-5, None) is None
+    with pytest.raises(TypeError):
+        nat.setup(1, 2)
+
+
 def test_python_layer_refuses_host_tensors():
     import torch
 
-    from kore_b200 import KoreError, serving
+    from kore_b200 import KoreError, _build, serving
 
+    _build.build_module()
     with pytest.raises(KoreError) as e:
         serving.sample(torch.zeros(2, 5), torch.zeros(2))
     assert "logits" in e.value.message
