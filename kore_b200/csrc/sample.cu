@@ -5,7 +5,7 @@
 // Weights are integers of 2^-44 (the largest is 2^44, 2^19 of them fit 63 bits): their sums do not depend on the order in
 // which atomics arrive, and a token's border moves by at most vocab 2^-45 of the largest weight.
 //
-// Bound by the latency of the passes and of the exchanges between CTAs (one row of 32000: 6.6 us without filters, 9.7 with
+// Bound by the latency of the passes and of the exchanges between CTAs (one row of 32000: 6.6 us without filters, 9.2 with
 // top-k, 16 with top-p), for many rows by how many clusters fit next to the f64 exponentials (13 f64 operations each): 128 rows
 // of 131072 with unlike settings take 76 us, the logits alone 10 us.  A row belongs to a cluster of 1 to 8 CTAs; each has a
 // slice of the row, in shared memory where it fits, otherwise in L2.  Top-k and top-p look for the element at which a running
@@ -38,7 +38,7 @@ constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int SAMPLE_BINS = 1024;
 constexpr int SAMPLE_OWN = 1024;  // elements that a CTA collects
-constexpr int SAMPLE_CAND = 256;  // counting what lies before each of c elements takes c^2 / 512 steps of a thread
+constexpr int SAMPLE_CAND = 256;  // of a list: counting what lies before each of c elements takes c^2 / 512 steps of a thread
 constexpr int SAMPLE_CTAS = 8;    // of a cluster, at most
 constexpr size_t SAMPLE_MAX_VOCAB = (size_t)1 << 19;
 
@@ -54,18 +54,14 @@ struct SampleParams {
     float *logprobs;
 };
 
-struct __align__(16) Candidate {
-    u64 comp;
-    double weight;  // a whole number; the sum of SAMPLE_CAND of them has 52 bits
-};
-
 struct SampleShared {
     u64 slot[8][SAMPLE_CTAS];  // one row per exchange between the CTAs
     u64 scratch[SAMPLE_WARPS], segment[SAMPLE_WARPS];
     double scale[32];               // see exp2_fixed
     uint32_t hist[2][SAMPLE_BINS];  // counts or shares; 64-bit sums take both (64-bit shared atomics are compare-and-swap loops)
     u64 own[SAMPLE_OWN], chosen[SAMPLE_CAND];  // collected by this CTA, and what is left of them in a part of the order
-    Candidate all[SAMPLE_CAND];                // of the whole row
+    __align__(16) u64 comp[SAMPLE_CAND];       // of the whole row, in order after sort_list
+    u64 weight[SAMPLE_CAND];
     uint32_t n_own, n_chosen;
     int bin[2];
     u64 before, upto, found;
@@ -329,14 +325,15 @@ struct Row {
         if (take_list(sh.own, count)) cut_list<false>(kept, (uint32_t)count, (u64)k);
         return (int)count;
     }
-    // the candidates of all CTAs (their numbers in slot 5) into sh.all, with their weights
+    // the candidates of all CTAs (their numbers in slot 5) into the list, with their weights
     __device__ void fetch_list(const u64 *from, u64 count) const {
         uint32_t c = 0;
         u64 base = 0;
         for (u64 i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
             while (i >= base + sh.slot[5][c]) base += sh.slot[5][c++];
             const u64 e = ld_cluster(from + (i - base), c);
-            sh.all[i] = {e, (double)weight(logit_of(e))};
+            sh.comp[i] = e;
+            sh.weight[i] = weight(logit_of(e));
         }
     }
     // the list of all that is kept, by the first CTA; the others have nothing left to do
@@ -347,7 +344,7 @@ struct Row {
     }
     // Cuts `kept` behind the element at which the measure of the kept elements, added up in order, reaches target(measure of
     // all); WEIGHT: measure = weight, otherwise 1.  Where only elements of weight 0 are at stake, nothing is cut.  Returns the
-    // length of the list in sh.all that holds all that is kept, or 0 where there is none; WEIGHT without a list: sh.segment
+    // length of the list that holds all that is kept, or 0 where there is none; WEIGHT without a list: sh.segment
     // has the warps' sums of the kept weights.
     template <bool WEIGHT, typename T>
     __device__ int cut(Kept &kept, T target_of) const {
@@ -544,46 +541,59 @@ struct Row {
     }
     __device__ __forceinline__ int quads_per_warp() const { return max(1, ((n + 3) / 4 + SAMPLE_WARPS - 1) / SAMPLE_WARPS); }
 
-    // Calls f(i, measure before it) for the elements of the list in sh.all, in the order that key(comp) gives; several threads
-    // add up what lies before an element, and the first of them calls.
-    template <bool WEIGHT, typename K, typename F>
-    __device__ __forceinline__ void in_order(uint32_t count, K key, F f) const {
+    // The first `count` elements of the list by key into the scratch space, comp and weight: an element's place is the number of
+    // smaller keys, which several threads count (c^2 / 512 steps of 2 keys: 1 us for 256 elements).  The histograms' space is free
+    // while there is a list.
+    __device__ __forceinline__ u64 *scratch_list() const { return reinterpret_cast<u64 *>(sh.hist); }
+    template <typename K>
+    __device__ __forceinline__ void place(uint32_t count, K key) const {
+        static_assert(sizeof(sh.hist) >= 2 * SAMPLE_CAND * sizeof(u64) && SAMPLE_CAND <= SAMPLE_THREADS, "");
         uint32_t per = 1;  // threads per element
         while (per < 32 && 2 * per * count <= SAMPLE_THREADS) per *= 2;
         __syncthreads();
-        for (uint32_t start = 0; start < count; start += SAMPLE_THREADS / per) {
-            const uint32_t i = start + threadIdx.x / per;
-            const auto c = i < count ? key(sh.all[i].comp) : key(0);
-            double before = 0.0;  // whole numbers of at most 52 bits
+        const uint32_t i = threadIdx.x / per;
+        const u64 e = sh.comp[min(i, count - 1)];
+        const auto c = key(e);
+        uint32_t before = 0;
 #pragma unroll 4
-            for (uint32_t j = threadIdx.x % per; j < count; j += per) {
-                const Candidate e = sh.all[j];
-                if (key(e.comp) < c) before += WEIGHT ? e.weight : 1.0;
-            }
-            for (uint32_t o = per / 2; o > 0; o /= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
-            if (i < count && threadIdx.x % per == 0) f(i, before);
+        for (uint32_t j = 2 * (threadIdx.x % per); j < count; j += 2 * per) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(sh.comp + j);
+            before += (key(two.x) < c ? 1 : 0) + (j + 1 < count && key(two.y) < c ? 1 : 0);
+        }
+        for (uint32_t o = per / 2; o > 0; o /= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
+        if (i < count && threadIdx.x % per == 0) {
+            scratch_list()[before] = e;
+            scratch_list()[SAMPLE_CAND + before] = sh.weight[i];
         }
         __syncthreads();
     }
-    // cuts behind the element of the list at which the measure reaches target
-    template <bool WEIGHT>
-    __device__ void cut_list(Kept &kept, uint32_t count, u64 target) const {
-        const double at = (double)target;
-        in_order<WEIGHT>(count, [](u64 c) { return c; }, [&](uint32_t i, double before) {
-            if (before < at && at <= before + (WEIGHT ? sh.all[i].weight : 1.0)) sh.found = sh.all[i].comp;
-        });
+    // cuts behind the element of the list, one a thread, at which the running sum of v reaches target(sum of all)
+    template <typename T>
+    __device__ __forceinline__ void cut_at(Kept &kept, u64 v, T target_of) const {
+        u64 upto = v;
+        block_scan(upto);
+        if (threadIdx.x == SAMPLE_THREADS - 1) sh.upto = upto;
+        __syncthreads();
+        const u64 target = target_of(sh.upto);
+        if (upto - v < target && target <= upto) sh.found = sh.comp[threadIdx.x];
+        __syncthreads();
         kept.cut(sh.found);
     }
-    // weight 0 for what is not kept any more; returns the sum of the others
-    __device__ u64 keep_list(const Kept &kept, uint32_t count) const {
-        u64 sum = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < count; i += SAMPLE_THREADS) {
-            const u64 c = sh.all[i].comp;
-            if (!kept(logit_of(c), (int)(uint32_t)c)) sh.all[i].weight = 0.0;
-            sum += (u64)sh.all[i].weight;
+    // puts the list in order and cuts behind the element at which the measure reaches target
+    template <bool WEIGHT>
+    __device__ void cut_list(Kept &kept, uint32_t count, u64 target) const {
+        place(count, [](u64 c) { return c; });
+        if (threadIdx.x < count) {
+            sh.comp[threadIdx.x] = scratch_list()[threadIdx.x];
+            sh.weight[threadIdx.x] = scratch_list()[SAMPLE_CAND + threadIdx.x];
         }
-        return block_reduce(sum, plus);
+        __syncthreads();
+        if (WEIGHT) cut_at(kept, threadIdx.x < count ? sh.weight[threadIdx.x] : 0ull, [&](u64) { return target; });
+        else kept.cut(sh.comp[min(target, (u64)count) - 1]);
+    }
+    __device__ __forceinline__ bool keeps(const Kept &kept, uint32_t count) const {  // this thread's element of the list
+        const u64 c = sh.comp[threadIdx.x % SAMPLE_CAND];
+        return threadIdx.x < count && kept(logit_of(c), (int)(uint32_t)c);
     }
 };
 
@@ -704,7 +714,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
     bool summed = false;
     if (tp < 1.0f) {
         if (list) {
-            row.cut_list<true>(kept, list, nucleus(row.keep_list(kept, list)));
+            row.cut_at(kept, row.keeps(kept, list) ? sh.weight[threadIdx.x] : 0ull, nucleus);
         } else {
             list = row.cut<true>(kept, nucleus);
             if (list && row.rank) return;
@@ -719,13 +729,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
             p.logprobs[r] = (float)(e - log((double)all * 0x1p-44));
         }
     };
-    if (list) {
-        const u64 all = row.keep_list(kept, list);
-        const double draw = (double)drawn(u, all);
-        row.in_order<true>(list, [](u64 c) { return (uint32_t)c; }, [&](uint32_t i, double before) {
-            const Candidate e = sh.all[i];
-            if (draw >= before && draw < before + e.weight) chosen(logit_of(e.comp), (int)(uint32_t)e.comp, all);
-        });
+    if (list) {  // in order: the kept ones are its first
+        const uint32_t many = __syncthreads_count(row.keeps(kept, list));
+        row.place(many, [](u64 c) { return (uint32_t)c; });
+        const u64 w = threadIdx.x < many ? row.scratch_list()[SAMPLE_CAND + threadIdx.x] : 0ull;
+        u64 upto = w;
+        row.block_scan(upto);
+        if (threadIdx.x == SAMPLE_THREADS - 1) sh.upto = upto;
+        __syncthreads();
+        const u64 all = sh.upto, draw = drawn(u, all);
+        if (draw >= upto - w && draw < upto) {
+            const u64 c = row.scratch_list()[threadIdx.x];
+            chosen(logit_of(c), (int)(uint32_t)c, all);
+        }
         return;
     }
     // ---- the draw: the warps' sums of kept weights, then the segment that holds the number is walked in index order
