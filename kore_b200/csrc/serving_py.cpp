@@ -216,6 +216,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t count) {
         if (count == ARGS) return F(args);
     } catch (...) {  // torch's exceptions, too (no memory): the caller meets them again
     }
+    PyErr_Clear();
     Py_RETURN_NONE;
 }
 
