@@ -39,7 +39,8 @@ def stale() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every CUDA source into one shared library; returns its path."""
+    """Compile every CUDA source into one shared library, and the Python module; returns the library's path."""
+    build_module(force)
     if not force and not stale():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -82,4 +83,3 @@ if __name__ == "__main__":
     import sys
 
     print(build(force=True, verbose="-v" in sys.argv))
-    print(build_module(force=True))
