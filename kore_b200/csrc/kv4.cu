@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 
 // ---- attention ---------------------------------------------------------------------------------
 // Bound by the bytes of the cache as long as the unpacking keeps up (8 sequences of 8191 .. 32768 positions, 8 KV heads of 128:
-// 49.6 us, 3.6 TB/s; 16 sequences of 513 .. 640, 32 KV heads of 100: 14.1 us, 6.5 of them in the five tiles of a warp): at the
+// 48.0 us, 3.7 TB/s; 16 sequences of 513 .. 640, 32 KV heads of 100: 13.6 us, 6.5 of them in the five tiles of a warp): at the
 // copy bandwidth an SM receives a position (K and V, 136 bytes for heads of 128) every 6 clocks, too few for a multiply-add per
 // value on the FP32 lanes.  So both products run on the matrix instruction m16n8k16 with f16 operands and f32 sums, and a 4-bit
 // code becomes an operand by masking alone: the bits 0x00f0 of a 16-bit lane ARE the f16 number code * 2^-20 (subnormal, exact,
@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 //   The other operand must keep f32 accuracy: queries and softmax weights are split into two f16 terms, x = hi + lo, 22
 // bits of x, for which rows are scaled by powers of two.
 //   Codes are the 16-row operand, queries and weights the 8-column one (S^T = K Q^T, O^T = V^T P^T): the two terms of four
-// query rows fill the columns, so four rows are served at the price of one, and the accumulators of 128 dims take 32
-// registers.  Up to eight rows take a second set of columns (NT = 2) over the same unpacked codes.
+// query rows fill the columns, so four rows are served at the price of one, and the accumulators of 128 dims, both terms in
+// one, take 16 registers.  Up to eight rows take a second set of columns (NT = 2) over the same unpacked codes.
 //   Lane (g, t) = (lane / 4, lane % 4).  The contraction over dims runs in any order as long as queries and keys agree, so
 // a lane takes whole words of key rows 2g and 2g + 1.  It gets hi and lo of query t at these positions, adds them, and after
 // the softmax packs hi and lo of the weight in the same place; a transposition of 8 x 8 tiles (movmatrix) makes them the
@@ -371,12 +371,9 @@ constexpr int ATT4_PER_SM = 4;   // resident CTAs: 128 registers a thread (five 
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
 constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
 constexpr int ATT4_GRAIN = ATT4_WARPS * ATT4_TILE;  // positions that give every warp a tile
-// A cache of so many grains is not split: 577 positions of one sequence and 32 KV heads take 6.8 us whole, 7.5 us in five chunks;
-// from ATT4_MANY units on two grains more (4 sequences of 760 positions, 8 KV heads, five tokens: 12.1 us whole, 15.1 split)
+// A cache of so many grains is not split: 577 positions of one sequence and 32 KV heads take 6.4 us whole, 7.3 us in five chunks;
+// from ATT4_MANY units on two grains more (4 sequences of 760 positions, 8 KV heads, five tokens: 10.8 us whole, 14.2 split)
 constexpr int ATT4_WHOLE = 5, ATT4_MANY = 32;
-// nor, among that many units, is the longest sequence that has so many grains more than an even share: 16 sequences of 1020
-// positions and 32 KV heads, 8 grains of 7, take 23.6 us and 32.1 us with a second chunk of one grain
-constexpr int ATT4_EXTRA = 4;
 constexpr int ATT4_ROUND = 32;  // chunks that the second kernel takes in a round
 constexpr float ATT4_SLACK = 8.0f;  // log2 of how far a weight may rise above the reference
 
@@ -423,11 +420,12 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
     // units alone take most of the slots the second one is used, and up to a CTA per unit more than the GPU holds
     const unsigned share = p.slots - p.least_ctas > p.slots / 2 ? p.slots - p.least_ctas : p.slots;
     const unsigned even = total >> 31 ? (unsigned)((total + share - 1) / share) : ((unsigned)total + share - 1) / share;
-    // A tile per warp is enough for a chunk (16 sequences of 641 positions and 8 KV heads: 13.1 us, in chunks of five 18.0); more
-    // than a round of them costs more than a second tile does (one sequence of 8000: 12.4 and 11.4 us).  No larger than the
+    // Sequences hardly longer than an even share stay whole: 16 sequences of 1020 positions and 32 KV heads, 8 grains of 7, take
+    // 22.8 us, and 32 us with second chunks of one grain.  Otherwise a tile per warp is enough for a chunk (16 sequences of 641 positions and 8 KV heads: 12.6 us, in chunks of five 18); more
+    // than a round of them costs more than a second tile does (one sequence of 8000: 12.4 us, and 11.3).  No larger than the
     // cache: many units over a long one would take the products below past 32 bits
     longest = __reduce_max_sync(0xffffffffu, longest);
-    const unsigned least = longest <= even + ATT4_EXTRA && p.batch * units >= ATT4_MANY ? longest : longest > ATT4_ROUND ? 2 : 1;
+    const unsigned least = 3 * longest <= 4 * even ? longest : longest > ATT4_ROUND ? 2 : 1;
     w.size = min(max(max(even, least), 1u), (unsigned)(p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
     int first = 0;  // running sum of CTAs over the sequences
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
@@ -464,8 +462,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 }
 // x -> (hi, lo), two f16 terms of it
 __device__ __forceinline__ uint32_t split_f16(float x) {
-    const __half hi = __float2half_rn(x);
-    const __half2 r = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
+    const __half2 r = __floats2half2_rn(x, x - __half2float(__float2half_rn(x)));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
@@ -519,7 +516,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
     using A = Attn4<W, NT>;
     constexpr int KC = A::KC, NBK = A::NBK, ROWS = A::ROWS;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ uint2 s_q[NT][2 * KC][32];  // query operands, in the order of the matrix instruction
+    __shared__ uint4 s_q[NT][KC][32];  // query operands, in the order of the matrix instruction
     __shared__ float s_fr[ROWS], s_qs[ROWS];
     __shared__ float s_m[ATT4_WARPS][ROWS], s_l[ATT4_WARPS][ROWS];
     __shared__ long long s_row[ROWS];  // index of the tile's rows in q and out
@@ -630,18 +627,18 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
             if (w >= 4 * KC) continue;
             const int tt = A::VEC ? w / KC : w & 3, c = A::VEC ? w % KC : w >> 2;
             const uint32_t y = split_f16(x[m][i] * up);
-            // step 2c + (n & 2) / 2, register n & 1, half n / 4; column 2 warp holds hi, the next one lo
-            __half *at = dst + ((size_t)(2 * c + ((n >> 1) & 1)) * 32 + warp * 8 + tt) * 4 + (n & 1) * 2 + (n >> 2);
+            // step (n & 2) / 2 of word c, register n & 1, half n / 4; column 2 warp holds hi, the next one lo
+            __half *at = dst + ((size_t)c * 32 + warp * 8 + tt) * 8 + ((n >> 1) & 1) * 4 + (n & 1) * 2 + (n >> 2);
             at[0] = __ushort_as_half((unsigned short)(y & 0xffffu));
-            at[16] = __ushort_as_half((unsigned short)(y >> 16));
+            at[32] = __ushort_as_half((unsigned short)(y >> 16));
         }
     }
     __syncthreads();
     const int least = min(c1, len - s_off[0]);  // the smallest limit of the tile's rows
-    uint2 qf[NT][2 * KC];  // held in registers where they fit
+    uint4 qf[KC];  // held in registers where they fit
     if (NT == 1) {
 #pragma unroll
-        for (int c = 0; c < 2 * KC; ++c) qf[0][c] = s_q[0][c][lane];
+        for (int c = 0; c < KC; ++c) qf[c] = s_q[0][c][lane];
     }
     int end[NT];  // positions of the chunk that this lane's row sees
     float fr[NT], qs[NT];
@@ -653,7 +650,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
         qs[n] = s_qs[r];
     }
 
-    float acc[NT][NBK][4][4];
+    float acc[NT][NBK][4][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -661,7 +658,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][k][j][i] = 0.0f;
+                for (int i = 0; i < 2; ++i) acc[n][k][j][i] = 0.0f;
     // of row t of each set: reference, sums over this lane's positions, the largest |weight * step| at the last rescaling, and
     // what weights are held times: 2^6 / 2^floor(log2 wref)
     float mref[NT], l[NT], alo[NT], wref[NT], ws[NT];
@@ -709,10 +706,10 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
                 const uint32_t a8[4] = {(x8 << 4) & 0x00f000f0u, (y8 << 4) & 0x00f000f0u, x8 & 0x00f000f0u, y8 & 0x00f000f0u};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint2 q0 = NT == 1 ? qf[n][2 * c] : s_q[n][2 * c][lane], q1 = NT == 1 ? qf[n][2 * c + 1] : s_q[n][2 * c + 1][lane];
-                    if (c == 0) mma_f16_first(sc[n], a[0], a[1], a[2], a[3], q0.x, q0.y);
-                    else mma_f16(sc[n], a[0], a[1], a[2], a[3], q0.x, q0.y);
-                    mma_f16(sc[n], a8[0], a8[1], a8[2], a8[3], q1.x, q1.y);
+                    const uint4 q = NT == 1 ? qf[c] : s_q[n][c][lane];
+                    if (c == 0) mma_f16_first(sc[n], a[0], a[1], a[2], a[3], q.x, q.y);
+                    else mma_f16(sc[n], a[0], a[1], a[2], a[3], q.x, q.y);
+                    mma_f16(sc[n], a8[0], a8[1], a8[2], a8[3], q.z, q.w);
                 }
             }
             const uint2 kp = *reinterpret_cast<const uint2 *>(sp + 16 * h + 2 * g);
@@ -788,7 +785,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[n][k][j][i] *= adj;
+                        for (int i = 0; i < 2; ++i) acc[n][k][j][i] *= adj;
             }
         }
         // ---- weighted sum of the codes
@@ -841,7 +838,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][k][j][i] += part[n][i];
+                    for (int i = 0; i < 2; ++i) acc[n][k][j][i] += part[n][2 * i] + part[n][2 * i + 1];
             }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -865,9 +862,8 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
             float4 *dst = reinterpret_cast<float4 *>(so + 8 * A::v_word(g, k));
 #pragma unroll
             for (int j = 0; j < 4; j += 2)
-                dst[j / 2] = make_float4(fmaf(acc[n][k][j][0] + acc[n][k][j][1], inv_ws, alo[n]), fmaf(acc[n][k][j][2] + acc[n][k][j][3], inv_ws, alo[n]),
-                                         fmaf(acc[n][k][j + 1][0] + acc[n][k][j + 1][1], inv_ws, alo[n]),
-                                         fmaf(acc[n][k][j + 1][2] + acc[n][k][j + 1][3], inv_ws, alo[n]));
+                dst[j / 2] = make_float4(fmaf(acc[n][k][j][0], inv_ws, alo[n]), fmaf(acc[n][k][j][1], inv_ws, alo[n]),
+                                         fmaf(acc[n][k][j + 1][0], inv_ws, alo[n]), fmaf(acc[n][k][j + 1][1], inv_ws, alo[n]));
         }
     }
     __syncthreads();
