@@ -418,8 +418,19 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
     const unsigned long long total = (unsigned long long)__reduce_add_sync(0xffffffffu, grains) * units;
     // sum of ceil(g / size) <= total / size + sequences * units, which is at most `slots` for the first size.  Where the
     // units alone take most of the slots the second one is used, and up to a CTA per unit more than the GPU holds
-    const unsigned share = p.slots - p.least_ctas > p.slots / 2 ? p.slots - p.least_ctas : p.slots;
-    const unsigned even = total >> 31 ? (unsigned)((total + share - 1) / share) : ((unsigned)total + share - 1) / share;
+    const bool once = p.slots - p.least_ctas > p.slots / 2;
+    const auto shares = [&](unsigned n) { return total >> 31 ? (unsigned)((total + n - 1) / n) : ((unsigned)total + n - 1) / n; };
+    unsigned even = shares(once ? p.slots - p.least_ctas : p.slots);
+    // the smallest size (to 3 %) with which the CTAs still are all resident: chunks of 19 grains instead of 20 for 8 sequences of
+    // 8191 .. 32768 positions, of 4 instead of 5 for 4 of 1501 .. 4001 with 24 units each (46.9 and 48.0 us, 19.9 and 21.9 us)
+    if (once && p.batch <= 32) {
+        unsigned low = shares(p.slots);
+        while (even - low > even / 32) {
+            const unsigned mid = (low + even) / 2, c = lane < p.batch ? max((grains + mid - 1) / mid, 1u) : 0u;
+            if (__reduce_add_sync(0xffffffffu, c) * units <= (unsigned)p.slots) even = mid;
+            else low = mid + 1;
+        }
+    }
     // Sequences hardly longer than an even share stay whole: 16 sequences of 1020 positions and 32 KV heads, 8 grains of 7, take
     // 22.8 us, and 32 us with second chunks of one grain.  Otherwise a tile per warp is enough for a chunk (16 sequences of 641 positions and 8 KV heads: 12.6 us, in chunks of five 18); more
     // than a round of them costs more than a second tile does (one sequence of 8000: 12.4 us, and 11.3).  No larger than the
