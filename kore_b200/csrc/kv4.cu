@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
 
 // ---- attention ---------------------------------------------------------------------------------
 // Bound by the bytes of the cache as long as the unpacking keeps up (8 sequences of 8191 .. 32768 positions, 8 KV heads of 128:
-// 48.0 us, 3.7 TB/s; 16 sequences of 513 .. 640, 32 KV heads of 100: 13.6 us, 6.5 of them in the five tiles of a warp): at the
+// 46.6 us, 3.8 TB/s; 16 sequences of 513 .. 640, 32 KV heads of 100: 13.6 us, 6.5 of them in the five tiles of a warp): at the
 // copy bandwidth an SM receives a position (K and V, 136 bytes for heads of 128) every 6 clocks, too few for a multiply-add per
 // value on the FP32 lanes.  So both products run on the matrix instruction m16n8k16 with f16 operands and f32 sums, and a 4-bit
 // code becomes an operand by masking alone: the bits 0x00f0 of a 16-bit lane ARE the f16 number code * 2^-20 (subnormal, exact,
@@ -421,8 +421,9 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
     const bool once = p.slots - p.least_ctas > p.slots / 2;
     const auto shares = [&](unsigned n) { return total >> 31 ? (unsigned)((total + n - 1) / n) : ((unsigned)total + n - 1) / n; };
     unsigned even = shares(once ? p.slots - p.least_ctas : p.slots);
-    // the smallest size (to 3 %) with which the CTAs still are all resident: chunks of 19 grains instead of 20 for 8 sequences of
-    // 8191 .. 32768 positions, of 4 instead of 5 for 4 of 1501 .. 4001 with 24 units each (46.9 and 48.0 us, 19.9 and 21.9 us)
+    // The smallest size (to 3 %) with which the CTAs still are all resident: chunks of 19 grains instead of 20 for 8 sequences of
+    // 8191 .. 32768 positions, of 4 instead of 5 for 4 of 1501 .. 4001 with 24 units each (46.6 and 48.0 us, 19.9 and 21.9 us).
+    // Where units take more than half of the slots, chunks of one round are larger and take 2 to 7 % longer than two rounds
     if (once && p.batch <= 32) {
         unsigned low = shares(p.slots);
         while (even - low > even / 32) {
@@ -432,9 +433,10 @@ __device__ __forceinline__ bool find_attn_work(const AttnParams &p, AttnWork &w)
         }
     }
     // Sequences hardly longer than an even share stay whole: 16 sequences of 1020 positions and 32 KV heads, 8 grains of 7, take
-    // 22.8 us, and 32 us with second chunks of one grain.  Otherwise a tile per warp is enough for a chunk (16 sequences of 641 positions and 8 KV heads: 12.6 us, in chunks of five 18); more
-    // than a round of them costs more than a second tile does (one sequence of 8000: 12.4 us, and 11.3).  No larger than the
-    // cache: many units over a long one would take the products below past 32 bits
+    // 22.8 us, and 32 us with second chunks of one grain.  Otherwise a tile per warp is enough for a chunk (16 sequences of 641
+    // positions and 8 KV heads: 12.6 us, in chunks of five 18); more than a round of them costs more than a second tile does (one
+    // sequence of 8000: 12.4 us, and 11.3).  No larger than the cache: many units over a long one would take the products below
+    // past 32 bits
     longest = __reduce_max_sync(0xffffffffu, longest);
     const unsigned least = 3 * longest <= 4 * even ? longest : longest > ATT4_ROUND ? 2 : 1;
     w.size = min(max(max(even, least), 1u), (unsigned)(p.lmax + ATT4_GRAIN - 1) / ATT4_GRAIN);
