@@ -56,6 +56,7 @@ struct AppendParams {
     int max_pos;
     const float *q_gamma, *k_gamma;
     float eps;
+    double per_dim;  // 1 / hd
     unsigned tasks, groups;  // tokens * groups of heads
     int n_heads, n_kv, hd;
     long long cache_len;  // n_seqs * lmax
@@ -126,22 +127,24 @@ __device__ __forceinline__ double warp_sum_of(double (&v)[HPW]) {
 }
 
 // Bound by one memory round trip for a few tokens (16 tokens, 32 heads of 100, norms, f32 cache: 2.7 us) and for many by the
-// bytes of the rows, which norms (64-bit sums) and the quantiser do not quite hide: 8192 tokens of 32 + 2 x 8 heads of 128 take
-// 80 us (3.9 TB/s; 62 us, 5.1 TB/s, without norms to an f32 cache).  A warp takes HPW heads of one token:
+// bytes of the rows, which the quantiser does not quite hide: 8192 tokens of 32 + 2 x 8 heads of 128 with norms take 66 us
+// (4.7 TB/s; 62 us, 5.1 TB/s, with an f32 cache).  A warp takes HPW heads of one token:
 // its lane l owns the rotation pairs 2l and 2l + 1, dims {2l, 2l + 1} of each half, so that its codes are whole bytes of the
 // row, a row needs no shared memory, and the token's angles are read once for all heads.
 // PAIRS: rows and tables are 8-byte aligned and half is even, a lane's two neighbours come and go in one access.
-template <bool Q4, int HPW, bool PAIRS>
+// FULL: heads of 128, every lane owns its pairs, so nothing is predicated and addresses are shifts (66 us against 80 us for the
+// 8192 tokens above, 62 and 72 us with an f32 cache).
+template <bool Q4, int HPW, bool PAIRS, bool FULL = false>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 8u + (threadIdx.x >> 5);
     release_and_wait();
     if (task >= p.tasks) return;
-    const int heads = p.n_heads + 2 * p.n_kv, hd = p.hd, half = hd / 2;
+    const int heads = p.n_heads + 2 * p.n_kv, hd = FULL ? 128 : p.hd, half = hd / 2;
     const unsigned t = task / p.groups;
     const int head0 = (int)(task - t * p.groups) * HPW;
     const int i0 = 2 * lane;
-    const bool own0 = i0 < half, own1 = i0 + 1 < half;
+    const bool own0 = FULL || i0 < half, own1 = FULL || i0 + 1 < half;
     float a[HPW][2], b[HPW][2];
     const float *row = p.qkv + (size_t)t * p.ld + (size_t)head0 * hd;
     auto load2 = [&](const float *src, float (&x)[2]) {
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) ss[j] = fma((double)a[j][i], (double)a[j][i], fma((double)b[j][i], (double)b[j][i], ss[j]));
         }
-        inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * (1.0 / hd) + (double)p.eps);
+        inv_of = (float)rsqrt_f64(warp_sum_of<HPW>(ss) * p.per_dim + (double)p.eps);
     }
     auto scale = [&](int j, const float (&ga)[2], const float (&gb)[2]) {
         const float inv = HPW == 1 ? inv_of : __shfl_sync(0xffffffffu, inv_of, 32 / HPW * j);
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
             bytes[lane] = byte_of(a[j]);
             bytes[half / 2 + lane] = byte_of(b[j]);
         }
-        if (lane < 4 * words - half) bytes[half + lane] = 0;  // tail of the last word
+        if (!FULL && lane < 4 * words - half) bytes[half + lane] = 0;  // tail of the last word
     }
 }
 
@@ -1014,6 +1017,7 @@ static int append(AppendParams &p, bool q4, size_t n, size_t max_pos, size_t n_s
         return fail(KB_ERR_UNSUPPORTED, "append: %zu tokens of %zu heads, %zu sequences", n, heads, n_seqs);
     p.max_pos = (int)max_pos;
     p.cache_len = (long long)n_seqs * p.lmax;
+    p.per_dim = 1.0 / p.hd;
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.qkv) | reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t) |
                           reinterpret_cast<uintptr_t>(p.q_gamma) | reinterpret_cast<uintptr_t>(p.k_gamma) | reinterpret_cast<uintptr_t>(p.q_out) |
                           reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache);
@@ -1026,8 +1030,8 @@ static int append(AppendParams &p, bool q4, size_t n, size_t max_pos, size_t n_s
     unsigned grid = 0;
     if (int rc = warp_grid(n, p.groups, &p.tasks, &grid)) return rc;
     void (*kern)(AppendParams) =
-        q4 ? (many ? (pairs ? append_kernel<true, 4, true> : append_kernel<true, 4, false>) : (pairs ? append_kernel<true, 1, true> : append_kernel<true, 1, false>))
-           : (many ? (pairs ? append_kernel<false, 4, true> : append_kernel<false, 4, false>) : (pairs ? append_kernel<false, 1, true> : append_kernel<false, 1, false>));
+        q4 ? (many ? (pairs ? (p.hd == 128 ? append_kernel<true, 4, true, true> : append_kernel<true, 4, true>) : append_kernel<true, 4, false>) : (pairs ? append_kernel<true, 1, true> : append_kernel<true, 1, false>))
+           : (many ? (pairs ? (p.hd == 128 ? append_kernel<false, 4, true, true> : append_kernel<false, 4, true>) : append_kernel<false, 4, false>) : (pairs ? append_kernel<false, 1, true> : append_kernel<false, 1, false>));
     const cudaError_t e = launch_after(kern, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "append launch");
 }

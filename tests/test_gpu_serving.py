@@ -83,6 +83,37 @@ def test_append_to_f32(env, n, heads, kv, hd, norm):
     assert (q.cpu().numpy() == rq).all() and (kd.cpu().numpy() == k).all() and (vd.cpu().numpy() == v).all()
 
 
+@pytest.mark.parametrize("heads,kv,hd,norm,odd", [(8, 2, 128, True, 0), (8, 2, 128, False, 0), (8, 2, 128, True, 1), (6, 3, 100, True, 0), (5, 1, 36, True, 0),
+                                                  (3, 3, 4, False, 0), (4, 4, 124, True, 1)])
+def test_append_of_many_tokens(env, heads, kv, hd, norm, odd):
+    """groups of four heads (queries, keys and values in one group, and a last one that is not full), both caches, odd addresses"""
+    n = 3000 // (heads + 2 * kv) + 5
+    rng = np.random.default_rng(hd + heads)
+    seqs, lmax = 4, (n + 3) // 4 * 4
+    qkv = (cases.gaussian(hd, (n, (heads + 2 * kv) * hd), 1.0) * np.exp(rng.uniform(-3, 3, (n, 1)))).astype(f32)
+    gq, gk = ((1 + cases.gaussian(i, (hd,), 0.2)).astype(f32) if norm else None for i in (5, 6))
+    cos, sin = tables(lmax, hd)
+    rows = rng.choice(seqs * lmax, n, replace=False).astype(np.int64)
+    pos = (rows % lmax).astype(np.int32)
+    src = env.torch.zeros((n, qkv.shape[1] + odd), device="cuda")[:, odd:]
+    src.copy_(env.dev(qkv))
+    rq, rk, rv = sr.append(qkv, pos, cos, sin, heads, kv, hd, gq, gk, 1e-6)
+    cache = filled_cache(env, seqs, kv, lmax, hd, 78)
+    want = planes_of(cache)
+    pair = [cases.gaussian(8 + i, (seqs, kv, lmax, hd), 1.0) for i in (0, 1)]
+    dev_pair = tuple(env.dev(x) for x in pair)
+    for to in (cache, dev_pair):
+        q = env.serving.qknorm_rope_append(src, env.dev(pos), env.dev(rows), env.dev(cos), env.dev(sin), to, heads,
+                                           q_gamma=None if gq is None else env.dev(gq), k_gamma=None if gk is None else env.dev(gk), eps=1e-6)
+        assert (q.cpu().numpy() == rq).all()
+    for at, x in ((0, rk), (2, rv)):
+        want[at][rows // lmax, :, rows % lmax], want[at + 1][rows // lmax, :, rows % lmax] = sr.quantise(x)
+        pair[at // 2][rows // lmax, :, rows % lmax] = x
+    for got, ref in zip(planes_of(cache), want):
+        assert (got == ref).all()
+    assert all((got.cpu().numpy() == ref).all() for got, ref in zip(dev_pair, pair))
+
+
 def test_append_without_norm_is_the_rotation_of_kb_rope_kv(env):
     """on the f32 cache the operator without gammas gives the numbers of the framework's own append"""
     from kore_b200 import _cabi
