@@ -872,14 +872,15 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         float *so = reinterpret_cast<float *>(smem) + (warp * ROWS + 4 * n + t) * A::OLD;
-        const float inv_ws = 0x1p20f / ws[n];
+        // 2^20 / ws in two factors: from weights times steps of 2^114 on their product leaves f32 where the sums do not
+        const float back = __uint_as_float(0x82000000u - __float_as_uint(ws[n]));  // 2^6 / ws
 #pragma unroll
         for (int k = 0; k < NBK; ++k) {
             float4 *dst = reinterpret_cast<float4 *>(so + 8 * A::v_word(g, k));
 #pragma unroll
             for (int j = 0; j < 4; j += 2)
-                dst[j / 2] = make_float4(fmaf(acc[n][k][j][0], inv_ws, alo[n]), fmaf(acc[n][k][j][1], inv_ws, alo[n]),
-                                         fmaf(acc[n][k][j + 1][0], inv_ws, alo[n]), fmaf(acc[n][k][j + 1][1], inv_ws, alo[n]));
+                dst[j / 2] = make_float4(fmaf(acc[n][k][j][0] * 0x1p14f, back, alo[n]), fmaf(acc[n][k][j][1] * 0x1p14f, back, alo[n]),
+                                         fmaf(acc[n][k][j + 1][0] * 0x1p14f, back, alo[n]), fmaf(acc[n][k][j + 1][1] * 0x1p14f, back, alo[n]));
         }
     }
     __syncthreads();
