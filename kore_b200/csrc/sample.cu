@@ -378,27 +378,28 @@ struct Row {
             // sums of shares are off by less than 2^-15: the border lies in the bins that reach target - slack .. target + slack
             const u64 all = told(3, plus);
             target = target_of(all);
-            const double aim = (double)target * 0x1p-44, slack = (double)all * 0x1p-58;
-            double w[2];
+            // In whole units of 2^-40, which the scan adds exactly: every number then lies in one bin
+            const u64 aim = target >> 4, slack = all >> 18, low = aim > slack ? aim - slack : 0ull, high = aim + slack;
+            u64 w[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k)
-                w[k] = (double)mine[k] * (1.0 / 65535) * (double)exp2f((float)(2 * threadIdx.x + k) * (-1.4426950408889634f * 32 / SAMPLE_BINS));
-            double upto = w[0] + w[1];
+                w[k] = (u64)((double)mine[k] * (0x1p40 / 65535) * (double)exp2f((float)(2 * threadIdx.x + k) * (-1.4426950408889634f * 32 / SAMPLE_BINS)));
+            u64 upto = w[0] + w[1];
             u64 shares = mine[0] + mine[1];  // up to bin[1]: 0.969 to 1 of 65535 for every element
             block_scan(upto, shares);
             if (threadIdx.x == SAMPLE_THREADS - 1) sh.upto = shares;
             __syncthreads();
 #pragma unroll
             for (int k = 1; k >= 0; --k) {
-                if (upto - w[k] < aim - slack && aim - slack <= upto) sh.bin[0] = 2 * threadIdx.x + k;
-                if (upto - w[k] < aim + slack && aim + slack <= upto) {
+                if (upto - w[k] < low && low <= upto) sh.bin[0] = 2 * threadIdx.x + k;
+                if (upto - w[k] < high && high <= upto) {
                     sh.bin[1] = 2 * threadIdx.x + k;
                     sh.upto = shares;
                 }
                 upto -= w[k];
                 shares -= mine[k];
             }
-            if (threadIdx.x == 0 && aim - slack <= 0.0) sh.bin[0] = 0;
+            if (threadIdx.x == 0 && low == 0) sh.bin[0] = 0;
         } else {
             target = target_of(0);
             find_bin(mine, target);

@@ -1,10 +1,10 @@
-"""Attention over the 4-bit cache at the ends of its ranges and to the accuracy that its header states."""
+"""Serving-step kernels where rare numbers meet: attention over the 4-bit cache at the ends of its ranges, borders of nuclei."""
 import numpy as np
 import pytest
 
 from oracle import serving_ref as sr
 from tests import cases
-from tests.test_gpu_serving import check_attention, env  # noqa: F401
+from tests.test_gpu_serving import check_attention, check_sample, env  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 f32 = np.float32
@@ -39,3 +39,25 @@ def test_attention_of_large_values_under_rising_weights(env):
     k = np.broadcast_to(np.where(late, 7.5 * np.log(2.0), 0.0)[:, None], (1, 1, n, hd)).astype(f32)  # 64 equal dims, queries of 1 / 8, scale 1 / 8
     v = (np.random.default_rng(1).uniform(-0.99, 0.99, (1, 1, n, hd)) * np.where(late, 2.0 ** 110, 2.0 ** 80)[:, None]).astype(f32)
     check_attention(env, np.full((1, 1, 1, hd), 1 / 8, f32), cache_of(env, k, v), [n])
+
+
+# seeds of rows and top_p whose border, less the accuracy of the sums that look for it, lies where running sums in f64 of
+# neighbouring threads do not meet: found by a search on the CPU over 2e8 rows
+BETWEEN = [(38773736, 0.932712317), (65209376, 0.979467869), (186987744, 0.996985555), (74197353, 0.98854059), (171723530, 0.690360785),
+           (57606035, 0.998813152), (28156044, 0.930305243), (52030044, 0.922126591), (61540356, 0.998595774), (124656509, 0.997032821),
+           (187341261, 0.796574116), (175736678, 0.892285883), (213259238, 0.889294267)]
+
+
+def test_sample_nuclei_that_end_between_two_sums(env):
+    """rows of 20 to 60 equal logits every 1/32: every row gets its token"""
+    rows = np.full((len(BETWEEN), 256 * 61), -np.inf, f32)
+    for row, (state, _) in zip(rows, BETWEEN):
+        row[0], at = 0.0, 1
+        for b in range(256):
+            state = (state * 1664525 + 1013904223) % 2 ** 32
+            n = 20 + (state >> 16) % 41
+            row[at:at + n] = -(b + 0.5) / 32
+            at += n
+    top_p = np.array([p for _, p in BETWEEN], f32)
+    for u in (0.02, 0.37, 0.75, 0.99):
+        check_sample(env, rows, np.full(len(rows), u, f32), top_p=top_p)
