@@ -251,7 +251,7 @@ class BitNetDecoder:
                                   self.vc[li].data_ptr(), sp))
             if prefill_shape is None and self.kv4 is not None:
                 serving.attend(B["q"].view(n, H, hd), self.kv4[li], lens, out=B["attn"].view(n, H, hd))
-                launches += 2
+                launches += 2 + (self.kv4[li]._workspace(1, H) > 0)  # split sequences are joined by a second launch
             elif prefill_shape is None:
                 ck(lib.kb_attn_decode(B["q"].data_ptr(), self.kc[li].data_ptr(), self.vc[li].data_ptr(), lens.data_ptr(),
                                       n, H, hd, cfg.max_len, B["attn"].data_ptr(), self.att_scratch.data_ptr(),
@@ -267,7 +267,6 @@ class BitNetDecoder:
                     vh = self.vc[li][:b, :, :t]
                 o = torch.nn.functional.scaled_dot_product_attention(qh, kh, vh, is_causal=True, enable_gqa=cfg.kv_heads != H)
                 B["attn"].view(b, t, H, hd).copy_(o.transpose(1, 2))
-                launches += 4
             ck(lib.kb_linear_forward_fused(L["o"].handle, B["attn"].data_ptr(), None, 0, None, None, n, B["hidden"].data_ptr(),
                                            B["hidden"].data_ptr(), 0, _cabi.PATH_AUTO, ws_ptr, B["ws_bytes"], sp))
             if fused:
@@ -288,7 +287,8 @@ class BitNetDecoder:
                                                B["sum"].data_ptr(), n, B["hidden"].data_ptr(), B["hidden"].data_ptr(), 0,
                                                _cabi.PATH_AUTO, None, 0, sp))
                 launches += 7 + (1 if n > 4 else 0)
-        self.launches_per_step = launches + 3
+        if prefill_shape is None:
+            self.launches_per_step = launches + 2 * (self.sampling is not None)  # the uniform numbers and the choice
         return B
 
     def _head(self, hidden_rows):
@@ -336,10 +336,12 @@ class BitNetDecoder:
                                               self.logits.data_ptr(), self.head_keys.data_ptr(), sp))
             _cabi.check(lib.kb_decode_advance(self.head_keys.data_ptr(), n, self.tokens.data_ptr(), self.positions.data_ptr(),
                                               self.lens.data_ptr(), self.cache_rows.data_ptr(), sp))
+            self.launches_per_step += 3
             self._sample()
             return
         logits = self._head(B["hidden"])
         self.torch.argmax(logits, dim=1, out=self.tokens)
+        self.launches_per_step += 6  # norm, product, argmax and three increments
         self._sample()
         self.positions.add_(1)
         self.lens.add_(1)
@@ -382,7 +384,7 @@ class BitNetDecoder:
             _cabi.check(self.lib.kb_decoder_step(self.persistent, self.tokens.data_ptr(), self.positions.data_ptr(),
                                                  self.lens.data_ptr(), self.cache_rows.data_ptr(), self.hidden_step.data_ptr(),
                                                  self.logits.data_ptr(), sp))
-            self.launches_per_step = 1
+            self.launches_per_step = 1 + 2 * (self.sampling is not None)
             self._sample()
             return
         if not use_graph:

@@ -143,6 +143,15 @@ class KV4Cache:
         a, b, c, d = self._held
         return a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr()
 
+    def _workspace(self, t: int, heads: int) -> int:
+        """Bytes of workspace of ``attend`` with t query tokens: 0 where no sequence is split, one launch instead of two."""
+        need = self._ws_bytes.get((t, heads))
+        if need is None:
+            with torch.cuda.device(self._dev):
+                need = self._ws_bytes[t, heads] = int(_cabi.lib().kb_attn_kv4_workspace_bytes(self.n_seqs, t, heads, self.n_kv_heads, self.head_dim,
+                                                                                             self.max_len))
+        return need
+
     def memory_bytes(self) -> int:
         return sum(t.numel() * 4 for t in self._held)
 
@@ -231,15 +240,11 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     out = torch.empty_like(q) if out is None else _need(out, "out", _F32, shape, dev)
     if q.numel() == 0:
         return out
-    lib, ws = _cabi.lib(), 0
-    need = cache._ws_bytes.get((t, heads))
-    if need is None:
-        with torch.cuda.device(dev):
-            need = cache._ws_bytes[t, heads] = lib.kb_attn_kv4_workspace_bytes(n, t, heads, cache.n_kv_heads, hd, cache.max_len)
+    ws, need = 0, cache._workspace(t, heads)
     if need:  # torch's allocator orders its reuse by stream and keeps a captured graph's blocks to that graph
         block = q.new_empty(need // 4)
         ws = block.data_ptr()
-    _run(dev, lib.kb_attn_kv4, q.data_ptr(), *cache._planes(), lens.data_ptr(), n, t, heads, cache.n_kv_heads, hd, cache.max_len, scale,
+    _run(dev, _cabi.lib().kb_attn_kv4, q.data_ptr(), *cache._planes(), lens.data_ptr(), n, t, heads, cache.n_kv_heads, hd, cache.max_len, scale,
          out.data_ptr(), ws, need)
     return out
 

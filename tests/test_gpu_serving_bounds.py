@@ -61,3 +61,47 @@ def test_sample_nuclei_that_end_between_two_sums(env):
     top_p = np.array([p for _, p in BETWEEN], f32)
     for u in (0.02, 0.37, 0.75, 0.99):
         check_sample(env, rows, np.full(len(rows), u, f32), top_p=top_p)
+
+
+# ---- the decoder's count of its launches ----------------------------------------------------------
+@pytest.mark.parametrize("batch,kv,bits,max_len", [(1, 4, 4, 32), (2, 2, 4, 4000), (6, 2, 4, 4000), (3, 4, 32, 32), (20, 4, 4, 32)])
+def test_decoder_counts_its_launches(env, batch, kv, bits, max_len):
+    """launches_per_step is the number of kernels of a captured step, and one more with sampling for the numbers drawn before it"""
+    from cuda.bindings import runtime
+
+    t = env.torch
+    cfg = env.decoder.DecoderConfig(n_layers=2, d_model=128, n_heads=4, d_ff=256, vocab=97, max_len=max_len, n_kv_heads=kv, kv_bits=bits)
+    dec = env.decoder.BitNetDecoder(cfg, env.decoder.random_weights(cfg, seed=4000), batch=batch)
+    prompt = t.zeros((batch, 3), dtype=t.int64, device="cuda")
+    assert dec.launches_per_step == 0
+    for sampling in (False, True):
+        dec.prefill(prompt)
+        if sampling:
+            dec.set_sampling(temperature=0.8)
+        stream = t.cuda.Stream()
+        stream.wait_stream(t.cuda.current_stream())
+        with t.cuda.stream(stream):
+            dec._decode_body()
+        t.cuda.synchronize()
+        g = t.cuda.CUDAGraph(keep_graph=True)
+        with t.cuda.graph(g, stream=stream):
+            dec._decode_body()
+        raw = g.raw_cuda_graph()
+        count = runtime.cudaGraphGetNodes(raw, 0)[2]
+        nodes = runtime.cudaGraphGetNodes(raw, count)[1]
+        kernels = sum(runtime.cudaGraphNodeGetType(x)[1] == runtime.cudaGraphNodeType.cudaGraphNodeTypeKernel for x in nodes)
+        assert dec.launches_per_step == kernels + sampling
+        dec.generate(prompt, 3)  # a prompt and its first choice are no step
+        assert dec.launches_per_step == kernels + sampling
+    dec.close()
+
+
+def test_decoder_counts_the_draw_behind_the_persistent_step(env):
+    cfg = env.decoder.DecoderConfig(n_layers=2, d_model=128, n_heads=4, d_ff=256, vocab=97, max_len=32)
+    dec = env.decoder.BitNetDecoder(cfg, env.decoder.random_weights(cfg, seed=4000), batch=1)
+    assert dec.persistent is not None
+    for temperature, launches in ((None, 1), (0.7, 3), (None, 1)):
+        dec.set_sampling(temperature)
+        dec.decode_step()
+        assert dec.launches_per_step == launches
+    dec.close()
