@@ -4,6 +4,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import warnings
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_PKG, "csrc")
@@ -39,20 +40,23 @@ def stale() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every CUDA source into one shared library, and the Python module; returns the library's path."""
-    build_module(force)
-    if not force and not stale():
-        return LIB_PATH
-    os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [nvcc(), *NVCC_FLAGS]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", LIB_PATH, *[os.path.join(CSRC, f) for f in SOURCES]]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    if verbose:
-        print(res.stdout + res.stderr)
+    """Compile every CUDA source into one shared library, then the Python module; returns the library's path.  The library needs
+    nvcc alone: where the module cannot be built (no torch headers, no C++ compiler) that is a warning."""
+    if force or stale():
+        os.makedirs(LIB_DIR, exist_ok=True)
+        cmd = [nvcc(), *NVCC_FLAGS]
+        if verbose:
+            cmd += ["-Xptxas", "-v"]
+        cmd += ["-o", LIB_PATH, *[os.path.join(CSRC, f) for f in SOURCES]]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if verbose:
+            print(res.stdout + res.stderr)
+    try:
+        build_module(force)
+    except Exception as e:
+        warnings.warn(f"the Python module of kore_b200.serving was not built: {e}", RuntimeWarning, stacklevel=2)
     return LIB_PATH
 
 

@@ -1,0 +1,49 @@
+"""The builds of the library and of the Python module beside it."""
+import os
+import subprocess
+
+import pytest
+
+from kore_b200 import _build
+
+
+class Runs:
+    """stands for subprocess.run: notes the programs, writes the outputs, fails where told to"""
+
+    def __init__(self, failing=()):
+        self.programs, self.failing = [], failing
+
+    def __call__(self, cmd, **kw):
+        name = os.path.basename(cmd[0])
+        self.programs.append(name)
+        rc = int(name in self.failing)
+        if not rc:
+            open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, rc, "", "no")
+
+
+@pytest.fixture
+def sandbox(monkeypatch, tmp_path):
+    """builds into an empty folder"""
+    monkeypatch.setattr(_build, "LIB_DIR", str(tmp_path))
+    monkeypatch.setattr(_build, "LIB_PATH", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(_build, "MODULE_PATH", str(tmp_path / "module.so"))
+    return tmp_path
+
+
+@pytest.mark.parametrize("why", ["no compiler", "no torch"])
+def test_the_library_is_built_without_the_module(monkeypatch, sandbox, why):
+    """nvcc is all that the library needs"""
+    runs = Runs(failing=("g++", "c++"))
+    monkeypatch.setattr(_build.subprocess, "run", runs)
+    if why == "no torch":
+        monkeypatch.setitem(__import__("sys").modules, "torch", None)
+    with pytest.warns(RuntimeWarning, match="serving"):
+        assert _build.build() == _build.LIB_PATH
+    assert runs.programs[0] == "nvcc" and os.path.exists(_build.LIB_PATH)
+
+
+def test_a_library_that_does_not_compile_is_an_error(monkeypatch, sandbox):
+    monkeypatch.setattr(_build.subprocess, "run", Runs(failing=("nvcc",)))
+    with pytest.raises(RuntimeError, match="nvcc"):
+        _build.build()
