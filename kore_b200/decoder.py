@@ -31,7 +31,7 @@ from typing import Dict, List, Optional
 
 import numpy as np
 
-from . import _cabi, nn, serving
+from . import _cabi, nn
 
 
 @dataclass
@@ -129,6 +129,8 @@ class BitNetDecoder:
                  persistent: Optional[bool] = None):
         import torch
 
+        from . import serving
+
         if cfg.kv_bits not in (4, 32):
             raise _cabi.KoreError(_cabi.ERR_UNSUPPORTED, f"kv_bits {cfg.kv_bits}: the cache is held in 32 or 4 bits")
         if cfg.n_heads % cfg.kv_heads:
@@ -136,7 +138,7 @@ class BitNetDecoder:
         if cfg.kv_bits == 32 and cfg.kv_heads != cfg.n_heads:
             raise _cabi.KoreError(_cabi.ERR_UNSUPPORTED, "grouped KV heads need kv_bits=4: the f32 cache has one per query head")
         self.cfg, self.batch, self.device = cfg, batch, device
-        self.torch = torch
+        self.torch, self.serving = torch, serving
         self.lib = _cabi.lib()
         self.dev = torch.device("cuda", device)
         d, f, v = cfg.d_model, cfg.d_ff, cfg.vocab
@@ -223,7 +225,7 @@ class BitNetDecoder:
 
     # ---- one pass over all layers for n tokens ----------------------------------------------
     def _layers(self, n, tokens, positions, cache_rows, lens, prefill_shape=None):
-        torch, cfg, lib, B = self.torch, self.cfg, self.lib, self._bufs[n]
+        torch, serving, cfg, lib, B = self.torch, self.serving, self.cfg, self.lib, self._bufs[n]
         sp = torch.cuda.current_stream(self.device).cuda_stream
         d, f, H, hd = cfg.d_model, cfg.d_ff, cfg.n_heads, cfg.head_dim
         ck = _cabi.check
@@ -368,7 +370,7 @@ class BitNetDecoder:
 
     def _sample(self):
         if self.sampling is not None:
-            serving.sample(self.logits, self.uniform, tokens=self.tokens, **self.sampling)
+            self.serving.sample(self.logits, self.uniform, tokens=self.tokens, **self.sampling)
 
     def _draw_uniform(self):
         if self.sampling is not None:

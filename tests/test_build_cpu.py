@@ -1,6 +1,7 @@
-"""The builds of the library and of the Python module beside it."""
+"""The builds of the library and of the Python module beside it, and what is imported without torch."""
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -37,7 +38,7 @@ def test_the_library_is_built_without_the_module(monkeypatch, sandbox, why):
     runs = Runs(failing=("g++", "c++"))
     monkeypatch.setattr(_build.subprocess, "run", runs)
     if why == "no torch":
-        monkeypatch.setitem(__import__("sys").modules, "torch", None)
+        monkeypatch.setitem(sys.modules, "torch", None)
     with pytest.warns(RuntimeWarning, match="serving"):
         assert _build.build() == _build.LIB_PATH
     assert runs.programs[0] == "nvcc" and os.path.exists(_build.LIB_PATH)
@@ -47,3 +48,13 @@ def test_a_library_that_does_not_compile_is_an_error(monkeypatch, sandbox):
     monkeypatch.setattr(_build.subprocess, "run", Runs(failing=("nvcc",)))
     with pytest.raises(RuntimeError, match="nvcc"):
         _build.build()
+
+
+def test_the_decoder_is_imported_without_torch():
+    """its configuration and angle tables need numpy alone"""
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "from kore_b200 import decoder\n"
+            "assert decoder.rope_tables(decoder.DecoderConfig())[0].shape == (640, 50)")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
