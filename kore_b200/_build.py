@@ -13,7 +13,6 @@ LIB_PATH = os.path.join(LIB_DIR, "libkore_b200.so")
 SOURCES = ["api.cu", "quant.cu", "gemv.cu", "gemv_group.cu", "gemv_mma.cu", "gemv_stream.cu", "gemm_tc.cu", "gemm_tcs.cu", "gemm_tc2.cu", "static_scratch.cu", "shard.cu", "decoder_ops.cu", "decode_step.cu", "kv4.cu", "sample.cu"]
 HEADERS = ["common.cuh", "device_utils.cuh", "tc_ptx.cuh", os.path.join("..", "..", "include", "kore_b200.h")]
 
-MODULE_PATH = os.path.join(LIB_DIR, "kore_b200_serving.so")  # a Python module against torch's C++ headers; loads without a GPU
 MODULE_SOURCE = "serving_py.cpp"
 
 NVCC_FLAGS = [
@@ -60,27 +59,38 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+def module_path() -> str:
+    """The Python module of kore_b200.serving, against torch's C++ headers; loads without a GPU.  Its name holds the Python and the
+    torch that it is for: another one's is neither taken for current nor loaded."""
+    import sysconfig
+
+    import torch
+
+    return os.path.join(LIB_DIR, f"kore_b200_serving.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so")
+
+
 def build_module(force: bool = False) -> str:
     """Compile the Python module of kore_b200.serving; returns its path."""
     import sysconfig
 
     import torch
 
+    path = module_path()
     deps = [os.path.join(CSRC, MODULE_SOURCE), os.path.join(CSRC, HEADERS[-1])]
-    if not force and os.path.exists(MODULE_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(MODULE_PATH) for d in deps):
-        return MODULE_PATH
+    if not force and os.path.exists(path) and all(os.path.getmtime(d) <= os.path.getmtime(path) for d in deps):
+        return path
     os.makedirs(LIB_DIR, exist_ok=True)
     base = os.path.dirname(torch.__file__)
     includes = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
                 os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"), sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    for path in includes:
-        cmd += ["-isystem", path]
-    cmd += ["-o", MODULE_PATH, deps[0], "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    for folder in includes:
+        cmd += ["-isystem", folder]
+    cmd += ["-o", path, deps[0], "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
-    return MODULE_PATH
+    return path
 
 
 if __name__ == "__main__":

@@ -32,7 +32,7 @@ def native():
     """The module of the calls (raises if it has not been built)."""
     global _native
     if _native is None:
-        lib, name, path = _cabi.lib(), "kore_b200_serving", _build.MODULE_PATH
+        lib, name, path = _cabi.lib(), "kore_b200_serving", _build.module_path()
         if not os.path.exists(path):
             raise RuntimeError(f"{path} is missing: the module has not been built (run `python -m kore_b200._build`)")
         loader = importlib.machinery.ExtensionFileLoader(name, path)

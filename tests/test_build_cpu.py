@@ -2,6 +2,7 @@
 import os
 import subprocess
 import sys
+import warnings
 
 import pytest
 
@@ -28,7 +29,6 @@ def sandbox(monkeypatch, tmp_path):
     """builds into an empty folder"""
     monkeypatch.setattr(_build, "LIB_DIR", str(tmp_path))
     monkeypatch.setattr(_build, "LIB_PATH", str(tmp_path / "lib.so"))
-    monkeypatch.setattr(_build, "MODULE_PATH", str(tmp_path / "module.so"))
     return tmp_path
 
 
@@ -58,3 +58,14 @@ def test_the_decoder_is_imported_without_torch():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
     assert res.returncode == 0, res.stderr
+
+
+def test_a_module_of_another_torch_is_not_taken_for_current(monkeypatch, sandbox):
+    import torch
+
+    runs = Runs()
+    monkeypatch.setattr(_build.subprocess, "run", runs)
+    first = _build.build_module()
+    assert _build.build_module() == first and runs.programs == ["g++"]
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert _build.build_module() != first and runs.programs == ["g++", "g++"]
