@@ -8,7 +8,7 @@ The reference's decoder loop has an f32 cache, one KV head per query head and a 
 (``crates/kore-edge/src/runtime.rs:106-294``).  All arithmetic runs in the CUDA library (``include/kore_b200.h`` states
 it down to the roundings); this file checks shapes and moves pointers.  Calls whose arguments need nothing else go through a
 small native module (``csrc/serving_py.cpp``: checks, results and launch in 5 us); it declines every other one, and what
-follows here copies strided operands, changes the device or says what is wrong.  Activations and logits are float32, as
+follows here, which also serves where the module has not been built, copies strided operands, changes the device or says what is wrong.  Activations and logits are float32, as
 everywhere in this package.  Results carry no gradient.
 """
 from __future__ import annotations
@@ -16,6 +16,7 @@ from __future__ import annotations
 import importlib.machinery
 import importlib.util
 import os
+import warnings
 
 import torch
 
@@ -28,10 +29,16 @@ _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
 _native = None
 
 
+class _Declines:
+    """stands for the module where there is none: every call goes the other way"""
+
+    append = read = attend = sample = staticmethod(lambda *args: None)
+
+
 def native():
-    """The module of the calls (raises if it has not been built)."""
+    """The module of the calls (raises if it has not been built for this Python and torch)."""
     global _native
-    if _native is None:
+    if _native is None or _native is _Declines:
         lib, name, path = _cabi.lib(), "kore_b200_serving", _build.module_path()
         if not os.path.exists(path):
             raise RuntimeError(f"{path} is missing: the module has not been built (run `python -m kore_b200._build`)")
@@ -42,6 +49,18 @@ def native():
                                                    lib.kb_attn_kv4_workspace_bytes, lib.kb_sample)))
         _native = module
     return _native
+
+
+def _calls():
+    """the module, or (with one warning) what declines every call: results are the same, a call takes some 5 to 9 us longer"""
+    global _native
+    _cabi.lib()  # without the CUDA library there is nothing to call: its error
+    try:
+        return native()
+    except (RuntimeError, ImportError) as e:
+        warnings.warn(f"calls of kore_b200.serving go without their native module: {e}", RuntimeWarning, stacklevel=3)
+        _native = _Declines
+        return _native
 
 
 def _refuse(t, name, dtype, shape, dev):
@@ -158,7 +177,7 @@ class KV4Cache:
     def read(self, cache_rows, k_out=None, v_out=None):
         """The f32 values of cache rows (int64 [n], row = sequence * max_len + position; zeros for a row outside the
         cache): K and V, each [n, n_kv_heads, head_dim]."""
-        done = (_native or native()).read(self._held, self.head_dim, cache_rows, k_out, v_out)
+        done = (_native or _calls()).read(self._held, self.head_dim, cache_rows, k_out, v_out)
         if done is not None:
             return done
         dev = self._dev
@@ -183,7 +202,7 @@ def qknorm_rope_append(qkv, positions, cache_rows, cos, sin, cache, n_heads: int
     ``cache`` is a KV4Cache or a pair (k, v) of float32 caches [n_seqs, n_kv_heads, max_len, head_dim].  Returns the
     queries, float32 [n, n_heads, head_dim].  Two tokens of one call must not name the same cache row."""
     four = isinstance(cache, KV4Cache)
-    done = (_native or native()).append(qkv, positions, cache_rows, cos, sin, cache._held if four else cache, cache.head_dim if four else 0,
+    done = (_native or _calls()).append(qkv, positions, cache_rows, cos, sin, cache._held if four else cache, cache.head_dim if four else 0,
                                         n_heads, q_gamma, k_gamma, eps, q_out)
     if done is not None:
         return done
@@ -225,7 +244,7 @@ def attend(q, cache: KV4Cache, lens, *, scale: float = 0.0, out=None):
     (or [n_seqs, n_heads, head_dim], t = 1), lens int32 [n_seqs] the cache positions up to and including the last of the t
     tokens.  Token i sees the positions below lens - (t - 1 - i); one that sees none gives zeros.  scale 0 is
     1 / sqrt(head_dim).  Returns float32 of q's shape."""
-    done = (_native or native()).attend(cache._held, cache.head_dim, q, lens, scale, out)
+    done = (_native or _calls()).attend(cache._held, cache.head_dim, q, lens, scale, out)
     if done is not None:
         return done
     hd, dev, n = cache.head_dim, cache._dev, cache.n_seqs
@@ -255,7 +274,7 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, r
     float32 [n], top_k int32 [n].  A temperature of 0 is greedy.  Top-k and min-p act on the tempered distribution, top-p
     on what they keep.  Returns int64 [n], with return_logprobs also float32 [n]: the log of the token's share of what was
     kept."""
-    done = (_native or native()).sample(logits, u, temperature, top_k, top_p, min_p, return_logprobs, tokens)
+    done = (_native or _calls()).sample(logits, u, temperature, top_k, top_p, min_p, return_logprobs, tokens)
     if done is not None:
         return done
     dev = _rows(logits, "logits", _F32, "[n, vocab]", 2)

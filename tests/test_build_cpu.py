@@ -69,3 +69,25 @@ def test_a_module_of_another_torch_is_not_taken_for_current(monkeypatch, sandbox
     assert _build.build_module() == first and runs.programs == ["g++"]
     monkeypatch.setattr(torch, "__version__", "0.0.1")
     assert _build.build_module() != first and runs.programs == ["g++", "g++"]
+
+
+@pytest.mark.parametrize("broken", [False, True])
+def test_calls_without_the_module_go_the_other_way(monkeypatch, tmp_path, broken):
+    """one warning, then the Python layer's own checks and errors; asking for the module itself is an error"""
+    import torch
+
+    from kore_b200 import KoreError, serving
+
+    path = tmp_path / "m.so"
+    if broken:
+        path.write_bytes(b"not a library")
+    monkeypatch.setattr(_build, "module_path", lambda: str(path))
+    monkeypatch.setattr(serving, "_native", None)
+    with pytest.warns(RuntimeWarning, match="native module"), pytest.raises(KoreError, match="logits"):
+        serving.sample(torch.zeros(2, 5), torch.zeros(2))
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with pytest.raises(KoreError, match="logits"):
+            serving.sample(torch.zeros(2, 5), torch.zeros(2))
+    with pytest.raises(ImportError if broken else RuntimeError):
+        serving.native()

@@ -105,3 +105,23 @@ def test_decoder_counts_the_draw_behind_the_persistent_step(env):
         dec.decode_step()
         assert dec.launches_per_step == launches
     dec.close()
+
+
+# ---- without the native module ------------------------------------------------------------------
+def test_results_without_the_native_module(env, monkeypatch):
+    """the four operators by way of the interpreter: the same bits"""
+    t, s = env.torch, env.serving
+    hd, lmax = 64, 2000
+    cos, sin = (env.dev(np.asarray(a, f32)) for a in (np.cos(np.arange(lmax))[:, None].repeat(hd // 2, 1), np.sin(np.arange(lmax))[:, None].repeat(hd // 2, 1)))
+    x, q = env.dev(cases.gaussian(1, (6, 8 * hd), 1.0)), env.dev(cases.gaussian(2, (2, 3, 4, hd), 1.0))
+    rows, lens = env.dev(np.array([0, 1, 2, lmax, lmax + 1, 2 * lmax - 1])), env.dev(np.array([3, lmax], np.int32))
+    pos = (rows % lmax).int()
+    logits, u = env.dev(cases.gaussian(3, (5, 3001), 2.0)), t.rand(5, device="cuda")
+
+    def run():
+        cache = s.KV4Cache(2, 2, lmax, hd)
+        out = [s.qknorm_rope_append(x, pos, rows, cos, sin, cache, 4), *cache.read(rows), s.attend(q, cache, lens)]
+        return out + list(s.sample(logits, u, top_p=t.full((5,), 0.9, device="cuda"), return_logprobs=True))
+    with_module = run()
+    monkeypatch.setattr(s, "_native", s._Declines)
+    assert all((a == b).all() for a, b in zip(with_module, run()))
