@@ -110,6 +110,11 @@ def _run(dev: int, fn, *args):
         _cabi.check(rc)
 
 
+def _check_head_dim(head_dim):
+    if head_dim < 4 or head_dim > 128 or head_dim % 4:
+        raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: head_dim {head_dim} must be a multiple of 4 up to 128")
+
+
 class KV4Cache:
     """K and V of ``n_seqs`` sequences in 4 bits: per (sequence, KV head, position) a row of codes and one (step, lo) pair
     of bfloat16 numbers, 4.25 bits a value for heads of 128 (f32 caches take 32).
@@ -122,6 +127,7 @@ class KV4Cache:
             raise KoreError(_cabi.ERR_INVALID, f"KV4Cache: {n_seqs} sequences, {n_kv_heads} KV heads, {max_len} positions")
         if max_len > 1 << 30:
             raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: {max_len} positions, at most {1 << 30}")
+        _check_head_dim(head_dim)
         max_len = (max_len + 3) // 4 * 4
         dev = torch.device("cuda", device)
         words = int(_cabi.lib().kb_kv4_row_words(head_dim))
@@ -137,8 +143,7 @@ class KV4Cache:
         return self
 
     def _adopt(self, k_codes, k_steps, v_codes, v_steps, head_dim):
-        if head_dim < 4 or head_dim > 128 or head_dim % 4:
-            raise KoreError(_cabi.ERR_UNSUPPORTED, f"KV4Cache: head_dim {head_dim} must be a multiple of 4 up to 128")
+        _check_head_dim(head_dim)
         dev = _rows(k_codes, "k_codes", _I32, "[n_seqs, n_kv_heads, max_len, words]", 4)
         shape = tuple(k_codes.shape[:3]) + ((head_dim + 7) // 8,)
         for t, name, want in ((k_codes, "k_codes", shape), (k_steps, "k_steps", shape[:3]), (v_codes, "v_codes", shape),
