@@ -265,8 +265,8 @@ int kb_decoder_status(kb_decoder *h, kb_stream stream, int *status);
  * to 2^30, the planes are 16-byte aligned.  A row is quantised from its own f32 values x:
  *   lo = bfloat16 at or below min(x);  step = bfloat16 at or above max((max(x) - lo) / 15, 2^-100);
  *   code = clamp(rne((x - lo) * (1 / step)), 0, 15)
- * with every f32 operation rounded once.  A row that holds an infinity or a NaN, or whose range overflows f32, is stored
- * with NaN for both numbers and reads back as NaN. */
+ * with every f32 operation rounded once.  A row that holds an infinity or a NaN, whose range overflows f32 or whose lowest
+ * value lies below the bfloat16 numbers is stored with NaN for both numbers and reads back as NaN. */
 size_t kb_kv4_row_words(int head_dim);
 
 /* Per token: RMSNorm of every query and key head over its head_dim (q_gamma / k_gamma [head_dim], each nullable: no norm),
@@ -295,9 +295,12 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
  * reads KV head h / (n_heads / n_kv_heads).  lens[b] counts the cache positions up to and including the last query token's
  * (clamped to 0 .. lmax): query token i sees the positions below lens[b] - (t - 1 - i).  A query that sees none gives
  * zeros; positions it does not see have no influence, whatever they hold.  scale multiplies the scores, 0 means
- * 1 / sqrt(head_dim).  Statistics and sums are f32; queries and softmax weights enter the products with 22 bits (results
- * within 1e-6 .. 2e-6 of 64-bit ones).  A query with an infinity or a NaN, or one that scale * log2(e) takes to 2^120 and
- * beyond, gives NaN.  Sums are held up to 2^8 times the weights and divided last, so values of V from 2^119 / lens on may
+ * 1 / sqrt(head_dim).  Statistics and sums are f32; queries and softmax weights enter the products with 22 bits, and the sums
+ * of a tile are cut off, not rounded, by the matrix instruction.  Against 64 bits a result is within 6e-6 for unit-normal
+ * queries, keys and values (about 1e-6 is measured), and for any within (2 e + 2^-16) max|v| with the bound of a score's
+ * error e = 2^-16 scale sum|q_d| max|k_d|.  A query with an infinity or a NaN, or one that scale * log2(e) takes to 2^120 and
+ * beyond, gives NaN; scores may overflow, to the same effect, where scale log2(e) sum|q_d| max|k_d| reaches 2^122.  Sums
+ * are held up to 2^8 times the weights and divided last, so values of V from 2^119 / lens on may
  * overflow.  The same call gives the same bits.  out may be q.  workspace: kb_attn_kv4_workspace_bytes bytes (for the
  * current device), 16-byte aligned, no initial contents needed, not shared by calls that overlap; NULL takes it from the
  * stream-ordered allocator. */

@@ -41,6 +41,41 @@ def test_attention_of_large_values_under_rising_weights(env):
     check_attention(env, np.full((1, 1, 1, hd), 1 / 8, f32), cache_of(env, k, v), [n])
 
 
+@pytest.mark.parametrize("rows", ["constant", "spread"])
+def test_attention_of_the_largest_scores(env, rows):
+    """scale log2(e) sum|q| max|k| of 2^121.5: one position has all the weight"""
+    hd, n, heads = 64, 300, 2
+    rng = np.random.default_rng(4)
+    q = np.abs(cases.gaussian(5, (1, 1, heads, hd), 30.0))
+    if rows == "spread":
+        q *= rng.choice([-1, 1], hd).astype(f32)
+        k = rng.uniform(-0.9, 0.9, (1, heads, n, hd))
+        k[0, :, 211] = np.sign(q[0, 0])
+    else:
+        k = np.broadcast_to((rng.permutation(n)[None, :, None] + 1.0) / n, (1, heads, n, hd))
+    k = (k * 2.0 ** 121.5 * np.log(2.0) * np.sqrt(hd) / np.abs(q).sum(-1).max()).astype(f32)
+    cache = cache_of(env, k, rng.standard_normal((1, heads, n, hd)).astype(f32))
+    got = env.serving.attend(env.dev(q), cache, env.dev(np.array([n], np.int32)))[0, 0].cpu().numpy()
+    at = 211 if rows == "spread" else int(k[0, 0, :, 0].argmax())
+    value = cache.read(env.dev(np.array([at])))[1][0].cpu().numpy()
+    # the next score is lower by far more than any rounding (1 / 300 of the largest at least): a weight of 1, held to 22 bits
+    assert (np.abs(got - value) <= 2.0 ** -20 * np.abs(value).max()).all()
+
+
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_rows_below_the_bfloat16_numbers(env, side):
+    """-3.4e38 is an f32 number, but no bfloat16 number lies at or below it; the next row is an ordinary one"""
+    hd = 8
+    x = np.full((2, 3 * hd), -1.0, f32)
+    x[0, slice(hd, 2 * hd) if side == "k" else slice(2 * hd, None)] = -3.4e38
+    cache, one, zero = env.serving.KV4Cache(1, 1, 4, hd), np.ones((4, hd // 2), f32), np.zeros((4, hd // 2), f32)
+    i = np.arange(2)
+    env.serving.qknorm_rope_append(env.dev(x), env.dev(i.astype(np.int32)), env.dev(i), env.dev(one), env.dev(zero), cache, 1)
+    for name, got in zip("kv", cache.read(env.dev(i))):
+        got = got.cpu().numpy()[:, 0]
+        assert (np.isnan(got[0]).all() if name == side else (got[0] == -1).all()) and (got[1] == -1).all()
+
+
 # seeds of rows and top_p whose border, less the accuracy of the sums that look for it, lies where running sums in f64 of
 # neighbouring threads do not meet: found by a search on the CPU over 2e8 rows
 BETWEEN = [(38773736, 0.932712317), (65209376, 0.979467869), (186987744, 0.996985555), (74197353, 0.98854059), (171723530, 0.690360785),
