@@ -29,31 +29,9 @@ namespace kb {
 
 // Every kernel here is launched with programmatic stream serialization, so its CTAs may be resident while the
 // producer of its inputs still runs.  Inputs that an earlier kernel of the step writes (activations, positions,
-// lengths, caches) are therefore plain pointers, read after the wait below: a `const __restrict__` pointer would let
+// lengths, caches) are therefore plain pointers, read after pdl_release_and_wait: a `const __restrict__` pointer would let
 // the compiler use the non-coherent path and hoist the loads above the wait (a head kernel did exactly that and read
 // the previous step's row).  Only true constants (weights, gamma, the RoPE tables) keep the qualifier.
-__device__ __forceinline__ void pdl_release_and_wait() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
-    static const bool pdl = [] {
-        const char *v = getenv("KB_GEMV_PDL");
-        return !(v && *v == '0');
-    }();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
-}
 
 __device__ __forceinline__ float block_reduce_sum_f(float v, float *scratch) {
 #pragma unroll
@@ -512,7 +490,6 @@ int kb_lm_head_argmax(const float *x, size_t n, size_t d, const float *w, size_t
     void (*kern)(const float *, int, int, const float *, int, float *, unsigned long long *) =
         tok == 2 ? lm_head_argmax_kernel<2> : (tok == 4 ? lm_head_argmax_kernel<4> : lm_head_argmax_kernel<HEAD_TOK>);
     if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, (int)smem, "lm_head smem attribute")) return rc;
-    static const bool pdl = [] { const char *v = getenv("KB_GEMV_PDL"); return !(v && *v == '0'); }();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)gx, groups);
     cfg.blockDim = dim3(HEAD_THREADS);
@@ -522,7 +499,7 @@ int kb_lm_head_argmax(const float *x, size_t n, size_t d, const float *w, size_t
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kern, x, (int)n, (int)d, w, (int)vocab, logits, keys);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "lm_head launch");
 }
@@ -543,7 +520,7 @@ int kb_rmsnorm_quant(const float *x, const float *gamma, size_t n, size_t d, flo
     if (d == 0 || d > (size_t)ROW_REGS * 256) return fail(KB_ERR_UNSUPPORTED, "rmsnorm: dim %zu outside 1..%d", d, ROW_REGS * 256);
     if (xq && (ldq < d || ldq > (size_t)ROW_REGS * 256 || ldq % 16)) return fail(KB_ERR_INVALID, "rmsnorm: bad ldq %zu", ldq);
     if (n == 0) return KB_OK;
-    cudaError_t e = launch_pdl(rmsnorm_quant_kernel, dim3((unsigned)n), dim3(256), static_cast<cudaStream_t>(stream), x, gamma,
+    cudaError_t e = launch_pdl(rmsnorm_quant_kernel, dim3((unsigned)n), dim3(256), 0, static_cast<cudaStream_t>(stream), x, gamma,
                                (int)d, eps, xn, xq, (int)ldq, sx, sumq);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "rmsnorm launch");
 }
@@ -556,9 +533,9 @@ static int swiglu_quant(bool pairs, const float *gate_up, size_t n, size_t f, si
     if (f == 0 || f > (size_t)ROW_REGS * 256 || ld < 2 * f) return fail(KB_ERR_UNSUPPORTED, "swiglu: width %zu outside 1..%d", f, ROW_REGS * 256);
     if (xq && (ldq < f || ldq > (size_t)ROW_REGS * 256 || ldq % 16)) return fail(KB_ERR_INVALID, "swiglu: bad ldq %zu", ldq);
     if (n == 0) return KB_OK;
-    cudaError_t e = pairs ? launch_pdl(swiglu_quant_kernel<true>, dim3((unsigned)n), dim3(256), static_cast<cudaStream_t>(stream),
+    cudaError_t e = pairs ? launch_pdl(swiglu_quant_kernel<true>, dim3((unsigned)n), dim3(256), 0, static_cast<cudaStream_t>(stream),
                                        gate_up, (int)f, ld, h, xq, (int)ldq, sx, sumq)
-                          : launch_pdl(swiglu_quant_kernel<false>, dim3((unsigned)n), dim3(256), static_cast<cudaStream_t>(stream),
+                          : launch_pdl(swiglu_quant_kernel<false>, dim3((unsigned)n), dim3(256), 0, static_cast<cudaStream_t>(stream),
                                        gate_up, (int)f, ld, h, xq, (int)ldq, sx, sumq);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "swiglu launch");
 }
@@ -582,7 +559,7 @@ int kb_rope_kv(const float *qkv, const int *positions, const long long *cache_ro
     if (lmax < 1) return fail(KB_ERR_INVALID, "rope: cache length %d", lmax);
     if (n == 0) return KB_OK;
     const unsigned chunks = (unsigned)((n_heads * (head_dim / 2) + 255) / 256);
-    cudaError_t e = launch_pdl(rope_kv_kernel, dim3((unsigned)n, chunks), dim3(256), static_cast<cudaStream_t>(stream), qkv,
+    cudaError_t e = launch_pdl(rope_kv_kernel, dim3((unsigned)n, chunks), dim3(256), 0, static_cast<cudaStream_t>(stream), qkv,
                                positions, cache_rows, cos_table, sin_table, n_heads, head_dim, lmax, q_out, k_cache, v_cache);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "rope launch");
 }
@@ -609,10 +586,10 @@ int kb_attn_decode(const float *q, const float *k_cache, const float *v_cache, c
     float *parts = scratch ? reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(scratch) + (bh * sizeof(int) + 255) / 256 * 256) : nullptr;
     const bool vec4 = head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
                                              reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0;
-    cudaError_t e = vec4 ? launch_pdl(attn_decode_kernel<true>, dim3((unsigned)(bh * splits)), dim3(ATT_WARPS * 32),
+    cudaError_t e = vec4 ? launch_pdl(attn_decode_kernel<true>, dim3((unsigned)(bh * splits)), dim3(ATT_WARPS * 32), 0,
                                       static_cast<cudaStream_t>(stream), q, k_cache, v_cache, lens, n_heads, head_dim, lmax,
                                       splits, parts, counters, out)
-                         : launch_pdl(attn_decode_kernel<false>, dim3((unsigned)(bh * splits)), dim3(ATT_WARPS * 32),
+                         : launch_pdl(attn_decode_kernel<false>, dim3((unsigned)(bh * splits)), dim3(ATT_WARPS * 32), 0,
                                       static_cast<cudaStream_t>(stream), q, k_cache, v_cache, lens, n_heads, head_dim, lmax,
                                       splits, parts, counters, out);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "attention launch");

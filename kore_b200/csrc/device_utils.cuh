@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 namespace kb {
 
@@ -84,5 +85,33 @@ __device__ __forceinline__ void st_pair(float *base, size_t o, float value, uint
                  : "memory");
 }
 
+
+// ---- programmatic stream serialization: a kernel starts while its predecessor runs, and waits before it touches anything that
+// an earlier kernel writes or reads.  Such inputs are plain pointers: a `const __restrict__` one may be loaded ahead of the wait
+__device__ __forceinline__ void pdl_release_and_wait() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+inline bool pdl_enabled() {
+    static const bool on = [] {
+        const char *v = getenv("KB_GEMV_PDL");
+        return !(v && *v == '0');
+    }();
+    return on;
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
+}
 
 }  // namespace kb

@@ -6,7 +6,6 @@
 //     step_j * sum_d(q_d c_jd) + lo_j * sum_d(q_d)      and an output      sum_j (p_j step_j) c_jd + sum_j p_j lo_j,
 // so both contractions run on bare codes and the pair touches one number per (query, position).
 #include <cuda_fp16.h>
-#include <stdlib.h>
 
 #include "common.cuh"
 #include "device_utils.cuh"
@@ -20,31 +19,6 @@ __host__ __device__ inline int kv4_words(int hd) { return (hd + 7) / 8; }
 
 __device__ __forceinline__ float kv4_step(uint32_t s) { return __uint_as_float(s << 16); }
 __device__ __forceinline__ float kv4_lo(uint32_t s) { return __uint_as_float(s & 0xffff0000u); }
-
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_after(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
-    static const bool pdl = [] {
-        const char *v = getenv("KB_GEMV_PDL");
-        return !(v && *v == '0');
-    }();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
-}
-
-// as in decoder_ops.cu: inputs that an earlier kernel of the step writes are plain pointers, read after this
-__device__ __forceinline__ void release_and_wait() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 
 // ---- norm + rotation + append ------------------------------------------------------------------
 struct AppendParams {
@@ -138,7 +112,7 @@ template <bool Q4, int HPW, bool PAIRS, bool FULL = false>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 8u + (threadIdx.x >> 5);
-    release_and_wait();
+    pdl_release_and_wait();
     if (task >= p.tasks) return;
     const int heads = p.n_heads + 2 * p.n_kv, hd = FULL ? 128 : p.hd, half = hd / 2;
     const unsigned t = task / p.groups;
@@ -308,7 +282,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint32_t *k_codes, 
                                                        int n_kv, int hd, long long cache_len, int lmax, float *k_out, float *v_out) {
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 8u + (threadIdx.x >> 5);
-    release_and_wait();
+    pdl_release_and_wait();
     if (task >= tasks || 4 * lane >= hd) return;
     const unsigned i = task / groups;
     const int head0 = (int)(task - i * groups) * READ_HEADS, words = kv4_words(hd);
@@ -539,7 +513,7 @@ __global__ void __launch_bounds__(ATT4_WARPS * 32, ATT4_PER_SM) attn_kv4_kernel(
     __shared__ int s_off[ROWS];        // positions behind the sequence's end that a row does not see
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rep = p.rep, hd = p.hd;
-    release_and_wait();
+    pdl_release_and_wait();
     AttnWork work;
     if (!find_attn_work(p, work)) return;
     const int b = work.b, kvh = work.unit / p.row_tiles, len = work.len;
@@ -917,7 +891,7 @@ static int launch_attn_kv4(const AttnParams &p, unsigned ctas, int dev, cudaStre
     void (*kern)(AttnParams) = one ? attn_kv4_kernel<W, 1> : attn_kv4_kernel<W, 2>;
     const size_t smem = one ? Attn4<W, 1>::SMEM : Attn4<W, 2>::SMEM;
     if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(kern), dev, (int)smem, "kv4 attention smem attribute")) return rc;
-    const cudaError_t e = launch_after(kern, dim3(ctas), dim3(ATT4_WARPS * 32), smem, stream, p);
+    const cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(ATT4_WARPS * 32), smem, stream, p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 attention launch");
 }
 
@@ -927,7 +901,7 @@ __global__ void __launch_bounds__(KV4_MAX_HD) attn_kv4_join_kernel(AttnParams p)
     const unsigned row = blockIdx.x, tok = row / p.n_heads;
     const int lane = threadIdx.x & 31, d = threadIdx.x, h = row - tok * p.n_heads, b = tok / p.t, i = tok - b * p.t;
     const int kvh = h / p.rep, r = i * p.rep + h - kvh * p.rep, tile = r / p.tile_rows;
-    release_and_wait();
+    pdl_release_and_wait();
     const int2 of = p.part_of[((size_t)b * p.n_kv + kvh) * p.row_tiles + tile];
     const int n = of.y;
     if (n == 1) return;  // the first kernel wrote it
@@ -1033,7 +1007,7 @@ static int append(AppendParams &p, bool q4, size_t n, size_t max_pos, size_t n_s
     void (*kern)(AppendParams) =
         q4 ? (many ? (pairs ? (p.hd == 128 ? append_kernel<true, 4, true, true> : append_kernel<true, 4, true>) : append_kernel<true, 4, false>) : (pairs ? append_kernel<true, 1, true> : append_kernel<true, 1, false>))
            : (many ? (pairs ? (p.hd == 128 ? append_kernel<false, 4, true, true> : append_kernel<false, 4, true>) : append_kernel<false, 4, false>) : (pairs ? append_kernel<false, 1, true> : append_kernel<false, 1, false>));
-    const cudaError_t e = launch_after(kern, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
+    const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "append launch");
 }
 
@@ -1090,7 +1064,7 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
     unsigned tasks = 0, grid = 0;
     const unsigned groups = (unsigned)(n_kv_heads + READ_HEADS - 1) / READ_HEADS;
     if (int rc = warp_grid(n, groups, &tasks, &grid)) return rc;
-    const cudaError_t e = launch_after(kv4_read_kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), k_codes, k_steps, v_codes,
+    const cudaError_t e = launch_pdl(kv4_read_kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), k_codes, k_steps, v_codes,
                                        v_steps, cache_rows, tasks, groups, n_kv_heads, head_dim, (long long)n_seqs * lmax, lmax, k_out, v_out);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "kv4 read launch");
 }
@@ -1140,7 +1114,7 @@ int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps
     }
     int rc = launch_attn_kv4<KV4_MAX_HD / 8>(p, (unsigned)plan.ctas, dev, st);
     if (rc == KB_OK && plan.slots) {
-        const cudaError_t e = launch_after(attn_kv4_join_kernel, dim3((unsigned)rows), dim3(KV4_MAX_HD), 0, st, p);
+        const cudaError_t e = launch_pdl(attn_kv4_join_kernel, dim3((unsigned)rows), dim3(KV4_MAX_HD), 0, st, p);
         if (e != cudaSuccess) rc = cuda_fail(e, "kv4 attention join launch");
     }
     if (own) {

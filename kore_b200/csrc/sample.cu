@@ -22,7 +22,6 @@
 // weights by segment already, and the CTA that holds the number walks the segment that does.
 #include <float.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include <type_traits>
 
@@ -624,8 +623,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(SampleParams 
         const double s = exp2(44.0 + (double)threadIdx.x * (1.0 / 32));
         sh.scale[threadIdx.x] = __hiloint2double(__double2hiint(s) - ((int)threadIdx.x << 15), __double2loint(s));
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_release_and_wait();
     const float *src = p.logits + r * p.ld + row.i0;
     row.l = src;
     row.wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
@@ -828,7 +826,6 @@ extern "C" int kb_sample(const float *logits, size_t n, size_t vocab, size_t ld,
     SampleParams p = {logits, ld, (int)vocab, slice, held, temperature, top_k, top_p, min_p, u, tokens, logprobs};
     const size_t smem = SAMPLE_FIXED + (held ? (size_t)slice * 4 : 0);
     if (int rc = set_dyn_smem_once(reinterpret_cast<const void *>(sample_kernel), dev, 200 * 1024, "sample smem attribute")) return rc;
-    static const bool pdl = [] { const char *v = getenv("KB_GEMV_PDL"); return !(v && *v == '0'); }();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ctas));
     cfg.blockDim = dim3(SAMPLE_THREADS);
@@ -841,7 +838,7 @@ extern "C" int kb_sample(const float *logits, size_t n, size_t vocab, size_t ld,
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 2 : 1;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel, p);
     return e == cudaSuccess ? KB_OK : cuda_fail(e, "sample launch");
 }
