@@ -101,8 +101,8 @@ __device__ __forceinline__ double warp_sum_of(double (&v)[HPW]) {
 }
 
 // Bound by one memory round trip for a few tokens (16 tokens, 32 heads of 100, norms, f32 cache: 2.7 us) and for many by the
-// bytes of the rows, which the quantiser does not quite hide: 8192 tokens of 32 + 2 x 8 heads of 128 with norms take 66 us
-// (4.7 TB/s; 62 us, 5.1 TB/s, with an f32 cache).  A warp takes HPW heads of one token:
+// bytes of the rows, which the quantiser does not quite hide: 8192 tokens of 32 + 2 x 8 heads of 128 with norms take 66 us for
+// 344 MB of rows read and written (5.2 TB/s; 62 us for 402 MB, 6.5 TB/s, with an f32 cache).  A warp takes HPW heads of one token:
 // its lane l owns the rotation pairs 2l and 2l + 1, dims {2l, 2l + 1} of each half, so that its codes are whole bytes of the
 // row, a row needs no shared memory, and the token's angles are read once for all heads.
 // PAIRS: rows and tables are 8-byte aligned and half is even, a lane's two neighbours come and go in one access.
@@ -158,7 +158,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
     const bool normed = p.q_gamma || p.k_gamma;
     float inv_of = 0.0f;  // of head lane / (32 / HPW)
     if (normed) {
-        double ss[HPW];  // f64: the order of the sum then cannot move a rounding of inv, so codes do not depend on it
+        // f64, in one order whatever HPW (lanes 16, 8, 4, 2, 1 apart), so that every launch gives the same codes.  A sum in
+        // another order rounds inv differently in about one row of 2^28
+        double ss[HPW];
 #pragma unroll
         for (int j = 0; j < HPW; ++j) {
             ss[j] = 0.0;
@@ -348,8 +350,11 @@ constexpr int ATT4_PER_SM = 4;   // resident CTAs: 128 registers a thread (five 
 constexpr int ATT4_TILE = 32;  // positions of a warp's tile
 constexpr int ATT4_ROWS = 4;   // query rows of a set of columns
 constexpr int ATT4_GRAIN = ATT4_WARPS * ATT4_TILE;  // positions that give every warp a tile
-// A cache of so many grains is not split: 577 positions of one sequence and 32 KV heads take 6.4 us whole, 7.3 us in five chunks;
-// from ATT4_MANY units on two grains more (4 sequences of 760 positions, 8 KV heads, five tokens: 10.8 us whole, 14.2 split)
+// A cache with room for so many grains is not split, so that the call is one launch without a search for work and a join: 577
+// positions of one sequence and 32 KV heads take 6.4 us, and 7.2 us split, in a cache of 1024; from ATT4_MANY units on two grains more
+// (4 sequences of 760 positions, 8 KV heads, five tokens: 10.8 us whole, 14.2 split).  By capacity, because the host does not know
+// the lengths: in a larger cache both kernels run, and sequences of these lengths are then better split than kept whole (the 577: 7.2
+// and 7.9 us; 16 sequences of 513 .. 640, 8 KV heads: 12.8 and 13.6 us), but for the shortest (16 of 100 .. 200: 9.9 and 8.0 us)
 constexpr int ATT4_WHOLE = 5, ATT4_MANY = 32;
 constexpr int ATT4_ROUND = 32;  // chunks that the second kernel takes in a round
 constexpr float ATT4_SLACK = 8.0f;  // log2 of how far a weight may rise above the reference
