@@ -297,13 +297,13 @@ int kb_kv4_read(const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t
  * zeros; positions it does not see have no influence, whatever they hold.  scale multiplies the scores, 0 means
  * 1 / sqrt(head_dim).  Statistics and sums are f32; queries and softmax weights enter the products with 22 bits, and the sums
  * of a tile are cut off, not rounded, by the matrix instruction.  Against 64 bits a result is within 6e-6 for unit-normal
- * queries, keys and values (1e-6 is usual, 3e-6 the most in half a million random calls), and for any within (2 e + 2^-16) max|v| with the bound of a score's
- * error e = 2^-16 scale sum|q_d| max|k_d|.  A query with an infinity or a NaN, or one that scale * log2(e) takes to 2^120 and
- * beyond, gives NaN; scores may overflow, to the same effect, where scale log2(e) sum|q_d| max|k_d| reaches 2^122.  Sums
- * are held up to 2^8 times the weights and divided last, so values of V from 2^119 / lens on may
- * overflow.  The same call gives the same bits.  out may be q.  workspace: kb_attn_kv4_workspace_bytes bytes (for the
- * current device), 16-byte aligned, no initial contents needed, not shared by calls that overlap; NULL takes it from the
- * stream-ordered allocator. */
+ * queries, keys and values (1e-6 is usual, 3e-6 the most in half a million random sequences), and for any within
+ * (2 e + 2^-16) max|v| with the bound of a score's error e = 2^-16 scale sum|q_d| max|k_d|.  A query with an infinity or a NaN,
+ * or one that scale * log2(e) takes to 2^120 and beyond, gives NaN; scores may overflow, to the same effect, where
+ * scale log2(e) sum|q_d| max|k_d| reaches 2^122.  Sums are held up to 2^8 times the weights and divided last, so values of V
+ * from 2^119 / lens on may overflow.  The same call gives the same bits.  out may be q.  workspace:
+ * kb_attn_kv4_workspace_bytes bytes (for the current device), 16-byte aligned, no initial contents needed, not shared by calls
+ * that overlap; NULL takes it from the stream-ordered allocator. */
 int kb_attn_kv4(const float *q, const uint32_t *k_codes, const uint32_t *k_steps, const uint32_t *v_codes,
                 const uint32_t *v_steps, const int *lens, size_t batch, int t, int n_heads, int n_kv_heads, int head_dim,
                 int lmax, float scale, float *out, void *workspace, size_t workspace_bytes, kb_stream stream);

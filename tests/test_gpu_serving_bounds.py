@@ -4,7 +4,7 @@ import pytest
 
 from oracle import serving_ref as sr
 from tests import cases
-from tests.test_gpu_serving import check_attention, check_sample, env  # noqa: F401
+from tests.test_gpu_serving import check_attention, check_sample, env, filled_cache, tables  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 f32 = np.float32
@@ -160,3 +160,59 @@ def test_results_without_the_native_module(env, monkeypatch):
     with_module = run()
     monkeypatch.setattr(s, "_native", s._Declines)
     assert all((a == b).all() for a, b in zip(with_module, run()))
+
+
+# ---- calls that the header allows --------------------------------------------------------------
+@pytest.mark.parametrize("scale", [-0.2, 1e-3, 3.0])
+@pytest.mark.parametrize("lmax", [300, 1500])
+def test_attention_scales(env, scale, lmax):
+    check_attention(env, cases.gaussian(70, (2, 2, 6, 44), 1.0), filled_cache(env, 2, 3, lmax, 44, 71), [lmax, lmax // 2 + 1], scale)
+
+
+@pytest.mark.parametrize("n", [3, 700])
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_append_with_one_gamma(env, n, which):
+    """norms of queries alone or of keys alone, for few and for many tokens"""
+    heads, kv, hd, lmax = 6, 2, 36, 704
+    qkv = cases.gaussian(n, (n, (heads + 2 * kv) * hd), 2.0)
+    gamma = (1 + cases.gaussian(7, (hd,), 0.2)).astype(f32)
+    gq, gk = (gamma, None) if which == "q" else (None, gamma)
+    cos, sin = tables(lmax, hd)
+    i = np.arange(n)
+    cache = env.serving.KV4Cache(1, kv, lmax, hd)
+    q = env.serving.qknorm_rope_append(env.dev(qkv), env.dev(i.astype(np.int32)), env.dev(i), env.dev(cos), env.dev(sin), cache, heads,
+                                       **{which + "_gamma": env.dev(gamma)})
+    rq, rk, rv = sr.append(qkv, i, cos, sin, heads, kv, hd, gq, gk)
+    assert (q.cpu().numpy() == rq).all()
+    for got, x in zip(cache.read(env.dev(i)), (rk, rv)):
+        assert (got.cpu().numpy() == sr.values(*sr.quantise(x), hd)).all()
+
+
+def test_read_of_one_side(env):
+    """a C caller may ask for keys or values alone, and then has no planes of the other"""
+    from kore_b200 import _cabi
+
+    t, seqs, kv, lmax, hd = env.torch, 2, 3, 40, 20
+    cache = filled_cache(env, seqs, kv, lmax, hd, 72)
+    rows = env.dev(np.array([0, 41, -1, 79, 80, 7]))
+    both = cache.read(rows)
+    stream = t.cuda.current_stream().cuda_stream
+    for side, planes in enumerate(((cache.k_codes, cache.k_steps), (cache.v_codes, cache.v_steps))):
+        out = t.full((6, kv, hd), 5.0, device="cuda")
+        a, b = (x.data_ptr() for x in planes)
+        args = (a, b, None, None) if side == 0 else (None, None, a, b)
+        outs = (out.data_ptr(), None) if side == 0 else (None, out.data_ptr())
+        _cabi.check(_cabi.lib().kb_kv4_read(*args, rows.data_ptr(), 6, kv, hd, seqs, lmax, *outs, stream))
+        t.cuda.synchronize()
+        assert (out == both[side]).all()
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_sample_rows_at_any_address(env, offset):
+    """slices of a wider matrix, one row and several, whose rows start at every place of 16 bytes"""
+    wide = env.dev(cases.gaussian(73, (3, 5011), 2.5))
+    for n in (1, 3):
+        view = wide[:n, offset:offset + 5003]
+        check_sample(env, view, np.array([0.2, 0.6, 0.93][:n], f32), top_p=0.9)
+        check_sample(env, view, np.array([0.2, 0.6, 0.93][:n], f32), top_k=30, temperature=0.7)
+        check_sample(env, view, np.array([0.2, 0.6, 0.93][:n], f32), temperature=0.0)
